@@ -474,6 +474,122 @@ int vedic_flash_attention_bwd_heads(const float* const* Q, const float* const* K
                                     int dh, float scale, int causal, int shunyam, int window, int stride,
                                     void* stream);
 
+/* ---- rows that choose their weights: routed experts, adapters ------------- */
+
+/* New: the reference has one feed-forward layer per block (include/FeedForward.hpp)
+ * and no adapters.  One plan serves them all: `rows` lists rows sorted by group
+ * (an expert, an adapter), offsets[g] .. offsets[g + 1] - 1 are group g's places in
+ * it.  Plans stay on the GPU: no call reads one on the host or waits for it.  What
+ * a plan holds is clamped where it is read (an offset to 0 .. n, a row or slot
+ * outside its matrix counts as none), so a bad plan gives wrong values but no
+ * access outside the arrays.  Limits: 1024 groups, leading dimensions below 2^22,
+ * counts below 2^30 (VEDIC_STATUS_TOO_LARGE). */
+
+/* The router: for each of T tokens the k largest of its E logits, a tie to the
+ * lower index, and their weights exp(x_j - max) / sum, the sum over the chosen
+ * ones (renorm != 0) or over all E (renorm == 0); then the T k pairs sorted by
+ * expert and, within one, by token.
+ *   ids, weights [T x k]   in descending order of the logits
+ *   offsets [E + 1]        the first sorted place of each expert, and the end
+ *   rows [T k]             the token of each place
+ *   slots [T x k]          the place of each pair
+ * A logit of -infinity is never chosen: a token with fewer than k others gets id
+ * -1, weight 0 and slot -1 in the rest, and the places behind offsets[E] have row
+ * -1.  NaN counts as larger than every number (and makes its token's weights NaN).
+ * k <= 64.  More than 64 tokens or 1024 pairs take a few KB of the stream's
+ * workspace block. */
+int vedic_route_topk(const float* logits, int64_t ld_logits, int T, int E, int k, int renorm, int* ids, float* weights,
+                     int* offsets, int* rows, int* slots, void* stream);
+
+/* Its backward: dlogits [T x E] from the choice, its weights and their gradient.
+ *   renorm: w_j (dw_j - sum w dw) at the chosen logits, 0 elsewhere;
+ *   else:   p_e (dw_e - sum w dw), p the softmax over all, dw_e = 0 if not chosen.
+ * The choice itself has no gradient. */
+int vedic_route_topk_bwd(const float* logits, int64_t ld_logits, const int* ids, const float* weights,
+                         const float* dweights, int T, int E, int k, int renorm, float* dlogits, int64_t ld_dlogits,
+                         void* stream);
+
+/* The plan alone: n entries of ids sorted by group, stable.  rows[place] = entry /
+ * per_row (1 for one group per row, k for [rows x k] ids), slots (may be NULL) the
+ * place of each entry; an id outside 0 .. groups - 1 belongs to no group (slot -1;
+ * row -1 in the places behind offsets[groups]). */
+int vedic_group_rows(const int* ids, int n, int per_row, int groups, int* offsets, int* rows, int* slots, void* stream);
+
+/* Products grouped by expert.  For the places i of group g:
+ *   NN  C[i] = epi(A[i] . B_g)      A [rows x K], B_g [K x N], C [rows x N]
+ *   NT  C[i] = epi(A[i] . B_g^T)    A [rows x K], B_g [N x K]
+ *   TN  C_g = beta C_g + sum over i of A[i]^T B[i]   A [rows x M], B [rows x N], C_g [M x N]
+ * with A[i] read at row row_index[i] of A's a_rows rows where a list is given (any
+ * row any number of times).  Rows of C behind offsets[groups] keep their content; a
+ * group without rows gives C_g = beta C_g.
+ * Types: F32 in and out; F16 in, fp32 accumulation, F32 or (NN, NT) F16 out,
+ * rounded to nearest even once.  preact has C's type.
+ * Epilogues: NN NONE, BIAS, BIAS_GELU (bias [groups x N]; preact, if set, receives
+ * the value before the GELU); NT NONE, GELU_BWD (times gelu_tanh'(preact)); TN
+ * NONE, and db_g = db_beta db_g + the column sums of group g's rows of B if db is set.
+ * The order of every sum is fixed.  Binary16 operands with 16-byte-aligned bases,
+ * leading dimensions and strides that are multiples of 8 and contiguous extents that
+ * are multiples of 8 run on the fast kernels, others on general ones.  TN with a row
+ * list, and a list into an A of 2 GiB or more, copy the listed rows into the stream's
+ * workspace block. */
+typedef struct {
+    int op, in_dtype, out_dtype, epilogue;
+    int groups;
+    int rows;    /* places: rows of C (NN, NT) or of B (TN) */
+    int M, N, K; /* M: TN only; K: NN and NT only */
+    const int* offsets;   /* [groups + 1] */
+    const int* row_index; /* NULL, or [rows] */
+    int a_rows;           /* rows of A, with row_index */
+    const void* A;
+    int64_t lda;
+    const void* B;
+    int64_t ldb;
+    int64_t stride_b; /* elements from B_g to B_(g+1) (NN, NT) */
+    void* C;
+    int64_t ldc;
+    int64_t stride_c; /* elements from C_g to C_(g+1) (TN) */
+    const float* bias;
+    void* preact;
+    int64_t ld_preact;
+    float beta; /* TN only */
+    float* db;  /* TN only: [groups x N] */
+    float db_beta;
+    void* stream;
+} vedic_grouped_desc_t;
+
+int vedic_gemm_grouped(const vedic_grouped_desc_t* desc);
+
+/* db_g = beta db_g + the column sums of group g's rows of dY (F32 or F16). */
+int vedic_bias_grad_grouped(const void* dY, int dtype, int64_t ld, int R, int N, const int* offsets, int groups, float beta,
+                            float* db, void* stream);
+
+/* Sorted rows back in token order:
+ *   out[t] = residual[t] + sum over j of weights[t, j] Y[slots[t, j]]
+ * (residual NULL: none, it may be out; weights NULL: ones, which is the backward of
+ * reading rows through a list).  Y F32 or F16 [R x D]; a slot outside adds nothing.
+ * Added in ascending j in fp32. */
+int vedic_combine_rows(const void* Y, int y_dtype, int64_t ldy, int R, const int* slots, const float* weights,
+                       const float* residual, int64_t ld_residual, float* out, int64_t ld_out, int T, int k, int D,
+                       void* stream);
+
+/* Its backward: dY[slots[t, j]] = weights[t, j] dout[t] (F32 or F16, rounded to
+ * nearest even), dweights[t, j] = <dout[t], Y[slots[t, j]]> (0 without a slot).  No
+ * two pairs may share a slot (those of a plan never do); rows of dY that no slot
+ * names keep their content. */
+int vedic_combine_rows_bwd(const float* dout, int64_t ld_dout, const void* Y, int y_dtype, int64_t ldy, int R,
+                           const int* slots, const float* weights, void* dY, int dy_dtype, int64_t ld_dy, float* dweights,
+                           int T, int k, int D, void* stream);
+
+/* Low-rank adapters of many requests beside a shared projection: for the places p
+ * of adapter g, i = rows[p]:  C[i] += scales[g] (X[i] . A_g) . B_g, A_g [K x r],
+ * B_g [r x N] contiguous, one after another; X, A, B all F32 or all F16, C fp32
+ * [M x N], scales NULL: ones.  The product with A_g stays in fp32.  A row may be listed
+ * once (two adapters on one row would add to it at the same time); rows not listed
+ * keep their content.  r <= 128.  Takes n r 4 bytes of the stream's workspace block. */
+int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, const void* A, const void* B, int groups, int r,
+                   const int* offsets, const int* rows, int n, const float* scales, float* C, int64_t ldc, int K, int N,
+                   void* stream);
+
 /* ---- test hooks --------------------------------------------------------- */
 
 /* Off by default.  When on, every GEMM with column sums allocates its

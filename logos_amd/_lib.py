@@ -62,6 +62,40 @@ class GemmDesc(ctypes.Structure):
     ]
 
 
+class GroupedDesc(ctypes.Structure):
+    """Mirror of vedic_grouped_desc_t."""
+
+    _fields_ = [
+        ("op", c_int),
+        ("in_dtype", c_int),
+        ("out_dtype", c_int),
+        ("epilogue", c_int),
+        ("groups", c_int),
+        ("rows", c_int),
+        ("M", c_int),
+        ("N", c_int),
+        ("K", c_int),
+        ("offsets", c_vp),
+        ("row_index", c_vp),
+        ("a_rows", c_int),
+        ("A", c_vp),
+        ("lda", c_i64),
+        ("B", c_vp),
+        ("ldb", c_i64),
+        ("stride_b", c_i64),
+        ("C", c_vp),
+        ("ldc", c_i64),
+        ("stride_c", c_i64),
+        ("bias", c_vp),
+        ("preact", c_vp),
+        ("ld_preact", c_i64),
+        ("beta", c_float),
+        ("db", c_vp),
+        ("db_beta", c_float),
+        ("stream", c_vp),
+    ]
+
+
 class VerifyResult(ctypes.Structure):
     """Mirror of vedic_verify_result_t."""
 
@@ -123,6 +157,21 @@ SIGNATURES = {
         c_int, [c_vp] * 9 + [c_int, c_int, c_float, c_int, c_int, c_int, c_int, c_vp]),
     "vedic_flash_attention_bwd_heads": (
         c_int, [ctypes.POINTER(c_vp)] * 9 + [c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int, c_vp]),
+    "vedic_route_topk": (c_int, [c_vp, c_i64, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "vedic_route_topk_bwd": (c_int, [c_vp, c_i64, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, c_i64, c_vp]),
+    "vedic_group_rows": (c_int, [c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp]),
+    "vedic_gemm_grouped": (c_int, [ctypes.POINTER(GroupedDesc)]),
+    "vedic_bias_grad_grouped": (c_int, [c_vp, c_int, c_i64, c_int, c_int, c_vp, c_int, c_float, c_vp, c_vp]),
+    "vedic_combine_rows": (
+        c_int, [c_vp, c_int, c_i64, c_int, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_int, c_int, c_int, c_vp]),
+    "vedic_combine_rows_bwd": (
+        c_int,
+        [c_vp, c_i64, c_vp, c_int, c_i64, c_int, c_vp, c_vp, c_vp, c_int, c_i64, c_vp, c_int, c_int, c_int, c_vp],
+    ),
+    "vedic_lora_add": (
+        c_int,
+        [c_vp, c_int, c_i64, c_int, c_vp, c_vp, c_int, c_int, c_vp, c_vp, c_int, c_vp, c_vp, c_i64, c_int, c_int, c_vp],
+    ),
     "vedic_debug_set_workspace_guard": (None, [c_int]),
     "vedic_debug_workspace_guard_hits": (ctypes.c_long, []),
     "vedic_uses_vendor_blas": (c_int, []),

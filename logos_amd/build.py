@@ -36,6 +36,15 @@ SOURCES = [
     "vedic_flash_attn_bwd.hip",
     "vedic_flash_probs.hip",
     "vedic_layernorm.hip",
+    "vedic_grouped_f16_nn.hip",
+    "vedic_grouped_f16_nt.hip",
+    "vedic_grouped_f16_tn.hip",
+    "vedic_grouped_any_nn.hip",
+    "vedic_grouped_any_nt.hip",
+    "vedic_grouped_any_tn.hip",
+    "vedic_route.hip",
+    "vedic_combine.hip",
+    "vedic_lora.hip",
     "vedic_capi.hip",
 ]
 

@@ -19,8 +19,18 @@
 #include "vedic_flash_attn.hpp"
 #include "vedic_common.hpp"
 #include "vedic_epilogue.hpp"
+#include "vedic_combine.hpp"
+#include "vedic_grouped.hpp"
+#include "vedic_lora.hpp"
+#include "vedic_route.hpp"
 
 namespace vedic {
+hipError_t launch_grouped_f16_nn(const GroupedArgs& a, int kind, bool f16out, hipStream_t s);
+hipError_t launch_grouped_f16_nt(const GroupedArgs& a, int kind, bool f16out, hipStream_t s);
+hipError_t launch_grouped_f16_tn(const GroupedArgs& a, int kind, bool f16out, hipStream_t s);
+hipError_t launch_grouped_any_nn(const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s);
+hipError_t launch_grouped_any_nt(const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s);
+hipError_t launch_grouped_any_tn(const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s);
 hipError_t launch_layernorm_f32(const float* X, const float* gamma, const float* beta, float* Y, void* Y16, int seq,
                                 int d, float eps, hipStream_t s);
 hipError_t launch_layernorm_f16(const void* X16, const float* gamma, const float* beta, void* Y16, int seq, int d,
@@ -1153,6 +1163,272 @@ extern "C" int vedic_bias_grad(const float* dY, float* db, int M, int N, float b
     Workspace pool;
     pool.s = static_cast<hipStream_t>(stream);
     return hip_status(colsum_matrix(dY, N, M, N, db, beta, pool));
+}
+
+// ------------------------------------------------- rows that choose their weights
+
+// Offsets, slots and row indexes count in int: products of the sizes stay below this.
+static constexpr int64_t kMaxCount = int64_t(1) << 30;
+
+extern "C" int vedic_route_topk(const float* logits, int64_t ld_logits, int T, int E, int k, int renorm, int* ids,
+                                float* weights, int* offsets, int* rows, int* slots, void* stream) {
+    if (T < 0 || E <= 0 || k <= 0 || k > E) return VEDIC_STATUS_BAD_DIM;
+    if (E > kMaxGroups || k > kMaxTopK || (int64_t)T * k >= kMaxCount) return VEDIC_STATUS_TOO_LARGE;
+    if (!offsets || (T > 0 && (!logits || !ids || !weights || !rows || !slots))) return VEDIC_STATUS_NULL_POINTER;
+    if (ld_logits < E) return VEDIC_STATUS_BAD_LD;
+    Workspace ws;
+    ws.s = static_cast<hipStream_t>(stream);
+    RouteArgs a{};
+    const size_t bytes = route_count_bytes(T, E, k);
+    if (bytes > 0) {
+        const hipError_t e = ws.get(&a.counts, bytes);
+        if (e != hipSuccess) return hip_status(e);
+    }
+    a.logits = logits;
+    a.ld = ld_logits;
+    a.T = T;
+    a.E = E;
+    a.k = k;
+    a.renorm = renorm != 0;
+    a.ids = ids;
+    a.weights = weights;
+    a.offsets = offsets;
+    a.rows = rows;
+    a.slots = slots;
+    hipError_t e = launch_route_topk(a, ws.s);
+    const hipError_t f = ws.put(a.counts);
+    return hip_status(e != hipSuccess ? e : f);
+}
+
+extern "C" int vedic_route_topk_bwd(const float* logits, int64_t ld_logits, const int* ids, const float* weights,
+                                    const float* dweights, int T, int E, int k, int renorm, float* dlogits,
+                                    int64_t ld_dlogits, void* stream) {
+    if (T < 0 || E <= 0 || k <= 0 || k > E) return VEDIC_STATUS_BAD_DIM;
+    if (E > kMaxGroups || k > kMaxTopK || (int64_t)T * k >= kMaxCount) return VEDIC_STATUS_TOO_LARGE;
+    if (T == 0) return VEDIC_STATUS_OK;
+    if (!logits || !ids || !weights || !dweights || !dlogits) return VEDIC_STATUS_NULL_POINTER;
+    if (ld_logits < E || ld_dlogits < E) return VEDIC_STATUS_BAD_LD;
+    return hip_status(launch_route_topk_bwd(logits, ld_logits, ids, weights, dweights, T, E, k, renorm != 0, dlogits,
+                                            ld_dlogits, static_cast<hipStream_t>(stream)));
+}
+
+extern "C" int vedic_group_rows(const int* ids, int n, int per_row, int groups, int* offsets, int* rows, int* slots,
+                                void* stream) {
+    if (n < 0 || groups <= 0 || per_row <= 0) return VEDIC_STATUS_BAD_DIM;
+    if (groups > kMaxGroups || n >= kMaxCount) return VEDIC_STATUS_TOO_LARGE;
+    if (!offsets || (n > 0 && (!ids || !rows))) return VEDIC_STATUS_NULL_POINTER;
+    Workspace ws;
+    ws.s = static_cast<hipStream_t>(stream);
+    int* counts = nullptr;
+    const size_t bytes = group_count_bytes(n, groups);
+    if (bytes > 0) {
+        const hipError_t e = ws.get(&counts, bytes);
+        if (e != hipSuccess) return hip_status(e);
+    }
+    const hipError_t e = launch_group_rows(ids, n, per_row, groups, counts, offsets, rows, slots, ws.s);
+    const hipError_t f = ws.put(counts);
+    return hip_status(e != hipSuccess ? e : f);
+}
+
+static hipError_t launch_grouped(int op, const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s) {
+    if (f16 && vec)
+        return op == VEDIC_OP_NN   ? launch_grouped_f16_nn(a, kind, f16out, s)
+               : op == VEDIC_OP_NT ? launch_grouped_f16_nt(a, kind, f16out, s)
+                                   : launch_grouped_f16_tn(a, kind, f16out, s);
+    return op == VEDIC_OP_NN   ? launch_grouped_any_nn(a, kind, f16, f16out, vec, s)
+           : op == VEDIC_OP_NT ? launch_grouped_any_nt(a, kind, f16, f16out, vec, s)
+                               : launch_grouped_any_tn(a, kind, f16, f16out, vec, s);
+}
+
+extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
+    if (!d) return VEDIC_STATUS_NULL_POINTER;
+    const bool tn = d->op == VEDIC_OP_TN;
+    if (d->op != VEDIC_OP_NN && d->op != VEDIC_OP_NT && !tn) return VEDIC_STATUS_BAD_LAYOUT;
+    if (d->in_dtype != VEDIC_DT_F32 && d->in_dtype != VEDIC_DT_F16) return VEDIC_STATUS_BAD_DTYPE;
+    const bool f16 = d->in_dtype == VEDIC_DT_F16, f16out = d->out_dtype == VEDIC_DT_F16;
+    if (d->out_dtype != VEDIC_DT_F32 && !(f16out && f16 && !tn)) return VEDIC_STATUS_BAD_DTYPE;
+    const int R = d->rows, N = d->N;
+    if (d->groups <= 0 || R < 0 || N <= 0 || (tn ? d->M : d->K) <= 0) return VEDIC_STATUS_BAD_DIM;
+    if (d->row_index && d->a_rows <= 0 && R > 0) return VEDIC_STATUS_BAD_DIM;
+    int kind;
+    switch (d->epilogue) {
+        case VEDIC_EPI_NONE: kind = GK_LINEAR; break;
+        case VEDIC_EPI_BIAS: kind = GK_LINEAR; break;
+        case VEDIC_EPI_BIAS_GELU: kind = GK_GELU; break;
+        case VEDIC_EPI_GELU_BWD: kind = GK_GELU_BWD; break;
+        default: return VEDIC_STATUS_BAD_EPILOGUE;
+    }
+    const bool wants_bias = d->epilogue == VEDIC_EPI_BIAS || d->epilogue == VEDIC_EPI_BIAS_GELU;
+    const bool reads_p = d->epilogue == VEDIC_EPI_GELU_BWD;
+    if ((wants_bias && (d->op != VEDIC_OP_NN || !d->bias)) || (reads_p && (d->op != VEDIC_OP_NT || !d->preact)))
+        return VEDIC_STATUS_BAD_EPILOGUE;
+    if (d->preact && kind != GK_GELU && kind != GK_GELU_BWD) return VEDIC_STATUS_BAD_EPILOGUE;
+    if ((!tn && (d->beta != 0.0f || d->db)) || d->beta != d->beta) return VEDIC_STATUS_BAD_EPILOGUE;
+    if (!d->offsets || (!d->C && (tn || R > 0)) || (R > 0 && (!d->A || !d->B))) return VEDIC_STATUS_NULL_POINTER;
+    const int a_cols = tn ? d->M : d->K, b_cols = d->op == VEDIC_OP_NT ? d->K : N;
+    if (d->lda < a_cols || d->ldb < b_cols || d->ldc < N || (d->preact && d->ld_preact < N)) return VEDIC_STATUS_BAD_LD;
+    // (groups of dW that overlap would be written by two workgroups at once)
+    if (d->stride_b < 0 || (tn && d->groups > 1 && d->stride_c < (int64_t)(d->M - 1) * d->ldc + N)) return VEDIC_STATUS_BAD_LD;
+    if (d->groups > kMaxGroups || R >= kMaxCount || d->a_rows >= kMaxCount || d->lda >= kMaxLd || d->ldb >= kMaxLd ||
+        d->ldc >= kMaxLd || d->ld_preact >= kMaxLd)
+        return VEDIC_STATUS_TOO_LARGE;
+    const int64_t row_tiles = tn ? (int64_t)d->groups * ((d->M + 63) / 64) : R / 64 + (int64_t)d->groups;
+    if (row_tiles * ((N + 63) / 64) >= kMaxCount) return VEDIC_STATUS_TOO_LARGE;
+    Workspace ws;
+    ws.s = static_cast<hipStream_t>(d->stream);
+    if (R == 0 && !tn) return VEDIC_STATUS_OK;
+
+    GroupedArgs a{};
+    a.A = d->A;
+    a.B = d->B;
+    a.C = d->C;
+    a.bias = wants_bias ? d->bias : nullptr;
+    a.P = d->preact;
+    a.offsets = d->offsets;
+    a.rows = R > 0 ? d->row_index : nullptr;
+    a.lda = d->lda;
+    a.ldb = d->ldb;
+    a.ldc = d->ldc;
+    a.ldp = d->ld_preact;
+    a.stride_b = d->stride_b;
+    a.stride_c = d->stride_c;
+    a.groups = d->groups;
+    a.R = R;
+    a.a_rows = d->a_rows;
+    a.M = d->M;
+    a.N = N;
+    a.K = d->K;
+    a.beta = d->beta;
+    if (tn && d->beta != 0.0f) kind = GK_BETA;
+    const int es = f16 ? 2 : 4, per16 = 16 / es;
+    // The rows of a list are copied into a workspace first where the kernels
+    // cannot follow it: along the contraction (TN), and past 32-bit offsets.
+    void* copy = nullptr;
+    if (a.rows && (tn || (int64_t)d->a_rows * d->lda * es >= (int64_t(1) << 31))) {
+        const int64_t ldn = ((int64_t)a_cols + 7) / 8 * 8;
+        hipError_t e = ws.get(&copy, (size_t)R * ldn * es);
+        if (e == hipSuccess)
+            e = launch_gather_rows(d->A, d->lda, d->a_rows, a.rows, R, a_cols, es, copy, ldn, ws.s);
+        if (e != hipSuccess) return hip_status(e);
+        a.A = copy;
+        a.lda = ldn;
+        a.rows = nullptr;
+    }
+    bool vec = aligned16(a.A) && a.lda % per16 == 0;
+    if (f16 || d->op == VEDIC_OP_NT) vec = vec && aligned16(a.B) && a.ldb % per16 == 0 && a.stride_b % per16 == 0;
+    vec = vec && a_cols % per16 == 0 && ((!f16 && d->op == VEDIC_OP_NN) || b_cols % per16 == 0);
+    hipError_t e = launch_grouped(d->op, a, kind, f16, f16out, vec, ws.s);
+    if (e == hipSuccess && d->db)
+        e = launch_group_colsum(d->B, f16, d->ldb, R, N, d->offsets, d->groups, d->db_beta, d->db, ws.s);
+    const hipError_t f = ws.put(copy);
+    return hip_status(e != hipSuccess ? e : f);
+}
+
+extern "C" int vedic_bias_grad_grouped(const void* dY, int dtype, int64_t ld, int R, int N, const int* offsets, int groups,
+                                       float beta, float* db, void* stream) {
+    if (dtype != VEDIC_DT_F32 && dtype != VEDIC_DT_F16) return VEDIC_STATUS_BAD_DTYPE;
+    if (R < 0 || N <= 0 || groups <= 0) return VEDIC_STATUS_BAD_DIM;
+    if (!offsets || !db || (R > 0 && !dY)) return VEDIC_STATUS_NULL_POINTER;
+    if (ld < N) return VEDIC_STATUS_BAD_LD;
+    if (groups > kMaxGroups) return VEDIC_STATUS_TOO_LARGE;
+    return hip_status(launch_group_colsum(dY, dtype == VEDIC_DT_F16, ld, R, N, offsets, groups, beta, db,
+                                          static_cast<hipStream_t>(stream)));
+}
+
+static int combine_checks(int y_dtype, int64_t ldy, int R, int T, int k, int D) {
+    if (y_dtype != VEDIC_DT_F32 && y_dtype != VEDIC_DT_F16) return VEDIC_STATUS_BAD_DTYPE;
+    if (T < 0 || k <= 0 || D <= 0 || R < 0) return VEDIC_STATUS_BAD_DIM;
+    if (ldy < D) return VEDIC_STATUS_BAD_LD;
+    if ((int64_t)T * k >= kMaxCount || R >= kMaxCount || (int64_t)T * ((D + 255) / 256) >= kMaxCount)
+        return VEDIC_STATUS_TOO_LARGE;
+    return VEDIC_STATUS_OK;
+}
+
+extern "C" int vedic_combine_rows(const void* Y, int y_dtype, int64_t ldy, int R, const int* slots, const float* weights,
+                                  const float* residual, int64_t ld_residual, float* out, int64_t ld_out, int T, int k,
+                                  int D, void* stream) {
+    const int st = combine_checks(y_dtype, ldy, R, T, k, D);
+    if (st != VEDIC_STATUS_OK) return st;
+    if (T == 0) return VEDIC_STATUS_OK;
+    if ((R > 0 && !Y) || !slots || !out) return VEDIC_STATUS_NULL_POINTER;
+    if (ld_out < D || (residual && ld_residual < D)) return VEDIC_STATUS_BAD_LD;
+    CombineArgs a{};
+    a.Y = Y;
+    a.ldy = ldy;
+    a.R = R;
+    a.slots = slots;
+    a.weights = weights;
+    a.residual = residual;
+    a.ldr = ld_residual;
+    a.out = out;
+    a.ldo = ld_out;
+    a.T = T;
+    a.k = k;
+    a.D = D;
+    return hip_status(launch_combine(a, y_dtype == VEDIC_DT_F16, static_cast<hipStream_t>(stream)));
+}
+
+extern "C" int vedic_combine_rows_bwd(const float* dout, int64_t ld_dout, const void* Y, int y_dtype, int64_t ldy, int R,
+                                      const int* slots, const float* weights, void* dY, int dy_dtype, int64_t ld_dy,
+                                      float* dweights, int T, int k, int D, void* stream) {
+    const int st = combine_checks(y_dtype, ldy, R, T, k, D);
+    if (st != VEDIC_STATUS_OK) return st;
+    if (dy_dtype != VEDIC_DT_F32 && dy_dtype != VEDIC_DT_F16) return VEDIC_STATUS_BAD_DTYPE;
+    if (T == 0) return VEDIC_STATUS_OK;
+    if (!dout || (R > 0 && (!Y || !dY)) || !slots || !weights || !dweights) return VEDIC_STATUS_NULL_POINTER;
+    if (ld_dout < D || ld_dy < D) return VEDIC_STATUS_BAD_LD;
+    CombineBwdArgs a{};
+    a.dout = dout;
+    a.ldg = ld_dout;
+    a.Y = Y;
+    a.ldy = ldy;
+    a.R = R;
+    a.slots = slots;
+    a.weights = weights;
+    a.dY = dY;
+    a.ldo = ld_dy;
+    a.dweights = dweights;
+    a.T = T;
+    a.k = k;
+    a.D = D;
+    return hip_status(launch_combine_bwd(a, y_dtype == VEDIC_DT_F16, dy_dtype == VEDIC_DT_F16,
+                                         static_cast<hipStream_t>(stream)));
+}
+
+extern "C" int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, const void* A, const void* B, int groups, int r,
+                              const int* offsets, const int* rows, int n, const float* scales, float* C, int64_t ldc, int K,
+                              int N, void* stream) {
+    if (dtype != VEDIC_DT_F32 && dtype != VEDIC_DT_F16) return VEDIC_STATUS_BAD_DTYPE;
+    if (M < 0 || n < 0 || groups <= 0 || r <= 0 || K <= 0 || N <= 0) return VEDIC_STATUS_BAD_DIM;
+    if (r > kLoraMaxRank || groups > kMaxGroups || M >= kMaxCount || n >= kMaxCount / 128 || ldx >= kMaxLd || ldc >= kMaxLd ||
+        ((int64_t)n / 8 + groups) * ((N + 255) / 256) >= kMaxCount)
+        return VEDIC_STATUS_TOO_LARGE;
+    if (ldx < K || ldc < N) return VEDIC_STATUS_BAD_LD;
+    if (n == 0 || M == 0) return VEDIC_STATUS_OK;
+    if (!X || !A || !B || !offsets || !rows || !C) return VEDIC_STATUS_NULL_POINTER;
+    Workspace ws;
+    ws.s = static_cast<hipStream_t>(stream);
+    LoraArgs a{};
+    hipError_t e = ws.get(&a.H, sizeof(float) * (size_t)n * r);
+    if (e != hipSuccess) return hip_status(e);
+    a.X = X;
+    a.ldx = ldx;
+    a.A = A;
+    a.B = B;
+    a.offsets = offsets;
+    a.rows = rows;
+    a.n = n;
+    a.groups = groups;
+    a.scales = scales;
+    a.C = C;
+    a.ldc = ldc;
+    a.M = M;
+    a.K = K;
+    a.N = N;
+    a.r = r;
+    e = launch_lora(a, dtype == VEDIC_DT_F16, ws.s);
+    const hipError_t f = ws.put(a.H);
+    return hip_status(e != hipSuccess ? e : f);
 }
 
 // ----------------------------------------------------------- elementwise

@@ -1,0 +1,45 @@
+// vedic_combine.hpp -- launch interface of vedic_combine.hip.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace vedic {
+
+struct CombineArgs {
+    const void* Y;  // [R x ldy]
+    int64_t ldy;
+    int R;
+    const int* slots;      // [T x k]; outside 0 .. R - 1: no row
+    const float* weights;  // [T x k], or null: ones
+    const float* residual; // or null
+    int64_t ldr;
+    float* out;
+    int64_t ldo;
+    int T, k, D;
+};
+
+struct CombineBwdArgs {
+    const float* dout;
+    int64_t ldg;
+    const void* Y;
+    int64_t ldy;
+    int R;
+    const int* slots;
+    const float* weights;
+    void* dY;
+    int64_t ldo;
+    float* dweights;
+    int T, k, D;
+};
+
+hipError_t launch_combine(const CombineArgs& a, bool f16, hipStream_t s);
+hipError_t launch_combine_bwd(const CombineBwdArgs& a, bool f16, bool out16, hipStream_t s);
+// dst[i] = src[rows[i]], `cols` values of es bytes (2 or 4); n > 0.
+hipError_t launch_gather_rows(const void* src, int64_t ld, int nsrc, const int* rows, int n, int cols, int es, void* dst,
+                              int64_t ldd, hipStream_t s);
+// db[e] = beta db[e] + column sums of the group's rows of X.
+hipError_t launch_group_colsum(const void* X, bool f16, int64_t ld, int R, int N, const int* offsets, int groups, float beta,
+                               float* db, hipStream_t s);
+
+}  // namespace vedic

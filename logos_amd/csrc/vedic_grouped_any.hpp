@@ -1,0 +1,344 @@
+// vedic_grouped_any.hpp -- the grouped products for binary32 operands and for
+// binary16 ones that the 16-byte kernels cannot load, any alignment.
+//
+// Every value is split into bf16 parts as it goes to LDS (vedic_split.hpp), six
+// v_mfma_f32_32x32x16_bf16 per 32 x 32 x 16 block, the arithmetic of the
+// ungrouped fp32 product (vedic_gemm_f32s.hpp), whose LDS layout this shares.
+// (A binary16 value has two parts; the third is zero.)  One 128 x 128 tile, or
+// 64 x 64 where those would leave CUs idle, per workgroup; per stage of 16
+// contraction steps the values of stage k + 2 are in registers on their way,
+// those of stage k + 1 are split into one LDS buffer while stage k's fragments
+// are read from the other.
+#pragma once
+
+#include "vedic_gemm_f32s.hpp"
+#include "vedic_grouped.hpp"
+
+namespace vedic {
+
+template <typename T>
+__device__ __forceinline__ float ld_value(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t soff) {
+    return ld_out<T>(rs, off, soff);
+}
+
+// One operand's staging (SideSplit with a value type and a row list): R rows of
+// the tile, NT threads.
+template <typename T, bool KC, bool VEC, int R, int NT>
+struct SideAny {
+    static constexpr bool PAIRS = KC && !VEC;
+    static constexpr int UNITS = PAIRS ? R * 8 : R * 2;
+    static constexpr int U = UNITS / NT;
+    static constexpr int PER = PAIRS ? 2 : 8;
+    static constexpr int ES = sizeof(T);
+    static_assert(UNITS % NT == 0, "units divide among the threads");
+    uint32_t off[U];
+    int k0[U];
+    typedef float Values[U][PER];
+
+    __device__ __forceinline__ static int row_of(int tid, int i) {
+        const int u = i * NT + tid;
+        return PAIRS ? u >> 3 : KC ? u >> 1 : u % R;
+    }
+    // list (KC): the tile's rows of the operand, `limit` of them there (a row
+    // outside is read as zeros); null: consecutive rows.
+    __device__ __forceinline__ void init(int tid, int64_t ld, int left, const int* list, int limit) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = i * NT + tid, row = row_of(tid, i);
+            k0[i] = PAIRS ? 2 * (u & 7) : KC ? 8 * (u & 1) : 8 * __builtin_amdgcn_readfirstlane(u / R);
+            bool ok = row < left;
+            if constexpr (KC) {
+                int64_t r = row;
+                if (list != nullptr) {
+                    const int x = ok ? list[row] : 0;
+                    ok = ok && (unsigned)x < (unsigned)limit;
+                    r = x;
+                }
+                off[i] = ok ? (uint32_t)(r * ld * ES + k0[i] * ES) : kOob;
+            } else {
+                off[i] = ok ? (uint32_t)(row * ES) : kOob;
+            }
+        }
+    }
+    // `steps` of the stage's 16 steps exist (maybe none); the others load as zeros.
+    __device__ __forceinline__ void load(Values& v, const T* base, int64_t ld, int steps) const {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            // (a stage past the range touches no memory: no records)
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<T*>(KC || steps <= k0[i] ? base : base + (int64_t)k0[i] * ld), 0,
+                steps > (KC ? 0 : k0[i]) ? 0x7FFFFFFF : 0, 0x00020000);
+            if constexpr (KC && VEC) {
+                constexpr int Q = 16 / ES;  // values per 16-byte load
+#pragma unroll
+                for (int q = 0; q < 8; q += Q) {
+                    const uint32_t o = k0[i] + q < steps ? off[i] : kOob;
+                    const u32x4_t w = __builtin_bit_cast(
+                        u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(o == kOob ? kOob : o + q * ES), 0, 0));
+                    if constexpr (ES == 4) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[i][q + e] = __builtin_bit_cast(float4_t, w)[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[i][q + e] = (float)__builtin_bit_cast(half8_t, w)[e];
+                    }
+                }
+            } else if constexpr (KC) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t o = k0[i] + e < steps ? off[i] : kOob;
+                    v[i][e] = ld_value<T>(rs, o == kOob ? kOob : o + ES * e, 0);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[i][e] = ld_value<T>(rs, k0[i] + e < steps ? off[i] : kOob, (uint32_t)e * (uint32_t)ld * ES);
+            }
+        }
+    }
+    __device__ __forceinline__ void commit(const Values& v, char* lds, int tid) const {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int row = row_of(tid, i);
+            char* dst = lds + row * kSplitRowBytes + split_half(row, k0[i] >> 3);
+            if constexpr (PAIRS) {
+                const SplitPair s = split_pair(v[i][0] * kSplitScale, v[i][1] * kSplitScale);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<uint32_t*>(dst + 32 * p + (k0[i] & 7) * 2) = s.p[p];
+            } else {
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = v[i][e] * kSplitScale;
+                const SplitFrag f = split8(w);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8_t*>(dst + 32 * p) = f.p[p];
+            }
+        }
+    }
+};
+
+// A wave's block on v_mfma_f32_32x32x2_f32 from the operands themselves: for
+// blocks whose split sums are not finite and for one or two steps.  pa, pb: this
+// lane's row and column (lane half h takes step 2 q + h), ka, kb the distance of
+// two steps' elements; a row that is not there has ok = false and counts as zeros.
+template <typename T, int MI, int NI>
+__device__ __forceinline__ void any_block_slow(const T* const (&pa)[MI], const bool (&oka)[MI], int64_t ka,
+                                               const T* const (&pb)[NI], int64_t kb, int K, int h,
+                                               float16_t (&acc)[MI][NI]) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = float16_t{};
+#pragma unroll 1
+    for (int k = h; k < K + h; k += 2) {
+        const bool in = k < K;
+        const int64_t q = in ? k : K - 1;
+        float x[MI], y[NI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) x[i] = in && oka[i] ? (float)pa[i][q * ka] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) y[j] = in ? (float)pb[j][q * kb] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[j], acc[i][j], 0, 0, 0);
+    }
+}
+
+// One BM x BN tile per workgroup.  NN / NT: work item w is column tile w mod
+// tiles_n of row tile w / tiles_n (row tiles counted through the groups).  TN: w
+// is tile w mod (tiles_m tiles_n) of group w / (tiles_m tiles_n).
+template <int OP, typename T, typename OT, bool VEC, int BM, int BN, int WGM, int WGN, int KIND>
+__global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs a) {
+    constexpr int NT = WGM * WGN * 64, WM = BM / WGM, WN = BN / WGN, MI = WM / 32, NI = WN / 32;
+    constexpr bool A_KC = OP != 2, B_KC = OP == 1;
+    constexpr int BYTES = (BM + BN) * kSplitRowBytes;
+    __shared__ __attribute__((aligned(1024))) char buf0[BYTES];
+    __shared__ __attribute__((aligned(1024))) char buf1[BYTES];
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int wm = wave / WGN, wn = wave % WGN;
+
+    int e, m0, n0, K, left, start, count;  // left: rows of C from m0 on
+    if constexpr (OP == 2) {
+        const int tiles = a.tiles_m * a.tiles_n;
+        e = blockIdx.x / tiles;
+        const int t = blockIdx.x - e * tiles;
+        m0 = t % a.tiles_m * BM;
+        n0 = t / a.tiles_m * BN;
+        start = min(max(a.offsets[e], 0), a.R);
+        count = max(0, min(max(a.offsets[e + 1], 0), a.R) - start);
+        K = count;
+        left = a.M - m0;
+    } else {
+        GroupIndex& ix = *reinterpret_cast<GroupIndex*>(buf0);
+        static_assert(sizeof(GroupIndex) <= BYTES, "the index fits a stage buffer");
+        group_index<NT>(a, ix, BM);
+        const int t = blockIdx.x / a.tiles_n;
+        if (t >= ix.pre[a.groups]) return;
+        e = group_of(ix, a.groups, t, lane);
+        start = __builtin_amdgcn_readfirstlane(ix.off[e]);
+        count = __builtin_amdgcn_readfirstlane(ix.off[e + 1]) - start;
+        m0 = (t - __builtin_amdgcn_readfirstlane(ix.pre[e])) * BM;
+        n0 = (blockIdx.x - t * a.tiles_n) * BN;
+        K = a.K;
+        left = count - m0;
+        __syncthreads();  // the index's LDS becomes a stage buffer
+    }
+    const T* A = static_cast<const T*>(a.A);
+    const int* list = nullptr;
+    if constexpr (OP == 2) {
+        A += (int64_t)start * a.lda + m0;
+    } else if (a.rows != nullptr) {
+        list = a.rows + start + m0;
+    } else {
+        A += (int64_t)(start + m0) * a.lda;
+    }
+    const T* B = static_cast<const T*>(a.B);
+    if constexpr (OP == 2) B += (int64_t)start * a.ldb + n0;
+    else B += (int64_t)e * a.stride_b + (B_KC ? (int64_t)n0 * a.ldb : n0);
+    const int64_t ka = A_KC ? 1 : a.lda, kb = B_KC ? 1 : a.ldb;
+
+    using SA = SideAny<T, A_KC, VEC, BM, NT>;
+    using SB = SideAny<T, B_KC, VEC, BN, NT>;
+    SA sa;
+    SB sb;
+    sa.init(tid, a.lda, left, list, a.a_rows);
+    sb.init(tid, a.ldb, a.N - n0, nullptr, 0);
+    typename SA::Values va;
+    typename SB::Values vb;
+    const bool few = K < kSplitMinK;
+    const int nk = few ? 0 : (K + kSplitK - 1) / kSplitK;
+    auto load = [&](int kt) {
+        const int64_t k = kt < nk ? (int64_t)kt * kSplitK : 0;
+        const int steps = kt < nk ? min(kSplitK, K - kt * kSplitK) : 0;
+        sa.load(va, A + k * ka, a.lda, steps);
+        sb.load(vb, B + k * kb, a.ldb, steps);
+    };
+    auto commit = [&](char* buf) {
+        sa.commit(va, buf, tid);
+        sb.commit(vb, buf + BM * kSplitRowBytes, tid);
+    };
+    float16_t acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = float16_t{};
+    auto stage = [&](const char* cur, char* nxt, int kt) {
+        SplitFrag fa[MI], fb[NI];
+#pragma unroll
+        for (int j = 0; j < NI; ++j) fb[j] = read_split(cur + BM * kSplitRowBytes, wn * WN + 32 * j, lane);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[i] = read_split(cur, wm * WM + 32 * i, lane);
+        commit(nxt);
+        load(kt + 2);
+#pragma unroll
+        for (int q = 0; q < kSplitProducts; ++q)
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i].p[kSplitA[q]], fb[j].p[kSplitB[q]],
+                                                                        acc[i][j], 0, 0, 0);
+        __syncthreads();
+    };
+    if (nk > 0) {
+        load(0);
+        commit(buf0);
+        load(1);
+        __syncthreads();
+        for (int kt = 0; kt < nk; kt += 2) {  // (a stage past the last is zeros)
+            stage(buf0, buf1, kt);
+            stage(buf1, buf0, kt + 1);
+        }
+    }
+    float probe = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            acc[i][j] *= kSplitUnscale2;
+            probe = nonfinite_probe(acc[i][j], probe);
+        }
+    if (few || __any(probe != 0.0f)) {
+        const T* pa[MI];
+        const T* pb[NI];
+        bool oka[MI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            int r = min(wm * WM + 32 * i + (lane & 31), left - 1);
+            oka[i] = true;
+            if (left <= 0) r = 0, oka[i] = false;
+            if (list != nullptr && oka[i]) {
+                r = list[r];
+                oka[i] = (unsigned)r < (unsigned)a.a_rows;
+                if (!oka[i]) r = 0;
+            }
+            pa[i] = A_KC ? A + (int64_t)r * a.lda : A + r;
+        }
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            const int n = min(wn * WN + 32 * j + (lane & 31), a.N - n0 - 1);
+            pb[j] = B_KC ? B + (int64_t)n * a.ldb : B + n;
+        }
+        any_block_slow<T, MI, NI>(pa, oka, ka, pb, kb, K, lane >> 5, acc);
+    }
+    const int row0 = m0 + wm * WM;
+    const int64_t crow = OP == 2 ? row0 : start + row0;
+    OT* C = static_cast<OT*>(a.C) + (OP == 2 ? (int64_t)e * a.stride_c : 0) + crow * a.ldc;
+    OT* P = a.P != nullptr ? static_cast<OT*>(a.P) + crow * a.ldp : nullptr;
+    grouped_epilogue<KIND, OT, true, MI, NI>(C, a.ldc, P, a.ldp, a.bias ? a.bias + (int64_t)e * a.N : nullptr, a.beta, acc,
+                                             left - wm * WM, a.N, n0 + wn * WN, lane);
+}
+
+struct CfgAMid {  // 128 x 128, four waves of 64 x 64
+    static constexpr int BM = 128, BN = 128, WGM = 2, WGN = 2;
+};
+struct CfgASmall {  // 64 x 64, two waves of 32 x 64
+    static constexpr int BM = 64, BN = 64, WGM = 2, WGN = 1;
+};
+
+// Row tiles that R rows in `groups` groups can have at most, and about have.
+inline int64_t grouped_row_tiles_max(int R, int groups, int bm) {
+    return R / bm + (groups < R ? groups : R);
+}
+inline double grouped_row_tiles(int R, int groups, int bm) {
+    return (double)R / bm + 0.5 * (groups < R ? groups : R);
+}
+
+template <int OP, typename T, typename OT, bool VEC, class Cfg, int KIND>
+static hipError_t launch_any(GroupedArgs a, hipStream_t s) {
+    a.tiles_n = (a.N + Cfg::BN - 1) / Cfg::BN;
+    a.tiles_m = OP == 2 ? (a.M + Cfg::BM - 1) / Cfg::BM : 0;
+    const int64_t work = OP == 2 ? (int64_t)a.groups * a.tiles_m * a.tiles_n
+                                 : grouped_row_tiles_max(a.R, a.groups, Cfg::BM) * a.tiles_n;
+    if (work > 0x7FFFFFFF) return hipErrorInvalidValue;  // (the caller has refused such sizes)
+    if (work == 0) return hipSuccess;
+    hipLaunchKernelGGL((grouped_any_kernel<OP, T, OT, VEC, Cfg::BM, Cfg::BN, Cfg::WGM, Cfg::WGN, KIND>), dim3((unsigned)work),
+                       dim3(Cfg::WGM * Cfg::WGN * 64), 0, s, a);
+    return hipGetLastError();
+}
+
+// 64 x 64 tiles where 128 x 128 ones would leave half the CUs without one.
+template <int OP, typename T, typename OT, bool VEC, int KIND>
+static hipError_t launch_any_tiles(const GroupedArgs& a, hipStream_t s) {
+    const double rows = OP == 2 ? (double)a.groups * ((a.M + 127) / 128) : grouped_row_tiles(a.R, a.groups, 128);
+    if (rows * ((a.N + 127) / 128) * 2 > device_cu_count()) return launch_any<OP, T, OT, VEC, CfgAMid, KIND>(a, s);
+    return launch_any<OP, T, OT, VEC, CfgASmall, KIND>(a, s);
+}
+
+// vec: rows that 16-byte loads can take (fp32 only; binary16 operands that have
+// them run on the kernels of vedic_grouped_f16.hpp).
+template <int OP, int KIND>
+static hipError_t launch_any_kind(const GroupedArgs& a, bool f16, bool f16out, bool vec, hipStream_t s) {
+    if (f16) {
+        if constexpr (OP != 2)
+            if (f16out) return launch_any_tiles<OP, _Float16, _Float16, false, KIND>(a, s);
+        return launch_any_tiles<OP, _Float16, float, false, KIND>(a, s);
+    }
+    if constexpr (OP != 2)
+        if (vec) return launch_any_tiles<OP, float, float, true, KIND>(a, s);
+    return launch_any_tiles<OP, float, float, false, KIND>(a, s);
+}
+
+}  // namespace vedic

@@ -1,0 +1,28 @@
+// vedic_lora.hpp -- launch interface of the adapters (vedic_lora.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace vedic {
+
+constexpr int kLoraMaxRank = 128;
+
+struct LoraArgs {
+    const void* X;  // [M x ldx]
+    int64_t ldx;
+    const void* A;  // [groups][K x r]
+    const void* B;  // [groups][r x N]
+    const int* offsets;
+    const int* rows;  // n positions, sorted by adapter
+    int n, groups;
+    const float* scales;  // [groups], or null: ones
+    float* C;             // [M x ldc]
+    int64_t ldc;
+    int M, K, N, r;
+    float* H;  // [n x r] workspace
+};
+
+hipError_t launch_lora(const LoraArgs& a, bool f16, hipStream_t s);
+
+}  // namespace vedic

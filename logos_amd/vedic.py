@@ -14,6 +14,12 @@ Names and argument meaning follow the reference:
   verify(A, B, C)                  cuda_vedic_verify (cuda/VedicGEMM.cu:765-814)
   flash_attention_fwd(Q, K, V)     cuda_flash_attention_fwd (cuda/VedicGEMM.cu:1065-1104)
 
+New here, with no counterpart in the reference: products whose rows choose their weights.
+  route_topk / route_topk_bwd      a router's choice, weights and plan, and its backward
+  gemm_grouped(op, A, B, offsets)  the experts' products, forward and backward (bias_grad_grouped, group_rows)
+  combine_rows / combine_rows_bwd  the experts' rows in token order, and the backward
+  gemm_lora / lora_add             low-rank adapters of many requests beside a shared projection
+
 Operands are torch tensors resident on the GPU (torch is used for device
 memory and streams only); every call runs on torch's current stream.  Shape
 errors raise ValueError (the reference's std::invalid_argument), device
@@ -23,6 +29,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -39,6 +46,8 @@ __all__ = [
     "cast_fp32_to_fp16",
     "cast_fp16_to_fp32", "verify", "gemm_checked", "VerifyResult", "uses_vendor_blas", "backend_name",
     "flash_attention_fwd", "flash_attention_fwd_heads", "flash_attention_bwd", "flash_attention_bwd_heads",
+    "Routing", "route_topk", "route_topk_bwd", "group_rows", "gemm_grouped", "bias_grad_grouped", "combine_rows",
+    "combine_rows_bwd", "lora_add", "gemm_lora",
 ]
 
 _DT = {torch.float32: DT_F32, torch.float16: DT_F16}
@@ -651,3 +660,317 @@ def flash_attention_bwd_heads(Qs, Ks, Vs, Os, dOs, lses, dQs=None, dKs=None, dVs
                                                        float(scale), int(causal), int(shunyam), int(window),
                                                        int(stride), _stream()))
     return tuple(out)
+
+
+# ---------------------------------------------------------------- rows that choose their weights
+
+
+def _on_current(t: torch.Tensor, name: str, dtype, dev: int) -> int:
+    """t's address, checked to be on the current device (whose stream the call runs on) and of `dtype`."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda or t.get_device() != dev:
+        raise ValueError(f"{name} must be on the current GPU (cuda:{dev})")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    return t.data_ptr()
+
+
+def _device() -> int:
+    if not torch.cuda.is_available():
+        raise ValueError("no GPU: the operands must be on the current GPU")
+    return torch.cuda.current_device()
+
+
+def _ints(t: torch.Tensor, name: str, shape: tuple, dev: int) -> int:
+    p = _on_current(t, name, torch.int32, dev)
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 of shape {shape}, got {tuple(t.shape)}")
+    return p
+
+
+def _floats(t: torch.Tensor, name: str, shape: tuple, dev: int) -> int:
+    p = _on_current(t, name, torch.float32, dev)
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous float32 of shape {shape}, got {tuple(t.shape)}")
+    return p
+
+
+def _rows2d(t: torch.Tensor, name: str, dtype, dev: int) -> tuple[int, int, int, int]:
+    """(address, rows, cols, leading dimension) of a row-major matrix of `dtype` on the current device."""
+    p = _on_current(t, name, dtype, dev)
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-D, got shape {tuple(t.shape)}")
+    r, c = t.shape
+    rs, cs = t.stride()
+    if r > 0 and c > 1 and cs != 1:
+        raise ValueError(f"{name} must be row-major with unit column stride")
+    if r > 1 and rs < c:
+        raise ValueError(f"{name}'s rows overlap (row stride {rs}, {c} columns)")
+    return p, r, c, rs if r > 1 else c
+
+
+class Routing(NamedTuple):
+    """What route_topk returns (int32 but for the float32 weights)."""
+
+    ids: torch.Tensor      # [T, k] experts in descending order of the logits; -1: none
+    weights: torch.Tensor  # [T, k]
+    offsets: torch.Tensor  # [E + 1] first sorted place of each expert
+    rows: torch.Tensor     # [T * k] token of each place
+    slots: torch.Tensor    # [T, k] place of each pair
+
+
+def route_topk(logits: torch.Tensor, k: int, renorm: bool = True) -> Routing:
+    """A router's choice: the k largest of each token's float32 logits [T, E] (a tie to the lower expert, -infinity
+    never), their softmax weights -- among the chosen (renorm) or within all E -- and the plan that gemm_grouped and
+    combine_rows read: the pairs sorted by expert.  See vedic_route_topk in logos_vedic.h."""
+    dev = _device()
+    p, T, E, ld = _rows2d(logits, "logits", torch.float32, dev)
+    if not 0 < k <= E:
+        raise ValueError(f"k must be 1 .. {E}, got {k}")
+    d = logits.device
+    ids = torch.empty((T, k), dtype=torch.int32, device=d)
+    weights = torch.empty((T, k), dtype=torch.float32, device=d)
+    offsets = torch.empty(E + 1, dtype=torch.int32, device=d)
+    rows = torch.empty(T * k, dtype=torch.int32, device=d)
+    slots = torch.empty((T, k), dtype=torch.int32, device=d)
+    _check(_lib.load().vedic_route_topk(p, ld, T, E, k, renorm, ids.data_ptr(), weights.data_ptr(), offsets.data_ptr(),
+                                        rows.data_ptr(), slots.data_ptr(), _stream()))
+    return Routing(ids, weights, offsets, rows, slots)
+
+
+def route_topk_bwd(logits: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, dweights: torch.Tensor,
+                   renorm: bool = True, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of route_topk's weights with respect to the logits, float32 [T, E]; renorm as in the forward."""
+    dev = _device()
+    p, T, E, ld = _rows2d(logits, "logits", torch.float32, dev)
+    if ids.dim() != 2 or ids.shape[0] != T or not 0 < ids.shape[1] <= E:
+        raise ValueError(f"ids must be [{T}, k] with k <= {E}, got {tuple(ids.shape)}")
+    shape = tuple(ids.shape)
+    pi, pw, pg = _ints(ids, "ids", shape, dev), _floats(weights, "weights", shape, dev), \
+        _floats(dweights, "dweights", shape, dev)
+    if out is None:
+        out = torch.empty((T, E), dtype=torch.float32, device=logits.device)
+    po, To, Eo, ldo = _rows2d(out, "out", torch.float32, dev)
+    if (To, Eo) != (T, E):
+        raise ValueError(f"out must be {T}x{E}")
+    _check(_lib.load().vedic_route_topk_bwd(p, ld, pi, pw, pg, T, E, shape[1], renorm, po, ldo, _stream()))
+    return out
+
+
+def group_rows(ids: torch.Tensor, groups: int, per_row: int = 1) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(offsets, rows, slots) of the plan that sorts the int32 `ids` by group, stable: rows[place] = entry // per_row.
+    An id outside 0 .. groups - 1 belongs to no group (slot -1)."""
+    dev = _device()
+    p = _ints(ids, "ids", tuple(ids.shape), dev)
+    n, d = ids.numel(), ids.device
+    offsets = torch.empty(max(groups, 0) + 1, dtype=torch.int32, device=d)
+    rows = torch.empty(n, dtype=torch.int32, device=d)
+    slots = torch.empty(ids.shape, dtype=torch.int32, device=d)
+    _check(_lib.load().vedic_group_rows(p, n, per_row, groups, offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(),
+                                        _stream()))
+    return offsets, rows, slots
+
+
+def _offsets(t: torch.Tensor, groups: int, dev: int) -> int:
+    return _ints(t, "offsets", (groups + 1,), dev)
+
+
+def gemm_grouped(op: int, A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor, C: torch.Tensor | None = None, *,
+                 rows: torch.Tensor | None = None, bias: torch.Tensor | None = None, epilogue: int = EPI_NONE,
+                 preact: torch.Tensor | None = None, beta: float = 0.0, db: torch.Tensor | None = None,
+                 db_beta: float = 0.0, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Products grouped by expert (vedic_gemm_grouped in logos_vedic.h): rows offsets[g] .. offsets[g + 1] - 1 take
+    group g's weight.
+
+      OP_NN  C[i] = epi(A[i] . B[g])       B [G, K, N]; epilogue NONE, BIAS or BIAS_GELU (bias [G, N], preact an output)
+      OP_NT  C[i] = epi(A[i] . B[g]^T)     B [G, N, K]; epilogue NONE or GELU_BWD (preact an input)
+      OP_TN  C[g] = beta C[g] + A_g^T . B_g  A [R, M], B [R, N], C [G, M, N]; db [G, N] = db_beta db + column sums of B
+
+    rows (int32 [R]): A[i] is row rows[i] of A.  A and B float16 or float32; C and preact float32, or float16
+    (out_dtype) with float16 operands and OP_NN / OP_NT.  Rows of C behind offsets[G] are left as they are."""
+    dev = _device()
+    dt = A.dtype
+    if dt not in _DT:
+        raise ValueError(f"A must be float16 or float32, got {dt}")
+    if op not in (OP_NN, OP_NT, OP_TN):
+        raise ValueError(f"unknown op {op}")
+    if epilogue not in ((EPI_NONE, EPI_BIAS, EPI_BIAS_GELU), (EPI_NONE, EPI_GELU_BWD), (EPI_NONE,))[op]:
+        raise ValueError("VedicGEMM: epilogue not offered with this op (NN: NONE, BIAS, BIAS_GELU; NT: NONE, GELU_BWD; "
+                         "TN: NONE)")
+    pa, a_rows, a_cols, lda = _rows2d(A, "A", dt, dev)
+    G = offsets.numel() - 1
+    if G < 1:
+        raise ValueError("offsets must hold groups + 1 values")
+    poff = _offsets(offsets, G, dev)
+    R = a_rows
+    pr = None
+    if rows is not None:
+        R = rows.numel()
+        pr = _ints(rows, "rows", (R,), dev)
+    d = A.device
+    stride_b = stride_c = 0
+    M = K = 0
+    if op == OP_TN:
+        pb, b_rows, N, ldb = _rows2d(B, "B", dt, dev)
+        M = a_cols
+        if b_rows != R:
+            raise ValueError(f"VedicGEMM: A gives {R} rows, B {b_rows}")
+        if C is None:
+            if beta != 0.0:
+                raise ValueError("beta != 0 needs an existing C")
+            C = torch.empty((G, M, N), dtype=torch.float32, device=d)
+        pc = _on_current(C, "C", torch.float32, dev)
+        if tuple(C.shape) != (G, M, N) or (N > 1 and C.stride(2) != 1) or (M > 1 and C.stride(1) < N):
+            raise ValueError(f"C must be float32 [{G}, {M}, {N}] with row-major matrices")
+        ldc, stride_c = (C.stride(1) if M > 1 else N), C.stride(0)
+    else:
+        pb = _on_current(B, "B", dt, dev)
+        if B.dim() != 3 or B.shape[0] != G:
+            raise ValueError(f"B must be [{G}, {'K, N' if op == OP_NN else 'N, K'}], got {tuple(B.shape)}")
+        br, bc = B.shape[1], B.shape[2]
+        K, N = (br, bc) if op == OP_NN else (bc, br)
+        if (bc > 1 and B.stride(2) != 1) or (br > 1 and B.stride(1) < bc):
+            raise ValueError("B must hold row-major matrices")
+        ldb, stride_b = (B.stride(1) if br > 1 else bc), B.stride(0)
+        if K != a_cols:
+            raise ValueError(f"VedicGEMM: inner dimensions differ (A gives K={a_cols}, B gives K={K})")
+        if beta != 0.0 or db is not None:
+            raise ValueError("beta and db belong to OP_TN")
+        if C is None:
+            C = torch.empty((R, N), dtype=out_dtype, device=d)
+        if C.dtype not in _DT or (C.dtype == torch.float16 and dt != torch.float16):
+            raise ValueError("C must be float32, or float16 with float16 operands")
+        pc, cr, cc, ldc = _rows2d(C, "C", C.dtype, dev)
+        if (cr, cc) != (R, N):
+            raise ValueError(f"C must be {R}x{N}, got {cr}x{cc}")
+    pbias = pp = pdb = None
+    if epilogue in (EPI_BIAS, EPI_BIAS_GELU):
+        if bias is None:
+            raise ValueError("this epilogue takes a bias")
+        pbias = _floats(bias, "bias", (G, N), dev)
+    elif bias is not None:
+        raise ValueError("a bias goes with EPI_BIAS or EPI_BIAS_GELU")
+    ldp = 0
+    if preact is not None:
+        pp, prow, pcol, ldp = _rows2d(preact, "preact", C.dtype, dev)
+        if (prow, pcol) != (R, N):
+            raise ValueError(f"preact must be {R}x{N}")
+    if db is not None:
+        pdb = _floats(db, "db", (G, N), dev)
+    desc = _lib.GroupedDesc(op, _DT[dt], _DT[C.dtype], epilogue, G, R, M, N, K, poff, pr, a_rows, pa, lda, pb, ldb, stride_b,
+                            pc, ldc, stride_c, pbias, pp, ldp, beta, pdb, db_beta, _stream())
+    _check(_lib.load().vedic_gemm_grouped(ctypes.byref(desc)))
+    return C
+
+
+def bias_grad_grouped(dY: torch.Tensor, offsets: torch.Tensor, db: torch.Tensor | None = None,
+                      beta: float = 0.0) -> torch.Tensor:
+    """db[g] = beta db[g] + the column sums of group g's rows of dY (float16 or float32 [R, N]), in a fixed order."""
+    dev = _device()
+    if dY.dtype not in _DT:
+        raise ValueError(f"dY must be float16 or float32, got {dY.dtype}")
+    p, R, N, ld = _rows2d(dY, "dY", dY.dtype, dev)
+    G = offsets.numel() - 1
+    po = _offsets(offsets, G, dev)
+    if db is None:
+        if beta != 0.0:
+            raise ValueError("beta != 0 needs an existing db")
+        db = torch.empty((G, N), dtype=torch.float32, device=dY.device)
+    pd = _floats(db, "db", (G, N), dev)
+    _check(_lib.load().vedic_bias_grad_grouped(p, _DT[dY.dtype], ld, R, N, po, G, beta, pd, _stream()))
+    return db
+
+
+def combine_rows(Y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None = None,
+                 residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """out[t] = residual[t] + sum over j of weights[t, j] Y[slots[t, j]], float32 [T, D]: the experts' rows back in token
+    order (weights None: ones, the backward of reading rows through a list; residual may be out)."""
+    dev = _device()
+    if Y.dtype not in _DT:
+        raise ValueError(f"Y must be float16 or float32, got {Y.dtype}")
+    p, R, D, ldy = _rows2d(Y, "Y", Y.dtype, dev)
+    if slots.dim() != 2:
+        raise ValueError("slots must be [T, k]")
+    T, k = slots.shape
+    ps = _ints(slots, "slots", (T, k), dev)
+    pw = None if weights is None else _floats(weights, "weights", (T, k), dev)
+    pres, ldr = None, 0
+    if residual is not None:
+        pres, rr, rc, ldr = _rows2d(residual, "residual", torch.float32, dev)
+        if (rr, rc) != (T, D):
+            raise ValueError(f"residual must be {T}x{D}")
+    if out is None:
+        out = torch.empty((T, D), dtype=torch.float32, device=Y.device)
+    po, To, Do, ldo = _rows2d(out, "out", torch.float32, dev)
+    if (To, Do) != (T, D):
+        raise ValueError(f"out must be {T}x{D}")
+    _check(_lib.load().vedic_combine_rows(p, _DT[Y.dtype], ldy, R, ps, pw, pres, ldr, po, ldo, T, k, D, _stream()))
+    return out
+
+
+def combine_rows_bwd(dout: torch.Tensor, Y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor,
+                     dY: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float32
+                     ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(dY, dweights) of combine_rows: dY[slots[t, j]] = weights[t, j] dout[t] in out_dtype (float32 or float16),
+    dweights[t, j] = <dout[t], Y[slots[t, j]]>.  Every slot at most once; rows that no slot names are left as they are
+    (undefined in a dY allocated here)."""
+    dev = _device()
+    if Y.dtype not in _DT:
+        raise ValueError(f"Y must be float16 or float32, got {Y.dtype}")
+    p, R, D, ldy = _rows2d(Y, "Y", Y.dtype, dev)
+    if slots.dim() != 2:
+        raise ValueError("slots must be [T, k]")
+    T, k = slots.shape
+    ps = _ints(slots, "slots", (T, k), dev)
+    pw = _floats(weights, "weights", (T, k), dev)
+    pg, gr, gc, ldg = _rows2d(dout, "dout", torch.float32, dev)
+    if (gr, gc) != (T, D):
+        raise ValueError(f"dout must be {T}x{D}")
+    if dY is None:
+        dY = torch.empty((R, D), dtype=out_dtype, device=Y.device)
+    if dY.dtype not in _DT:
+        raise ValueError("dY must be float16 or float32")
+    po, orr, oc, ldo = _rows2d(dY, "dY", dY.dtype, dev)
+    if (orr, oc) != (R, D):
+        raise ValueError(f"dY must be {R}x{D}")
+    dw = torch.empty((T, k), dtype=torch.float32, device=Y.device)
+    _check(_lib.load().vedic_combine_rows_bwd(pg, ldg, p, _DT[Y.dtype], ldy, R, ps, pw, po, _DT[dY.dtype], ldo,
+                                              dw.data_ptr(), T, k, D, _stream()))
+    return dY, dw
+
+
+def lora_add(C: torch.Tensor, X: torch.Tensor, A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor,
+             rows: torch.Tensor, scales: torch.Tensor | None = None) -> torch.Tensor:
+    """C[i] += scales[g] (X[i] . A[g]) . B[g], in place, for the rows i = rows[offsets[g] .. offsets[g + 1] - 1] of each
+    adapter g (a plan of group_rows).  X [M, K], A [G, K, r], B [G, r, N] all float16 or all float32, C float32 [M, N];
+    r <= 128.  A row is listed at most once; others keep their content."""
+    dev = _device()
+    dt = X.dtype
+    if dt not in _DT:
+        raise ValueError(f"X must be float16 or float32, got {dt}")
+    px, M, K, ldx = _rows2d(X, "X", dt, dev)
+    pa, pb = _on_current(A, "A", dt, dev), _on_current(B, "B", dt, dev)
+    pc, Mc, N, ldc = _rows2d(C, "C", torch.float32, dev)
+    if A.dim() != 3 or not A.is_contiguous() or A.shape[1] != K:
+        raise ValueError(f"A must be contiguous [G, {K}, r], got {tuple(A.shape)}")
+    G, _, r = A.shape
+    if tuple(B.shape) != (G, r, N) or not B.is_contiguous():
+        raise ValueError(f"B must be contiguous [{G}, {r}, {N}], got {tuple(B.shape)}")
+    if Mc != M:
+        raise ValueError(f"C must have {M} rows, got {Mc}")
+    n = rows.numel()
+    po, pr = _offsets(offsets, G, dev), _ints(rows, "rows", (n,), dev)
+    psc = None if scales is None else _floats(scales, "scales", (G,), dev)
+    _check(_lib.load().vedic_lora_add(px, _DT[dt], ldx, M, pa, pb, G, r, po, pr, n, psc, pc, ldc, K, N, _stream()))
+    return C
+
+
+def gemm_lora(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor,
+              rows: torch.Tensor, bias: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """Y = X . W (+ bias), float32, with every listed row's adapter added (lora_add): one shared projection for the
+    requests of a batch, each with low-rank weights of its own."""
+    _on_current(X, "X", W.dtype, _device())
+    Y = gemm(OP_NN, X, W, out, bias=bias, epilogue=EPI_BIAS if bias is not None else EPI_NONE)
+    return lora_add(Y, X, A, B, offsets, rows, scales)
