@@ -1409,7 +1409,9 @@ extern "C" int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, cons
     Workspace ws;
     ws.s = static_cast<hipStream_t>(stream);
     LoraArgs a{};
-    hipError_t e = ws.get(&a.H, sizeof(float) * (size_t)n * r);
+    const bool f16 = dtype == VEDIC_DT_F16;
+    void* work = nullptr;
+    hipError_t e = ws.get(&work, lora_bytes(n, r, f16));
     if (e != hipSuccess) return hip_status(e);
     a.X = X;
     a.ldx = ldx;
@@ -1426,8 +1428,8 @@ extern "C" int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, cons
     a.K = K;
     a.N = N;
     a.r = r;
-    e = launch_lora(a, dtype == VEDIC_DT_F16, ws.s);
-    const hipError_t f = ws.put(a.H);
+    e = launch_lora(a, f16, work, ws.s);
+    const hipError_t f = ws.put(work);
     return hip_status(e != hipSuccess ? e : f);
 }
 

@@ -1,8 +1,10 @@
 // vedic_lora.hip -- low-rank adapters of many requests in one batch: for the rows
 // i of adapter g (list position p, rows[p] = i),
 //   C[i] += scale[g] (X[i] . A_g) . B_g,   A_g [K x r], B_g [r x N].
-// Two launches, H = X A_g into a workspace in fp32 (never rounded), then C.
+// Two launches, H = X A_g into a workspace (fp32, or the same as two binary16
+// values), then C.
 #include "vedic_common.hpp"
+#include "vedic_gemm_f16.hpp"
 #include "vedic_grouped.hpp"
 #include "vedic_lora.hpp"
 
@@ -101,8 +103,236 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
     }
 }
 
+// ------------------------------------------------ binary16, 16-byte rows
+
+typedef short lora_short4_t __attribute__((ext_vector_type(4)));
+
+// MFMA operand of 16 columns n0 .. n0 + 15 (lane l: column l mod 16) and the 32
+// steps k0 .. k0 + 31 (lane l: 8 (l / 16) .. + 7) of an LDS matrix [k][pitch bytes],
+// by two transposing reads; XOR16: the 16-byte slots of row k are XORed by 4 (k mod 4).
+template <bool XOR16>
+__device__ __forceinline__ half8_t read_tr16(const char* lds, int pitch, int k0, int n0, int lane) {
+    const int g = lane >> 4, s = lane & 15;
+    union {
+        lora_short4_t q[2];
+        half8_t h;
+    } u;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int k = k0 + 8 * g + 4 * t + (s >> 2), n = n0 + 4 * (s & 3);
+        const int off = XOR16 ? k * pitch + (((n >> 3) ^ (4 * (k & 3))) << 4) + 2 * (n & 7) : k * pitch + 2 * n;
+        u.q[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) lora_short4_t*)(lds + off));
+    }
+    return u.h;
+}
+
+// H = X A_g of 16 places by one workgroup, eight waves each taking an eighth of K
+// through two LDS stages of its own (A_g's rows k .. k + KC - 1 are one piece of
+// memory; a wave reads what it loaded itself, so no barrier until the sum).  X's
+// rows go straight into the MFMA's operand registers.
+//
+// H stays at fp32 precision as two binary16 values: row p is scaled by 2^-x so that
+// its largest value lies in [2^14, 2^15), and h = hi + lo, hi = f16(h), lo = f16(h -
+// hi), leaves at most 2^-22 of h or 2^-25, 2^-39 of the largest, behind.
+// factor[p] = scale 2^x then multiplies the product's fp32 sums.
+template <int RP, int KC>
+__global__ void __launch_bounds__(512) lora_shrink_f16_kernel(LoraArgs a) {
+    constexpr int NB = RP / 16, SB = KC * RP * 2, NI = (SB + 1023) / 1024, STAGE = NI * 1024;
+    constexpr int RS = RP < 32 ? 32 : RP;  // columns of hi, of lo
+    static_assert(8 * 16 * RP * 4 <= 8 * 2 * STAGE, "the partial sums fit the stages");
+    __shared__ __attribute__((aligned(1024))) char s0[8 * STAGE];
+    __shared__ __attribute__((aligned(1024))) char s1[8 * STAGE];
+    __shared__ GroupIndex ix;
+    GroupedArgs q{};
+    q.offsets = a.offsets;
+    q.groups = a.groups;
+    q.R = a.n;
+    group_index<512>(q, ix, 16);
+    const int tid = threadIdx.x, lane = tid & 63, t = blockIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (t >= ix.pre[a.groups]) return;
+    const int g = group_of(ix, a.groups, t, lane);
+    const int p0 = __builtin_amdgcn_readfirstlane(ix.off[g]) + (t - __builtin_amdgcn_readfirstlane(ix.pre[g])) * 16;
+    const int np = min(16, __builtin_amdgcn_readfirstlane(ix.off[g + 1]) - p0);
+    // this lane's row of X and the wave's range of K, whole stages
+    const int row = (lane & 15) < np ? a.rows[p0 + (lane & 15)] : -1;
+    const bool ok = (unsigned)row < (unsigned)a.M;
+    const half8_t* x =
+        reinterpret_cast<const half8_t*>(static_cast<const _Float16*>(a.X) + (int64_t)(ok ? row : 0) * a.ldx);
+    const int kw = (a.K + 8 * KC - 1) / (8 * KC) * KC;
+    const int kb = min(a.K, wave * kw), ke = min(a.K, kb + kw);
+    const char* A = static_cast<const char*>(a.A) + ((int64_t)g * a.K) * a.r * 2;
+    const int rb = a.r * 2;
+    auto issue = [&](int k, char* dst) {
+        const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(A + (int64_t)(k < ke ? k : 0) * rb);
+        const int left = k < ke ? min(KC, ke - k) * rb : 0;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int off = i * 1024 + lane * 16;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(dst + wave * STAGE + i * 1024), 16,
+                                                     off + 16 <= left ? (uint32_t)off : kOob, 0, 0, 0);
+        }
+        asm volatile("" ::: "memory");
+    };
+    // (loads without a condition, so that every stage has the same number in flight:
+    // past the range the row's start, whose product with A_g's zeros is masked to zero)
+    half8_t xf[2][KC / 32];
+    auto fetch = [&](int k, half8_t (&f)[KC / 32]) {
+#pragma unroll
+        for (int c = 0; c < KC / 32; ++c) {
+            const int kk = k + 32 * c + 8 * (lane >> 4);
+            f[c] = x[kk < ke ? kk >> 3 : 0];
+        }
+        asm volatile("" ::: "memory");
+    };
+    float4_t acc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    auto multiply = [&](const char* src, int k, half8_t (&f)[KC / 32]) {
+#pragma unroll
+        for (int c = 0; c < KC / 32; ++c) {
+            if (!ok || k + 32 * c + 8 * (lane >> 4) >= ke) f[c] = half8_t{};
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    f[c], read_tr16<false>(src + wave * STAGE, rb, 32 * c, 16 * b, lane), acc[b], 0, 0, 0);
+        }
+    };
+    issue(kb, s0);
+    fetch(kb, xf[0]);
+    for (int k = kb; k < ke; k += 2 * KC) {
+        issue(k + KC, s1);
+        fetch(k + KC, xf[1]);
+        wait_vmcnt<NI + KC / 32>();
+        multiply(s0, k, xf[0]);
+        wait_lgkmcnt0();
+        issue(k + 2 * KC, s0);
+        fetch(k + 2 * KC, xf[0]);
+        wait_vmcnt<NI + KC / 32>();
+        multiply(s1, k + KC, xf[1]);
+        wait_lgkmcnt0();
+    }
+    wait_vmcnt<0>();
+    __syncthreads();
+    // sum of the eight partials in wave order: part[wave][row][column]
+    float* part0 = reinterpret_cast<float*>(s0);
+    float* part1 = reinterpret_cast<float*>(s1);
+    constexpr int PW = 16 * RP;  // floats a wave
+    auto part = [&](int w) { return w < 4 ? part0 + w * PW : part1 + (w - 4) * PW; };
+    static_assert(4 * PW * 4 <= 8 * STAGE, "four waves' partials in each stage object");
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part(wave)[(4 * (lane >> 4) + e) * RP + 16 * b + (lane & 15)] = acc[b][e];
+    __syncthreads();
+    // 32 threads a row, columns c, c + 32, ...
+    const int i = tid >> 5, c0 = tid & 31;
+    constexpr int NC = (RS + 31) / 32;
+    float h[NC], top = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NC; ++v) {
+        const int c = c0 + 32 * v;
+        h[v] = 0.0f;
+        if (c < a.r && c < RP)
+            for (int w = 0; w < 8; ++w) h[v] += part(w)[i * RP + c];
+        top = fmaxf(top, fabsf(h[v]));
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 32));
+    if (i < np) {
+        // (a row of zeros, or one that is not finite, keeps its scale)
+        int ex = 0;
+        if (top > 0.0f && top < __builtin_inff()) {
+            (void)frexpf(top, &ex);  // top = m 2^ex, m in [0.5, 1)
+            ex -= 15;
+        }
+        const float down = ldexpf(1.0f, ex < -126 ? 126 : ex > 126 ? -126 : -ex);
+        _Float16* o = a.Hs + (int64_t)(p0 + i) * (2 * RS);
+#pragma unroll
+        for (int v = 0; v < NC; ++v) {
+            const int c = c0 + 32 * v;
+            const float s = h[v] * down;
+            const _Float16 hi = (_Float16)s;
+            const float rest = s - (float)hi;
+            o[c] = hi;
+            o[RS + c] = fabsf((float)hi) < __builtin_inff() ? (_Float16)rest : (_Float16)0.0f;
+        }
+        if (c0 == 0) a.factor[p0 + i] = (a.scales ? a.scales[g] : 1.0f) / down;
+    }
+}
+
+// C[rows[p]] += factor[p] (hi + lo) B_g: 16 places by 256 columns, a wave 64 of
+// them.  B_g's columns are staged in LDS once for both parts; the product is taken
+// transposed, so that a lane holds four neighbouring columns of one row.
+template <int RS>
+__global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
+    __shared__ __attribute__((aligned(1024))) char sb[RS * 512];
+    __shared__ GroupIndex ix;
+    GroupedArgs q{};
+    q.offsets = a.offsets;
+    q.groups = a.groups;
+    q.R = a.n;
+    group_index<256>(q, ix, 16);
+    const int strips = (a.N + 255) / 256;
+    const int tid = threadIdx.x, lane = tid & 63, t = blockIdx.x / strips;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (t >= ix.pre[a.groups]) return;
+    const int g = group_of(ix, a.groups, t, lane);
+    const int p0 = __builtin_amdgcn_readfirstlane(ix.off[g]) + (t - __builtin_amdgcn_readfirstlane(ix.pre[g])) * 16;
+    const int np = min(16, __builtin_amdgcn_readfirstlane(ix.off[g + 1]) - p0);
+    const int n0 = (blockIdx.x - t * strips) * 256;
+    const _Float16* B = static_cast<const _Float16*>(a.B) + (int64_t)g * a.r * a.N + n0;
+    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(B);
+#pragma unroll
+    for (int i = 0; i < RS / 8; ++i) {  // an instruction: two rows of 32 slots
+        const int k = 8 * i + 2 * wave + (lane >> 5), slot = (lane & 31) ^ (4 * (k & 3));
+        const bool in = k < a.r && n0 + 8 * slot < a.N;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(sb + (8 * i + 2 * wave) * 512), 16,
+                                                 in ? (uint32_t)(k * a.N * 2 + slot * 16) : kOob, 0, 0, 0);
+    }
+    const int p = lane & 15;
+    const _Float16* h = a.Hs + (int64_t)(p0 + (p < np ? p : 0)) * (2 * RS) + 8 * (lane >> 4);
+    half8_t hi[RS / 32], lo[RS / 32];
+#pragma unroll
+    for (int c = 0; c < RS / 32; ++c) {
+        hi[c] = *reinterpret_cast<const half8_t*>(h + 32 * c);
+        lo[c] = *reinterpret_cast<const half8_t*>(h + RS + 32 * c);
+    }
+    const float f = a.factor[p0 + (p < np ? p : 0)];
+    const int row = p < np ? a.rows[p0 + p] : -1;
+    const bool ok = (unsigned)row < (unsigned)a.M;
+    float* crow = a.C + (int64_t)(ok ? row : 0) * a.ldc + n0 + 64 * wave + 4 * (lane >> 4);
+    float4_t old[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        old[b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        if (ok && n0 + 64 * wave + 16 * b + 4 * (lane >> 4) < a.N) old[b] = *reinterpret_cast<const float4_t*>(crow + 16 * b);
+    }
+    wait_vmcnt<0>();
+    __syncthreads();
+    float4_t acc[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) acc[b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < RS / 32; ++c)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const half8_t w = read_tr16<true>(sb, 512, 32 * c, 64 * wave + 16 * b, lane);
+            acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, lo[c], acc[b], 0, 0, 0);
+            acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, hi[c], acc[b], 0, 0, 0);
+        }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+        if (ok && n0 + 64 * wave + 16 * b + 4 * (lane >> 4) < a.N) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) old[b][e] = __builtin_fmaf(f, acc[b][e], old[b][e]);
+            store16_hold(crow + 16 * b, old[b]);
+        }
+}
+
 template <typename T>
-hipError_t launch(const LoraArgs& a, hipStream_t s) {
+hipError_t launch_any(const LoraArgs& a, hipStream_t s) {
     const int64_t tiles = a.n / kLoraRows + (a.groups < a.n ? a.groups : a.n);
     hipLaunchKernelGGL((lora_shrink_kernel<T>), dim3((unsigned)tiles), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
@@ -111,10 +341,44 @@ hipError_t launch(const LoraArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
+template <int RP, int KC>
+hipError_t launch_f16(const LoraArgs& a, hipStream_t s) {
+    const int64_t tiles = a.n / 16 + (a.groups < a.n ? a.groups : a.n);
+    hipLaunchKernelGGL((lora_shrink_f16_kernel<RP, KC>), dim3((unsigned)tiles), dim3(512), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((lora_expand_f16_kernel<(RP < 32 ? 32 : RP)>), dim3((unsigned)(tiles * ((a.N + 255) / 256))), dim3(256),
+                       0, s, a);
+    return hipGetLastError();
+}
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Whether the matrix-core kernels take the call: whole 16-byte loads of every operand.
+bool vec16(const LoraArgs& a) {
+    return al16(a.X) && al16(a.A) && al16(a.B) && al16(a.C) && a.ldx % 8 == 0 && a.K % 8 == 0 && a.N % 8 == 0 && a.r % 4 == 0 &&
+           a.ldc % 4 == 0;
+}
+
 }  // namespace
 
-hipError_t launch_lora(const LoraArgs& a, bool f16, hipStream_t s) {
-    return f16 ? launch<_Float16>(a, s) : launch<float>(a, s);
+size_t lora_bytes(int n, int r, bool f16) {
+    const size_t rs = (size_t)(r <= 32 ? 32 : r <= 64 ? 64 : 128);
+    // (fp32: n r values; binary16: hi and lo of rs each, and the factors)
+    return f16 ? (size_t)n * (rs * 4 + 4) : (size_t)n * r * 4;
+}
+
+hipError_t launch_lora(LoraArgs a, bool f16, void* work, hipStream_t s) {
+    a.H = static_cast<float*>(work);
+    if (!f16) return launch_any<float>(a, s);
+    if (!vec16(a)) return launch_any<_Float16>(a, s);
+    const size_t rs = (size_t)(a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128);
+    a.Hs = static_cast<_Float16*>(work);
+    a.factor = reinterpret_cast<float*>(a.Hs + (size_t)a.n * 2 * rs);
+    if (a.r <= 16) return launch_f16<16, 64>(a, s);
+    if (a.r <= 32) return launch_f16<32, 64>(a, s);
+    if (a.r <= 64) return launch_f16<64, 64>(a, s);
+    return launch_f16<128, 32>(a, s);
 }
 
 }  // namespace vedic

@@ -20,9 +20,14 @@ struct LoraArgs {
     float* C;             // [M x ldc]
     int64_t ldc;
     int M, K, N, r;
-    float* H;  // [n x r] workspace
+    // set by the launch
+    float* H;       // [n x r]
+    _Float16* Hs;   // [n][hi, lo]
+    float* factor;  // [n]
 };
 
-hipError_t launch_lora(const LoraArgs& a, bool f16, hipStream_t s);
+// Workspace of a call, and the call (work: that many bytes, 256-byte aligned).
+size_t lora_bytes(int n, int r, bool f16);
+hipError_t launch_lora(LoraArgs a, bool f16, void* work, hipStream_t s);
 
 }  // namespace vedic
