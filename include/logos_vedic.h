@@ -494,8 +494,8 @@ int vedic_flash_attention_bwd_heads(const float* const* Q, const float* const* K
  *   rows [T k]             the token of each place
  *   slots [T x k]          the place of each pair
  * A logit of -infinity is never chosen: a token with fewer than k others gets id
- * -1, weight 0 and slot -1 in the rest, and the places behind offsets[E] have row
- * -1.  NaN counts as larger than every number (and makes its token's weights NaN).
+ * -1, weight 0 and slot -1 in the rest, whose tokens fill the places behind
+ * offsets[E].  NaN counts as larger than every number (and makes its token's weights NaN).
  * k <= 64.  More than 64 tokens or 1024 pairs take a few KB of the stream's
  * workspace block. */
 int vedic_route_topk(const float* logits, int64_t ld_logits, int T, int E, int k, int renorm, int* ids, float* weights,
@@ -511,8 +511,8 @@ int vedic_route_topk_bwd(const float* logits, int64_t ld_logits, const int* ids,
 
 /* The plan alone: n entries of ids sorted by group, stable.  rows[place] = entry /
  * per_row (1 for one group per row, k for [rows x k] ids), slots (may be NULL) the
- * place of each entry; an id outside 0 .. groups - 1 belongs to no group (slot -1;
- * row -1 in the places behind offsets[groups]). */
+ * place of each entry; an id outside 0 .. groups - 1 belongs to no group (slot -1) and
+ * its row is among those behind offsets[groups]. */
 int vedic_group_rows(const int* ids, int n, int per_row, int groups, int* offsets, int* rows, int* slots, void* stream);
 
 /* Products grouped by expert.  For the places i of group g:

@@ -1254,7 +1254,7 @@ extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
     switch (d->epilogue) {
         case VEDIC_EPI_NONE: kind = GK_LINEAR; break;
         case VEDIC_EPI_BIAS: kind = GK_LINEAR; break;
-        case VEDIC_EPI_BIAS_GELU: kind = GK_GELU; break;
+        case VEDIC_EPI_BIAS_GELU: kind = d->preact ? GK_GELU_P : GK_GELU; break;
         case VEDIC_EPI_GELU_BWD: kind = GK_GELU_BWD; break;
         default: return VEDIC_STATUS_BAD_EPILOGUE;
     }
@@ -1262,7 +1262,7 @@ extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
     const bool reads_p = d->epilogue == VEDIC_EPI_GELU_BWD;
     if ((wants_bias && (d->op != VEDIC_OP_NN || !d->bias)) || (reads_p && (d->op != VEDIC_OP_NT || !d->preact)))
         return VEDIC_STATUS_BAD_EPILOGUE;
-    if (d->preact && kind != GK_GELU && kind != GK_GELU_BWD) return VEDIC_STATUS_BAD_EPILOGUE;
+    if (d->preact && kind != GK_GELU_P && kind != GK_GELU_BWD) return VEDIC_STATUS_BAD_EPILOGUE;
     if ((!tn && (d->beta != 0.0f || d->db)) || d->beta != d->beta) return VEDIC_STATUS_BAD_EPILOGUE;
     if (!d->offsets || (!d->C && (tn || R > 0)) || (R > 0 && (!d->A || !d->B))) return VEDIC_STATUS_NULL_POINTER;
     const int a_cols = tn ? d->M : d->K, b_cols = d->op == VEDIC_OP_NT ? d->K : N;
@@ -1301,10 +1301,19 @@ extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
     a.beta = d->beta;
     if (tn && d->beta != 0.0f) kind = GK_BETA;
     const int es = f16 ? 2 : 4, per16 = 16 / es;
+    a.db = d->db;
+    a.db_beta = d->db_beta;
+    auto vec_of = [&]() {
+        bool vec = aligned16(a.A) && a.lda % per16 == 0;
+        if (f16 || d->op == VEDIC_OP_NT) vec = vec && aligned16(a.B) && a.ldb % per16 == 0 && a.stride_b % per16 == 0;
+        return vec && a_cols % per16 == 0 && ((!f16 && d->op == VEDIC_OP_NN) || b_cols % per16 == 0);
+    };
+    bool vec = vec_of();
     // The rows of a list are copied into a workspace first where the kernels
-    // cannot follow it: along the contraction (TN), and past 32-bit offsets.
+    // cannot follow it: past 32-bit offsets, and along the contraction (TN) but for
+    // the 16-byte binary16 kernels.
     void* copy = nullptr;
-    if (a.rows && (tn || (int64_t)d->a_rows * d->lda * es >= (int64_t(1) << 31))) {
+    if (a.rows && ((tn && !(f16 && vec)) || (int64_t)d->a_rows * d->lda * es >= (int64_t(1) << 31))) {
         const int64_t ldn = ((int64_t)a_cols + 7) / 8 * 8;
         hipError_t e = ws.get(&copy, (size_t)R * ldn * es);
         if (e == hipSuccess)
@@ -1313,12 +1322,11 @@ extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
         a.A = copy;
         a.lda = ldn;
         a.rows = nullptr;
+        vec = vec_of();
     }
-    bool vec = aligned16(a.A) && a.lda % per16 == 0;
-    if (f16 || d->op == VEDIC_OP_NT) vec = vec && aligned16(a.B) && a.ldb % per16 == 0 && a.stride_b % per16 == 0;
-    vec = vec && a_cols % per16 == 0 && ((!f16 && d->op == VEDIC_OP_NN) || b_cols % per16 == 0);
     hipError_t e = launch_grouped(d->op, a, kind, f16, f16out, vec, ws.s);
-    if (e == hipSuccess && d->db)
+    // (the 16-byte binary16 kernels sum the columns on the way)
+    if (e == hipSuccess && d->db && !(f16 && vec))
         e = launch_group_colsum(d->B, f16, d->ldb, R, N, d->offsets, d->groups, d->db_beta, d->db, ws.s);
     const hipError_t f = ws.put(copy);
     return hip_status(e != hipSuccess ? e : f);

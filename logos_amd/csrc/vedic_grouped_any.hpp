@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs 
     constexpr int BYTES = (BM + BN) * kSplitRowBytes;
     __shared__ __attribute__((aligned(1024))) char buf0[BYTES];
     __shared__ __attribute__((aligned(1024))) char buf1[BYTES];
+    __shared__ __attribute__((aligned(16))) float sbias[BN];
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int wm = wave / WGN, wn = wave % WGN;
@@ -166,25 +167,27 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs 
         const int t = blockIdx.x - e * tiles;
         m0 = t % a.tiles_m * BM;
         n0 = t / a.tiles_m * BN;
-        start = min(max(a.offsets[e], 0), a.R);
-        count = max(0, min(max(a.offsets[e + 1], 0), a.R) - start);
+        start = group_start(a, e);
+        count = group_count(a, e);
         K = count;
         left = a.M - m0;
     } else {
         GroupIndex& ix = *reinterpret_cast<GroupIndex*>(buf0);
-        static_assert(sizeof(GroupIndex) <= BYTES, "the index fits a stage buffer");
-        group_index<NT>(a, ix, BM);
+        static_assert(BN <= NT && sizeof(GroupIndex) <= BYTES, "the index fits a stage buffer");
+        group_index(a, ix, BM);
         const int t = blockIdx.x / a.tiles_n;
         if (t >= ix.pre[a.groups]) return;
         e = group_of(ix, a.groups, t, lane);
-        start = __builtin_amdgcn_readfirstlane(ix.off[e]);
-        count = __builtin_amdgcn_readfirstlane(ix.off[e + 1]) - start;
+        start = group_start(a, e);
+        count = group_count(a, e);
         m0 = (t - __builtin_amdgcn_readfirstlane(ix.pre[e])) * BM;
         n0 = (blockIdx.x - t * a.tiles_n) * BN;
         K = a.K;
         left = count - m0;
         __syncthreads();  // the index's LDS becomes a stage buffer
     }
+    // (read after the barriers of the stages or the one before the epilogue)
+    if (tid < BN) sbias[tid] = a.bias != nullptr && n0 + tid < a.N ? a.bias[(int64_t)e * a.N + n0 + tid] : 0.0f;
     const T* A = static_cast<const T*>(a.A);
     const int* list = nullptr;
     if constexpr (OP == 2) {
@@ -287,8 +290,13 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs 
     const int64_t crow = OP == 2 ? row0 : start + row0;
     OT* C = static_cast<OT*>(a.C) + (OP == 2 ? (int64_t)e * a.stride_c : 0) + crow * a.ldc;
     OT* P = a.P != nullptr ? static_cast<OT*>(a.P) + crow * a.ldp : nullptr;
-    grouped_epilogue<KIND, OT, true, MI, NI>(C, a.ldc, P, a.ldp, a.bias ? a.bias + (int64_t)e * a.N : nullptr, a.beta, acc,
-                                             left - wm * WM, a.N, n0 + wn * WN, lane);
+    __syncthreads();
+    if (grouped_reads(KIND) && a.wide)
+        grouped_epilogue<KIND, OT, true, true, MI, NI>(C, a.ldc, P, a.ldp, sbias + wn * WN, a.beta, acc, left - wm * WM, a.N,
+                                                       n0 + wn * WN, lane);
+    else
+        grouped_epilogue<KIND, OT, true, false, MI, NI>(C, a.ldc, P, a.ldp, sbias + wn * WN, a.beta, acc, left - wm * WM, a.N,
+                                                        n0 + wn * WN, lane);
 }
 
 struct CfgAMid {  // 128 x 128, four waves of 64 x 64
@@ -310,6 +318,7 @@ template <int OP, typename T, typename OT, bool VEC, class Cfg, int KIND>
 static hipError_t launch_any(GroupedArgs a, hipStream_t s) {
     a.tiles_n = (a.N + Cfg::BN - 1) / Cfg::BN;
     a.tiles_m = OP == 2 ? (a.M + Cfg::BM - 1) / Cfg::BM : 0;
+    a.wide = grouped_wide_rows(a, sizeof(OT));
     const int64_t work = OP == 2 ? (int64_t)a.groups * a.tiles_m * a.tiles_n
                                  : grouped_row_tiles_max(a.R, a.groups, Cfg::BM) * a.tiles_n;
     if (work > 0x7FFFFFFF) return hipErrorInvalidValue;  // (the caller has refused such sizes)

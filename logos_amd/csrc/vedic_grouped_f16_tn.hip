@@ -3,8 +3,8 @@
 
 namespace vedic {
 
-VEDIC_GROUPED_INSTANTIATE(2, GK_LINEAR, float);
-VEDIC_GROUPED_INSTANTIATE(2, GK_BETA, float);
+VEDIC_GROUPED_INSTANTIATE_TN(GK_LINEAR);
+VEDIC_GROUPED_INSTANTIATE_TN(GK_BETA);
 
 hipError_t launch_grouped_f16_tn(const GroupedArgs& a, int kind, bool /*f16out*/, hipStream_t s) {
     if (kind == GK_BETA) return launch_grouped_tiles<2, GK_BETA, float>(a, s);

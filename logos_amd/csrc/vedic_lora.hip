@@ -24,12 +24,12 @@ __global__ void __launch_bounds__(256) lora_shrink_kernel(LoraArgs a) {
     q.offsets = a.offsets;
     q.groups = a.groups;
     q.R = a.n;
-    group_index<256>(q, ix, kLoraRows);
+    group_index(q, ix, kLoraRows);
     const int lane = threadIdx.x & 63, t = blockIdx.x;
     if (t >= ix.pre[a.groups]) return;
     const int g = group_of(ix, a.groups, t, lane);
-    const int p0 = ix.off[g] + (t - ix.pre[g]) * kLoraRows;
-    const int np = min(kLoraRows, ix.off[g + 1] - p0);
+    const int b0 = (t - ix.pre[g]) * kLoraRows, p0 = group_start(q, g) + b0;
+    const int np = min(kLoraRows, group_count(q, g) - b0);
     const T* A = static_cast<const T*>(a.A) + (int64_t)g * a.K * a.r;
     const T* X = static_cast<const T*>(a.X);
     const T* x[kLoraRows];
@@ -72,13 +72,13 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
     q.offsets = a.offsets;
     q.groups = a.groups;
     q.R = a.n;
-    group_index<256>(q, ix, kLoraRows);
+    group_index(q, ix, kLoraRows);
     const int strips = (a.N + 255) / 256;
     const int lane = threadIdx.x & 63, t = blockIdx.x / strips;
     if (t >= ix.pre[a.groups]) return;
     const int g = group_of(ix, a.groups, t, lane);
-    const int p0 = ix.off[g] + (t - ix.pre[g]) * kLoraRows;
-    const int np = min(kLoraRows, ix.off[g + 1] - p0);
+    const int b0 = (t - ix.pre[g]) * kLoraRows, p0 = group_start(q, g) + b0;
+    const int np = min(kLoraRows, group_count(q, g) - b0);
     for (int o = threadIdx.x; o < kLoraRows * a.r; o += 256) {
         const int i = o / a.r;
         h[i][o % a.r] = i < np ? a.H[(int64_t)(p0 + i) * a.r + o % a.r] : 0.0f;
@@ -148,13 +148,13 @@ __global__ void __launch_bounds__(512) lora_shrink_f16_kernel(LoraArgs a) {
     q.offsets = a.offsets;
     q.groups = a.groups;
     q.R = a.n;
-    group_index<512>(q, ix, 16);
+    group_index(q, ix, 16);
     const int tid = threadIdx.x, lane = tid & 63, t = blockIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (t >= ix.pre[a.groups]) return;
     const int g = group_of(ix, a.groups, t, lane);
-    const int p0 = __builtin_amdgcn_readfirstlane(ix.off[g]) + (t - __builtin_amdgcn_readfirstlane(ix.pre[g])) * 16;
-    const int np = min(16, __builtin_amdgcn_readfirstlane(ix.off[g + 1]) - p0);
+    const int b0 = (t - __builtin_amdgcn_readfirstlane(ix.pre[g])) * 16, p0 = group_start(q, g) + b0;
+    const int np = min(16, group_count(q, g) - b0);
     // this lane's row of X and the wave's range of K, whole stages
     const int row = (lane & 15) < np ? a.rows[p0 + (lane & 15)] : -1;
     const bool ok = (unsigned)row < (unsigned)a.M;
@@ -273,14 +273,14 @@ __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
     q.offsets = a.offsets;
     q.groups = a.groups;
     q.R = a.n;
-    group_index<256>(q, ix, 16);
+    group_index(q, ix, 16);
     const int strips = (a.N + 255) / 256;
     const int tid = threadIdx.x, lane = tid & 63, t = blockIdx.x / strips;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (t >= ix.pre[a.groups]) return;
     const int g = group_of(ix, a.groups, t, lane);
-    const int p0 = __builtin_amdgcn_readfirstlane(ix.off[g]) + (t - __builtin_amdgcn_readfirstlane(ix.pre[g])) * 16;
-    const int np = min(16, __builtin_amdgcn_readfirstlane(ix.off[g + 1]) - p0);
+    const int b0 = (t - __builtin_amdgcn_readfirstlane(ix.pre[g])) * 16, p0 = group_start(q, g) + b0;
+    const int np = min(16, group_count(q, g) - b0);
     const int n0 = (blockIdx.x - t * strips) * 256;
     const _Float16* B = static_cast<const _Float16*>(a.B) + (int64_t)g * a.r * a.N + n0;
     const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(B);

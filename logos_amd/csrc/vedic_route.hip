@@ -2,11 +2,13 @@
 // token's E logits, their softmax weights, and the tokens sorted by expert; and
 // the logits' gradient.
 //
-// Choice.  One wave per token, lane l holding logits EPL l .. EPL l + EPL - 1 as
-// unsigned keys in the order of the values.  A pick is the largest key of the
-// wave (six DPP steps), the lowest lane that has it and that lane's lowest place:
-// the lowest expert among equals, without comparing indexes.  The weights are
-// exp(x_j - x_max) over their sum, in fp32.
+// Choice.  16 lanes per token, four tokens a wave (64 lanes, one token, past 256
+// experts or 16 choices), lane l of a token holding logits EPL l .. EPL l + EPL - 1
+// as unsigned keys in the order of the values.  A pick is the largest key of the
+// token's lanes (one v_max_u32 with DPP per halving), the lowest lane that has it and
+// that lane's lowest place: the lowest expert among equals, without comparing
+// indexes.  The weights are exp(x_j - x_max) over their sum, in fp32.  Instructions
+// bound it: with a wave per token 8192 tokens of 128 experts, 8 chosen, took 66 us.
 //
 // Sorting is a stable counting sort by expert in two launches: the choice leaves
 // each workgroup's counts per expert, and the placement adds the counts of the
@@ -20,20 +22,36 @@ namespace vedic {
 
 namespace {
 
-// Largest value of the wave, in every lane (v_max_u32 with DPP; identity 0).
+// v_max_u32 with DPP (identity 0).
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
     const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true);
     return v > o ? v : o;
 }
+// Largest value of the lane's 16 lanes, in every lane of them: rotations by 8, 4, 2, 1.
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    v = dpp_max<0x128, 0xF>(v);
+    v = dpp_max<0x124, 0xF>(v);
+    v = dpp_max<0x122, 0xF>(v);
+    return dpp_max<0x121, 0xF>(v);
+}
+// Largest value of the wave, in every lane.
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-    v = dpp_max<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
-    v = dpp_max<0x112, 0xF>(v);
-    v = dpp_max<0x114, 0xF>(v);
-    v = dpp_max<0x118, 0xF>(v);
+    v = row_max(v);
     v = dpp_max<0x142, 0xA>(v);  // row_bcast 15, 31: the last lane has all
     v = dpp_max<0x143, 0xC>(v);
     return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+template <int LPT>
+__device__ __forceinline__ uint32_t token_max(uint32_t v) {
+    if constexpr (LPT == 16) return row_max(v);
+    else return wave_max(v);
+}
+template <int LPT>
+__device__ __forceinline__ float token_sum(float v) {
+#pragma unroll
+    for (int d = LPT / 2; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    return v;
 }
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -53,27 +71,28 @@ __device__ __forceinline__ float value_of(uint32_t key) {  // of a chosen one
     return __builtin_bit_cast(float, key >> 31 ? key == 0xFFFFFFFFu ? key : key & 0x7FFFFFFFu : ~key);
 }
 
-// One token by one wave: lane j < k gets the j-th choice (id -1 and weight 0 where
-// fewer than k logits are above -infinity).
-template <int EPL>
-__device__ __forceinline__ void choose(const float* x, int E, int k, bool renorm, int lane, int& id, float& w) {
+// One token by LPT lanes, `l` of them this one: lane j < k gets the j-th choice (id -1
+// and weight 0 where fewer than k logits are above -infinity).  All lanes of a wave
+// take k picks; x may be null for lanes without a token.
+template <int LPT, int EPL>
+__device__ __forceinline__ void choose(const float* x, int E, int k, bool renorm, int l, int& id, float& w) {
     uint32_t key[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-        const int e = lane * EPL + i;
-        key[i] = e < E ? key_of(x[e]) : 0u;
+        const int e = l * EPL + i;
+        key[i] = x != nullptr && e < E ? key_of(x[e]) : 0u;
     }
     uint32_t top = 0;  // this lane's largest
 #pragma unroll
     for (int i = 0; i < EPL; ++i) top = top > key[i] ? top : key[i];
-    uint32_t first = 0;
-    float total = 0.0f, mine = 0.0f;
+    uint32_t first = 0, mine = 0;
+    float total = 0.0f;
     id = -1;
     for (int j = 0; j < k; ++j) {
-        const uint32_t m = wave_max(top);
+        const uint32_t m = token_max<LPT>(top);
         if (j == 0) {
             first = m;
-            if (!renorm && m != 0) {
+            if (!renorm) {
                 // the softmax over all experts: summed before the keys are spent
                 const float x0 = value_of(m);
 #pragma unroll
@@ -81,27 +100,36 @@ __device__ __forceinline__ void choose(const float* x, int E, int k, bool renorm
                     if (key[i] != 0) total += expf(value_of(key[i]) - x0);
             }
         }
-        if (m == 0) break;
-        const int from = __ffsll((unsigned long long)__ballot(top == m)) - 1;
+        // the lowest of the token's lanes that holds it (none left: m is 0, and every
+        // lane's top is)
+        const unsigned long long hold = __ballot(top == m);
+        const int shift = LPT == 16 ? (threadIdx.x & 48) : 0;
+        const unsigned long long mask = LPT == 16 ? (hold >> shift) & 0xFFFFull : hold;
+        const int from = __ffsll(mask) - 1;
+        const bool winner = l == from && m != 0;
         int place = 0;
 #pragma unroll
         for (int i = EPL - 1; i >= 0; --i) place = key[i] == m ? i : place;
-        const int e = __builtin_amdgcn_readlane(place, from) + from * EPL;
-        if (lane == j) {
-            id = e;
-            mine = value_of(m);
+        // (expert + 1 of the winner in every lane of the token; 0: none)
+        const uint32_t e = token_max<LPT>(winner ? (uint32_t)(l * EPL + place + 1) : 0u);
+        if (l == j) {
+            id = (int)e - 1;
+            mine = m;
         }
-        if (lane == from) {
-            top = 0;
+        if (EPL == 1) {
+            top = winner ? 0u : top;
+        } else {
+            uint32_t t = 0;
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
-                if (i == place) key[i] = 0;
-                top = top > key[i] ? top : key[i];
+                key[i] = winner && i == place ? 0u : key[i];
+                t = t > key[i] ? t : key[i];
             }
+            top = t;
         }
     }
-    const float ex = id >= 0 ? expf(mine - value_of(first)) : 0.0f;
-    total = wave_sum(renorm ? ex : total);
+    const float ex = id >= 0 ? expf(value_of(mine) - value_of(first)) : 0.0f;
+    total = token_sum<LPT>(renorm ? ex : total);
     w = id >= 0 ? ex / total : 0.0f;
 }
 
@@ -179,7 +207,7 @@ __device__ __forceinline__ void place(PlaceLds& l, const int* ids, int p0, int p
         if (there) {
             for (int v = 0; v < wave; ++v) at += l.wave[v][bin];
             at += l.base[bin];
-            rows[at] = bin < groups ? p / per_row : -1;
+            rows[at] = p / per_row;
             if (slots) slots[p] = bin < groups ? at : -1;
         }
         if (q + kPlaceThreads < p1) {
@@ -196,37 +224,39 @@ __device__ __forceinline__ void place(PlaceLds& l, const int* ids, int p0, int p
 
 // Tokens [t0, t1) of this workgroup: choices, weights, and the counts per expert
 // in cnt (LDS).
-template <int EPL>
+template <int LPT, int EPL>
 __device__ __forceinline__ void choose_tokens(const RouteArgs& a, int t0, int t1, int nwaves, int* cnt) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    for (int t = t0 + wave; t < t1; t += nwaves) {
+    constexpr int TPW = 64 / LPT;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & (LPT - 1);
+    for (int tw = t0 + wave * TPW; tw < t1; tw += nwaves * TPW) {
+        const int t = tw + (threadIdx.x & 63) / LPT;
         int id;
         float w;
-        choose<EPL>(a.logits + (int64_t)t * a.ld, a.E, a.k, a.renorm, lane, id, w);
-        if (lane < a.k) {
-            a.ids[(int64_t)t * a.k + lane] = id;
-            a.weights[(int64_t)t * a.k + lane] = w;
+        choose<LPT, EPL>(t < t1 ? a.logits + (int64_t)t * a.ld : nullptr, a.E, a.k, a.renorm, l, id, w);
+        if (t < t1 && l < a.k) {
+            a.ids[(int64_t)t * a.k + l] = id;
+            a.weights[(int64_t)t * a.k + l] = w;
             if (cnt) atomicAdd(&cnt[bin_of(id, a.E)], 1);  // (an integer count: any order)
         }
     }
 }
 
-template <int EPL>
+template <int LPT, int EPL>
 __global__ void __launch_bounds__(256) route_choose_kernel(RouteArgs a) {
     __shared__ int cnt[kMaxGroups + 1];
     for (int e = threadIdx.x; e <= a.E; e += 256) cnt[e] = 0;
     __syncthreads();
-    const int t0 = blockIdx.x * a.chunk;
-    choose_tokens<EPL>(a, t0, min(a.T, t0 + a.chunk), 4, cnt);
+    const int t0 = blockIdx.x * a.tokens;
+    choose_tokens<LPT, EPL>(a, t0, min(a.T, t0 + a.tokens), 4, cnt);
     __syncthreads();
     for (int e = threadIdx.x; e <= a.E; e += 256) a.counts[(int64_t)blockIdx.x * (a.E + 1) + e] = cnt[e];
 }
 
 // Few tokens: choice and placement by one workgroup.
-template <int EPL>
+template <int LPT, int EPL>
 __global__ void __launch_bounds__(kPlaceThreads) route_small_kernel(RouteArgs a) {
     __shared__ PlaceLds l;
-    choose_tokens<EPL>(a, 0, a.T, kPlaceWaves, nullptr);
+    choose_tokens<LPT, EPL>(a, 0, a.T, kPlaceWaves, nullptr);
     __threadfence_block();
     __syncthreads();
     place<true>(l, a.ids, 0, a.T * a.k, a.k, a.E, a.bits, a.offsets, a.rows, a.slots);
@@ -244,21 +274,30 @@ __global__ void __launch_bounds__(256) group_count_kernel(const int* ids, int n,
     for (int e = threadIdx.x; e <= groups; e += 256) counts[(int64_t)blockIdx.x * (groups + 1) + e] = cnt[e];
 }
 
-// Placement of chunk blockIdx.x; counts [gridDim.x][groups + 1].
+// Placement of chunk blockIdx.x; counts [rows][groups + 1], `per` rows a chunk.
+// Thread t sums bin t mod bins of every (1024 / bins)-th row of counts, in registers;
+// the rest is added in LDS (integers: any order).
 __global__ void __launch_bounds__(kPlaceThreads) group_place_kernel(const int* ids, int n, int per_row, int groups, int bits,
-                                                                     int chunk, const int* counts, int* offsets, int* rows,
-                                                                     int* slots) {
+                                                                     int chunk, const int* counts, int nrow, int per,
+                                                                     int* offsets, int* rows, int* slots) {
     __shared__ PlaceLds l;
-    const int tid = threadIdx.x, bins = groups + 1;
+    const int tid = threadIdx.x, bins = groups + 1, me = blockIdx.x;
     for (int b = tid; b < bins; b += kPlaceThreads) l.base[b] = l.before[b] = 0;
     __syncthreads();
-    const int nb = gridDim.x, me = blockIdx.x;
-    const int64_t cells = (int64_t)nb * bins;
-    for (int64_t i = tid; i < cells; i += kPlaceThreads) {
-        const int c = counts[i], b = (int)(i % bins);
-        if (c != 0) {
-            atomicAdd(&l.base[b], c);
-            if (i / bins < me) atomicAdd(&l.before[b], c);
+    const int lanes = bins < kPlaceThreads ? kPlaceThreads / bins : 1;  // rows at a time
+    for (int b0 = 0; b0 < bins; b0 += kPlaceThreads) {  // (more bins than threads: 1025)
+        const int b = b0 + tid % bins, r0 = tid / bins;
+        if (b < bins && r0 < lanes) {
+            int all = 0, mine = 0;
+            const int* c = counts + b;
+#pragma unroll 8
+            for (int r = r0; r < nrow; r += lanes) {
+                const int v = c[(int64_t)r * bins];
+                all += v;
+                mine += r < me * per ? v : 0;
+            }
+            if (all) atomicAdd(&l.base[b], all);
+            if (mine) atomicAdd(&l.before[b], mine);
         }
     }
     __syncthreads();
@@ -336,19 +375,34 @@ int bits_for(int bins) {
     return b;
 }
 
-// Pairs per workgroup of the placement: whole tokens, 1024 or the multiple of it
-// that keeps the workgroups, whose counts each of them reads, to about 128.
-int chunk_tokens(int64_t T, int k) {
-    const int64_t pairs = T * k;
-    const int64_t per = 1024 * ((pairs + 128 * 1024 - 1) / (128 * 1024));
-    const int64_t t = per / k;
-    return (int)(t < 1 ? 1 : t);
+// Entries per workgroup of the placement: 1024, or the multiple of it that keeps the
+// workgroups, which read each others' counts, to about 128.
+int64_t place_chunk(int64_t n) { return 1024 * ((n + 128 * 1024 - 1) / (128 * 1024)); }
+
+// Tokens per workgroup of the choice: 16 a pass (4 with a wave per token), for about
+// 512 workgroups, and whole rows of counts per chunk of the placement.
+struct RoutePlan {
+    int tokens, per;  // tokens a workgroup, workgroups a chunk
+    int64_t blocks, chunks;
+    bool wide;  // a wave per token
+};
+RoutePlan route_plan(int64_t T, int E, int k) {
+    RoutePlan p;
+    p.wide = E > 256 || k > 16;
+    const int pass = p.wide ? 4 : 16;
+    const int64_t t = T > 512 ? (T + 511) / 512 : 1;
+    p.tokens = (int)((t + pass - 1) / pass * pass);
+    const int64_t want = place_chunk(T * k) / k;  // tokens a chunk
+    p.per = (int)(want > p.tokens ? want / p.tokens : 1);
+    p.blocks = (T + p.tokens - 1) / p.tokens;
+    p.chunks = (p.blocks + p.per - 1) / p.per;
+    return p;
 }
 
-template <int EPL>
-hipError_t launch_route(const RouteArgs& a, bool small, int blocks, hipStream_t s) {
-    if (small) hipLaunchKernelGGL((route_small_kernel<EPL>), dim3(1), dim3(kPlaceThreads), 0, s, a);
-    else hipLaunchKernelGGL((route_choose_kernel<EPL>), dim3(blocks), dim3(256), 0, s, a);
+template <int LPT, int EPL>
+hipError_t launch_route(const RouteArgs& a, bool small, int64_t blocks, hipStream_t s) {
+    if (small) hipLaunchKernelGGL((route_small_kernel<LPT, EPL>), dim3(1), dim3(kPlaceThreads), 0, s, a);
+    else hipLaunchKernelGGL((route_choose_kernel<LPT, EPL>), dim3((unsigned)blocks), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
@@ -361,29 +415,34 @@ static bool route_small(int64_t T, int k) { return T <= kRouteSmall && T * k <= 
 
 size_t route_count_bytes(int64_t T, int E, int k) {
     if (route_small(T, k)) return 0;
-    const int64_t c = chunk_tokens(T, k);
-    return sizeof(int) * (size_t)((T + c - 1) / c) * (E + 1);
+    return sizeof(int) * (size_t)route_plan(T, E, k).blocks * (E + 1);
 }
 
 hipError_t launch_route_topk(RouteArgs a, hipStream_t s) {
     const bool small = route_small(a.T, a.k);
+    const RoutePlan p = route_plan(a.T, a.E, a.k);
     a.bits = bits_for(a.E + 1);
-    a.chunk = chunk_tokens(a.T, a.k);
-    const int blocks = (a.T + a.chunk - 1) / a.chunk;
-    hipError_t e = a.E <= 64    ? launch_route<1>(a, small, blocks, s)
-                   : a.E <= 128 ? launch_route<2>(a, small, blocks, s)
-                   : a.E <= 256 ? launch_route<4>(a, small, blocks, s)
-                   : a.E <= 512 ? launch_route<8>(a, small, blocks, s)
-                                : launch_route<16>(a, small, blocks, s);
+    a.tokens = p.tokens;
+    hipError_t e;
+    if (p.wide)
+        e = a.E <= 64    ? launch_route<64, 1>(a, small, p.blocks, s)
+            : a.E <= 256 ? launch_route<64, 4>(a, small, p.blocks, s)
+                         : launch_route<64, 16>(a, small, p.blocks, s);
+    else
+        e = a.E <= 16    ? launch_route<16, 1>(a, small, p.blocks, s)
+            : a.E <= 32  ? launch_route<16, 2>(a, small, p.blocks, s)
+            : a.E <= 64  ? launch_route<16, 4>(a, small, p.blocks, s)
+            : a.E <= 128 ? launch_route<16, 8>(a, small, p.blocks, s)
+                         : launch_route<16, 16>(a, small, p.blocks, s);
     if (e != hipSuccess || small) return e;
-    hipLaunchKernelGGL(group_place_kernel, dim3(blocks), dim3(kPlaceThreads), 0, s, a.ids, a.T * a.k, a.k, a.E, a.bits,
-                       a.chunk * a.k, a.counts, a.offsets, a.rows, a.slots);
+    hipLaunchKernelGGL(group_place_kernel, dim3((unsigned)p.chunks), dim3(kPlaceThreads), 0, s, a.ids, a.T * a.k, a.k, a.E,
+                       a.bits, p.tokens * p.per * a.k, a.counts, (int)p.blocks, p.per, a.offsets, a.rows, a.slots);
     return hipGetLastError();
 }
 
 size_t group_count_bytes(int64_t n, int groups) {
     if (n <= kPlaceThreads) return 0;
-    const int64_t c = chunk_tokens(n, 1);
+    const int64_t c = place_chunk(n);
     return sizeof(int) * (size_t)((n + c - 1) / c) * (groups + 1);
 }
 
@@ -395,12 +454,12 @@ hipError_t launch_group_rows(const int* ids, int n, int per_row, int groups, int
                            rows, slots);
         return hipGetLastError();
     }
-    const int chunk = chunk_tokens(n, 1), blocks = (n + chunk - 1) / chunk;
-    hipLaunchKernelGGL(group_count_kernel, dim3(blocks), dim3(256), 0, s, ids, n, groups, chunk, counts);
+    const int64_t chunk = place_chunk(n), blocks = (n + chunk - 1) / chunk;
+    hipLaunchKernelGGL(group_count_kernel, dim3((unsigned)blocks), dim3(256), 0, s, ids, n, groups, (int)chunk, counts);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(group_place_kernel, dim3(blocks), dim3(kPlaceThreads), 0, s, ids, n, per_row, groups, bits, chunk,
-                       counts, offsets, rows, slots);
+    hipLaunchKernelGGL(group_place_kernel, dim3((unsigned)blocks), dim3(kPlaceThreads), 0, s, ids, n, per_row, groups, bits,
+                       (int)chunk, counts, (int)blocks, 1, offsets, rows, slots);
     return hipGetLastError();
 }
 

@@ -21,7 +21,7 @@ struct RouteArgs {
     int* rows;       // [T k]
     int* slots;      // [T x k]
     int* counts;     // route_count_bytes() of workspace
-    int bits, chunk; // set by the launch
+    int bits, tokens;  // set by the launch
 };
 
 size_t route_count_bytes(int64_t T, int E, int k);

@@ -760,7 +760,8 @@ def route_topk_bwd(logits: torch.Tensor, ids: torch.Tensor, weights: torch.Tenso
 
 def group_rows(ids: torch.Tensor, groups: int, per_row: int = 1) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(offsets, rows, slots) of the plan that sorts the int32 `ids` by group, stable: rows[place] = entry // per_row.
-    An id outside 0 .. groups - 1 belongs to no group (slot -1)."""
+    An id outside 0 .. groups - 1 belongs to no group (slot -1); its row comes
+    behind offsets[groups]."""
     dev = _device()
     p = _ints(ids, "ids", tuple(ids.shape), dev)
     n, d = ids.numel(), ids.device

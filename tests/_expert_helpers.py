@@ -41,12 +41,12 @@ def weights(logits, ids, renorm):
 
 
 def plan(ids, groups, per_row):
-    """(offsets, rows, slots), stable; ids outside belong to no group."""
+    """(offsets, rows, slots), stable; ids outside belong to no group, their rows come last."""
     flat = ids.reshape(-1)
     key = np.where((flat >= 0) & (flat < groups), flat, groups)
     order = np.argsort(key, kind="stable")
     offsets = np.array([(key < g).sum() for g in range(groups + 1)], np.int32)
-    rows = np.where(key[order] < groups, order // per_row, -1).astype(np.int32)
+    rows = (order // per_row).astype(np.int32)
     slots = np.empty_like(order)
     slots[order] = np.arange(order.size)
     slots = np.where(key < groups, slots, -1).astype(np.int32).reshape(ids.shape)

@@ -157,8 +157,14 @@ def test_tn(case, dt, listed):
                    terms=np.abs(dot[i]) + np.abs(c0[i]))
         check_rows(db0[i].double().cpu().numpy(), dy[seg[i]].sum(0) + b0[i], np.abs(dy[seg[i]]).sum(0), n, F32, f"db beta {i}",
                    terms=np.abs(dy[seg[i]].sum(0)) + np.abs(b0[i]))
+    # alone: another fixed order of the same n terms, which the same bound of n u sum |dY| holds for
     alone = v.bias_grad_grouped(dY, ints(off))
-    assert torch.equal(alone, db)
+    for i in range(G):
+        check_rows(alone[i].double().cpu().numpy(), dy[seg[i]].sum(0), np.abs(dy[seg[i]]).sum(0), max(1, sizes[i]), F32,
+                   f"db alone {i}")
+    assert torch.equal(alone, v.bias_grad_grouped(dY, ints(off)))
+    db2 = torch.empty_like(db)
+    assert torch.equal(dW, v.gemm_grouped(v.OP_TN, X, dY, ints(off), rows=rl, db=db2)) and torch.equal(db, db2)
 
 
 @pytest.mark.parametrize("dt", [F16, F32])
