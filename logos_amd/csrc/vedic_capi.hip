@@ -28,9 +28,9 @@ namespace vedic {
 hipError_t launch_grouped_f16_nn(const GroupedArgs& a, int kind, bool f16out, hipStream_t s);
 hipError_t launch_grouped_f16_nt(const GroupedArgs& a, int kind, bool f16out, hipStream_t s);
 hipError_t launch_grouped_f16_tn(const GroupedArgs& a, int kind, bool f16out, hipStream_t s);
-hipError_t launch_grouped_any_nn(const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s);
-hipError_t launch_grouped_any_nt(const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s);
-hipError_t launch_grouped_any_tn(const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s);
+hipError_t launch_grouped_any_nn(const GroupedArgs& a, int kind, bool f16, bool f16out, hipStream_t s);
+hipError_t launch_grouped_any_nt(const GroupedArgs& a, int kind, bool f16, bool f16out, hipStream_t s);
+hipError_t launch_grouped_any_tn(const GroupedArgs& a, int kind, bool f16, bool f16out, hipStream_t s);
 hipError_t launch_layernorm_f32(const float* X, const float* gamma, const float* beta, float* Y, void* Y16, int seq,
                                 int d, float eps, hipStream_t s);
 hipError_t launch_layernorm_f16(const void* X16, const float* gamma, const float* beta, void* Y16, int seq, int d,
@@ -1230,14 +1230,15 @@ extern "C" int vedic_group_rows(const int* ids, int n, int per_row, int groups, 
     return hip_status(e != hipSuccess ? e : f);
 }
 
+// vec: binary16 operands whose rows 16-byte loads can take.
 static hipError_t launch_grouped(int op, const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s) {
-    if (f16 && vec)
+    if (vec)
         return op == VEDIC_OP_NN   ? launch_grouped_f16_nn(a, kind, f16out, s)
                : op == VEDIC_OP_NT ? launch_grouped_f16_nt(a, kind, f16out, s)
                                    : launch_grouped_f16_tn(a, kind, f16out, s);
-    return op == VEDIC_OP_NN   ? launch_grouped_any_nn(a, kind, f16, f16out, vec, s)
-           : op == VEDIC_OP_NT ? launch_grouped_any_nt(a, kind, f16, f16out, vec, s)
-                               : launch_grouped_any_tn(a, kind, f16, f16out, vec, s);
+    return op == VEDIC_OP_NN   ? launch_grouped_any_nn(a, kind, f16, f16out, s)
+           : op == VEDIC_OP_NT ? launch_grouped_any_nt(a, kind, f16, f16out, s)
+                               : launch_grouped_any_tn(a, kind, f16, f16out, s);
 }
 
 extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
@@ -1300,20 +1301,18 @@ extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
     a.K = d->K;
     a.beta = d->beta;
     if (tn && d->beta != 0.0f) kind = GK_BETA;
-    const int es = f16 ? 2 : 4, per16 = 16 / es;
+    const int es = f16 ? 2 : 4;
     a.db = d->db;
     a.db_beta = d->db_beta;
     auto vec_of = [&]() {
-        bool vec = aligned16(a.A) && a.lda % per16 == 0;
-        if (f16 || d->op == VEDIC_OP_NT) vec = vec && aligned16(a.B) && a.ldb % per16 == 0 && a.stride_b % per16 == 0;
-        return vec && a_cols % per16 == 0 && ((!f16 && d->op == VEDIC_OP_NN) || b_cols % per16 == 0);
+        return f16 && aligned16(a.A) && aligned16(a.B) && ((a.lda | a.ldb | a.stride_b) & 7) == 0 && ((a_cols | b_cols) & 7) == 0;
     };
     bool vec = vec_of();
     // The rows of a list are copied into a workspace first where the kernels
     // cannot follow it: past 32-bit offsets, and along the contraction (TN) but for
     // the 16-byte binary16 kernels.
     void* copy = nullptr;
-    if (a.rows && ((tn && !(f16 && vec)) || (int64_t)d->a_rows * d->lda * es >= (int64_t(1) << 31))) {
+    if (a.rows && ((tn && !vec) || (int64_t)d->a_rows * d->lda * es >= (int64_t(1) << 31))) {
         const int64_t ldn = ((int64_t)a_cols + 7) / 8 * 8;
         hipError_t e = ws.get(&copy, (size_t)R * ldn * es);
         if (e == hipSuccess)
@@ -1326,7 +1325,7 @@ extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
     }
     hipError_t e = launch_grouped(d->op, a, kind, f16, f16out, vec, ws.s);
     // (the 16-byte binary16 kernels sum the columns on the way)
-    if (e == hipSuccess && d->db && !(f16 && vec))
+    if (e == hipSuccess && d->db && !vec)
         e = launch_group_colsum(d->B, f16, d->ldb, R, N, d->offsets, d->groups, d->db_beta, d->db, ws.s);
     const hipError_t f = ws.put(copy);
     return hip_status(e != hipSuccess ? e : f);

@@ -22,14 +22,18 @@ __device__ __forceinline__ float ld_value(__amdgpu_buffer_rsrc_t rs, uint32_t of
 }
 
 // One operand's staging (SideSplit with a value type and a row list): R rows of
-// the tile, NT threads.
-template <typename T, bool KC, bool VEC, int R, int NT>
+// the tile, NT threads.  Contraction contiguous (KC): fp32, eight steps of one row per
+// thread by two 16-byte loads, which need no more than the values' own 4-byte
+// alignment (whole fours of steps: the caller adds the last three or fewer); binary16 in pairs of steps,
+// value by value, as it may lie at any 2 bytes.  Otherwise eight values down one
+// column, coalesced across the lanes.
+template <typename T, bool KC, int R, int NT>
 struct SideAny {
-    static constexpr bool PAIRS = KC && !VEC;
+    static constexpr int ES = sizeof(T);
+    static constexpr bool PAIRS = KC && ES == 2;
     static constexpr int UNITS = PAIRS ? R * 8 : R * 2;
     static constexpr int U = UNITS / NT;
     static constexpr int PER = PAIRS ? 2 : 8;
-    static constexpr int ES = sizeof(T);
     static_assert(UNITS % NT == 0, "units divide among the threads");
     uint32_t off[U];
     int k0[U];
@@ -68,20 +72,14 @@ struct SideAny {
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
                 const_cast<T*>(KC || steps <= k0[i] ? base : base + (int64_t)k0[i] * ld), 0,
                 steps > (KC ? 0 : k0[i]) ? 0x7FFFFFFF : 0, 0x00020000);
-            if constexpr (KC && VEC) {
-                constexpr int Q = 16 / ES;  // values per 16-byte load
+            if constexpr (KC && !PAIRS) {
 #pragma unroll
-                for (int q = 0; q < 8; q += Q) {
+                for (int q = 0; q < 8; q += 4) {
                     const uint32_t o = k0[i] + q < steps ? off[i] : kOob;
-                    const u32x4_t w = __builtin_bit_cast(
-                        u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(o == kOob ? kOob : o + q * ES), 0, 0));
-                    if constexpr (ES == 4) {
+                    const float4_t w = __builtin_bit_cast(
+                        float4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(o == kOob ? kOob : o + q * ES), 0, 0));
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[i][q + e] = __builtin_bit_cast(float4_t, w)[e];
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[i][q + e] = (float)__builtin_bit_cast(half8_t, w)[e];
-                    }
+                    for (int e = 0; e < 4; ++e) v[i][q + e] = w[e];
                 }
             } else if constexpr (KC) {
 #pragma unroll
@@ -117,27 +115,24 @@ struct SideAny {
     }
 };
 
-// A wave's block on v_mfma_f32_32x32x2_f32 from the operands themselves: for
-// blocks whose split sums are not finite and for one or two steps.  pa, pb: this
-// lane's row and column (lane half h takes step 2 q + h), ka, kb the distance of
-// two steps' elements; a row that is not there has ok = false and counts as zeros.
+// acc += a wave's block over steps kb .. K - 1 on v_mfma_f32_32x32x2_f32 from the
+// operands themselves: for blocks whose split sums are not finite, for one or two
+// steps, and for the steps behind the last four.  pa, pb: this lane's row and column
+// (lane half h takes step kb + 2 q + h), ka, kb_ the distance of two steps' elements; a
+// row that is not there has oka = false and counts as zeros.
 template <typename T, int MI, int NI>
 __device__ __forceinline__ void any_block_slow(const T* const (&pa)[MI], const bool (&oka)[MI], int64_t ka,
-                                               const T* const (&pb)[NI], int64_t kb, int K, int h,
+                                               const T* const (&pb)[NI], int64_t kb_, int kb, int K, int h,
                                                float16_t (&acc)[MI][NI]) {
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = float16_t{};
 #pragma unroll 1
-    for (int k = h; k < K + h; k += 2) {
+    for (int k = kb + h; k < K + h; k += 2) {
         const bool in = k < K;
         const int64_t q = in ? k : K - 1;
         float x[MI], y[NI];
 #pragma unroll
         for (int i = 0; i < MI; ++i) x[i] = in && oka[i] ? (float)pa[i][q * ka] : 0.0f;
 #pragma unroll
-        for (int j = 0; j < NI; ++j) y[j] = in ? (float)pb[j][q * kb] : 0.0f;
+        for (int j = 0; j < NI; ++j) y[j] = in ? (float)pb[j][q * kb_] : 0.0f;
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -148,16 +143,25 @@ __device__ __forceinline__ void any_block_slow(const T* const (&pa)[MI], const b
 // One BM x BN tile per workgroup.  NN / NT: work item w is column tile w mod
 // tiles_n of row tile w / tiles_n (row tiles counted through the groups).  TN: w
 // is tile w mod (tiles_m tiles_n) of group w / (tiles_m tiles_n).
-template <int OP, typename T, typename OT, bool VEC, int BM, int BN, int WGM, int WGN, int KIND>
-__global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs a) {
+//
+// WGK > 1: that many groups of WGM x WGN waves, each with LDS buffers of its own and
+// a part of the contraction (whole stages); the others leave their sums in LDS for the
+// first, which adds them in order and runs the epilogue.
+template <int OP, typename T, typename OT, int BM, int BN, int WGM, int WGN, int WGK, int KIND>
+__global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(GroupedArgs a) {
     constexpr int NT = WGM * WGN * 64, WM = BM / WGM, WN = BN / WGN, MI = WM / 32, NI = WN / 32;
     constexpr bool A_KC = OP != 2, B_KC = OP == 1;
     constexpr int BYTES = (BM + BN) * kSplitRowBytes;
-    __shared__ __attribute__((aligned(1024))) char buf0[BYTES];
-    __shared__ __attribute__((aligned(1024))) char buf1[BYTES];
+    // VALU instructions placed after each MFMA: the split's 7 per element
+    constexpr int VPM = (7 * (BM + BN) * kSplitK / NT + kSplitProducts * MI * NI - 1) / (kSplitProducts * MI * NI);
+    __shared__ __attribute__((aligned(1024))) char all0[WGK * BYTES];
+    __shared__ __attribute__((aligned(1024))) char all1[WGK * BYTES];
     __shared__ __attribute__((aligned(16))) float sbias[BN];
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x % NT;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int wk = WGK > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
+    char* const buf0 = all0 + wk * BYTES;
+    char* const buf1 = all1 + wk * BYTES;
     const int wm = wave / WGN, wn = wave % WGN;
 
     int e, m0, n0, K, left, start, count;  // left: rows of C from m0 on
@@ -172,7 +176,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs 
         K = count;
         left = a.M - m0;
     } else {
-        GroupIndex& ix = *reinterpret_cast<GroupIndex*>(buf0);
+        GroupIndex& ix = *reinterpret_cast<GroupIndex*>(all0);
         static_assert(BN <= NT && sizeof(GroupIndex) <= BYTES, "the index fits a stage buffer");
         group_index(a, ix, BM);
         const int t = blockIdx.x / a.tiles_n;
@@ -187,7 +191,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs 
         __syncthreads();  // the index's LDS becomes a stage buffer
     }
     // (read after the barriers of the stages or the one before the epilogue)
-    if (tid < BN) sbias[tid] = a.bias != nullptr && n0 + tid < a.N ? a.bias[(int64_t)e * a.N + n0 + tid] : 0.0f;
+    if (wk == 0 && tid < BN) sbias[tid] = a.bias != nullptr && n0 + tid < a.N ? a.bias[(int64_t)e * a.N + n0 + tid] : 0.0f;
     const T* A = static_cast<const T*>(a.A);
     const int* list = nullptr;
     if constexpr (OP == 2) {
@@ -202,8 +206,8 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs 
     else B += (int64_t)e * a.stride_b + (B_KC ? (int64_t)n0 * a.ldb : n0);
     const int64_t ka = A_KC ? 1 : a.lda, kb = B_KC ? 1 : a.ldb;
 
-    using SA = SideAny<T, A_KC, VEC, BM, NT>;
-    using SB = SideAny<T, B_KC, VEC, BN, NT>;
+    using SA = SideAny<T, A_KC, BM, NT>;
+    using SB = SideAny<T, B_KC, BN, NT>;
     SA sa;
     SB sb;
     sa.init(tid, a.lda, left, list, a.a_rows);
@@ -211,10 +215,14 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs 
     typename SA::Values va;
     typename SB::Values vb;
     const bool few = K < kSplitMinK;
-    const int nk = few ? 0 : (K + kSplitK - 1) / kSplitK;
+    // (fp32 rows are loaded four steps at a time: the last K mod 4 come at the end)
+    const int Kq = OP != 2 && sizeof(T) == 4 ? K & ~3 : K;
+    const int nk_all = few ? 0 : (Kq + kSplitK - 1) / kSplitK;
+    const int nk = (nk_all + WGK - 1) / WGK, kt0 = wk * nk;  // stages of this wave group, the first of them
     auto load = [&](int kt) {
-        const int64_t k = kt < nk ? (int64_t)kt * kSplitK : 0;
-        const int steps = kt < nk ? min(kSplitK, K - kt * kSplitK) : 0;
+        const bool in = kt < nk && kt0 + kt < nk_all;
+        const int64_t k = in ? (int64_t)(kt0 + kt) * kSplitK : 0;
+        const int steps = in ? min(kSplitK, Kq - (kt0 + kt) * kSplitK) : 0;
         sa.load(va, A + k * ka, a.lda, steps);
         sb.load(vb, B + k * kb, a.ldb, steps);
     };
@@ -243,17 +251,60 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs 
                 for (int j = 0; j < NI; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i].p[kSplitA[q]], fb[j].p[kSplitB[q]],
                                                                         acc[i][j], 0, 0, 0);
-        __syncthreads();
+        // the fragment reads, then a few VALU instructions of the split (and an LDS
+        // write once there is one) after every MFMA
+        __builtin_amdgcn_sched_group_barrier(0x100, 3 * (MI + NI), 0);
+#pragma unroll
+        for (int x = 0; x < kSplitProducts * MI * NI; ++x) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, VPM, 0);
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        stage_barrier();  // (not a fence: stage kt + 2's loads stay in flight)
     };
     if (nk > 0) {
         load(0);
         commit(buf0);
         load(1);
-        __syncthreads();
+        stage_barrier();
         for (int kt = 0; kt < nk; kt += 2) {  // (a stage past the last is zeros)
             stage(buf0, buf1, kt);
             stage(buf1, buf0, kt + 1);
         }
+    }
+    if constexpr (WGK > 1) {
+        // partial (group, i) of a wave: 32 x WN sums
+        constexpr int PIECE = WGM * WGN * 32 * WN * 4, PER = WGK * BYTES / PIECE;
+        static_assert((WGK - 1) * MI <= 2 * PER, "the partial sums fit the buffers");
+        auto piece = [&](int p) {
+            return reinterpret_cast<float4_t*>((p < PER ? all0 : all1) + (p % PER) * PIECE + wave * (32 * WN * 4));
+        };
+        __syncthreads();
+        if (wk > 0) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        piece((wk - 1) * MI + i)[(j * 4 + q) * 64 + lane] =
+                            float4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        }
+        __syncthreads();
+        if (wk > 0) return;
+#pragma unroll
+        for (int g = 0; g < WGK - 1; ++g)
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float4_t v = piece(g * MI + i)[(j * 4 + q) * 64 + lane];
+#pragma unroll
+                        for (int e2 = 0; e2 < 4; ++e2) acc[i][j][4 * q + e2] += v[e2];
+                    }
     }
     float probe = 0.0f;
 #pragma unroll
@@ -263,7 +314,8 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs 
             acc[i][j] *= kSplitUnscale2;
             probe = nonfinite_probe(acc[i][j], probe);
         }
-    if (few || __any(probe != 0.0f)) {
+    const bool again = few || __any(probe != 0.0f);
+    if (again || Kq < K) {
         const T* pa[MI];
         const T* pb[NI];
         bool oka[MI];
@@ -284,13 +336,19 @@ __global__ void __launch_bounds__(WGM* WGN * 64) grouped_any_kernel(GroupedArgs 
             const int n = min(wn * WN + 32 * j + (lane & 31), a.N - n0 - 1);
             pb[j] = B_KC ? B + (int64_t)n * a.ldb : B + n;
         }
-        any_block_slow<T, MI, NI>(pa, oka, ka, pb, kb, K, lane >> 5, acc);
+        if (again) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = float16_t{};
+        }
+        any_block_slow<T, MI, NI>(pa, oka, ka, pb, kb, again ? 0 : Kq, K, lane >> 5, acc);
     }
     const int row0 = m0 + wm * WM;
     const int64_t crow = OP == 2 ? row0 : start + row0;
     OT* C = static_cast<OT*>(a.C) + (OP == 2 ? (int64_t)e * a.stride_c : 0) + crow * a.ldc;
     OT* P = a.P != nullptr ? static_cast<OT*>(a.P) + crow * a.ldp : nullptr;
-    __syncthreads();
+    if constexpr (WGK == 1) __syncthreads();  // the bias (the sums' barriers have shown it otherwise)
     if (grouped_reads(KIND) && a.wide)
         grouped_epilogue<KIND, OT, true, true, MI, NI>(C, a.ldc, P, a.ldp, sbias + wn * WN, a.beta, acc, left - wm * WM, a.N,
                                                        n0 + wn * WN, lane);
@@ -305,6 +363,7 @@ struct CfgAMid {  // 128 x 128, four waves of 64 x 64
 struct CfgASmall {  // 64 x 64, two waves of 32 x 64
     static constexpr int BM = 64, BN = 64, WGM = 2, WGN = 1;
 };
+constexpr int kAnyGroups = 3;  // wave groups of a workgroup where few tiles share the CUs
 
 // Row tiles that R rows in `groups` groups can have at most, and about have.
 inline int64_t grouped_row_tiles_max(int R, int groups, int bm) {
@@ -314,7 +373,7 @@ inline double grouped_row_tiles(int R, int groups, int bm) {
     return (double)R / bm + 0.5 * (groups < R ? groups : R);
 }
 
-template <int OP, typename T, typename OT, bool VEC, class Cfg, int KIND>
+template <int OP, typename T, typename OT, class Cfg, int WGK, int KIND>
 static hipError_t launch_any(GroupedArgs a, hipStream_t s) {
     a.tiles_n = (a.N + Cfg::BN - 1) / Cfg::BN;
     a.tiles_m = OP == 2 ? (a.M + Cfg::BM - 1) / Cfg::BM : 0;
@@ -323,31 +382,42 @@ static hipError_t launch_any(GroupedArgs a, hipStream_t s) {
                                  : grouped_row_tiles_max(a.R, a.groups, Cfg::BM) * a.tiles_n;
     if (work > 0x7FFFFFFF) return hipErrorInvalidValue;  // (the caller has refused such sizes)
     if (work == 0) return hipSuccess;
-    hipLaunchKernelGGL((grouped_any_kernel<OP, T, OT, VEC, Cfg::BM, Cfg::BN, Cfg::WGM, Cfg::WGN, KIND>), dim3((unsigned)work),
-                       dim3(Cfg::WGM * Cfg::WGN * 64), 0, s, a);
+    hipLaunchKernelGGL((grouped_any_kernel<OP, T, OT, Cfg::BM, Cfg::BN, Cfg::WGM, Cfg::WGN, WGK, KIND>),
+                       dim3((unsigned)work), dim3(Cfg::WGM * Cfg::WGN * WGK * 64), 0, s, a);
     return hipGetLastError();
 }
 
-// 64 x 64 tiles where 128 x 128 ones would leave half the CUs without one.
-template <int OP, typename T, typename OT, bool VEC, int KIND>
+// 64 x 64 tiles where 128 x 128 ones would leave half the CUs without one.  Three wave
+// groups where a CU gets no more than one 128 x 128 tile, and with the small ones, for
+// contractions long enough to share (us, one group / three: 2006 rows in 7 groups of
+// 2000 into 1000, 156 tiles, NN 103 / 79, NT 101 / 74; the same TN, 896 tiles of 286 steps,
+// 63 / 73; 16 rows of 1024 into 4096 in 8 groups 55 / 45; 300 rows of 512 into 777 24 / 17).
+template <int OP, typename T, typename OT, int KIND>
 static hipError_t launch_any_tiles(const GroupedArgs& a, hipStream_t s) {
-    const double rows = OP == 2 ? (double)a.groups * ((a.M + 127) / 128) : grouped_row_tiles(a.R, a.groups, 128);
-    if (rows * ((a.N + 127) / 128) * 2 > device_cu_count()) return launch_any<OP, T, OT, VEC, CfgAMid, KIND>(a, s);
-    return launch_any<OP, T, OT, VEC, CfgASmall, KIND>(a, s);
+    auto tiles = [&](int b) {
+        return (OP == 2 ? (double)a.groups * ((a.M + b - 1) / b) : grouped_row_tiles(a.R, a.groups, b)) * ((a.N + b - 1) / b);
+    };
+    const int cus = device_cu_count();
+    const bool split = (OP == 2 ? a.R / a.groups : a.K) >= 256;
+    if (tiles(128) * 2 > cus) {
+        if (split && tiles(128) <= cus) return launch_any<OP, T, OT, CfgAMid, kAnyGroups, KIND>(a, s);
+        return launch_any<OP, T, OT, CfgAMid, 1, KIND>(a, s);
+    }
+    if (split) return launch_any<OP, T, OT, CfgASmall, kAnyGroups, KIND>(a, s);
+    return launch_any<OP, T, OT, CfgASmall, 1, KIND>(a, s);
 }
 
-// vec: rows that 16-byte loads can take (fp32 only; binary16 operands that have
-// them run on the kernels of vedic_grouped_f16.hpp).
 template <int OP, int KIND>
-static hipError_t launch_any_kind(const GroupedArgs& a, bool f16, bool f16out, bool vec, hipStream_t s) {
-    if (f16) {
-        if constexpr (OP != 2)
-            if (f16out) return launch_any_tiles<OP, _Float16, _Float16, false, KIND>(a, s);
-        return launch_any_tiles<OP, _Float16, float, false, KIND>(a, s);
-    }
+static hipError_t launch_any_kind(const GroupedArgs& a, bool f16, bool f16out, hipStream_t s) {
     if constexpr (OP != 2)
-        if (vec) return launch_any_tiles<OP, float, float, true, KIND>(a, s);
-    return launch_any_tiles<OP, float, float, false, KIND>(a, s);
+        if (f16out) return launch_any_tiles<OP, _Float16, _Float16, KIND>(a, s);
+    return f16 ? launch_any_tiles<OP, _Float16, float, KIND>(a, s) : launch_any_tiles<OP, float, float, KIND>(a, s);
 }
+
+#define VEDIC_ANY_KERNELS(OP, T, OT, KIND)                                                               \
+    template __global__ void grouped_any_kernel<OP, T, OT, 128, 128, 2, 2, 1, KIND>(GroupedArgs);          \
+    template __global__ void grouped_any_kernel<OP, T, OT, 128, 128, 2, 2, kAnyGroups, KIND>(GroupedArgs); \
+    template __global__ void grouped_any_kernel<OP, T, OT, 64, 64, 2, 1, 1, KIND>(GroupedArgs);            \
+    template __global__ void grouped_any_kernel<OP, T, OT, 64, 64, 2, 1, kAnyGroups, KIND>(GroupedArgs)
 
 }  // namespace vedic

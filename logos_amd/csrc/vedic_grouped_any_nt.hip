@@ -3,26 +3,16 @@
 
 namespace vedic {
 
-template __global__ void grouped_any_kernel<1, float, float, false, 128, 128, 2, 2, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, float, float, false, 64, 64, 2, 1, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, _Float16, float, false, 128, 128, 2, 2, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, _Float16, float, false, 64, 64, 2, 1, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, float, float, true, 128, 128, 2, 2, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, float, float, true, 64, 64, 2, 1, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, _Float16, _Float16, false, 128, 128, 2, 2, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, _Float16, _Float16, false, 64, 64, 2, 1, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, float, float, false, 128, 128, 2, 2, GK_GELU_BWD>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, float, float, false, 64, 64, 2, 1, GK_GELU_BWD>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, _Float16, float, false, 128, 128, 2, 2, GK_GELU_BWD>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, _Float16, float, false, 64, 64, 2, 1, GK_GELU_BWD>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, float, float, true, 128, 128, 2, 2, GK_GELU_BWD>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, float, float, true, 64, 64, 2, 1, GK_GELU_BWD>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, _Float16, _Float16, false, 128, 128, 2, 2, GK_GELU_BWD>(GroupedArgs);
-template __global__ void grouped_any_kernel<1, _Float16, _Float16, false, 64, 64, 2, 1, GK_GELU_BWD>(GroupedArgs);
+VEDIC_ANY_KERNELS(1, float, float, GK_LINEAR);
+VEDIC_ANY_KERNELS(1, _Float16, float, GK_LINEAR);
+VEDIC_ANY_KERNELS(1, _Float16, _Float16, GK_LINEAR);
+VEDIC_ANY_KERNELS(1, float, float, GK_GELU_BWD);
+VEDIC_ANY_KERNELS(1, _Float16, float, GK_GELU_BWD);
+VEDIC_ANY_KERNELS(1, _Float16, _Float16, GK_GELU_BWD);
 
-hipError_t launch_grouped_any_nt(const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s) {
-    if (kind == GK_GELU_BWD) return launch_any_kind<1, GK_GELU_BWD>(a, f16, f16out, vec, s);
-    return launch_any_kind<1, GK_LINEAR>(a, f16, f16out, vec, s);
+hipError_t launch_grouped_any_nt(const GroupedArgs& a, int kind, bool f16, bool f16out, hipStream_t s) {
+    if (kind == GK_GELU_BWD) return launch_any_kind<1, GK_GELU_BWD>(a, f16, f16out, s);
+    return launch_any_kind<1, GK_LINEAR>(a, f16, f16out, s);
 }
 
 }  // namespace vedic

@@ -3,18 +3,14 @@
 
 namespace vedic {
 
-template __global__ void grouped_any_kernel<2, float, float, false, 128, 128, 2, 2, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<2, float, float, false, 64, 64, 2, 1, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<2, _Float16, float, false, 128, 128, 2, 2, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<2, _Float16, float, false, 64, 64, 2, 1, GK_LINEAR>(GroupedArgs);
-template __global__ void grouped_any_kernel<2, float, float, false, 128, 128, 2, 2, GK_BETA>(GroupedArgs);
-template __global__ void grouped_any_kernel<2, float, float, false, 64, 64, 2, 1, GK_BETA>(GroupedArgs);
-template __global__ void grouped_any_kernel<2, _Float16, float, false, 128, 128, 2, 2, GK_BETA>(GroupedArgs);
-template __global__ void grouped_any_kernel<2, _Float16, float, false, 64, 64, 2, 1, GK_BETA>(GroupedArgs);
+VEDIC_ANY_KERNELS(2, float, float, GK_LINEAR);
+VEDIC_ANY_KERNELS(2, _Float16, float, GK_LINEAR);
+VEDIC_ANY_KERNELS(2, float, float, GK_BETA);
+VEDIC_ANY_KERNELS(2, _Float16, float, GK_BETA);
 
-hipError_t launch_grouped_any_tn(const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s) {
-    if (kind == GK_BETA) return launch_any_kind<2, GK_BETA>(a, f16, f16out, vec, s);
-    return launch_any_kind<2, GK_LINEAR>(a, f16, f16out, vec, s);
+hipError_t launch_grouped_any_tn(const GroupedArgs& a, int kind, bool f16, bool f16out, hipStream_t s) {
+    if (kind == GK_BETA) return launch_any_kind<2, GK_BETA>(a, f16, f16out, s);
+    return launch_any_kind<2, GK_LINEAR>(a, f16, f16out, s);
 }
 
 }  // namespace vedic

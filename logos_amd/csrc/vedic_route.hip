@@ -75,12 +75,24 @@ __device__ __forceinline__ float value_of(uint32_t key) {  // of a chosen one
 // and weight 0 where fewer than k logits are above -infinity).  All lanes of a wave
 // take k picks; x may be null for lanes without a token.
 template <int LPT, int EPL>
-__device__ __forceinline__ void choose(const float* x, int E, int k, bool renorm, int l, int& id, float& w) {
+__device__ __forceinline__ void choose(const float* x, int E, int k, bool renorm, bool wide, int l, int& id, float& w) {
     uint32_t key[EPL];
+    if (EPL >= 4 && wide) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-        const int e = l * EPL + i;
-        key[i] = x != nullptr && e < E ? key_of(x[e]) : 0u;
+        for (int i = 0; i < EPL; i += 4) {
+            const int e = l * EPL + i;
+            const bool in = x != nullptr && e < E;
+            float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (in) v = *reinterpret_cast<const float4_t*>(x + e);
+#pragma unroll
+            for (int q = 0; q < 4 && q < EPL; ++q) key[i + q] = in ? key_of(v[q]) : 0u;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+            const int e = l * EPL + i;
+            key[i] = x != nullptr && e < E ? key_of(x[e]) : 0u;
+        }
     }
     uint32_t top = 0;  // this lane's largest
 #pragma unroll
@@ -133,6 +145,10 @@ __device__ __forceinline__ void choose(const float* x, int E, int k, bool renorm
     w = id >= 0 ? ex / total : 0.0f;
 }
 
+// Distance of two workgroups' counts: groups + 1 of them, whole 16-byte accesses.
+__host__ __device__ inline int count_pitch(int groups) { return (groups + 4) / 4 * 4; }
+
+constexpr int kChooseThreads = 512;
 constexpr int kPlaceThreads = 1024, kPlaceWaves = kPlaceThreads / 64;
 
 // Where pairs go.  base[bin]: the next free position of each bin (bin `groups`:
@@ -232,7 +248,7 @@ __device__ __forceinline__ void choose_tokens(const RouteArgs& a, int t0, int t1
         const int t = tw + (threadIdx.x & 63) / LPT;
         int id;
         float w;
-        choose<LPT, EPL>(t < t1 ? a.logits + (int64_t)t * a.ld : nullptr, a.E, a.k, a.renorm, l, id, w);
+        choose<LPT, EPL>(t < t1 ? a.logits + (int64_t)t * a.ld : nullptr, a.E, a.k, a.renorm, a.wide, l, id, w);
         if (t < t1 && l < a.k) {
             a.ids[(int64_t)t * a.k + l] = id;
             a.weights[(int64_t)t * a.k + l] = w;
@@ -242,14 +258,14 @@ __device__ __forceinline__ void choose_tokens(const RouteArgs& a, int t0, int t1
 }
 
 template <int LPT, int EPL>
-__global__ void __launch_bounds__(256) route_choose_kernel(RouteArgs a) {
+__global__ void __launch_bounds__(kChooseThreads) route_choose_kernel(RouteArgs a) {
     __shared__ int cnt[kMaxGroups + 1];
-    for (int e = threadIdx.x; e <= a.E; e += 256) cnt[e] = 0;
+    for (int e = threadIdx.x; e <= a.E; e += kChooseThreads) cnt[e] = 0;
     __syncthreads();
     const int t0 = blockIdx.x * a.tokens;
-    choose_tokens<LPT, EPL>(a, t0, min(a.T, t0 + a.tokens), 4, cnt);
+    choose_tokens<LPT, EPL>(a, t0, min(a.T, t0 + a.tokens), kChooseThreads / 64, cnt);
     __syncthreads();
-    for (int e = threadIdx.x; e <= a.E; e += 256) a.counts[(int64_t)blockIdx.x * (a.E + 1) + e] = cnt[e];
+    for (int e = threadIdx.x; e <= a.E; e += kChooseThreads) a.counts[(int64_t)blockIdx.x * count_pitch(a.E) + e] = cnt[e];
 }
 
 // Few tokens: choice and placement by one workgroup.
@@ -271,34 +287,37 @@ __global__ void __launch_bounds__(256) group_count_kernel(const int* ids, int n,
     const int64_t p1 = min((int64_t)n, p0 + chunk);
     for (int64_t p = p0 + threadIdx.x; p < p1; p += 256) atomicAdd(&cnt[bin_of(ids[p], groups)], 1);
     __syncthreads();
-    for (int e = threadIdx.x; e <= groups; e += 256) counts[(int64_t)blockIdx.x * (groups + 1) + e] = cnt[e];
+    for (int e = threadIdx.x; e <= groups; e += 256) counts[(int64_t)blockIdx.x * count_pitch(groups) + e] = cnt[e];
 }
 
-// Placement of chunk blockIdx.x; counts [rows][groups + 1], `per` rows a chunk.
-// Thread t sums bin t mod bins of every (1024 / bins)-th row of counts, in registers;
-// the rest is added in LDS (integers: any order).
+// Placement of chunk blockIdx.x; counts [nrow][count_pitch], `per` rows a chunk.
+// Thread t sums four bins of every (1024 / quads)-th row of counts, in registers; the
+// rest is added in LDS (integers: any order).
 __global__ void __launch_bounds__(kPlaceThreads) group_place_kernel(const int* ids, int n, int per_row, int groups, int bits,
                                                                      int chunk, const int* counts, int nrow, int per,
                                                                      int* offsets, int* rows, int* slots) {
     __shared__ PlaceLds l;
     const int tid = threadIdx.x, bins = groups + 1, me = blockIdx.x;
+    typedef int int4_t __attribute__((ext_vector_type(4)));
+    const int quads = count_pitch(groups) / 4, lanes = kPlaceThreads / quads, q = tid % quads, r0 = tid / quads;
+    int4_t all = {0, 0, 0, 0}, mine = {0, 0, 0, 0};
+    if (r0 < lanes) {
+#pragma unroll 8
+        for (int r = r0; r < nrow; r += lanes) {
+            const int4_t v = reinterpret_cast<const int4_t*>(counts)[(int64_t)r * quads + q];
+            all += v;
+            if (r < me * per) mine += v;
+        }
+    }
     for (int b = tid; b < bins; b += kPlaceThreads) l.base[b] = l.before[b] = 0;
     __syncthreads();
-    const int lanes = bins < kPlaceThreads ? kPlaceThreads / bins : 1;  // rows at a time
-    for (int b0 = 0; b0 < bins; b0 += kPlaceThreads) {  // (more bins than threads: 1025)
-        const int b = b0 + tid % bins, r0 = tid / bins;
-        if (b < bins && r0 < lanes) {
-            int all = 0, mine = 0;
-            const int* c = counts + b;
-#pragma unroll 8
-            for (int r = r0; r < nrow; r += lanes) {
-                const int v = c[(int64_t)r * bins];
-                all += v;
-                mine += r < me * per ? v : 0;
+    if (r0 < lanes) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (4 * q + e < bins) {
+                if (all[e]) atomicAdd(&l.base[4 * q + e], all[e]);
+                if (mine[e]) atomicAdd(&l.before[4 * q + e], mine[e]);
             }
-            if (all) atomicAdd(&l.base[b], all);
-            if (mine) atomicAdd(&l.before[b], mine);
-        }
     }
     __syncthreads();
     scan_base(l, bins);
@@ -379,7 +398,7 @@ int bits_for(int bins) {
 // workgroups, which read each others' counts, to about 128.
 int64_t place_chunk(int64_t n) { return 1024 * ((n + 128 * 1024 - 1) / (128 * 1024)); }
 
-// Tokens per workgroup of the choice: 16 a pass (4 with a wave per token), for about
+// Tokens per workgroup of the choice: 32 a pass (8 with a wave per token), at most
 // 512 workgroups, and whole rows of counts per chunk of the placement.
 struct RoutePlan {
     int tokens, per;  // tokens a workgroup, workgroups a chunk
@@ -389,7 +408,7 @@ struct RoutePlan {
 RoutePlan route_plan(int64_t T, int E, int k) {
     RoutePlan p;
     p.wide = E > 256 || k > 16;
-    const int pass = p.wide ? 4 : 16;
+    const int pass = kChooseThreads / (p.wide ? 64 : 16);
     const int64_t t = T > 512 ? (T + 511) / 512 : 1;
     p.tokens = (int)((t + pass - 1) / pass * pass);
     const int64_t want = place_chunk(T * k) / k;  // tokens a chunk
@@ -402,7 +421,7 @@ RoutePlan route_plan(int64_t T, int E, int k) {
 template <int LPT, int EPL>
 hipError_t launch_route(const RouteArgs& a, bool small, int64_t blocks, hipStream_t s) {
     if (small) hipLaunchKernelGGL((route_small_kernel<LPT, EPL>), dim3(1), dim3(kPlaceThreads), 0, s, a);
-    else hipLaunchKernelGGL((route_choose_kernel<LPT, EPL>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((route_choose_kernel<LPT, EPL>), dim3((unsigned)blocks), dim3(kChooseThreads), 0, s, a);
     return hipGetLastError();
 }
 
@@ -415,13 +434,14 @@ static bool route_small(int64_t T, int k) { return T <= kRouteSmall && T * k <= 
 
 size_t route_count_bytes(int64_t T, int E, int k) {
     if (route_small(T, k)) return 0;
-    return sizeof(int) * (size_t)route_plan(T, E, k).blocks * (E + 1);
+    return sizeof(int) * (size_t)route_plan(T, E, k).blocks * count_pitch(E);
 }
 
 hipError_t launch_route_topk(RouteArgs a, hipStream_t s) {
     const bool small = route_small(a.T, a.k);
     const RoutePlan p = route_plan(a.T, a.E, a.k);
     a.bits = bits_for(a.E + 1);
+    a.wide = a.E % 4 == 0 && a.ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
     a.tokens = p.tokens;
     hipError_t e;
     if (p.wide)
@@ -443,7 +463,7 @@ hipError_t launch_route_topk(RouteArgs a, hipStream_t s) {
 size_t group_count_bytes(int64_t n, int groups) {
     if (n <= kPlaceThreads) return 0;
     const int64_t c = place_chunk(n);
-    return sizeof(int) * (size_t)((n + c - 1) / c) * (groups + 1);
+    return sizeof(int) * (size_t)((n + c - 1) / c) * count_pitch(groups);
 }
 
 hipError_t launch_group_rows(const int* ids, int n, int per_row, int groups, int* counts, int* offsets, int* rows, int* slots,

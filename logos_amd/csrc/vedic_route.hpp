@@ -22,6 +22,7 @@ struct RouteArgs {
     int* slots;      // [T x k]
     int* counts;     // route_count_bytes() of workspace
     int bits, tokens;  // set by the launch
+    bool wide;         // 16-byte loads of the logits
 };
 
 size_t route_count_bytes(int64_t T, int E, int k);
