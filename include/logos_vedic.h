@@ -590,6 +590,12 @@ int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, const void* A, 
                    const int* offsets, const int* rows, int n, const float* scales, float* C, int64_t ldc, int K, int N,
                    void* stream);
 
+/* The shared projection with them: vedic_gemm(base), then vedic_lora_add of base->A
+ * onto base->C.  base: op NN, F32 or F16 in, F32 out, epilogue NONE or BIAS, no preact
+ * or colsum. */
+int vedic_gemm_lora(const vedic_gemm_desc_t* base, const void* A, const void* B, int groups, int r, const int* offsets,
+                    const int* rows, int n, const float* scales);
+
 /* ---- test hooks --------------------------------------------------------- */
 
 /* Off by default.  When on, every GEMM with column sums allocates its

@@ -172,6 +172,8 @@ SIGNATURES = {
         c_int,
         [c_vp, c_int, c_i64, c_int, c_vp, c_vp, c_int, c_int, c_vp, c_vp, c_int, c_vp, c_vp, c_i64, c_int, c_int, c_vp],
     ),
+    "vedic_gemm_lora": (
+        c_int, [ctypes.POINTER(GemmDesc), c_vp, c_vp, c_int, c_int, c_vp, c_vp, c_int, c_vp]),
     "vedic_debug_set_workspace_guard": (None, [c_int]),
     "vedic_debug_workspace_guard_hits": (ctypes.c_long, []),
     "vedic_uses_vendor_blas": (c_int, []),

@@ -39,6 +39,7 @@ SOURCES = [
     "vedic_grouped_f16_nn.hip",
     "vedic_grouped_f16_nt.hip",
     "vedic_grouped_f16_tn.hip",
+    "vedic_grouped_skinny.hip",
     "vedic_grouped_any_nn.hip",
     "vedic_grouped_any_nt.hip",
     "vedic_grouped_any_tn.hip",

@@ -28,6 +28,7 @@ namespace vedic {
 hipError_t launch_grouped_f16_nn(const GroupedArgs& a, int kind, bool f16out, hipStream_t s);
 hipError_t launch_grouped_f16_nt(const GroupedArgs& a, int kind, bool f16out, hipStream_t s);
 hipError_t launch_grouped_f16_tn(const GroupedArgs& a, int kind, bool f16out, hipStream_t s);
+hipError_t launch_grouped_f16_skinny(int op, const GroupedArgs& a, int kind, bool f16out, hipStream_t s);
 hipError_t launch_grouped_any_nn(const GroupedArgs& a, int kind, bool f16, bool f16out, hipStream_t s);
 hipError_t launch_grouped_any_nt(const GroupedArgs& a, int kind, bool f16, bool f16out, hipStream_t s);
 hipError_t launch_grouped_any_tn(const GroupedArgs& a, int kind, bool f16, bool f16out, hipStream_t s);
@@ -1232,6 +1233,10 @@ extern "C" int vedic_group_rows(const int* ids, int n, int per_row, int groups, 
 
 // vec: binary16 operands whose rows 16-byte loads can take.
 static hipError_t launch_grouped(int op, const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s) {
+    // At most eight rows a group (us, tiles / few-row kernel, 8 groups: NN 1024 into 4096, 8
+    // rows 16.2 / 12.2, 32 rows 20.0 / 18.7, 64 rows 19.6 / 19.4, 128 rows 20.0 / 27.0; 4096
+    // into 1024, 64 rows 39.0 / 27.6; NT 4096 into 1024, 64 rows 38.6 / 15.5).
+    if (vec && op != VEDIC_OP_TN && a.R <= 8 * a.groups) return launch_grouped_f16_skinny(op, a, kind, f16out, s);
     if (vec)
         return op == VEDIC_OP_NN   ? launch_grouped_f16_nn(a, kind, f16out, s)
                : op == VEDIC_OP_NT ? launch_grouped_f16_nt(a, kind, f16out, s)
@@ -1402,23 +1407,29 @@ extern "C" int vedic_combine_rows_bwd(const float* dout, int64_t ld_dout, const 
                                          static_cast<hipStream_t>(stream)));
 }
 
-extern "C" int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, const void* A, const void* B, int groups, int r,
-                              const int* offsets, const int* rows, int n, const float* scales, float* C, int64_t ldc, int K,
-                              int N, void* stream) {
+static int lora_checks(const void* X, int dtype, int64_t ldx, int M, const void* A, const void* B, int groups, int r,
+                       const int* offsets, const int* rows, int n, const float* C, int64_t ldc, int K, int N) {
     if (dtype != VEDIC_DT_F32 && dtype != VEDIC_DT_F16) return VEDIC_STATUS_BAD_DTYPE;
     if (M < 0 || n < 0 || groups <= 0 || r <= 0 || K <= 0 || N <= 0) return VEDIC_STATUS_BAD_DIM;
     if (r > kLoraMaxRank || groups > kMaxGroups || M >= kMaxCount || n >= kMaxCount / 128 || ldx >= kMaxLd || ldc >= kMaxLd ||
-        ((int64_t)n / 8 + groups) * ((N + 255) / 256) >= kMaxCount)
+        ((int64_t)n / 8 + groups) * ((N + 63) / 64) >= kMaxCount)
         return VEDIC_STATUS_TOO_LARGE;
     if (ldx < K || ldc < N) return VEDIC_STATUS_BAD_LD;
-    if (n == 0 || M == 0) return VEDIC_STATUS_OK;
-    if (!X || !A || !B || !offsets || !rows || !C) return VEDIC_STATUS_NULL_POINTER;
+    if (n > 0 && M > 0 && (!X || !A || !B || !offsets || !rows || !C)) return VEDIC_STATUS_NULL_POINTER;
+    return VEDIC_STATUS_OK;
+}
+
+extern "C" int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, const void* A, const void* B, int groups, int r,
+                              const int* offsets, const int* rows, int n, const float* scales, float* C, int64_t ldc, int K,
+                              int N, void* stream) {
+    const int st = lora_checks(X, dtype, ldx, M, A, B, groups, r, offsets, rows, n, C, ldc, K, N);
+    if (st != VEDIC_STATUS_OK || n == 0 || M == 0) return st;
     Workspace ws;
     ws.s = static_cast<hipStream_t>(stream);
     LoraArgs a{};
     const bool f16 = dtype == VEDIC_DT_F16;
     void* work = nullptr;
-    hipError_t e = ws.get(&work, lora_bytes(n, r, f16));
+    hipError_t e = ws.get(&work, lora_bytes(n, r, f16, M, ldx, K));
     if (e != hipSuccess) return hip_status(e);
     a.X = X;
     a.ldx = ldx;
@@ -1438,6 +1449,23 @@ extern "C" int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, cons
     e = launch_lora(a, f16, work, ws.s);
     const hipError_t f = ws.put(work);
     return hip_status(e != hipSuccess ? e : f);
+}
+
+extern "C" int vedic_gemm_lora(const vedic_gemm_desc_t* base, const void* A, const void* B, int groups, int r,
+                               const int* offsets, const int* rows, int n, const float* scales) {
+    if (!base) return VEDIC_STATUS_NULL_POINTER;
+    if (base->op != VEDIC_OP_NN) return VEDIC_STATUS_BAD_LAYOUT;
+    if (base->in_dtype == VEDIC_DT_F32_F16 || base->out_dtype != VEDIC_DT_F32) return VEDIC_STATUS_BAD_DTYPE;
+    if ((base->epilogue != VEDIC_EPI_NONE && base->epilogue != VEDIC_EPI_BIAS) || base->preact || base->colsum)
+        return VEDIC_STATUS_BAD_EPILOGUE;
+    // (the adapters' arguments first: a refused call leaves C as it was)
+    int st = lora_checks(base->A, base->in_dtype, base->lda, base->M, A, B, groups, r, offsets, rows, n,
+                         static_cast<float*>(base->C), base->ldc, base->K, base->N);
+    if (st != VEDIC_STATUS_OK) return st;
+    st = vedic_gemm(base);
+    if (st != VEDIC_STATUS_OK || n == 0) return st;
+    return vedic_lora_add(base->A, base->in_dtype, base->lda, base->M, A, B, groups, r, offsets, rows, n, scales,
+                          static_cast<float*>(base->C), base->ldc, base->K, base->N, base->stream);
 }
 
 // ----------------------------------------------------------- elementwise

@@ -30,6 +30,7 @@ enum GroupedKind : int {
     GK_GELU_P = 2,    // P = acc (+ b), C = gelu(P)
     GK_GELU_BWD = 3,  // C = acc * gelu'(P)
     GK_BETA = 4,      // C = acc + beta C
+    GK_ADD = 5,       // C[out_rows[i]] += scales[group] acc[i]   (fp32 adapters)
 };
 
 // Whether a kind reads P or the old C; the others add a bias.
@@ -49,6 +50,9 @@ struct GroupedArgs {
     int a_rows;  // rows of A
     int M, N, K; // NN / NT: N and K; TN: M and N
     float beta;
+    const int* out_rows;  // GK_ADD: [R] rows of C, out_limit of them there
+    int out_limit;
+    const float* scales;  // GK_ADD: [groups], or null
     float* db;  // TN: [groups x N] column sums of B, or null
     float db_beta;
     int tiles_m, tiles_n;
@@ -301,6 +305,29 @@ __device__ __forceinline__ void grouped_epilogue(void* C, int64_t ldc, void* P, 
             __builtin_amdgcn_sched_barrier(0);  // one block's offsets at a time
         }
     }
+}
+
+// GK_ADD: adds a (32 MI) x (32 NI) wave tile, times `scale`, to the rows of C that
+// `rows` lists (nrow of them; a row outside 0 .. limit - 1 takes nothing).
+template <int MI, int NI>
+__device__ __forceinline__ void grouped_add(float* C, int64_t ldc, const int* rows, int limit, float scale,
+                                            const float16_t (&acc)[MI][NI], int nrow, int N, int col0, int lane) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int u = 32 * i + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+            const int row = u < nrow ? rows[u] : -1;
+            if ((unsigned)row >= (unsigned)limit) continue;
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const int col = col0 + 32 * j + (lane & 31);
+                if (col < N) {
+                    float* c = C + (int64_t)row * ldc + col;
+                    *c = __builtin_fmaf(scale, acc[i][j][e], *c);
+                }
+            }
+        }
 }
 
 // Whether C and P allow the epilogue's wide accesses (strides in elements; every

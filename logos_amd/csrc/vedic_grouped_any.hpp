@@ -344,6 +344,11 @@ __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(Groupe
         }
         any_block_slow<T, MI, NI>(pa, oka, ka, pb, kb, again ? 0 : Kq, K, lane >> 5, acc);
     }
+    if constexpr (KIND == GK_ADD) {
+        grouped_add<MI, NI>(static_cast<float*>(a.C), a.ldc, a.out_rows + start + m0 + wm * WM, a.out_limit,
+                            a.scales ? a.scales[e] : 1.0f, acc, left - wm * WM, a.N, n0 + wn * WN, lane);
+        return;
+    }
     const int row0 = m0 + wm * WM;
     const int64_t crow = OP == 2 ? row0 : start + row0;
     OT* C = static_cast<OT*>(a.C) + (OP == 2 ? (int64_t)e * a.stride_c : 0) + crow * a.ldc;

@@ -2,7 +2,8 @@
 // i of adapter g (list position p, rows[p] = i),
 //   C[i] += scale[g] (X[i] . A_g) . B_g,   A_g [K x r], B_g [r x N].
 // Two launches, H = X A_g into a workspace (fp32, or the same as two binary16
-// values), then C.
+// values), then C.  fp32 operands take the grouped fp32 products for both.
+#include "vedic_combine.hpp"
 #include "vedic_common.hpp"
 #include "vedic_gemm_f16.hpp"
 #include "vedic_grouped.hpp"
@@ -10,14 +11,18 @@
 
 namespace vedic {
 
+hipError_t launch_grouped_any_nn(const GroupedArgs& a, int kind, bool f16, bool f16out, hipStream_t s);
+
 namespace {
+
+// ------------------------------------------------ binary16, any alignment
 
 constexpr int kLoraRows = 8;  // rows per workgroup of one adapter
 
 // H[p][0 .. r) of a tile of eight list positions: thread t takes rank t % RT of
 // the steps k = t / RT, t / RT + ST, ...
-template <typename T>
 __global__ void __launch_bounds__(256) lora_shrink_kernel(LoraArgs a) {
+    typedef _Float16 T;
     __shared__ GroupIndex ix;
     __shared__ float part[256][kLoraRows + 1];
     GroupedArgs q{};
@@ -64,8 +69,8 @@ __global__ void __launch_bounds__(256) lora_shrink_kernel(LoraArgs a) {
 }
 
 // C += scale H B_g: a tile of eight rows by 256 columns, one column a thread.
-template <typename T>
 __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
+    typedef _Float16 T;
     __shared__ GroupIndex ix;
     __shared__ float h[kLoraRows][kLoraMaxRank];
     GroupedArgs q{};
@@ -331,14 +336,58 @@ __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
         }
 }
 
-template <typename T>
 hipError_t launch_any(const LoraArgs& a, hipStream_t s) {
     const int64_t tiles = a.n / kLoraRows + (a.groups < a.n ? a.groups : a.n);
-    hipLaunchKernelGGL((lora_shrink_kernel<T>), dim3((unsigned)tiles), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(lora_shrink_kernel, dim3((unsigned)tiles), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((lora_expand_kernel<T>), dim3((unsigned)(tiles * ((a.N + 255) / 256))), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(lora_expand_kernel, dim3((unsigned)(tiles * ((a.N + 255) / 256))), dim3(256), 0, s, a);
     return hipGetLastError();
+}
+
+// fp32: two grouped products, the second adding to the listed rows of C.  (`copy`:
+// the listed rows, where X is past the products' 32-bit offsets.)
+bool copies_rows(int M, int64_t ldx, bool f16) { return !f16 && (int64_t)M * ldx * 4 >= (int64_t(1) << 31); }
+
+hipError_t launch_f32(const LoraArgs& a, float* copy, hipStream_t s) {
+    GroupedArgs q{};
+    q.A = a.X;
+    q.lda = a.ldx;
+    q.rows = a.rows;
+    q.a_rows = a.M;
+    if (copies_rows(a.M, a.ldx, false)) {
+        const hipError_t e = launch_gather_rows(a.X, a.ldx, a.M, a.rows, a.n, a.K, 4, copy, a.K, s);
+        if (e != hipSuccess) return e;
+        q.A = copy;
+        q.lda = a.K;
+        q.rows = nullptr;
+    }
+    q.B = a.A;
+    q.ldb = a.r;
+    q.stride_b = (int64_t)a.K * a.r;
+    q.C = a.H;
+    q.ldc = a.r;
+    q.offsets = a.offsets;
+    q.groups = a.groups;
+    q.R = a.n;
+    q.N = a.r;
+    q.K = a.K;
+    const hipError_t e = launch_grouped_any_nn(q, GK_LINEAR, false, false, s);
+    if (e != hipSuccess) return e;
+    q.A = a.H;
+    q.lda = a.r;
+    q.rows = nullptr;
+    q.B = a.B;
+    q.ldb = a.N;
+    q.stride_b = (int64_t)a.r * a.N;
+    q.C = a.C;
+    q.ldc = a.ldc;
+    q.N = a.N;
+    q.K = a.r;
+    q.out_rows = a.rows;
+    q.out_limit = a.M;
+    q.scales = a.scales;
+    return launch_grouped_any_nn(q, GK_ADD, false, false, s);
 }
 
 template <int RP, int KC>
@@ -362,16 +411,18 @@ bool vec16(const LoraArgs& a) {
 
 }  // namespace
 
-size_t lora_bytes(int n, int r, bool f16) {
+static size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+size_t lora_bytes(int n, int r, bool f16, int M, int64_t ldx, int K) {
     const size_t rs = (size_t)(r <= 32 ? 32 : r <= 64 ? 64 : 128);
-    // (fp32: n r values; binary16: hi and lo of rs each, and the factors)
-    return f16 ? (size_t)n * (rs * 4 + 4) : (size_t)n * r * 4;
+    // (fp32: n r values, and the copied rows; binary16: hi and lo of rs each, and the factors)
+    return f16 ? (size_t)n * (rs * 4 + 4) : rounded((size_t)n * r * 4) + (copies_rows(M, ldx, f16) ? (size_t)n * K * 4 : 0);
 }
 
 hipError_t launch_lora(LoraArgs a, bool f16, void* work, hipStream_t s) {
     a.H = static_cast<float*>(work);
-    if (!f16) return launch_any<float>(a, s);
-    if (!vec16(a)) return launch_any<_Float16>(a, s);
+    if (!f16) return launch_f32(a, reinterpret_cast<float*>(static_cast<char*>(work) + rounded((size_t)a.n * a.r * 4)), s);
+    if (!vec16(a)) return launch_any(a, s);
     const size_t rs = (size_t)(a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128);
     a.Hs = static_cast<_Float16*>(work);
     a.factor = reinterpret_cast<float*>(a.Hs + (size_t)a.n * 2 * rs);

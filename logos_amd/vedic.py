@@ -950,24 +950,28 @@ def lora_add(C: torch.Tensor, X: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     adapter g (a plan of group_rows).  X [M, K], A [G, K, r], B [G, r, N] all float16 or all float32, C float32 [M, N];
     r <= 128.  A row is listed at most once; others keep their content."""
     dev = _device(X)
+    px, M, K, ldx, pa, pb, N, G, r, n, po, pr, psc = _lora_args(X, A, B, offsets, rows, scales, dev)
+    pc, Mc, Nc, ldc = _rows2d(C, "C", torch.float32, dev)
+    if (Mc, Nc) != (M, N):
+        raise ValueError(f"C must be {M}x{N}, got {Mc}x{Nc}")
+    _check(_lib.load().vedic_lora_add(px, _DT[X.dtype], ldx, M, pa, pb, G, r, po, pr, n, psc, pc, ldc, K, N, _stream()))
+    return C
+
+
+def _lora_args(X, A, B, offsets, rows, scales, dev):
     dt = X.dtype
     if dt not in _DT:
         raise ValueError(f"X must be float16 or float32, got {dt}")
     px, M, K, ldx = _rows2d(X, "X", dt, dev)
     pa, pb = _on_current(A, "A", dt, dev), _on_current(B, "B", dt, dev)
-    pc, Mc, N, ldc = _rows2d(C, "C", torch.float32, dev)
     if A.dim() != 3 or not A.is_contiguous() or A.shape[1] != K:
         raise ValueError(f"A must be contiguous [G, {K}, r], got {tuple(A.shape)}")
     G, _, r = A.shape
-    if tuple(B.shape) != (G, r, N) or not B.is_contiguous():
-        raise ValueError(f"B must be contiguous [{G}, {r}, {N}], got {tuple(B.shape)}")
-    if Mc != M:
-        raise ValueError(f"C must have {M} rows, got {Mc}")
+    if B.dim() != 3 or B.shape[0] != G or B.shape[1] != r or not B.is_contiguous():
+        raise ValueError(f"B must be contiguous [{G}, {r}, N], got {tuple(B.shape)}")
     n = rows.numel()
-    po, pr = _offsets(offsets, G, dev), _ints(rows, "rows", (n,), dev)
     psc = None if scales is None else _floats(scales, "scales", (G,), dev)
-    _check(_lib.load().vedic_lora_add(px, _DT[dt], ldx, M, pa, pb, G, r, po, pr, n, psc, pc, ldc, K, N, _stream()))
-    return C
+    return px, M, K, ldx, pa, pb, B.shape[2], G, r, n, _offsets(offsets, G, dev), _ints(rows, "rows", (n,), dev), psc
 
 
 def gemm_lora(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor,
@@ -975,6 +979,19 @@ def gemm_lora(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Tensor
               out: torch.Tensor | None = None) -> torch.Tensor:
     """Y = X . W (+ bias), float32, with every listed row's adapter added (lora_add): one shared projection for the
     requests of a batch, each with low-rank weights of its own."""
-    _on_current(X, "X", W.dtype, _device(X))
-    Y = gemm(OP_NN, X, W, out, bias=bias, epilogue=EPI_BIAS if bias is not None else EPI_NONE)
-    return lora_add(Y, X, A, B, offsets, rows, scales)
+    dev = _device(X)
+    px, M, K, ldx, pa, pb, N, G, r, n, po, pr, psc = _lora_args(X, A, B, offsets, rows, scales, dev)
+    pw, Kw, Nw, ldw = _rows2d(W, "W", X.dtype, dev)
+    if (Kw, Nw) != (K, N):
+        raise ValueError(f"VedicGEMM: W must be {K}x{N}, got {Kw}x{Nw}")
+    if out is None:
+        out = X.new_empty((M, N), dtype=torch.float32)
+    pc, Mc, Nc, ldc = _rows2d(out, "out", torch.float32, dev)
+    if (Mc, Nc) != (M, N):
+        raise ValueError(f"out must be {M}x{N}")
+    pbias = None if bias is None else _floats(bias, "bias", (N,), dev)
+    dt = _DT[X.dtype]
+    d = _lib.GemmDesc(OP_NN, dt, DT_F32, M, N, K, px, ldx, pw, ldw, pc, ldc, 1.0, 0.0, pbias,
+                      EPI_NONE if bias is None else EPI_BIAS, None, 0, _stream(), None, 0.0)
+    _check(_lib.load().vedic_gemm_lora(ctypes.byref(d), pa, pb, G, r, po, pr, n, psc))
+    return out

@@ -129,6 +129,24 @@ def test_lora(args, status):
     assert _lib.load().vedic_lora_add(*args) == status
 
 
+@pytest.mark.parametrize("kw,args,status", [
+    (dict(op=1), (P, P, 2, 4, P, P, 4, None), _lib.STATUS_BAD_LAYOUT),
+    (dict(in_dtype=2), (P, P, 2, 4, P, P, 4, None), _lib.STATUS_BAD_DTYPE),
+    (dict(out_dtype=1), (P, P, 2, 4, P, P, 4, None), _lib.STATUS_BAD_DTYPE),
+    (dict(epilogue=2, bias=P), (P, P, 2, 4, P, P, 4, None), _lib.STATUS_BAD_EPILOGUE),
+    (dict(preact=P), (P, P, 2, 4, P, P, 4, None), _lib.STATUS_BAD_EPILOGUE),
+    (dict(), (P, P, 2, 129, P, P, 4, None), _lib.STATUS_TOO_LARGE),
+    (dict(), (None, P, 2, 4, P, P, 4, None), _lib.STATUS_NULL_POINTER),
+    (dict(epilogue=1), (P, P, 2, 4, P, P, 4, None), _lib.STATUS_BAD_EPILOGUE),  # the product's own refusal: no bias
+])
+def test_gemm_lora(kw, args, status):
+    d = dict(op=0, in_dtype=1, out_dtype=0, M=8, N=8, K=8, A=P, lda=8, B=P, ldb=8, C=P, ldc=8, alpha=1.0, beta=0.0,
+             bias=None, epilogue=0, preact=None, ld_preact=0, stream=None)
+    d.update(kw)
+    assert _lib.load().vedic_gemm_lora(ctypes.byref(_lib.GemmDesc(**d)), *args) == status
+    assert _lib.load().vedic_gemm_lora(None, *args) == _lib.STATUS_NULL_POINTER
+
+
 @pytest.mark.parametrize("args,status", [
     ((P, 2, 8, 4, 8, P, 2, 0.0, P, None), _lib.STATUS_BAD_DTYPE),
     ((P, 1, 7, 4, 8, P, 2, 0.0, P, None), _lib.STATUS_BAD_LD),
