@@ -483,7 +483,8 @@ int vedic_flash_attention_bwd_heads(const float* const* Q, const float* const* K
  * a plan holds is clamped where it is read (an offset to 0 .. n, a row or slot
  * outside its matrix counts as none), so a bad plan gives wrong values but no
  * access outside the arrays.  Limits: 1024 groups, leading dimensions below 2^22,
- * counts below 2^30 (VEDIC_STATUS_TOO_LARGE). */
+ * counts below 2^30 (places of a grouped product 2^27, of adapters 2^23;
+ * VEDIC_STATUS_TOO_LARGE). */
 
 /* The router: for each of T tokens the k largest of its E logits, a tie to the
  * lower index, and their weights exp(x_j - max) / sum, the sum over the chosen
@@ -529,9 +530,10 @@ int vedic_group_rows(const int* ids, int n, int per_row, int groups, int* offset
  * NONE, and db_g = db_beta db_g + the column sums of group g's rows of B if db is set.
  * The order of every sum is fixed.  Binary16 operands with 16-byte-aligned bases,
  * leading dimensions and strides that are multiples of 8 and contiguous extents that
- * are multiples of 8 run on the fast kernels, others on general ones.  TN with a row
- * list, and a list into an A of 2 GiB or more, copy the listed rows into the stream's
- * workspace block. */
+ * are multiples of 8 run on the fast kernels as they are; others are copied into padded
+ * rows in the stream's workspace block first, up to 256 MiB of them, or run on general
+ * kernels.  Also in that block: the listed rows of fp32 TN products and of an A of 2 GiB
+ * or more, and the slabs of TN products with few tiles and long groups (at most 16 MiB). */
 typedef struct {
     int op, in_dtype, out_dtype, epilogue;
     int groups;

@@ -189,6 +189,8 @@ _lib: ctypes.CDLL | None = None
 def load() -> ctypes.CDLL:
     """Loads liblogos_vedic.so once; raises if it has not been built."""
     global _lib
+    if _lib is not None:  # (set once, after the signatures)
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):

@@ -1170,6 +1170,8 @@ extern "C" int vedic_bias_grad(const float* dY, float* db, int M, int N, float b
 
 // Offsets, slots and row indexes count in int: products of the sizes stay below this.
 static constexpr int64_t kMaxCount = int64_t(1) << 30;
+// Padded copies of unaligned binary16 operands, at most (the stream's block keeps it).
+static constexpr size_t kPadBytes = size_t(256) << 20;
 
 extern "C" int vedic_route_topk(const float* logits, int64_t ld_logits, int T, int E, int k, int renorm, int* ids,
                                 float* weights, int* offsets, int* rows, int* slots, void* stream) {
@@ -1231,6 +1233,17 @@ extern "C" int vedic_group_rows(const int* ids, int n, int per_row, int groups, 
     return hip_status(e != hipSuccess ? e : f);
 }
 
+// Slices of a TN product whose 128 x 128 tiles number at most half the CUs: as many as
+// give every CU one, of 512 rows on average at least (1: none).
+static int grouped_ksplit(int groups, int M, int N, int R, int cus) {
+    const int64_t tiles = (int64_t)groups * ((M + 127) / 128) * ((N + 127) / 128);
+    if (tiles * 2 > cus) return 1;
+    int64_t s = cus / tiles;
+    s = s < R / groups / 512 ? s : R / groups / 512;
+    s = s < 16 ? s : 16;
+    return s >= 2 ? (int)s : 1;
+}
+
 // vec: binary16 operands whose rows 16-byte loads can take.
 static hipError_t launch_grouped(int op, const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s) {
     // At most eight rows a group (us, tiles / few-row kernel, 8 groups: NN 1024 into 4096, 8
@@ -1246,8 +1259,8 @@ static hipError_t launch_grouped(int op, const GroupedArgs& a, int kind, bool f1
                                : launch_grouped_any_tn(a, kind, f16, f16out, s);
 }
 
-extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
-    if (!d) return VEDIC_STATUS_NULL_POINTER;
+// A grouped product (d->offsets null: one group of all rows).
+static int run_grouped(const vedic_grouped_desc_t* d) {
     const bool tn = d->op == VEDIC_OP_TN;
     if (d->op != VEDIC_OP_NN && d->op != VEDIC_OP_NT && !tn) return VEDIC_STATUS_BAD_LAYOUT;
     if (d->in_dtype != VEDIC_DT_F32 && d->in_dtype != VEDIC_DT_F16) return VEDIC_STATUS_BAD_DTYPE;
@@ -1270,12 +1283,12 @@ extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
         return VEDIC_STATUS_BAD_EPILOGUE;
     if (d->preact && kind != GK_GELU_P && kind != GK_GELU_BWD) return VEDIC_STATUS_BAD_EPILOGUE;
     if ((!tn && (d->beta != 0.0f || d->db)) || d->beta != d->beta) return VEDIC_STATUS_BAD_EPILOGUE;
-    if (!d->offsets || (!d->C && (tn || R > 0)) || (R > 0 && (!d->A || !d->B))) return VEDIC_STATUS_NULL_POINTER;
+    if ((!d->C && (tn || R > 0)) || (R > 0 && (!d->A || !d->B))) return VEDIC_STATUS_NULL_POINTER;
     const int a_cols = tn ? d->M : d->K, b_cols = d->op == VEDIC_OP_NT ? d->K : N;
     if (d->lda < a_cols || d->ldb < b_cols || d->ldc < N || (d->preact && d->ld_preact < N)) return VEDIC_STATUS_BAD_LD;
     // (groups of dW that overlap would be written by two workgroups at once)
     if (d->stride_b < 0 || (tn && d->groups > 1 && d->stride_c < (int64_t)(d->M - 1) * d->ldc + N)) return VEDIC_STATUS_BAD_LD;
-    if (d->groups > kMaxGroups || R >= kMaxCount || d->a_rows >= kMaxCount || d->lda >= kMaxLd || d->ldb >= kMaxLd ||
+    if (d->groups > kMaxGroups || R >= kMaxCount / 8 || d->a_rows >= kMaxCount || d->lda >= kMaxLd || d->ldb >= kMaxLd ||
         d->ldc >= kMaxLd || d->ld_preact >= kMaxLd)
         return VEDIC_STATUS_TOO_LARGE;
     const int64_t row_tiles = tn ? (int64_t)d->groups * ((d->M + 63) / 64) : R / 64 + (int64_t)d->groups;
@@ -1312,7 +1325,49 @@ extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
     auto vec_of = [&]() {
         return f16 && aligned16(a.A) && aligned16(a.B) && ((a.lda | a.ldb | a.stride_b) & 7) == 0 && ((a_cols | b_cols) & 7) == 0;
     };
+    a.Mp = a.M;
+    a.Np = N;
     bool vec = vec_of();
+    // Binary16 operands that 16-byte loads cannot take are copied into rows of whole
+    // 16-byte pieces where that is not too much memory: the copies cost less than the
+    // general kernels' six bf16 products per value and loads of single values (two groups
+    // of 4494 rows, 423 x 960 TN, 250 us without).
+    if (f16 && !vec && R > 0) {
+        auto whole = [](int c) { return (int64_t)(c + 7) / 8 * 8; };
+        const bool ca = !aligned16(a.A) || (a.lda & 7) || (a_cols & 7);
+        const bool cb = !aligned16(a.B) || ((a.ldb | a.stride_b) & 7) || (b_cols & 7);
+        const bool gather = a.rows && (tn || R < d->a_rows);  // listed rows rather than all of A
+        const int64_t na = gather || !a.rows ? R : d->a_rows, per_b = tn ? R : d->op == VEDIC_OP_NN ? d->K : N;
+        const int64_t nb = tn ? R : per_b * d->groups;
+        const size_t bytes_a = ca ? (size_t)na * whole(a_cols) * 2 : 0, bytes_b = cb ? (size_t)nb * whole(b_cols) * 2 : 0;
+        if (bytes_a + bytes_b <= kPadBytes && ws.room(bytes_a + bytes_b + 256)) {
+            void* pa = nullptr;
+            void* pb = nullptr;
+            hipError_t e = ca ? ws.get(&pa, bytes_a) : hipSuccess;
+            if (e == hipSuccess && cb) e = ws.get(&pb, bytes_b);
+            if (e == hipSuccess && ca)
+                e = launch_pad_rows(a.A, a.lda, (int)na, 0, d->a_rows, gather ? a.rows : nullptr, na, a_cols, pa, ws.s);
+            if (e == hipSuccess && cb) e = launch_pad_rows(a.B, a.ldb, (int)per_b, a.stride_b, 0, nullptr, nb, b_cols, pb, ws.s);
+            if (e != hipSuccess) return hip_status(e);
+            if (ca) {
+                a.A = pa;
+                a.lda = whole(a_cols);
+                a.Mp = (int)whole(a.M);
+                if (gather) a.rows = nullptr;
+            }
+            if (cb) {
+                a.B = pb;
+                a.ldb = whole(b_cols);
+                a.stride_b = per_b * a.ldb;
+                if (d->op != VEDIC_OP_NT) a.Np = (int)whole(N);
+            }
+            if (!tn) {
+                a.K = (int)whole(d->K);
+                a.kpad = d->op == VEDIC_OP_NN ? a.K - d->K : 0;
+            }
+            vec = true;
+        }
+    }
     // The rows of a list are copied into a workspace first where the kernels
     // cannot follow it: past 32-bit offsets, and along the contraction (TN) but for
     // the 16-byte binary16 kernels.
@@ -1326,14 +1381,43 @@ extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
         a.A = copy;
         a.lda = ldn;
         a.rows = nullptr;
-        vec = vec_of();
+        if (!vec) vec = vec_of();
     }
+    // TN with few tiles and long groups: slices of the contraction into slabs, then their
+    // sums in order.
+    const int ks = tn && vec ? grouped_ksplit(d->groups, d->M, N, R, device_cu_count()) : 1;
+    const size_t slab = (size_t)d->groups * d->M * N, sums = (size_t)d->groups * N;
+    if (ks > 1 && ws.room(4 * ks * (slab + sums) + 512)) {
+        float* cw = nullptr;
+        float* dw = nullptr;
+        hipError_t e = ws.get(&cw, 4 * ks * slab);
+        if (e == hipSuccess && d->db) e = ws.get(&dw, 4 * ks * sums);
+        if (e != hipSuccess) return hip_status(e);
+        a.C = cw;
+        a.ldc = N;
+        a.stride_c = (int64_t)d->M * N;
+        a.split_c = (int64_t)slab;
+        a.ksplit = ks;
+        a.db = dw;
+        a.db_beta = 0.0f;
+        e = launch_grouped(d->op, a, GK_LINEAR, f16, f16out, vec, ws.s);
+        if (e == hipSuccess)
+            e = launch_slab_sum(cw, ks, d->groups, d->M, N, static_cast<float*>(d->C), d->ldc, d->stride_c, d->beta, ws.s);
+        if (e == hipSuccess && dw) e = launch_slab_sum(dw, ks, d->groups, 1, N, d->db, N, N, d->db_beta, ws.s);
+        return hip_status(e);
+    }
+    a.ksplit = 1;
     hipError_t e = launch_grouped(d->op, a, kind, f16, f16out, vec, ws.s);
     // (the 16-byte binary16 kernels sum the columns on the way)
     if (e == hipSuccess && d->db && !vec)
         e = launch_group_colsum(d->B, f16, d->ldb, R, N, d->offsets, d->groups, d->db_beta, d->db, ws.s);
     const hipError_t f = ws.put(copy);
     return hip_status(e != hipSuccess ? e : f);
+}
+
+extern "C" int vedic_gemm_grouped(const vedic_grouped_desc_t* d) {
+    if (!d || !d->offsets) return VEDIC_STATUS_NULL_POINTER;
+    return run_grouped(d);
 }
 
 extern "C" int vedic_bias_grad_grouped(const void* dY, int dtype, int64_t ld, int R, int N, const int* offsets, int groups,
@@ -1419,18 +1503,55 @@ static int lora_checks(const void* X, int dtype, int64_t ldx, int M, const void*
     return VEDIC_STATUS_OK;
 }
 
-extern "C" int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, const void* A, const void* B, int groups, int r,
-                              const int* offsets, const int* rows, int n, const float* scales, float* C, int64_t ldc, int K,
-                              int N, void* stream) {
-    const int st = lora_checks(X, dtype, ldx, M, A, B, groups, r, offsets, rows, n, C, ldc, K, N);
-    if (st != VEDIC_STATUS_OK || n == 0 || M == 0) return st;
+// The shared projection.  Operands that 16-byte loads cannot take run as a grouped
+// product of one group, whose kernels have more for them (us, vedic_gemm / one group:
+// binary16 1 x 320 x 1747 53 / 12, 1848 x 459 x 1024 87 / 16, fp32 2707 x 632 x 909 45 / 33).
+static int run_base(const vedic_gemm_desc_t* b) {
+    const int es = b->in_dtype == VEDIC_DT_F16 ? 2 : 4, per16 = 16 / es;
+    const bool aligned = aligned16(b->A) && aligned16(b->B) && b->lda % per16 == 0 && b->ldb % per16 == 0 &&
+                         b->K % per16 == 0 && b->N % per16 == 0;
+    if (aligned || b->alpha != 1.0f || b->beta != 0.0f || b->ldc >= kMaxLd) return vedic_gemm(b);
+    vedic_grouped_desc_t d = {};
+    d.op = VEDIC_OP_NN;
+    d.in_dtype = b->in_dtype;
+    d.out_dtype = b->out_dtype;
+    d.epilogue = b->epilogue;
+    d.groups = 1;
+    d.rows = b->M;
+    d.N = b->N;
+    d.K = b->K;
+    d.A = b->A;
+    d.lda = b->lda;
+    d.B = b->B;
+    d.ldb = b->ldb;
+    d.C = b->C;
+    d.ldc = b->ldc;
+    d.bias = b->bias;
+    d.stream = b->stream;
+    return run_grouped(&d);
+}
+
+// C += the adapters' products, after `base` where one is given (the workspace first: a
+// call that cannot have it has done nothing).
+static int run_lora(const vedic_gemm_desc_t* base, const LoraArgs& a, bool f16, void* stream) {
     Workspace ws;
     ws.s = static_cast<hipStream_t>(stream);
-    LoraArgs a{};
-    const bool f16 = dtype == VEDIC_DT_F16;
     void* work = nullptr;
-    hipError_t e = ws.get(&work, lora_bytes(n, r, f16, M, ldx, K));
+    hipError_t e = ws.get(&work, lora_bytes(a, f16));
     if (e != hipSuccess) return hip_status(e);
+    if (base) {
+        const int st = run_base(base);
+        if (st != VEDIC_STATUS_OK) return st;
+    }
+    e = launch_lora(a, f16, work, ws.s);
+    const hipError_t f = ws.put(work);
+    return hip_status(e != hipSuccess ? e : f);
+}
+
+static LoraArgs lora_args(const void* X, int64_t ldx, int M, const void* A, const void* B, int groups, int r,
+                          const int* offsets, const int* rows, int n, const float* scales, float* C, int64_t ldc, int K,
+                          int N) {
+    LoraArgs a{};
     a.X = X;
     a.ldx = ldx;
     a.A = A;
@@ -1446,9 +1567,16 @@ extern "C" int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, cons
     a.K = K;
     a.N = N;
     a.r = r;
-    e = launch_lora(a, f16, work, ws.s);
-    const hipError_t f = ws.put(work);
-    return hip_status(e != hipSuccess ? e : f);
+    return a;
+}
+
+extern "C" int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, const void* A, const void* B, int groups, int r,
+                              const int* offsets, const int* rows, int n, const float* scales, float* C, int64_t ldc, int K,
+                              int N, void* stream) {
+    const int st = lora_checks(X, dtype, ldx, M, A, B, groups, r, offsets, rows, n, C, ldc, K, N);
+    if (st != VEDIC_STATUS_OK || n == 0 || M == 0) return st;
+    return run_lora(nullptr, lora_args(X, ldx, M, A, B, groups, r, offsets, rows, n, scales, C, ldc, K, N),
+                    dtype == VEDIC_DT_F16, stream);
 }
 
 extern "C" int vedic_gemm_lora(const vedic_gemm_desc_t* base, const void* A, const void* B, int groups, int r,
@@ -1459,13 +1587,17 @@ extern "C" int vedic_gemm_lora(const vedic_gemm_desc_t* base, const void* A, con
     if ((base->epilogue != VEDIC_EPI_NONE && base->epilogue != VEDIC_EPI_BIAS) || base->preact || base->colsum)
         return VEDIC_STATUS_BAD_EPILOGUE;
     // (the adapters' arguments first: a refused call leaves C as it was)
-    int st = lora_checks(base->A, base->in_dtype, base->lda, base->M, A, B, groups, r, offsets, rows, n,
+    const int st = lora_checks(base->A, base->in_dtype, base->lda, base->M, A, B, groups, r, offsets, rows, n,
                          static_cast<float*>(base->C), base->ldc, base->K, base->N);
     if (st != VEDIC_STATUS_OK) return st;
-    st = vedic_gemm(base);
-    if (st != VEDIC_STATUS_OK || n == 0) return st;
-    return vedic_lora_add(base->A, base->in_dtype, base->lda, base->M, A, B, groups, r, offsets, rows, n, scales,
-                          static_cast<float*>(base->C), base->ldc, base->K, base->N, base->stream);
+    if (n == 0 || base->M <= 0) return vedic_gemm(base);
+    if (base->epilogue == VEDIC_EPI_BIAS && !base->bias) return VEDIC_STATUS_BAD_EPILOGUE;
+    if (!base->B) return VEDIC_STATUS_NULL_POINTER;
+    if (base->ldb < base->N) return VEDIC_STATUS_BAD_LD;
+    return run_lora(base,
+                    lora_args(base->A, base->lda, base->M, A, B, groups, r, offsets, rows, n, scales,
+                              static_cast<float*>(base->C), base->ldc, base->K, base->N),
+                    base->in_dtype == VEDIC_DT_F16, base->stream);
 }
 
 // ----------------------------------------------------------- elementwise

@@ -159,6 +159,29 @@ __global__ void __launch_bounds__(256) gather_rows16_kernel(const u32x4_t* src, 
     }
 }
 
+// dst[i][0 .. 8 octs) = binary16 src row i (row rows[i], zeros outside nsrc, where a
+// list is given), zeros past `cols`; src rows in matrices of `per` rows, `stride` apart.
+// 16-byte stores; loads of any alignment.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const _Float16* src, int64_t ld, int per, int64_t stride, int nsrc,
+                                                        const int* rows, int64_t n, int cols, int octs, half8_t* dst) {
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n * octs; q += (int64_t)gridDim.x * 256) {
+        const int64_t i = q / octs;
+        const int c = (int)(q - i * octs) * 8;
+        int64_t r = i;
+        bool ok = true;
+        if (rows != nullptr) {
+            r = rows[i];
+            ok = (uint64_t)r < (uint64_t)nsrc;
+        }
+        const int64_t m = ok ? r / per : 0;
+        const _Float16* s = src + m * stride + (ok ? r - m * per : 0) * ld + c;
+        half8_t v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = ok && c + e < cols ? s[e] : (_Float16)0.0f;
+        dst[q] = v;
+    }
+}
+
 // db[e][j] = beta db[e][j] + sum of X[i][j] over the group's rows.  One workgroup
 // per group and strip of columns, phase p of PH adding rows p, p + PH, ... in
 // order and the phases then in order.  VEC: 64 columns by 16-byte loads; else one
@@ -203,6 +226,20 @@ __global__ void __launch_bounds__(256) group_colsum_kernel(const T* X, int64_t l
             float* o = db + (int64_t)e * N + col;
             *o = beta == 0.0f ? t : __builtin_fmaf(beta, *o, t);
         }
+    }
+}
+
+// C_g = beta C_g + the sum of S slabs [groups][M x N], in order.
+__global__ void __launch_bounds__(256) slab_sum_kernel(const float* ws, int S, int64_t slab, int M, int N, float* C, int64_t ldc,
+                                                        int64_t stride_c, float beta) {
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < slab; q += (int64_t)gridDim.x * 256) {
+        float t = ws[q];
+        for (int s = 1; s < S; ++s) t += ws[s * slab + q];
+        const int64_t row = q / N;
+        const int n = (int)(q - row * N);
+        const int64_t g = row / M;
+        float* c = C + g * stride_c + (row - g * M) * ldc + n;
+        *c = beta == 0.0f ? t : __builtin_fmaf(beta, *c, t);
     }
 }
 
@@ -256,6 +293,25 @@ hipError_t launch_gather_rows(const void* src, int64_t ld, int nsrc, const int* 
         hipLaunchKernelGGL(gather_rows_kernel, dim3((unsigned)n), dim3(256), 0, s, static_cast<const uint16_t*>(src),
                            ld * (es / 2), nsrc, rows, n, cols * (es / 2), static_cast<uint16_t*>(dst), ldd * (es / 2));
     }
+    return hipGetLastError();
+}
+
+hipError_t launch_slab_sum(const float* ws, int S, int groups, int M, int N, float* C, int64_t ldc, int64_t stride_c, float beta,
+                           hipStream_t s) {
+    const int64_t slab = (int64_t)groups * M * N;
+    int64_t blocks = (slab + 255) / 256;
+    if (blocks > 65536) blocks = 65536;
+    hipLaunchKernelGGL(slab_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, s, ws, S, slab, M, N, C, ldc, stride_c, beta);
+    return hipGetLastError();
+}
+
+hipError_t launch_pad_rows(const void* src, int64_t ld, int per, int64_t stride, int nsrc, const int* rows, int64_t n, int cols,
+                           void* dst, hipStream_t s) {
+    const int octs = (cols + 7) / 8;
+    int64_t blocks = (n * octs + 255) / 256;
+    if (blocks > 65536) blocks = 65536;
+    hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const _Float16*>(src), ld, per,
+                       stride, nsrc, rows, n, cols, octs, static_cast<half8_t*>(dst));
     return hipGetLastError();
 }
 

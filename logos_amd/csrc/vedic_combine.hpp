@@ -38,6 +38,13 @@ hipError_t launch_combine_bwd(const CombineBwdArgs& a, bool f16, bool out16, hip
 // dst[i] = src[rows[i]], `cols` values of es bytes (2 or 4); n > 0.
 hipError_t launch_gather_rows(const void* src, int64_t ld, int nsrc, const int* rows, int n, int cols, int es, void* dst,
                               int64_t ldd, hipStream_t s);
+// C_g = beta C_g + the sum of S slabs [groups][M x N], in order.
+hipError_t launch_slab_sum(const float* ws, int S, int groups, int M, int N, float* C, int64_t ldc, int64_t stride_c, float beta,
+                           hipStream_t s);
+// dst [n x roundup(cols, 8)] binary16 = n rows of `cols` values of src (matrices of `per`
+// rows, `stride` apart; or its rows rows[i], nsrc of them there), padded with zeros; n > 0.
+hipError_t launch_pad_rows(const void* src, int64_t ld, int per, int64_t stride, int nsrc, const int* rows, int64_t n, int cols,
+                           void* dst, hipStream_t s);
 // db[e] = beta db[e] + column sums of the group's rows of X.
 hipError_t launch_group_colsum(const void* X, bool f16, int64_t ld, int R, int N, const int* offsets, int groups, float beta,
                                float* db, hipStream_t s);

@@ -49,17 +49,29 @@ struct GroupedArgs {
     int R;       // rows of C (NN / NT), of B (TN): offsets are clamped to it
     int a_rows;  // rows of A
     int M, N, K; // NN / NT: N and K; TN: M and N
+    // Binary16 kernels: the columns that A (TN) and B (NN, TN) have, which a padded copy
+    // has more of than M and N, and the steps of K that are A's padding alone (NN).
+    int Mp, Np, kpad;
     float beta;
     const int* out_rows;  // GK_ADD: [R] rows of C, out_limit of them there
     int out_limit;
     const float* scales;  // GK_ADD: [groups], or null
     float* db;  // TN: [groups x N] column sums of B, or null
     float db_beta;
+    // TN split over the contraction: slice s of a group's rows goes to C + s split_c (C
+    // then a workspace of [ksplit][groups][M x N]) and db + s groups N.  1: no split.
+    int ksplit;
+    int64_t split_c;
     int tiles_m, tiles_n;
+    int most;   // work items that a plan in order can have at most
     bool wide;  // grouped_wide_rows
 };
 
-__device__ __forceinline__ int group_start(const GroupedArgs& a, int e) { return min(max(a.offsets[e], 0), a.R); }
+// (no offsets: one group of all rows)
+__device__ __forceinline__ int group_start(const GroupedArgs& a, int e) {
+    if (a.offsets == nullptr) return e > 0 ? a.R : 0;
+    return min(max(a.offsets[e], 0), a.R);
+}
 __device__ __forceinline__ int group_count(const GroupedArgs& a, int e) {
     return max(0, group_start(a, e + 1) - group_start(a, e));
 }
@@ -132,7 +144,8 @@ __device__ __forceinline__ int group_of(const GroupIndex& ix, int groups, int t,
     int e = 0;
     for (int e0 = 0; e0 < groups; e0 += 64)
         e += __popcll(__ballot(e0 + lane < groups && ix.pre[min(e0 + lane, groups - 1) + 1] <= t));
-    return __builtin_amdgcn_readfirstlane(e);
+    // (a bad plan's tiles can exceed what the grid was made for: never past the last group)
+    return __builtin_amdgcn_readfirstlane(min(e, groups - 1));
 }
 
 // gelu_tanh'(x) = s + 2 c x s (1 - s) (1 + 3 * 0.044715 x^2), s = 1 / (1 + e), e =

@@ -120,9 +120,9 @@ struct SideAny {
 // steps, and for the steps behind the last four.  pa, pb: this lane's row and column
 // (lane half h takes step kb + 2 q + h), ka, kb_ the distance of two steps' elements; a
 // row that is not there has oka = false and counts as zeros.
-template <typename T, int MI, int NI>
+template <typename T, typename TB, int MI, int NI>
 __device__ __forceinline__ void any_block_slow(const T* const (&pa)[MI], const bool (&oka)[MI], int64_t ka,
-                                               const T* const (&pb)[NI], int64_t kb_, int kb, int K, int h,
+                                               const TB* const (&pb)[NI], int64_t kb_, int kb, int K, int h,
                                                float16_t (&acc)[MI][NI]) {
 #pragma unroll 1
     for (int k = kb + h; k < K + h; k += 2) {
@@ -147,7 +147,8 @@ __device__ __forceinline__ void any_block_slow(const T* const (&pa)[MI], const b
 // WGK > 1: that many groups of WGM x WGN waves, each with LDS buffers of its own and
 // a part of the contraction (whole stages); the others leave their sums in LDS for the
 // first, which adds them in order and runs the epilogue.
-template <int OP, typename T, typename OT, int BM, int BN, int WGM, int WGN, int WGK, int KIND>
+// T, TB, OT: the types of A, B and C.
+template <int OP, typename T, typename TB, typename OT, int BM, int BN, int WGM, int WGN, int WGK, int KIND>
 __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(GroupedArgs a) {
     constexpr int NT = WGM * WGN * 64, WM = BM / WGM, WN = BN / WGN, MI = WM / 32, NI = WN / 32;
     constexpr bool A_KC = OP != 2, B_KC = OP == 1;
@@ -201,13 +202,13 @@ __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(Groupe
     } else {
         A += (int64_t)(start + m0) * a.lda;
     }
-    const T* B = static_cast<const T*>(a.B);
+    const TB* B = static_cast<const TB*>(a.B);
     if constexpr (OP == 2) B += (int64_t)start * a.ldb + n0;
     else B += (int64_t)e * a.stride_b + (B_KC ? (int64_t)n0 * a.ldb : n0);
     const int64_t ka = A_KC ? 1 : a.lda, kb = B_KC ? 1 : a.ldb;
 
     using SA = SideAny<T, A_KC, BM, NT>;
-    using SB = SideAny<T, B_KC, BN, NT>;
+    using SB = SideAny<TB, B_KC, BN, NT>;
     SA sa;
     SB sb;
     sa.init(tid, a.lda, left, list, a.a_rows);
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(Groupe
     const bool again = few || __any(probe != 0.0f);
     if (again || Kq < K) {
         const T* pa[MI];
-        const T* pb[NI];
+        const TB* pb[NI];
         bool oka[MI];
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(Groupe
 #pragma unroll
                 for (int j = 0; j < NI; ++j) acc[i][j] = float16_t{};
         }
-        any_block_slow<T, MI, NI>(pa, oka, ka, pb, kb, again ? 0 : Kq, K, lane >> 5, acc);
+        any_block_slow<T, TB, MI, NI>(pa, oka, ka, pb, kb, again ? 0 : Kq, K, lane >> 5, acc);
     }
     if constexpr (KIND == GK_ADD) {
         grouped_add<MI, NI>(static_cast<float*>(a.C), a.ldc, a.out_rows + start + m0 + wm * WM, a.out_limit,
@@ -378,7 +379,7 @@ inline double grouped_row_tiles(int R, int groups, int bm) {
     return (double)R / bm + 0.5 * (groups < R ? groups : R);
 }
 
-template <int OP, typename T, typename OT, class Cfg, int WGK, int KIND>
+template <int OP, typename T, typename TB, typename OT, class Cfg, int WGK, int KIND>
 static hipError_t launch_any(GroupedArgs a, hipStream_t s) {
     a.tiles_n = (a.N + Cfg::BN - 1) / Cfg::BN;
     a.tiles_m = OP == 2 ? (a.M + Cfg::BM - 1) / Cfg::BM : 0;
@@ -387,7 +388,7 @@ static hipError_t launch_any(GroupedArgs a, hipStream_t s) {
                                  : grouped_row_tiles_max(a.R, a.groups, Cfg::BM) * a.tiles_n;
     if (work > 0x7FFFFFFF) return hipErrorInvalidValue;  // (the caller has refused such sizes)
     if (work == 0) return hipSuccess;
-    hipLaunchKernelGGL((grouped_any_kernel<OP, T, OT, Cfg::BM, Cfg::BN, Cfg::WGM, Cfg::WGN, WGK, KIND>),
+    hipLaunchKernelGGL((grouped_any_kernel<OP, T, TB, OT, Cfg::BM, Cfg::BN, Cfg::WGM, Cfg::WGN, WGK, KIND>),
                        dim3((unsigned)work), dim3(Cfg::WGM * Cfg::WGN * WGK * 64), 0, s, a);
     return hipGetLastError();
 }
@@ -397,7 +398,7 @@ static hipError_t launch_any(GroupedArgs a, hipStream_t s) {
 // contractions long enough to share (us, one group / three: 2006 rows in 7 groups of
 // 2000 into 1000, 156 tiles, NN 103 / 79, NT 101 / 74; the same TN, 896 tiles of 286 steps,
 // 63 / 73; 16 rows of 1024 into 4096 in 8 groups 55 / 45; 300 rows of 512 into 777 24 / 17).
-template <int OP, typename T, typename OT, int KIND>
+template <int OP, typename T, typename TB, typename OT, int KIND>
 static hipError_t launch_any_tiles(const GroupedArgs& a, hipStream_t s) {
     auto tiles = [&](int b) {
         return (OP == 2 ? (double)a.groups * ((a.M + b - 1) / b) : grouped_row_tiles(a.R, a.groups, b)) * ((a.N + b - 1) / b);
@@ -405,24 +406,24 @@ static hipError_t launch_any_tiles(const GroupedArgs& a, hipStream_t s) {
     const int cus = device_cu_count();
     const bool split = (OP == 2 ? a.R / a.groups : a.K) >= 256;
     if (tiles(128) * 2 > cus) {
-        if (split && tiles(128) <= cus) return launch_any<OP, T, OT, CfgAMid, kAnyGroups, KIND>(a, s);
-        return launch_any<OP, T, OT, CfgAMid, 1, KIND>(a, s);
+        if (split && tiles(128) <= cus) return launch_any<OP, T, TB, OT, CfgAMid, kAnyGroups, KIND>(a, s);
+        return launch_any<OP, T, TB, OT, CfgAMid, 1, KIND>(a, s);
     }
-    if (split) return launch_any<OP, T, OT, CfgASmall, kAnyGroups, KIND>(a, s);
-    return launch_any<OP, T, OT, CfgASmall, 1, KIND>(a, s);
+    if (split) return launch_any<OP, T, TB, OT, CfgASmall, kAnyGroups, KIND>(a, s);
+    return launch_any<OP, T, TB, OT, CfgASmall, 1, KIND>(a, s);
 }
 
 template <int OP, int KIND>
 static hipError_t launch_any_kind(const GroupedArgs& a, bool f16, bool f16out, hipStream_t s) {
     if constexpr (OP != 2)
-        if (f16out) return launch_any_tiles<OP, _Float16, _Float16, KIND>(a, s);
-    return f16 ? launch_any_tiles<OP, _Float16, float, KIND>(a, s) : launch_any_tiles<OP, float, float, KIND>(a, s);
+        if (f16out) return launch_any_tiles<OP, _Float16, _Float16, _Float16, KIND>(a, s);
+    return f16 ? launch_any_tiles<OP, _Float16, _Float16, float, KIND>(a, s) : launch_any_tiles<OP, float, float, float, KIND>(a, s);
 }
 
-#define VEDIC_ANY_KERNELS(OP, T, OT, KIND)                                                               \
-    template __global__ void grouped_any_kernel<OP, T, OT, 128, 128, 2, 2, 1, KIND>(GroupedArgs);          \
-    template __global__ void grouped_any_kernel<OP, T, OT, 128, 128, 2, 2, kAnyGroups, KIND>(GroupedArgs); \
-    template __global__ void grouped_any_kernel<OP, T, OT, 64, 64, 2, 1, 1, KIND>(GroupedArgs);            \
-    template __global__ void grouped_any_kernel<OP, T, OT, 64, 64, 2, 1, kAnyGroups, KIND>(GroupedArgs)
+#define VEDIC_ANY_KERNELS(OP, T, TB, OT, KIND)                                                               \
+    template __global__ void grouped_any_kernel<OP, T, TB, OT, 128, 128, 2, 2, 1, KIND>(GroupedArgs);          \
+    template __global__ void grouped_any_kernel<OP, T, TB, OT, 128, 128, 2, 2, kAnyGroups, KIND>(GroupedArgs); \
+    template __global__ void grouped_any_kernel<OP, T, TB, OT, 64, 64, 2, 1, 1, KIND>(GroupedArgs);            \
+    template __global__ void grouped_any_kernel<OP, T, TB, OT, 64, 64, 2, 1, kAnyGroups, KIND>(GroupedArgs)
 
 }  // namespace vedic

@@ -144,7 +144,7 @@ struct StageSums {
 
 // One work item: a tile of one group.
 struct GroupedItem {
-    int e, start, m0, n0, left, K, nk;
+    int e, start, m0, n0, left, K, nk, slice;
 };
 
 // Work item w counts tiles of PM x PN; with SM x SN > 1 a tile is cut into that
@@ -157,11 +157,14 @@ __device__ __forceinline__ GroupedItem grouped_item(const GroupedArgs& a, const 
     w /= SM * SN;
     if constexpr (OP == 2) {
         const int tiles = a.tiles_m * a.tiles_n;
+        it.slice = __builtin_amdgcn_readfirstlane(w / (a.groups * tiles));
+        w -= it.slice * a.groups * tiles;
         const int place = w / tiles, t = w - place * tiles;
         it.e = __builtin_amdgcn_readfirstlane(ix.pre[place]);
         it.m0 = t % a.tiles_m * PM;
         it.n0 = t / a.tiles_m * PN;
-        it.K = group_count(a, it.e);
+        const int count = group_count(a, it.e), len = ((count + a.ksplit - 1) / a.ksplit + BK - 1) / BK * BK;
+        it.K = max(0, min(len, count - it.slice * len));
         it.left = a.M;
     } else {
         it.e = group_of(ix, a.groups, w / a.tiles_n, lane);
@@ -180,6 +183,14 @@ __device__ __forceinline__ GroupedItem grouped_item(const GroupedArgs& a, const 
     // (uniform, said so that the loads' resources stay in scalar registers)
     it.e = __builtin_amdgcn_readfirstlane(it.e);
     it.start = __builtin_amdgcn_readfirstlane(group_start(a, it.e));
+    if constexpr (OP == 2) {
+        if (a.ksplit > 1) {
+            // (an empty slice may start past the group's end: nothing is read there)
+            const int count = group_count(a, it.e);
+            it.start += min(count, it.slice * (((count + a.ksplit - 1) / a.ksplit + BK - 1) / BK * BK));
+            it.start = __builtin_amdgcn_readfirstlane(it.start);
+        }
+    }
     it.m0 = __builtin_amdgcn_readfirstlane(it.m0);
     it.n0 = __builtin_amdgcn_readfirstlane(it.n0);
     it.left = __builtin_amdgcn_readfirstlane(it.left) - it.m0;
@@ -190,13 +201,13 @@ __device__ __forceinline__ GroupedItem grouped_item(const GroupedArgs& a, const 
 
 // The loads of the next stage into (la) and (lb), and the operands moved on (past
 // the range nothing is read: the stage has no steps left).
-#define VEDIC_G_ISSUE(la, lb)                      \
-    do {                                           \
-        sa.load(Ab, (la), wave, lane, krem);       \
-        sb.load(Bb, (lb), wave, lane, krem);       \
-        Ab += A_KC ? (int64_t)BK : astep;          \
-        Bb += B_KC ? (int64_t)BK : BK * a.ldb;     \
-        krem -= BK;                                \
+#define VEDIC_G_ISSUE(la, lb)                       \
+    do {                                            \
+        sa.load(Ab, (la), wave, lane, krem);        \
+        sb.load(Bb, (lb), wave, lane, krem - kpad); \
+        Ab += A_KC ? (int64_t)BK : astep;           \
+        Bb += B_KC ? (int64_t)BK : BK * a.ldb;      \
+        krem -= BK;                                 \
     } while (0)
 // A pointer said to be uniform: its halves in scalar registers.
 __device__ __forceinline__ const _Float16* uniform(const _Float16* p) {
@@ -222,13 +233,13 @@ __device__ __forceinline__ const _Float16* uniform(const _Float16* p) {
         if constexpr (OP == 2) {                                                                               \
             Ab += (LIST ? 0 : (int64_t)it.start * a.lda) + it.m0;                                              \
             Bb += (int64_t)it.start * a.ldb + it.n0;                                                           \
-            sa.init(wave, lane, a.lda, it.m0, a.M, a.rows, it.start, a.R, a.a_rows);                           \
+            sa.init(wave, lane, a.lda, it.m0, a.Mp, a.rows, it.start, a.R, a.a_rows);                          \
         } else {                                                                                               \
             Bb += (int64_t)it.e * a.stride_b + (B_KC ? (int64_t)it.n0 * a.ldb : it.n0);                        \
             if (!a.rows) Ab += (int64_t)(it.start + it.m0) * a.lda;                                            \
             sa.init(wave, lane, a.lda, a.rows ? a.a_rows : BM);                                                \
         }                                                                                                      \
-        sb.init(wave, lane, a.ldb, it.n0, a.N);                                                                \
+        sb.init(wave, lane, a.ldb, it.n0, B_KC ? a.N : a.Np);                                                  \
         if (kBias && (int)threadIdx.x < BN) sbias[par][threadIdx.x] = bnext;                                   \
         Ab = uniform(Ab);                                                                                      \
         Bb = uniform(Bb);                                                                                      \
@@ -266,6 +277,7 @@ __device__ __forceinline__ void grouped_tiles(const GroupedArgs& a, const GroupI
     const _Float16* Bb;
     float bnext = 0.0f;
     int krem;  // contraction steps not yet loaded
+    const int kpad = OP == 0 ? a.kpad : 0;
     const int64_t astep = LIST ? 0 : BK * a.lda;  // (TN)
     VEDIC_G_NEXT();
     VEDIC_G_START();
@@ -315,7 +327,7 @@ __device__ __forceinline__ void grouped_tiles(const GroupedArgs& a, const GroupI
             if (sums) {
                 wait_vmcnt<0>();  // (zero loads past the range may still write the buffers)
                 __syncthreads();
-                ss.finish(reinterpret_cast<float*>(t0), a.db + (int64_t)it.e * a.N + it.n0, a.N - it.n0, a.db_beta, wave, lane);
+                ss.finish(reinterpret_cast<float*>(t0), a.db + ((int64_t)it.slice * a.groups + it.e) * a.N + it.n0, a.N - it.n0, a.db_beta, wave, lane);
             }
         }
         const GroupedItem done = it;
@@ -329,7 +341,7 @@ __device__ __forceinline__ void grouped_tiles(const GroupedArgs& a, const GroupI
         }
         const int row0 = done.m0 + wm * WM, col0 = done.n0 + wn * WN, left = done.left - wm * WM;
         const int64_t crow = OP == 2 ? row0 : done.start + row0;
-        OT* const C = static_cast<OT*>(a.C) + (OP == 2 ? (int64_t)done.e * a.stride_c : 0) + crow * a.ldc;
+        OT* const C = static_cast<OT*>(a.C) + (OP == 2 ? done.slice * a.split_c + (int64_t)done.e * a.stride_c : 0) + crow * a.ldc;
         OT* const P = a.P != nullptr ? static_cast<OT*>(a.P) + crow * a.ldp : nullptr;
         if (nk == 0) __syncthreads();  // (no stage's barrier has shown the bias)
         if (grouped_reads(KIND) && !a.wide)
@@ -363,8 +375,8 @@ __global__ void __launch_bounds__(512) grouped_f16_large_kernel(GroupedArgs a) {
     __shared__ __attribute__((aligned(16))) float sb1[256];
     if constexpr (OP != 2) group_index(a, ix, 256);
     else group_order<512>(a, ix, reinterpret_cast<int*>(t0));
-    const int nwork = OP == 2 ? a.groups * a.tiles_m * a.tiles_n
-                              : __builtin_amdgcn_readfirstlane(ix.pre[a.groups]) * a.tiles_n;
+    const int nwork = OP == 2 ? a.groups * a.tiles_m * a.tiles_n * a.ksplit
+                              : min((int64_t)__builtin_amdgcn_readfirstlane(ix.pre[a.groups]) * a.tiles_n, (int64_t)a.most);
     const int G = gridDim.x, b = blockIdx.x;
     const int w = (G & 7) == 0 ? (b & 7) * (G >> 3) + (b >> 3) : b;
     const int rest = nwork % G, whole = rest * 2 <= G ? nwork - rest : nwork;
@@ -392,7 +404,7 @@ __global__ void __launch_bounds__(256) grouped_f16_small_kernel(GroupedArgs a) {
     __shared__ __attribute__((aligned(16))) float sb0[128];
     __shared__ __attribute__((aligned(16))) float sb1[128];
     group_index(a, ix, 128);
-    const int nwork = __builtin_amdgcn_readfirstlane(ix.pre[a.groups]) * a.tiles_n;
+    const int nwork = min((int64_t)__builtin_amdgcn_readfirstlane(ix.pre[a.groups]) * a.tiles_n, (int64_t)a.most);
     const int G = gridDim.x, b = blockIdx.x;
     const int w = (G & 7) == 0 ? (b & 7) * (G >> 3) + (b >> 3) : b;
     if (w < nwork)
@@ -411,9 +423,11 @@ inline hipError_t grouped_grid(int op, GroupedArgs& a, int b, int parts, int es_
     a.tiles_n = (a.N + b - 1) / b;
     a.tiles_m = op == 2 ? (a.M + b - 1) / b : 0;
     a.wide = grouped_wide_rows(a, es_out);
-    const int64_t most = op == 2 ? (int64_t)a.groups * a.tiles_m * a.tiles_n
+    if (a.ksplit < 1) a.ksplit = 1;
+    const int64_t most = op == 2 ? (int64_t)a.groups * a.tiles_m * a.tiles_n * a.ksplit
                                  : (int64_t)(a.R / b + (a.groups < a.R ? a.groups : a.R)) * a.tiles_n;
     if (most * parts > 0x7FFFFFFF) return hipErrorInvalidValue;  // (the caller has refused such sizes)
+    a.most = (int)most;
     const int cus = device_cu_count();
     grid = most * parts < cus ? (int)(most * parts) : cus;
     return hipSuccess;

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(256) grouped_f16_skinny_kernel(GroupedArgs a) 
             bk[i] = 8 * c + 8;
         } else {  // eight k rows of two blocks of 32 columns (64 bytes) an instruction
             const int k = 8 * i + ((lane & 31) >> 2), col = 32 * (lane >> 5) + 8 * (lane & 3);
-            boff[i] = n0 + col + 8 <= a.N ? (uint32_t)((int64_t)k * a.ldb * 2 + col * 2) : kOob;
+            boff[i] = n0 + col + 8 <= a.Np ? (uint32_t)((int64_t)k * a.ldb * 2 + col * 2) : kOob;
             bk[i] = k + 1;
         }
     }
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(256) grouped_f16_skinny_kernel(GroupedArgs a) 
         const int krem = ke - k;
         const int64_t kk = krem > 0 ? k : 0;
         skinny_load<NA>(A + kk, aoff, ak, krem, buf + wave * kStage);
-        skinny_load<4>(B_KC ? B + kk : B + kk * a.ldb, boff, bk, krem, buf + wave * kStage + kABytes);
+        skinny_load<4>(B_KC ? B + kk : B + kk * a.ldb, boff, bk, min(krem, a.K - (B_KC ? 0 : a.kpad) - k), buf + wave * kStage + kABytes);
     };
     float16_t acc[1][NB] = {};
     // (rows 16 .. 31 of the MFMA's A read other LDS: they feed rows that are not stored)

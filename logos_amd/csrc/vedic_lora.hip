@@ -2,7 +2,8 @@
 // i of adapter g (list position p, rows[p] = i),
 //   C[i] += scale[g] (X[i] . A_g) . B_g,   A_g [K x r], B_g [r x N].
 // Two launches, H = X A_g into a workspace (fp32, or the same as two binary16
-// values), then C.  fp32 operands take the grouped fp32 products for both.
+// values), then C.  fp32 operands, and rows that 16-byte loads cannot take, run as two
+// grouped products (vedic_grouped_any.hpp).
 #include "vedic_combine.hpp"
 #include "vedic_common.hpp"
 #include "vedic_gemm_f16.hpp"
@@ -14,99 +15,6 @@ namespace vedic {
 hipError_t launch_grouped_any_nn(const GroupedArgs& a, int kind, bool f16, bool f16out, hipStream_t s);
 
 namespace {
-
-// ------------------------------------------------ binary16, any alignment
-
-constexpr int kLoraRows = 8;  // rows per workgroup of one adapter
-
-// H[p][0 .. r) of a tile of eight list positions: thread t takes rank t % RT of
-// the steps k = t / RT, t / RT + ST, ...
-__global__ void __launch_bounds__(256) lora_shrink_kernel(LoraArgs a) {
-    typedef _Float16 T;
-    __shared__ GroupIndex ix;
-    __shared__ float part[256][kLoraRows + 1];
-    GroupedArgs q{};
-    q.offsets = a.offsets;
-    q.groups = a.groups;
-    q.R = a.n;
-    group_index(q, ix, kLoraRows);
-    const int lane = threadIdx.x & 63, t = blockIdx.x;
-    if (t >= ix.pre[a.groups]) return;
-    const int g = group_of(ix, a.groups, t, lane);
-    const int b0 = (t - ix.pre[g]) * kLoraRows, p0 = group_start(q, g) + b0;
-    const int np = min(kLoraRows, group_count(q, g) - b0);
-    const T* A = static_cast<const T*>(a.A) + (int64_t)g * a.K * a.r;
-    const T* X = static_cast<const T*>(a.X);
-    const T* x[kLoraRows];
-    bool ok[kLoraRows];
-#pragma unroll
-    for (int i = 0; i < kLoraRows; ++i) {
-        const int row = i < np ? a.rows[p0 + i] : -1;
-        ok[i] = (unsigned)row < (unsigned)a.M;
-        x[i] = X + (int64_t)(ok[i] ? row : 0) * a.ldx;
-    }
-    int rt = 1;
-    while (rt < a.r) rt <<= 1;  // ranks across the threads, a power of two
-    const int c = threadIdx.x % rt, kp = threadIdx.x / rt, ks = 256 / rt;
-    float acc[kLoraRows] = {};
-    if (c < a.r)
-        for (int k = kp; k < a.K; k += ks) {
-            const float w = (float)A[(int64_t)k * a.r + c];
-#pragma unroll
-            for (int i = 0; i < kLoraRows; ++i) acc[i] = __builtin_fmaf(ok[i] ? (float)x[i][k] : 0.0f, w, acc[i]);
-        }
-#pragma unroll
-    for (int i = 0; i < kLoraRows; ++i) part[threadIdx.x][i] = acc[i];
-    __syncthreads();
-    for (int o = threadIdx.x; o < a.r * kLoraRows; o += 256) {
-        const int cc = o % a.r, i = o / a.r;
-        if (i < np) {
-            float s = 0.0f;
-            for (int v = 0; v < ks; ++v) s += part[v * rt + cc][i];
-            a.H[(int64_t)(p0 + i) * a.r + cc] = s;
-        }
-    }
-}
-
-// C += scale H B_g: a tile of eight rows by 256 columns, one column a thread.
-__global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
-    typedef _Float16 T;
-    __shared__ GroupIndex ix;
-    __shared__ float h[kLoraRows][kLoraMaxRank];
-    GroupedArgs q{};
-    q.offsets = a.offsets;
-    q.groups = a.groups;
-    q.R = a.n;
-    group_index(q, ix, kLoraRows);
-    const int strips = (a.N + 255) / 256;
-    const int lane = threadIdx.x & 63, t = blockIdx.x / strips;
-    if (t >= ix.pre[a.groups]) return;
-    const int g = group_of(ix, a.groups, t, lane);
-    const int b0 = (t - ix.pre[g]) * kLoraRows, p0 = group_start(q, g) + b0;
-    const int np = min(kLoraRows, group_count(q, g) - b0);
-    for (int o = threadIdx.x; o < kLoraRows * a.r; o += 256) {
-        const int i = o / a.r;
-        h[i][o % a.r] = i < np ? a.H[(int64_t)(p0 + i) * a.r + o % a.r] : 0.0f;
-    }
-    __syncthreads();
-    const int col = (blockIdx.x - t * strips) * 256 + threadIdx.x;
-    if (col >= a.N) return;
-    const T* B = static_cast<const T*>(a.B) + (int64_t)g * a.r * a.N + col;
-    float acc[kLoraRows] = {};
-    for (int k = 0; k < a.r; ++k) {
-        const float w = (float)B[(int64_t)k * a.N];
-#pragma unroll
-        for (int i = 0; i < kLoraRows; ++i) acc[i] = __builtin_fmaf(h[i][k], w, acc[i]);
-    }
-    const float sc = a.scales ? a.scales[g] : 1.0f;
-    for (int i = 0; i < np; ++i) {
-        const int row = a.rows[p0 + i];
-        if ((unsigned)row < (unsigned)a.M) {
-            float* c = a.C + (int64_t)row * a.ldc + col;
-            *c = __builtin_fmaf(sc, acc[i], *c);
-        }
-    }
-}
 
 // ------------------------------------------------ binary16, 16-byte rows
 
@@ -336,27 +244,18 @@ __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
         }
 }
 
-hipError_t launch_any(const LoraArgs& a, hipStream_t s) {
-    const int64_t tiles = a.n / kLoraRows + (a.groups < a.n ? a.groups : a.n);
-    hipLaunchKernelGGL(lora_shrink_kernel, dim3((unsigned)tiles), dim3(256), 0, s, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(lora_expand_kernel, dim3((unsigned)(tiles * ((a.N + 255) / 256))), dim3(256), 0, s, a);
-    return hipGetLastError();
-}
+// Any types and alignment: two grouped products, the second adding to the listed rows
+// of C.  (`copy`: the listed rows, where X is past the products' 32-bit offsets.)
+bool copies_rows(const LoraArgs& a, bool f16) { return (int64_t)a.M * a.ldx * (f16 ? 2 : 4) >= (int64_t(1) << 31); }
 
-// fp32: two grouped products, the second adding to the listed rows of C.  (`copy`:
-// the listed rows, where X is past the products' 32-bit offsets.)
-bool copies_rows(int M, int64_t ldx, bool f16) { return !f16 && (int64_t)M * ldx * 4 >= (int64_t(1) << 31); }
-
-hipError_t launch_f32(const LoraArgs& a, float* copy, hipStream_t s) {
+hipError_t launch_any(const LoraArgs& a, bool f16, void* copy, hipStream_t s) {
     GroupedArgs q{};
     q.A = a.X;
     q.lda = a.ldx;
     q.rows = a.rows;
     q.a_rows = a.M;
-    if (copies_rows(a.M, a.ldx, false)) {
-        const hipError_t e = launch_gather_rows(a.X, a.ldx, a.M, a.rows, a.n, a.K, 4, copy, a.K, s);
+    if (copies_rows(a, f16)) {
+        const hipError_t e = launch_gather_rows(a.X, a.ldx, a.M, a.rows, a.n, a.K, f16 ? 2 : 4, copy, a.K, s);
         if (e != hipSuccess) return e;
         q.A = copy;
         q.lda = a.K;
@@ -372,7 +271,7 @@ hipError_t launch_f32(const LoraArgs& a, float* copy, hipStream_t s) {
     q.R = a.n;
     q.N = a.r;
     q.K = a.K;
-    const hipError_t e = launch_grouped_any_nn(q, GK_LINEAR, false, false, s);
+    const hipError_t e = launch_grouped_any_nn(q, GK_LINEAR, f16, false, s);
     if (e != hipSuccess) return e;
     q.A = a.H;
     q.lda = a.r;
@@ -387,7 +286,7 @@ hipError_t launch_f32(const LoraArgs& a, float* copy, hipStream_t s) {
     q.out_rows = a.rows;
     q.out_limit = a.M;
     q.scales = a.scales;
-    return launch_grouped_any_nn(q, GK_ADD, false, false, s);
+    return launch_grouped_any_nn(q, GK_ADD, f16, false, s);
 }
 
 template <int RP, int KC>
@@ -413,16 +312,18 @@ bool vec16(const LoraArgs& a) {
 
 static size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-size_t lora_bytes(int n, int r, bool f16, int M, int64_t ldx, int K) {
-    const size_t rs = (size_t)(r <= 32 ? 32 : r <= 64 ? 64 : 128);
-    // (fp32: n r values, and the copied rows; binary16: hi and lo of rs each, and the factors)
-    return f16 ? (size_t)n * (rs * 4 + 4) : rounded((size_t)n * r * 4) + (copies_rows(M, ldx, f16) ? (size_t)n * K * 4 : 0);
+size_t lora_bytes(const LoraArgs& a, bool f16) {
+    if (f16 && vec16(a)) {  // hi and lo of rs values each, and the factors
+        const size_t rs = (size_t)(a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128);
+        return (size_t)a.n * (rs * 4 + 4);
+    }
+    return rounded((size_t)a.n * a.r * 4) + (copies_rows(a, f16) ? (size_t)a.n * a.K * (f16 ? 2 : 4) : 0);
 }
 
 hipError_t launch_lora(LoraArgs a, bool f16, void* work, hipStream_t s) {
     a.H = static_cast<float*>(work);
-    if (!f16) return launch_f32(a, reinterpret_cast<float*>(static_cast<char*>(work) + rounded((size_t)a.n * a.r * 4)), s);
-    if (!vec16(a)) return launch_any(a, s);
+    if (!f16 || !vec16(a))
+        return launch_any(a, f16, static_cast<char*>(work) + rounded((size_t)a.n * a.r * 4), s);
     const size_t rs = (size_t)(a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128);
     a.Hs = static_cast<_Float16*>(work);
     a.factor = reinterpret_cast<float*>(a.Hs + (size_t)a.n * 2 * rs);

@@ -27,7 +27,7 @@ struct LoraArgs {
 };
 
 // Workspace of a call, and the call (work: that many bytes, 256-byte aligned).
-size_t lora_bytes(int n, int r, bool f16, int M, int64_t ldx, int K);
+size_t lora_bytes(const LoraArgs& a, bool f16);
 hipError_t launch_lora(LoraArgs a, bool f16, void* work, hipStream_t s);
 
 }  // namespace vedic

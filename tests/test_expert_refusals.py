@@ -137,7 +137,10 @@ def test_lora(args, status):
     (dict(preact=P), (P, P, 2, 4, P, P, 4, None), _lib.STATUS_BAD_EPILOGUE),
     (dict(), (P, P, 2, 129, P, P, 4, None), _lib.STATUS_TOO_LARGE),
     (dict(), (None, P, 2, 4, P, P, 4, None), _lib.STATUS_NULL_POINTER),
-    (dict(epilogue=1), (P, P, 2, 4, P, P, 4, None), _lib.STATUS_BAD_EPILOGUE),  # the product's own refusal: no bias
+    (dict(epilogue=1), (P, P, 2, 4, P, P, 0, None), _lib.STATUS_BAD_EPILOGUE),  # the product's own refusal: no bias
+    (dict(epilogue=1), (P, P, 2, 4, P, P, 4, None), _lib.STATUS_BAD_EPILOGUE),
+    (dict(B=None), (P, P, 2, 4, P, P, 4, None), _lib.STATUS_NULL_POINTER),
+    (dict(ldb=7), (P, P, 2, 4, P, P, 4, None), _lib.STATUS_BAD_LD),
 ])
 def test_gemm_lora(kw, args, status):
     d = dict(op=0, in_dtype=1, out_dtype=0, M=8, N=8, K=8, A=P, lda=8, B=P, ldb=8, C=P, ldc=8, alpha=1.0, beta=0.0,

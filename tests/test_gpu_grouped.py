@@ -53,6 +53,7 @@ SIZES = [
     ([33, 12], 2, 8),
     ([12, 31], 17, 33),                     # nothing aligned
     ([150, 90], 131, 259),
+    ([2100, 1, 3000], 40, 56),              # few tiles and long groups: the contraction is shared (TN)
 ]
 COMBOS = [(F16, F16), (F16, F32), (F32, F32)]
 
