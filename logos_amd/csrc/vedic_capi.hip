@@ -109,6 +109,7 @@ struct StreamArena {
     std::recursive_mutex mu;
     ArenaBlock main;
     size_t want = 0;
+    size_t pooled = 0;  // pieces of the calls under way that did not fit the block
     std::vector<ArenaBlock*> held;  // blocks of captures
 
     // Makes the block as large as the largest call so far (the old one is freed
@@ -210,7 +211,7 @@ struct Workspace {
     StreamArena* arena = nullptr;  // locked while this workspace is alive
     ArenaBlock* block = nullptr;   // the arena's block that serves this call
     size_t mark = 0;               // its fill when this workspace took it
-    size_t asked = 0;              // all pieces of this call so far
+    size_t pooled = 0;             // bytes of this call's pieces from the pool
     void* extra[8] = {};           // pieces from the pool (did not fit the arena)
     int captured = -1;             // whether the stream is being captured (-1: not asked yet)
     unsigned long long capture_id = 0;
@@ -223,6 +224,7 @@ struct Workspace {
             if (p) (void)hipFreeAsync(p, s);
         if (block) block->used = mark;
         if (arena) {
+            arena->pooled -= pooled;
             if (!capturing()) arena->grow(s);  // so that one call is enough before a capture
             arena->mu.unlock();
         }
@@ -263,14 +265,16 @@ struct Workspace {
             return hipSuccess;
         }
         open();
-        asked += take;
         if (block && take <= block->cap - block->used) {
             *p = reinterpret_cast<T*>(block->base + block->used);
             block->used += take;
             return hipSuccess;
         }
         if (capturing()) return hipErrorStreamCaptureUnsupported;
-        if (mark + asked > arena->want) arena->want = mark + asked;
+        // (with what the calls around this one have, so that the block fits them together)
+        pooled += take;
+        arena->pooled += take;
+        if (block->used + arena->pooled > arena->want) arena->want = block->used + arena->pooled;
         for (void*& slot : extra)
             if (!slot) {
                 const hipError_t e = hipMallocAsync(reinterpret_cast<void**>(p), bytes, s);
@@ -1340,7 +1344,7 @@ static int run_grouped(const vedic_grouped_desc_t* d) {
         const int64_t na = gather || !a.rows ? R : d->a_rows, per_b = tn ? R : d->op == VEDIC_OP_NN ? d->K : N;
         const int64_t nb = tn ? R : per_b * d->groups;
         const size_t bytes_a = ca ? (size_t)na * whole(a_cols) * 2 : 0, bytes_b = cb ? (size_t)nb * whole(b_cols) * 2 : 0;
-        if (bytes_a + bytes_b <= kPadBytes && ws.room(bytes_a + bytes_b + 256)) {
+        if (bytes_a + bytes_b <= kPadBytes && ws.room(Workspace::rounded(bytes_a) + Workspace::rounded(bytes_b))) {
             void* pa = nullptr;
             void* pb = nullptr;
             hipError_t e = ca ? ws.get(&pa, bytes_a) : hipSuccess;
@@ -1387,7 +1391,7 @@ static int run_grouped(const vedic_grouped_desc_t* d) {
     // sums in order.
     const int ks = tn && vec ? grouped_ksplit(d->groups, d->M, N, R, device_cu_count()) : 1;
     const size_t slab = (size_t)d->groups * d->M * N, sums = (size_t)d->groups * N;
-    if (ks > 1 && ws.room(4 * ks * (slab + sums) + 512)) {
+    if (ks > 1 && ws.room(Workspace::rounded(4 * ks * slab) + (d->db ? Workspace::rounded(4 * ks * sums) : 0))) {
         float* cw = nullptr;
         float* dw = nullptr;
         hipError_t e = ws.get(&cw, 4 * ks * slab);
