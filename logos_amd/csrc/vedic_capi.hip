@@ -1238,14 +1238,18 @@ extern "C" int vedic_group_rows(const int* ids, int n, int per_row, int groups, 
 }
 
 // Slices of a TN product whose 128 x 128 tiles number at most half the CUs: as many as
-// give every CU one, of 512 rows on average at least (1: none).
+// give every CU one, of 512 rows on average at least (1: none).  A tile takes about 8 us
+// per 1024 rows and the slabs with their sum 6 to 10, so the slices have to save 1536 rows
+// (us, unsplit / split: two groups of 4500 rows 424 x 960 44.0 / 28.0, two of 8192 rows 512 x 512
+// 66.1 / 23.6, one of 8192 1024 x 1024 67.6 / 33.3; eight of 1024 512 x 256 13.0 / 18.7).
 static int grouped_ksplit(int groups, int M, int N, int R, int cus) {
     const int64_t tiles = (int64_t)groups * ((M + 127) / 128) * ((N + 127) / 128);
     if (tiles * 2 > cus) return 1;
+    const int64_t each = R / groups;
     int64_t s = cus / tiles;
-    s = s < R / groups / 512 ? s : R / groups / 512;
+    s = s < each / 512 ? s : each / 512;
     s = s < 16 ? s : 16;
-    return s >= 2 ? (int)s : 1;
+    return each * (s - 1) >= 1536 * s ? (int)s : 1;
 }
 
 // vec: binary16 operands whose rows 16-byte loads can take.
