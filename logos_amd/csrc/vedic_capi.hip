@@ -1252,6 +1252,24 @@ static int grouped_ksplit(int groups, int M, int N, int R, int cus) {
     return each * (s - 1) >= 1536 * s ? (int)s : 1;
 }
 
+// Slices of an NN or NT product without GELU whose tiles number at most half the CUs (128 x
+// 128 on the 16-byte binary16 kernels, else 64 x 64 and three wave groups).  The binary16
+// kernel takes about 8 us per 1024 steps, so slices have to save that many; the other takes
+// 17 and any slice of 256 steps pays (us, unsplit / split, binary16 rows, groups, K -> N: 1920, 6,
+// 3624 -> 448 40.2 / 29.7; 438, 12, 3456 -> 320 30.8 / 16.4; 512, 4, 2048 -> 512 21.0 / 15.7; 1000, 2,
+// 1024 -> 1024 15.7 / 19.1; fp32 438, 12, 3456 -> 320 67.0 / 30.0; 512, 4, 2048 -> 512 43.3 / 23.1;
+// 1000, 2, 1024 -> 1024 28.0 / 26.2; 64, 2, 512 -> 512 16.1 / 13.2).
+static int grouped_ksplit_rows(int groups, int R, int N, int K, bool vec, int cus) {
+    if (vec && R <= 8 * groups) return 1;  // (the few-row kernel splits among its waves)
+    const int b = vec ? 128 : 64;
+    const double tiles = ((double)R / b + 0.5 * (groups < R ? groups : R)) * ((N + b - 1) / b);
+    if (tiles * 2 > cus) return 1;
+    const int fit = (int)(cus / tiles), most = K / (vec ? 512 : 256);
+    int s = fit < most ? fit : most;
+    s = s < 8 ? s : 8;
+    return s >= 2 && (!vec || (int64_t)K * (s - 1) >= (int64_t)1024 * s) ? s : 1;
+}
+
 // vec: binary16 operands whose rows 16-byte loads can take.
 static hipError_t launch_grouped(int op, const GroupedArgs& a, int kind, bool f16, bool f16out, bool vec, hipStream_t s) {
     // At most eight rows a group (us, tiles / few-row kernel, 8 groups: NN 1024 into 4096, 8
@@ -1412,6 +1430,22 @@ static int run_grouped(const vedic_grouped_desc_t* d) {
         if (e == hipSuccess)
             e = launch_slab_sum(cw, ks, d->groups, d->M, N, static_cast<float*>(d->C), d->ldc, d->stride_c, d->beta, ws.s);
         if (e == hipSuccess && dw) e = launch_slab_sum(dw, ks, d->groups, 1, N, d->db, N, N, d->db_beta, ws.s);
+        return hip_status(e);
+    }
+    // NN and NT with few tiles and a long contraction the same way.
+    const int kr = !tn && kind == GK_LINEAR ? grouped_ksplit_rows(d->groups, R, N, d->K, vec, device_cu_count()) : 1;
+    if (kr > 1 && ws.room(Workspace::rounded(4 * (size_t)kr * R * N))) {
+        float* cw = nullptr;
+        hipError_t e = ws.get(&cw, 4 * (size_t)kr * R * N);
+        if (e != hipSuccess) return hip_status(e);
+        a.C = cw;
+        a.ldc = N;
+        a.bias = nullptr;
+        a.split_c = (int64_t)R * N;
+        a.ksplit = kr;
+        e = launch_grouped(d->op, a, kind, f16, false, vec, ws.s);
+        if (e == hipSuccess)
+            e = launch_slab_rows(cw, kr, R, N, d->offsets, d->groups, wants_bias ? d->bias : nullptr, d->C, d->ldc, f16out, ws.s);
         return hip_status(e);
     }
     a.ksplit = 1;

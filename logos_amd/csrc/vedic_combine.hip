@@ -243,6 +243,34 @@ __global__ void __launch_bounds__(256) slab_sum_kernel(const float* ws, int S, i
     }
 }
 
+// C = the sum of S slabs [R x N], in order, plus the group's bias, in the groups' rows.
+// One row per workgroup row (blockIdx.y), found among the groups by bisection.
+template <typename OT>
+__global__ void __launch_bounds__(256) slab_rows_kernel(const float* ws, int S, int R, int N, const int* offsets, int groups,
+                                                        const float* bias, OT* C, int64_t ldc) {
+    const int n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= N) return;
+    for (int r = blockIdx.y; r < R; r += gridDim.y) {
+        int e = 0;
+        if (offsets != nullptr) {
+            // (the last group that starts at or before r: the groups before it end there)
+            int lo = 0, hi = groups;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (offsets[mid] <= r) lo = mid;
+                else hi = mid - 1;
+            }
+            e = lo;
+            if (e >= groups || offsets[0] > r) continue;
+        }
+        const float* w = ws + (int64_t)r * N + n;
+        float t = w[0];
+        for (int s = 1; s < S; ++s) t += w[(int64_t)s * R * N];
+        if (bias != nullptr) t += bias[(int64_t)e * N + n];
+        C[r * ldc + n] = (OT)t;
+    }
+}
+
 bool rows_ok(const void* p, int64_t ld, int es, int chunk) {
     return p == nullptr || ((reinterpret_cast<uintptr_t>(p) % chunk) == 0 && (ld * es) % chunk == 0);
 }
@@ -302,6 +330,16 @@ hipError_t launch_slab_sum(const float* ws, int S, int groups, int M, int N, flo
     int64_t blocks = (slab + 255) / 256;
     if (blocks > 65536) blocks = 65536;
     hipLaunchKernelGGL(slab_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, s, ws, S, slab, M, N, C, ldc, stride_c, beta);
+    return hipGetLastError();
+}
+
+hipError_t launch_slab_rows(const float* ws, int S, int R, int N, const int* offsets, int groups, const float* bias, void* C,
+                            int64_t ldc, bool out16, hipStream_t s) {
+    const dim3 g((unsigned)((N + 255) / 256), (unsigned)(R < 32768 ? R : 32768)), b(256);
+    if (out16)
+        hipLaunchKernelGGL(slab_rows_kernel<_Float16>, g, b, 0, s, ws, S, R, N, offsets, groups, bias, static_cast<_Float16*>(C), ldc);
+    else
+        hipLaunchKernelGGL(slab_rows_kernel<float>, g, b, 0, s, ws, S, R, N, offsets, groups, bias, static_cast<float*>(C), ldc);
     return hipGetLastError();
 }
 

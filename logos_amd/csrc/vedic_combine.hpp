@@ -41,6 +41,10 @@ hipError_t launch_gather_rows(const void* src, int64_t ld, int nsrc, const int* 
 // C_g = beta C_g + the sum of S slabs [groups][M x N], in order.
 hipError_t launch_slab_sum(const float* ws, int S, int groups, int M, int N, float* C, int64_t ldc, int64_t stride_c, float beta,
                            hipStream_t s);
+// C (binary16 with out16) = the sum of S slabs [R x N], in order, plus the group's bias (or
+// none) in the rows 0 .. offsets[groups] - 1 (null offsets: one group of all rows).
+hipError_t launch_slab_rows(const float* ws, int S, int R, int N, const int* offsets, int groups, const float* bias, void* C,
+                            int64_t ldc, bool out16, hipStream_t s);
 // dst [n x roundup(cols, 8)] binary16 = n rows of `cols` values of src (matrices of `per`
 // rows, `stride` apart; or its rows rows[i], nsrc of them there), padded with zeros; n > 0.
 hipError_t launch_pad_rows(const void* src, int64_t ld, int per, int64_t stride, int nsrc, const int* rows, int64_t n, int cols,

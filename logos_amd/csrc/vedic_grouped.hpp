@@ -58,8 +58,9 @@ struct GroupedArgs {
     const float* scales;  // GK_ADD: [groups], or null
     float* db;  // TN: [groups x N] column sums of B, or null
     float db_beta;
-    // TN split over the contraction: slice s of a group's rows goes to C + s split_c (C
-    // then a workspace of [ksplit][groups][M x N]) and db + s groups N.  1: no split.
+    // The contraction split over workgroups: slice s goes to C + s split_c (C then a
+    // workspace of [ksplit][groups][M x N], NN and NT [ksplit][R x N]) and db + s groups
+    // N.  1: no split.
     int ksplit;
     int64_t split_c;
     int tiles_m, tiles_n;

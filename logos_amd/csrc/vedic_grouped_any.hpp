@@ -147,6 +147,8 @@ __device__ __forceinline__ void any_block_slow(const T* const (&pa)[MI], const b
 // WGK > 1: that many groups of WGM x WGN waves, each with LDS buffers of its own and
 // a part of the contraction (whole stages); the others leave their sums in LDS for the
 // first, which adds them in order and runs the epilogue.
+// NN and NT with a.ksplit > 1: the grid's second dimension counts slices of the
+// contraction, each into its own slab (vedic_grouped.hpp).
 // T, TB, OT: the types of A, B and C.
 template <int OP, typename T, typename TB, typename OT, int BM, int BN, int WGM, int WGN, int WGK, int KIND>
 __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(GroupedArgs a) {
@@ -219,7 +221,10 @@ __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(Groupe
     // (fp32 rows are loaded four steps at a time: the last K mod 4 come at the end)
     const int Kq = OP != 2 && sizeof(T) == 4 ? K & ~3 : K;
     const int nk_all = few ? 0 : (Kq + kSplitK - 1) / kSplitK;
-    const int nk = (nk_all + WGK - 1) / WGK, kt0 = wk * nk;  // stages of this wave group, the first of them
+    const int slices = OP == 2 ? 1 : gridDim.y, slice = OP == 2 ? 0 : blockIdx.y;
+    const int nk = (nk_all + WGK * slices - 1) / (WGK * slices);  // stages of a wave group
+    const int kt0 = (slice * WGK + wk) * nk;                      // the first of this one's
+    const int Ka = min(Kq, slice * WGK * nk * kSplitK), Kz = slice + 1 < slices ? min(Kq, Ka + WGK * nk * kSplitK) : K;
     auto load = [&](int kt) {
         const bool in = kt < nk && kt0 + kt < nk_all;
         const int64_t k = in ? (int64_t)(kt0 + kt) * kSplitK : 0;
@@ -316,7 +321,7 @@ __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(Groupe
             probe = nonfinite_probe(acc[i][j], probe);
         }
     const bool again = few || __any(probe != 0.0f);
-    if (again || Kq < K) {
+    if (again || Kq < Kz) {
         const T* pa[MI];
         const TB* pb[NI];
         bool oka[MI];
@@ -343,7 +348,7 @@ __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(Groupe
 #pragma unroll
                 for (int j = 0; j < NI; ++j) acc[i][j] = float16_t{};
         }
-        any_block_slow<T, TB, MI, NI>(pa, oka, ka, pb, kb, again ? 0 : Kq, K, lane >> 5, acc);
+        any_block_slow<T, TB, MI, NI>(pa, oka, ka, pb, kb, again ? Ka : Kq, Kz, lane >> 5, acc);
     }
     if constexpr (KIND == GK_ADD) {
         grouped_add<MI, NI>(static_cast<float*>(a.C), a.ldc, a.out_rows + start + m0 + wm * WM, a.out_limit,
@@ -352,7 +357,7 @@ __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(Groupe
     }
     const int row0 = m0 + wm * WM;
     const int64_t crow = OP == 2 ? row0 : start + row0;
-    OT* C = static_cast<OT*>(a.C) + (OP == 2 ? (int64_t)e * a.stride_c : 0) + crow * a.ldc;
+    OT* C = static_cast<OT*>(a.C) + (OP == 2 ? (int64_t)e * a.stride_c : slice * a.split_c) + crow * a.ldc;
     OT* P = a.P != nullptr ? static_cast<OT*>(a.P) + crow * a.ldp : nullptr;
     if constexpr (WGK == 1) __syncthreads();  // the bias (the sums' barriers have shown it otherwise)
     if (grouped_reads(KIND) && a.wide)
@@ -389,7 +394,7 @@ static hipError_t launch_any(GroupedArgs a, hipStream_t s) {
     if (work > 0x7FFFFFFF) return hipErrorInvalidValue;  // (the caller has refused such sizes)
     if (work == 0) return hipSuccess;
     hipLaunchKernelGGL((grouped_any_kernel<OP, T, TB, OT, Cfg::BM, Cfg::BN, Cfg::WGM, Cfg::WGN, WGK, KIND>),
-                       dim3((unsigned)work), dim3(Cfg::WGM * Cfg::WGN * WGK * 64), 0, s, a);
+                       dim3((unsigned)work, OP != 2 && a.ksplit > 1 ? a.ksplit : 1), dim3(Cfg::WGM * Cfg::WGN * WGK * 64), 0, s, a);
     return hipGetLastError();
 }
 

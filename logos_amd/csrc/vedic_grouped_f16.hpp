@@ -144,12 +144,12 @@ struct StageSums {
 
 // One work item: a tile of one group.
 struct GroupedItem {
-    int e, start, m0, n0, left, K, nk, slice;
+    int e, start, m0, n0, left, K, nk, slice, k0;  // k0: NN and NT, the slice's first step
 };
 
 // Work item w counts tiles of PM x PN; with SM x SN > 1 a tile is cut into that
 // many parts of BM x BN and w counts the parts.
-template <int OP, int BM, int BN, int BK, int SM, int SN>
+template <int OP, int BM, int BN, int BK, int SM, int SN, bool SPLIT>
 __device__ __forceinline__ GroupedItem grouped_item(const GroupedArgs& a, const GroupIndex& ix, int w, int lane) {
     constexpr int PM = BM * SM, PN = BN * SN;
     GroupedItem it;
@@ -167,6 +167,18 @@ __device__ __forceinline__ GroupedItem grouped_item(const GroupedArgs& a, const 
         it.K = max(0, min(len, count - it.slice * len));
         it.left = a.M;
     } else {
+        it.slice = it.k0 = 0;
+        it.K = a.K;
+        if constexpr (SPLIT) {
+            if (a.ksplit > 1) {
+                const int len = ((a.K + a.ksplit - 1) / a.ksplit + BK - 1) / BK * BK;
+                const int each = __builtin_amdgcn_readfirstlane(ix.pre[a.groups]) * a.tiles_n;
+                it.slice = __builtin_amdgcn_readfirstlane(w / each);
+                w -= it.slice * each;
+                it.k0 = min(a.K, it.slice * len);
+                it.K = min(len, a.K - it.k0);
+            }
+        }
         it.e = group_of(ix, a.groups, w / a.tiles_n, lane);
         const int p0 = __builtin_amdgcn_readfirstlane(ix.pre[it.e]);
         const int mt = __builtin_amdgcn_readfirstlane(ix.pre[it.e + 1]) - p0;
@@ -176,7 +188,6 @@ __device__ __forceinline__ GroupedItem grouped_item(const GroupedArgs& a, const 
         it.m0 = (first + in % rows) * PM;
         it.n0 = in / rows * PN;
         it.left = group_count(a, it.e);
-        it.K = a.K;
     }
     it.m0 += part % SM * BM;
     it.n0 += part / SM * BN;
@@ -237,6 +248,11 @@ __device__ __forceinline__ const _Float16* uniform(const _Float16* p) {
         } else {                                                                                               \
             Bb += (int64_t)it.e * a.stride_b + (B_KC ? (int64_t)it.n0 * a.ldb : it.n0);                        \
             if (!a.rows) Ab += (int64_t)(it.start + it.m0) * a.lda;                                            \
+            if constexpr (SPLIT) {                                                                             \
+                Ab += it.k0;                                                                                   \
+                Bb += B_KC ? (int64_t)it.k0 : it.k0 * a.ldb;                                                   \
+                kpad = OP == 0 && it.k0 + it.K == a.K ? a.kpad : 0;                                            \
+            }                                                                                                  \
             sa.init(wave, lane, a.lda, a.rows ? a.a_rows : BM);                                                \
         }                                                                                                      \
         sb.init(wave, lane, a.ldb, it.n0, B_KC ? a.N : a.Np);                                                  \
@@ -260,6 +276,7 @@ __device__ __forceinline__ void grouped_tiles(const GroupedArgs& a, const GroupI
     constexpr int L = SA::NLD + SB::NLD;
     static_assert(ST >= 2 && ST <= 3, "2 or 3 LDS stages");
     constexpr bool kInterleave = BM * BN >= 256 * 256;
+    constexpr bool SPLIT = OP != 2 && ST == 3;  // (the small kernel's tiles)
     constexpr bool kBias = !grouped_reads(KIND);
     char* const As[3] = {t0, t1, t2};
     char* const Bs[3] = {t0 + SA::BYTES, t1 + SA::BYTES, t2 + SA::BYTES};
@@ -269,7 +286,7 @@ __device__ __forceinline__ void grouped_tiles(const GroupedArgs& a, const GroupI
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int wm = wave / WGN, wn = wave % WGN;
-    GroupedItem it = grouped_item<OP, BM, BN, BK, SM, SN>(a, ix, first, lane), nx = it;
+    GroupedItem it = grouped_item<OP, BM, BN, BK, SM, SN, SPLIT>(a, ix, first, lane), nx = it;
     if (SM * SN > 1 && (it.left <= 0 || it.n0 >= a.N)) return;  // a part past the tile's edge
     SA sa;
     SB sb;
@@ -277,7 +294,7 @@ __device__ __forceinline__ void grouped_tiles(const GroupedArgs& a, const GroupI
     const _Float16* Bb;
     float bnext = 0.0f;
     int krem;  // contraction steps not yet loaded
-    const int kpad = OP == 0 ? a.kpad : 0;
+    int kpad = OP == 0 ? a.kpad : 0;
     const int64_t astep = LIST ? 0 : BK * a.lda;  // (TN)
     VEDIC_G_NEXT();
     VEDIC_G_START();
@@ -289,7 +306,7 @@ __device__ __forceinline__ void grouped_tiles(const GroupedArgs& a, const GroupI
         const int wn_ = OP == 2 && LOOP && (round & 1) ? first + round * step + (step - 1 - 2 * (first % step)) : first + round * step;
         const bool more = LOOP && wn_ < nwork;
         if (more) {
-            nx = grouped_item<OP, BM, BN, BK, SM, SN>(a, ix, wn_, lane);
+            nx = grouped_item<OP, BM, BN, BK, SM, SN, SPLIT>(a, ix, wn_, lane);
             VEDIC_G_NEXT();
         }
         float16_t acc[MI][NI];
@@ -341,7 +358,8 @@ __device__ __forceinline__ void grouped_tiles(const GroupedArgs& a, const GroupI
         }
         const int row0 = done.m0 + wm * WM, col0 = done.n0 + wn * WN, left = done.left - wm * WM;
         const int64_t crow = OP == 2 ? row0 : done.start + row0;
-        OT* const C = static_cast<OT*>(a.C) + (OP == 2 ? done.slice * a.split_c + (int64_t)done.e * a.stride_c : 0) + crow * a.ldc;
+        OT* const C = static_cast<OT*>(a.C) + (OP == 2 ? done.slice * a.split_c + (int64_t)done.e * a.stride_c : SPLIT ? done.slice * a.split_c : 0) +
+                      crow * a.ldc;
         OT* const P = a.P != nullptr ? static_cast<OT*>(a.P) + crow * a.ldp : nullptr;
         if (nk == 0) __syncthreads();  // (no stage's barrier has shown the bias)
         if (grouped_reads(KIND) && !a.wide)
@@ -404,7 +422,7 @@ __global__ void __launch_bounds__(256) grouped_f16_small_kernel(GroupedArgs a) {
     __shared__ __attribute__((aligned(16))) float sb0[128];
     __shared__ __attribute__((aligned(16))) float sb1[128];
     group_index(a, ix, 128);
-    const int nwork = min((int64_t)__builtin_amdgcn_readfirstlane(ix.pre[a.groups]) * a.tiles_n, (int64_t)a.most);
+    const int nwork = min((int64_t)__builtin_amdgcn_readfirstlane(ix.pre[a.groups]) * a.tiles_n * a.ksplit, (int64_t)a.most);
     const int G = gridDim.x, b = blockIdx.x;
     const int w = (G & 7) == 0 ? (b & 7) * (G >> 3) + (b >> 3) : b;
     if (w < nwork)
@@ -426,10 +444,10 @@ inline hipError_t grouped_grid(int op, GroupedArgs& a, int b, int parts, int es_
     if (a.ksplit < 1) a.ksplit = 1;
     const int64_t most = op == 2 ? (int64_t)a.groups * a.tiles_m * a.tiles_n * a.ksplit
                                  : (int64_t)(a.R / b + (a.groups < a.R ? a.groups : a.R)) * a.tiles_n;
-    if (most * parts > 0x7FFFFFFF) return hipErrorInvalidValue;  // (the caller has refused such sizes)
-    a.most = (int)most;
+    if (most * parts * (op == 2 ? 1 : a.ksplit) > 0x7FFFFFFF) return hipErrorInvalidValue;  // (the caller has refused such sizes)
+    a.most = (int)(op == 2 ? most : most * a.ksplit);
     const int cus = device_cu_count();
-    grid = most * parts < cus ? (int)(most * parts) : cus;
+    grid = (int64_t)a.most * parts < cus ? a.most * parts : cus;
     return hipSuccess;
 }
 

@@ -54,6 +54,8 @@ SIZES = [
     ([12, 31], 17, 33),                     # nothing aligned
     ([150, 90], 131, 259),
     ([2100, 1, 3000], 40, 56),              # few tiles and long groups: the contraction is shared (TN)
+    ([130, 0, 5, 111], 2056, 104),          # and a long one of few rows (NN, NT)
+    ([60, 1], 2051, 67),
 ]
 COMBOS = [(F16, F16), (F16, F32), (F32, F32)]
 
@@ -241,6 +243,39 @@ def test_values_that_are_not_finite(dt):
     keep[5] = keep[70] = False
     keep[:48, 7] = False
     torch.testing.assert_close(got[keep], clean[keep], rtol=0, atol=64 * 2.0 ** -19)  # 2 K u sum |ab|, the sum below 16
+
+
+@pytest.mark.parametrize("out", [F16, F32])
+@pytest.mark.parametrize("dt,K", [(F16, 2056), (F16, 2051), (F32, 2050)])
+def test_shared_contraction(dt, K, out):
+    """A long contraction of few rows: values that are not finite in each part of it, pitched rows, rows behind the last
+    group and between C's rows."""
+    if out == F16 and dt == F32:
+        pytest.skip("float32 operands give float32")
+    v = vedic()
+    rng = np.random.default_rng(K)
+    sizes, N, extra = [40, 0, 24], 72, 5
+    off, R = sizes_to_offsets(sizes), 64
+    X, x = make(rng, (R + extra, K), dt)
+    W, w = make(rng, (3, K, N), dt, K ** -0.5)
+    bad = {3: (7, float("inf")), 11: (K // 2, float("nan")), 50: (K - 1, float("-inf"))}
+    for r, (k, value) in bad.items():
+        X[r, k] = value
+    X[R:] = float("nan")
+    b, bv = make(rng, (3, N), F32)
+    g = np.repeat(np.arange(3), sizes)
+    dot = np.einsum("rk,rkn->rn", x[:R], w[g])
+    absdot = np.einsum("rk,rkn->rn", np.abs(x[:R]), np.abs(w[g]))
+    keep = np.array([r not in bad for r in range(R)])
+    for op, B in ((v.OP_NN, W), (v.OP_NT, W.transpose(1, 2).contiguous())):
+        kw, t = (dict(bias=b, epilogue=v.EPI_BIAS), bv[g]) if op == v.OP_NN else ({}, np.zeros((R, N)))
+        C = pitched(torch.full((R + extra, N), 7.0, device="cuda", dtype=out), 8)
+        got = v.gemm_grouped(op, pitched(X, 8), B, ints(off), C, **kw)
+        check_rows(got[:R].double().cpu().numpy()[keep], (dot + t)[keep], absdot[keep], K, out, "shared",
+                   terms=(np.abs(dot) + np.abs(t))[keep])
+        assert not torch.isfinite(got[:R].float()[torch.from_numpy(~keep).cuda()]).any()
+        assert torch.all(got[R:] == 7.0)
+        assert torch.isnan(C._base.view(R + extra, N + 8)[:, N:]).all()
 
 
 @pytest.mark.parametrize("op", ["NN", "TN"])
