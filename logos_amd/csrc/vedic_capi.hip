@@ -1570,7 +1570,8 @@ static int run_base(const vedic_gemm_desc_t* b) {
     d.ldc = b->ldc;
     d.bias = b->bias;
     d.stream = b->stream;
-    return run_grouped(&d);
+    const int st = run_grouped(&d);
+    return st == VEDIC_STATUS_TOO_LARGE ? vedic_gemm(b) : st;  // (refused: nothing has run)
 }
 
 // C += the adapters' products, after `base` where one is given (the workspace first: a

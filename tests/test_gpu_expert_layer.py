@@ -114,8 +114,15 @@ def test_layer_in_a_graph():
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
 
+    long = torch.randn(64, 2048, device="cuda")
+    Wl = torch.randn(2, 2048, 96, device="cuda")
+    tall, dt = torch.randn(8192, 64, device="cuda").half(), torch.randn(8192, 128, device="cuda").half()
+    ends = {n: torch.tensor([0, n // 3, n], dtype=torch.int32, device="cuda") for n in (64, 8192)}
+
     def work():
-        return [L.step(), odd.step(), dict(lora=v.gemm_lora(la["X"], la["W"], la["A"], la["B"], off, rows))]
+        # (a long contraction shared by several workgroups, fp32 NN and binary16 TN)
+        shared = dict(nn=v.gemm_grouped(v.OP_NN, long, Wl, ends[64]), tn=v.gemm_grouped(v.OP_TN, tall, dt, ends[8192]))
+        return [L.step(), odd.step(), shared, dict(lora=v.gemm_lora(la["X"], la["W"], la["A"], la["B"], off, rows))]
 
     with torch.cuda.stream(s):
         work()  # the stream's workspace block
@@ -129,6 +136,8 @@ def test_layer_in_a_graph():
             layer.x.copy_(torch.randn_like(layer.x))
             layer.dout.copy_(torch.randn_like(layer.dout))
         la["X"].copy_(torch.randn_like(la["X"]))
+        long.copy_(torch.randn_like(long))
+        tall.copy_(torch.randn_like(tall))
         g.replay()
         torch.cuda.synchronize()
         eager = work()
@@ -164,6 +173,38 @@ def test_capture_without_a_block_is_refused():
     torch.cuda.synchronize()
     assert torch.all(C == 7.0)
     torch.testing.assert_close(D, want, rtol=0, atol=41 * 2.0 ** -17)  # 2 K u sum |ab|, the sum below 64
+
+
+def test_rows_past_two_gibibytes():
+    """Row lists into operands whose offsets pass 32 bits, and outputs that do."""
+    v = vedic()
+    rows = torch.tensor([0, 1_099_999, 7, 600_123, 1_048_577], dtype=torch.int32, device="cuda")
+    for dt, T in ((F16, 1_100_000), (torch.float32, 1_100_000)):
+        X = torch.empty(T, 1024, dtype=dt, device="cuda")
+        x = torch.randn(5, 1024, device="cuda").to(dt)
+        X[rows.long()] = x
+        W = (torch.randn(2, 1024, 64, device="cuda") / 32).to(dt)
+        off = torch.tensor([0, 2, 5], dtype=torch.int32, device="cuda")
+        assert torch.equal(v.gemm_grouped(v.OP_NN, X, W, off, rows=rows), v.gemm_grouped(v.OP_NN, x, W, off))
+        dY = torch.randn(5, 64, device="cuda").to(dt)
+        assert torch.equal(v.gemm_grouped(v.OP_TN, X, dY, off, rows=rows), v.gemm_grouped(v.OP_TN, x, dY, off))
+        A, B = (torch.randn(2, 1024, 8, device="cuda") / 32).to(dt), torch.randn(2, 8, 1024, device="cuda").to(dt)
+        C = torch.empty(T, 1024, device="cuda")
+        C[rows.long()] = 0.0
+        want = torch.zeros(5, 1024, device="cuda")
+        v.lora_add(want, x, A, B, off, torch.arange(5, dtype=torch.int32, device="cuda"))
+        got = v.lora_add(C, X, A, B, off, rows)
+        assert torch.equal(got[rows.long()], want)
+        # (slots that far into Y, and dY)
+        w = torch.tensor([[0.5, 2.0]], device="cuda")
+        slots = torch.tensor([[1_099_999, 600_123]], dtype=torch.int32, device="cuda")
+        out = v.combine_rows(X, slots, w)
+        torch.testing.assert_close(out[0], 0.5 * x[1].float() + 2.0 * x[3].float(), rtol=2.0 ** -22, atol=2.0 ** -20)
+        g = torch.randn(1, 1024, device="cuda")
+        dYf, dw = v.combine_rows_bwd(g, X, slots, w, dY=C)
+        assert torch.equal(dYf[1_099_999], 0.5 * g[0]) and torch.equal(dYf[600_123], 2.0 * g[0])
+        torch.testing.assert_close(dw[0].double(), x[[1, 3]].double() @ g[0].double(), rtol=0, atol=1024 * 2.0 ** -20)
+        del X, C, dYf
 
 
 def test_streams_and_threads():
