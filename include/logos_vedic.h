@@ -533,7 +533,11 @@ int vedic_group_rows(const int* ids, int n, int per_row, int groups, int* offset
  * are multiples of 8 run on the fast kernels as they are; others are copied into padded
  * rows in the stream's workspace block first, up to 256 MiB of them, or run on general
  * kernels.  Also in that block: the listed rows of fp32 TN products and of an A of 2 GiB
- * or more, and the slabs of TN products with few tiles and long groups (at most 16 MiB). */
+ * or more, and the slabs of products with few tiles and a long contraction, which several
+ * workgroups then share (at most 16 MiB; epilogues NONE and BIAS).  A captured call whose
+ * stream has no such block, or one too small, does without the padded copies and the
+ * slabs (results may then differ in rounding), and is refused where it needs the listed
+ * rows. */
 typedef struct {
     int op, in_dtype, out_dtype, epilogue;
     int groups;
@@ -587,14 +591,18 @@ int vedic_combine_rows_bwd(const float* dout, int64_t ld_dout, const void* Y, in
  * B_g [r x N] contiguous, one after another; X, A, B all F32 or all F16, C fp32
  * [M x N], scales NULL: ones.  The product with A_g stays in fp32.  A row may be listed
  * once (two adapters on one row would add to it at the same time); rows not listed
- * keep their content.  r <= 128.  Takes n r 4 bytes of the stream's workspace block. */
+ * keep their content.  r <= 128.  Takes about 4 n r bytes of the stream's workspace block
+ * (r rounded up to 32, 64 or 128), and n K values where X is 2 GiB or more and is F32 or
+ * not 16-byte aligned. */
 int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, const void* A, const void* B, int groups, int r,
                    const int* offsets, const int* rows, int n, const float* scales, float* C, int64_t ldc, int K, int N,
                    void* stream);
 
-/* The shared projection with them: vedic_gemm(base), then vedic_lora_add of base->A
+/* The shared projection with them: base's product, then vedic_lora_add of base->A
  * onto base->C.  base: op NN, F32 or F16 in, F32 out, epilogue NONE or BIAS, no preact
- * or colsum. */
+ * or colsum.  Operands that are not 16-byte aligned run on the grouped kernels (one
+ * group), whose sums may round differently from vedic_gemm's.  A refused call has
+ * written nothing. */
 int vedic_gemm_lora(const vedic_gemm_desc_t* base, const void* A, const void* B, int groups, int r, const int* offsets,
                     const int* rows, int n, const float* scales);
 

@@ -1258,16 +1258,24 @@ static int grouped_ksplit(int groups, int M, int N, int R, int cus) {
 // 17 and any slice of 256 steps pays (us, unsplit / split, binary16 rows, groups, K -> N: 1920, 6,
 // 3624 -> 448 40.2 / 29.7; 438, 12, 3456 -> 320 30.8 / 16.4; 512, 4, 2048 -> 512 21.0 / 15.7; 1000, 2,
 // 1024 -> 1024 15.7 / 19.1; fp32 438, 12, 3456 -> 320 67.0 / 30.0; 512, 4, 2048 -> 512 43.3 / 23.1;
-// 1000, 2, 1024 -> 1024 28.0 / 26.2; 64, 2, 512 -> 512 16.1 / 13.2).
+// 64, 2, 512 -> 512 16.1 / 13.2).  Where 64 x 64 tiles are more than that and 128 x 128 ones
+// are not, slices of 384 steps of the latter (64 x 64 unsplit / 128 x 128 split: 1920, 6, 3624 -> 448
+// 80.9 / 63.5; 4414, 8, 1368 -> 355 66.1 / 49.6; 3000, 4, 1000 -> 500 49.1 / 36.6; 1000, 2, 1024 ->
+// 1024 26.1 / 31.3; with slices of 300 steps 2000, 3, 600 -> 400 19.2 / 26.1).
 static int grouped_ksplit_rows(int groups, int R, int N, int K, bool vec, int cus) {
     if (vec && R <= 8 * groups) return 1;  // (the few-row kernel splits among its waves)
-    const int b = vec ? 128 : 64;
-    const double tiles = ((double)R / b + 0.5 * (groups < R ? groups : R)) * ((N + b - 1) / b);
+    auto tiles_of = [&](int b) { return ((double)R / b + 0.5 * (groups < R ? groups : R)) * ((N + b - 1) / b); };
+    double tiles = tiles_of(vec ? 128 : 64);
+    const bool large = !vec && tiles * 2 > cus;
+    const double rounds = tiles > cus ? tiles / cus : 1.0;
+    if (large) tiles = tiles_of(128);  // (launch_any_tiles takes those then)
     if (tiles * 2 > cus) return 1;
-    const int fit = (int)(cus / tiles), most = K / (vec ? 512 : 256);
+    const int fit = (int)(cus / tiles), most = K / (vec ? 512 : large ? 384 : 256);
     int s = fit < most ? fit : most;
     s = s < 8 ? s : 8;
-    return s >= 2 && (!vec || (int64_t)K * (s - 1) >= (int64_t)1024 * s) ? s : 1;
+    if (s < 2 || (vec && (int64_t)K * (s - 1) < (int64_t)1024 * s)) return 1;
+    // (a stage of the larger tiles takes 1.8 times as long, the slabs as long as 384 steps)
+    return large && rounds * K < 1.8 * K / s + 384.0 ? 1 : s;
 }
 
 // vec: binary16 operands whose rows 16-byte loads can take.
@@ -1610,6 +1618,7 @@ static LoraArgs lora_args(const void* X, int64_t ldx, int M, const void* A, cons
     a.K = K;
     a.N = N;
     a.r = r;
+    a.ksplit = grouped_ksplit_rows(groups, n, r, K, false, device_cu_count());
     return a;
 }
 

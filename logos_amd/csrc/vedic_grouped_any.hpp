@@ -4,8 +4,10 @@
 // Every value is split into bf16 parts as it goes to LDS (vedic_split.hpp), six
 // v_mfma_f32_32x32x16_bf16 per 32 x 32 x 16 block, the arithmetic of the
 // ungrouped fp32 product (vedic_gemm_f32s.hpp), whose LDS layout this shares.
-// (A binary16 value has two parts; the third is zero.)  One 128 x 128 tile, or
-// 64 x 64 where those would leave CUs idle, per workgroup; per stage of 16
+// (A binary16 value has two parts; the third is zero.)  The matrix pipe and the split's
+// VALU work bound it, at small sizes each stage's latency: 2006 rows in 7 groups, 1999 into
+// 1001, take 77 us (104 TFLOP/s; the ungrouped library product of this card does 153).
+// One 128 x 128 tile, or 64 x 64 where those would leave CUs idle, per workgroup; per stage of 16
 // contraction steps the values of stage k + 2 are in registers on their way,
 // those of stage k + 1 are split into one LDS buffer while stage k's fragments
 // are read from the other.
@@ -410,7 +412,7 @@ static hipError_t launch_any_tiles(const GroupedArgs& a, hipStream_t s) {
     };
     const int cus = device_cu_count();
     const bool split = (OP == 2 ? a.R / a.groups : a.K) >= 256;
-    if (tiles(128) * 2 > cus) {
+    if (tiles(128) * 2 > cus || (OP != 2 && a.ksplit > 1 && tiles(64) * 2 > cus)) {
         if (split && tiles(128) <= cus) return launch_any<OP, T, TB, OT, CfgAMid, kAnyGroups, KIND>(a, s);
         return launch_any<OP, T, TB, OT, CfgAMid, 1, KIND>(a, s);
     }

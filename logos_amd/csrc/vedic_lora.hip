@@ -4,6 +4,10 @@
 // Two launches, H = X A_g into a workspace (fp32, or the same as two binary16
 // values), then C.  fp32 operands, and rows that 16-byte loads cannot take, run as two
 // grouped products (vedic_grouped_any.hpp).
+//
+// 4096 rows, 1024 into 4096, 12 adapters of rank 64 (all but a twelfth of the rows): 7.9 us
+// for H, bound by the latency of its few workgroups, and 30.2 us for C, bound by reading and
+// writing it (125 MB, 4.1 TB/s); 16 rows of rank 16 4.6 and 4.8 us, two launches' latency.
 #include "vedic_combine.hpp"
 #include "vedic_common.hpp"
 #include "vedic_gemm_f16.hpp"
@@ -245,10 +249,13 @@ __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
 }
 
 // Any types and alignment: two grouped products, the second adding to the listed rows
-// of C.  (`copy`: the listed rows, where X is past the products' 32-bit offsets.)
+// of C.  (`copy`: the listed rows, where X is past the products' 32-bit offsets; `slabs`:
+// H's slices with a.ksplit > 1, as the grouped products share a long contraction: us, one
+// slice / as many as fit, projection included, one row of 768 into 256, rank 4
+// 32.4 / 27.6; 898 rows of 896 into 2496, rank 64 106 / 98.)
 bool copies_rows(const LoraArgs& a, bool f16) { return (int64_t)a.M * a.ldx * (f16 ? 2 : 4) >= (int64_t(1) << 31); }
 
-hipError_t launch_any(const LoraArgs& a, bool f16, void* copy, hipStream_t s) {
+hipError_t launch_any(const LoraArgs& a, bool f16, float* slabs, void* copy, hipStream_t s) {
     GroupedArgs q{};
     q.A = a.X;
     q.lda = a.ldx;
@@ -264,15 +271,20 @@ hipError_t launch_any(const LoraArgs& a, bool f16, void* copy, hipStream_t s) {
     q.B = a.A;
     q.ldb = a.r;
     q.stride_b = (int64_t)a.K * a.r;
-    q.C = a.H;
+    q.C = a.ksplit > 1 ? slabs : a.H;
     q.ldc = a.r;
+    q.ksplit = a.ksplit;
+    q.split_c = (int64_t)a.n * a.r;
     q.offsets = a.offsets;
     q.groups = a.groups;
     q.R = a.n;
     q.N = a.r;
     q.K = a.K;
-    const hipError_t e = launch_grouped_any_nn(q, GK_LINEAR, f16, false, s);
+    hipError_t e = launch_grouped_any_nn(q, GK_LINEAR, f16, false, s);
+    if (e == hipSuccess && a.ksplit > 1)
+        e = launch_slab_rows(slabs, a.ksplit, a.n, a.r, a.offsets, a.groups, nullptr, a.H, a.r, false, s);
     if (e != hipSuccess) return e;
+    q.ksplit = 1;
     q.A = a.H;
     q.lda = a.r;
     q.rows = nullptr;
@@ -317,13 +329,17 @@ size_t lora_bytes(const LoraArgs& a, bool f16) {
         const size_t rs = (size_t)(a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128);
         return (size_t)a.n * (rs * 4 + 4);
     }
-    return rounded((size_t)a.n * a.r * 4) + (copies_rows(a, f16) ? (size_t)a.n * a.K * (f16 ? 2 : 4) : 0);
+    const size_t h = (size_t)a.n * a.r * 4;
+    return rounded(h) + (a.ksplit > 1 ? rounded(a.ksplit * h) : 0) + (copies_rows(a, f16) ? (size_t)a.n * a.K * (f16 ? 2 : 4) : 0);
 }
 
 hipError_t launch_lora(LoraArgs a, bool f16, void* work, hipStream_t s) {
     a.H = static_cast<float*>(work);
-    if (!f16 || !vec16(a))
-        return launch_any(a, f16, static_cast<char*>(work) + rounded((size_t)a.n * a.r * 4), s);
+    if (!f16 || !vec16(a)) {
+        const size_t h = (size_t)a.n * a.r * 4;
+        char* const slabs = static_cast<char*>(work) + rounded(h);
+        return launch_any(a, f16, reinterpret_cast<float*>(slabs), slabs + (a.ksplit > 1 ? rounded(a.ksplit * h) : 0), s);
+    }
     const size_t rs = (size_t)(a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128);
     a.Hs = static_cast<_Float16*>(work);
     a.factor = reinterpret_cast<float*>(a.Hs + (size_t)a.n * 2 * rs);

@@ -20,6 +20,7 @@ struct LoraArgs {
     float* C;             // [M x ldc]
     int64_t ldc;
     int M, K, N, r;
+    int ksplit;  // slices of K in H's product, where that is a grouped product
     // set by the launch
     float* H;       // [n x r]
     _Float16* Hs;   // [n][hi, lo]

@@ -8,7 +8,8 @@
 // token's lanes (one v_max_u32 with DPP per halving), the lowest lane that has it and
 // that lane's lowest place: the lowest expert among equals, without comparing
 // indexes.  The weights are exp(x_j - x_max) over their sum, in fp32.  Instructions
-// bound it: with a wave per token 8192 tokens of 128 experts, 8 chosen, took 66 us.
+// bound it: 8192 tokens of 128 experts, 8 chosen, take 6.3 us (66 with a wave per token)
+// and their placement 7.9; the 5.2 MB they read and write would take 1.1.
 //
 // Sorting is a stable counting sort by expert in two launches: the choice leaves
 // each workgroup's counts per expert, and the placement adds the counts of the
