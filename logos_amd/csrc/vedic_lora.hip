@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
 // of C.  (`copy`: the listed rows, where X is past the products' 32-bit offsets; `slabs`:
 // H's slices with a.ksplit > 1, as the grouped products share a long contraction: us, one
 // slice / as many as fit, projection included, one row of 768 into 256, rank 4
-// 32.4 / 27.6; 898 rows of 896 into 2496, rank 64 106 / 98.)
+// 32.4 / 27.6; 898 rows of 896 into 2496, rank 64 98.3 / 90.6.)
 bool copies_rows(const LoraArgs& a, bool f16) { return (int64_t)a.M * a.ldx * (f16 ? 2 : 4) >= (int64_t(1) << 31); }
 
 hipError_t launch_any(const LoraArgs& a, bool f16, float* slabs, void* copy, hipStream_t s) {
