@@ -1252,6 +1252,21 @@ static int grouped_ksplit(int groups, int M, int N, int R, int cus) {
     return each * (s - 1) >= 1536 * s ? (int)s : 1;
 }
 
+// Slices on the general kernels, of K steps on `t64` tiles of 64 x 64 or `t128` of 128 x 128
+// (TN, us, unsplit / split, rows, groups, M x N: 4096, 2, 256 x 256 44.2 / 16.7; 16384, 4, 512 x 512
+// 84.4 / 57.3; 2000, 2, 1000 x 1000 49.9 / 39.4; NN and NT: grouped_ksplit_rows).
+static int any_ksplit(double t64, double t128, int K, int cus) {
+    const bool large = t64 * 2 > cus;  // (launch_any_tiles takes the larger tiles then)
+    const double tiles = large ? t128 : t64, rounds = t64 > cus ? t64 / cus : 1.0;
+    if (tiles * 2 > cus) return 1;
+    const int fit = (int)(cus / tiles), most = K / (large ? 384 : 256);
+    int s = fit < most ? fit : most;
+    s = s < 8 ? s : 8;
+    if (s < 2) return 1;
+    // (a stage of the larger tiles takes 1.8 times as long, the slabs as long as 384 steps)
+    return large && rounds * K < 1.8 * K / s + 384.0 ? 1 : s;
+}
+
 // Slices of an NN or NT product without GELU whose tiles number at most half the CUs (128 x
 // 128 on the 16-byte binary16 kernels, else 64 x 64 and three wave groups).  The binary16
 // kernel takes about 8 us per 1024 steps, so slices have to save that many; the other takes
@@ -1263,19 +1278,13 @@ static int grouped_ksplit(int groups, int M, int N, int R, int cus) {
 // 80.9 / 63.5; 4414, 8, 1368 -> 355 66.1 / 49.6; 3000, 4, 1000 -> 500 49.1 / 36.6; 1000, 2, 1024 ->
 // 1024 26.1 / 31.3; with slices of 300 steps 2000, 3, 600 -> 400 19.2 / 26.1).
 static int grouped_ksplit_rows(int groups, int R, int N, int K, bool vec, int cus) {
-    if (vec && R <= 8 * groups) return 1;  // (the few-row kernel splits among its waves)
-    auto tiles_of = [&](int b) { return ((double)R / b + 0.5 * (groups < R ? groups : R)) * ((N + b - 1) / b); };
-    double tiles = tiles_of(vec ? 128 : 64);
-    const bool large = !vec && tiles * 2 > cus;
-    const double rounds = tiles > cus ? tiles / cus : 1.0;
-    if (large) tiles = tiles_of(128);  // (launch_any_tiles takes those then)
-    if (tiles * 2 > cus) return 1;
-    const int fit = (int)(cus / tiles), most = K / (vec ? 512 : large ? 384 : 256);
+    auto tiles = [&](int b) { return ((double)R / b + 0.5 * (groups < R ? groups : R)) * ((N + b - 1) / b); };
+    if (!vec) return any_ksplit(tiles(64), tiles(128), K, cus);
+    if (R <= 8 * groups || tiles(128) * 2 > cus) return 1;  // (the few-row kernel splits among its waves)
+    const int fit = (int)(cus / tiles(128)), most = K / 512;
     int s = fit < most ? fit : most;
     s = s < 8 ? s : 8;
-    if (s < 2 || (vec && (int64_t)K * (s - 1) < (int64_t)1024 * s)) return 1;
-    // (a stage of the larger tiles takes 1.8 times as long, the slabs as long as 384 steps)
-    return large && rounds * K < 1.8 * K / s + 384.0 ? 1 : s;
+    return s >= 2 && (int64_t)K * (s - 1) >= (int64_t)1024 * s ? s : 1;
 }
 
 // vec: binary16 operands whose rows 16-byte loads can take.
@@ -1419,13 +1428,17 @@ static int run_grouped(const vedic_grouped_desc_t* d) {
     }
     // TN with few tiles and long groups: slices of the contraction into slabs, then their
     // sums in order.
-    const int ks = tn && vec ? grouped_ksplit(d->groups, d->M, N, R, device_cu_count()) : 1;
+    auto tn_tiles = [&](int b) { return (double)d->groups * ((d->M + b - 1) / b) * ((N + b - 1) / b); };
+    const int ks = !tn ? 1
+                   : vec ? grouped_ksplit(d->groups, d->M, N, R, device_cu_count())
+                         : any_ksplit(tn_tiles(64), tn_tiles(128), R / d->groups, device_cu_count());
+    const bool sums_inside = d->db && vec;  // (the 16-byte binary16 kernels sum the columns on the way)
     const size_t slab = (size_t)d->groups * d->M * N, sums = (size_t)d->groups * N;
-    if (ks > 1 && ws.room(Workspace::rounded(4 * ks * slab) + (d->db ? Workspace::rounded(4 * ks * sums) : 0))) {
+    if (ks > 1 && ws.room(Workspace::rounded(4 * ks * slab) + (sums_inside ? Workspace::rounded(4 * ks * sums) : 0))) {
         float* cw = nullptr;
         float* dw = nullptr;
         hipError_t e = ws.get(&cw, 4 * ks * slab);
-        if (e == hipSuccess && d->db) e = ws.get(&dw, 4 * ks * sums);
+        if (e == hipSuccess && sums_inside) e = ws.get(&dw, 4 * ks * sums);
         if (e != hipSuccess) return hip_status(e);
         a.C = cw;
         a.ldc = N;
@@ -1438,6 +1451,8 @@ static int run_grouped(const vedic_grouped_desc_t* d) {
         if (e == hipSuccess)
             e = launch_slab_sum(cw, ks, d->groups, d->M, N, static_cast<float*>(d->C), d->ldc, d->stride_c, d->beta, ws.s);
         if (e == hipSuccess && dw) e = launch_slab_sum(dw, ks, d->groups, 1, N, d->db, N, N, d->db_beta, ws.s);
+        if (e == hipSuccess && d->db && !vec)
+            e = launch_group_colsum(d->B, f16, d->ldb, R, N, d->offsets, d->groups, d->db_beta, d->db, ws.s);
         return hip_status(e);
     }
     // NN and NT with few tiles and a long contraction the same way.
@@ -1458,7 +1473,6 @@ static int run_grouped(const vedic_grouped_desc_t* d) {
     }
     a.ksplit = 1;
     hipError_t e = launch_grouped(d->op, a, kind, f16, f16out, vec, ws.s);
-    // (the 16-byte binary16 kernels sum the columns on the way)
     if (e == hipSuccess && d->db && !vec)
         e = launch_group_colsum(d->B, f16, d->ldb, R, N, d->offsets, d->groups, d->db_beta, d->db, ws.s);
     const hipError_t f = ws.put(copy);

@@ -149,8 +149,8 @@ __device__ __forceinline__ void any_block_slow(const T* const (&pa)[MI], const b
 // WGK > 1: that many groups of WGM x WGN waves, each with LDS buffers of its own and
 // a part of the contraction (whole stages); the others leave their sums in LDS for the
 // first, which adds them in order and runs the epilogue.
-// NN and NT with a.ksplit > 1: the grid's second dimension counts slices of the
-// contraction, each into its own slab (vedic_grouped.hpp).
+// a.ksplit > 1: the grid's second dimension counts slices of the
+// contraction (TN: of each group's), each into its own slab (vedic_grouped.hpp).
 // T, TB, OT: the types of A, B and C.
 template <int OP, typename T, typename TB, typename OT, int BM, int BN, int WGM, int WGN, int WGK, int KIND>
 __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(GroupedArgs a) {
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(Groupe
     // (fp32 rows are loaded four steps at a time: the last K mod 4 come at the end)
     const int Kq = OP != 2 && sizeof(T) == 4 ? K & ~3 : K;
     const int nk_all = few ? 0 : (Kq + kSplitK - 1) / kSplitK;
-    const int slices = OP == 2 ? 1 : gridDim.y, slice = OP == 2 ? 0 : blockIdx.y;
+    const int slices = gridDim.y, slice = blockIdx.y;
     const int nk = (nk_all + WGK * slices - 1) / (WGK * slices);  // stages of a wave group
     const int kt0 = (slice * WGK + wk) * nk;                      // the first of this one's
     const int Ka = min(Kq, slice * WGK * nk * kSplitK), Kz = slice + 1 < slices ? min(Kq, Ka + WGK * nk * kSplitK) : K;
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(WGM* WGN * WGK * 64) grouped_any_kernel(Groupe
     }
     const int row0 = m0 + wm * WM;
     const int64_t crow = OP == 2 ? row0 : start + row0;
-    OT* C = static_cast<OT*>(a.C) + (OP == 2 ? (int64_t)e * a.stride_c : slice * a.split_c) + crow * a.ldc;
+    OT* C = static_cast<OT*>(a.C) + slice * a.split_c + (OP == 2 ? (int64_t)e * a.stride_c : 0) + crow * a.ldc;
     OT* P = a.P != nullptr ? static_cast<OT*>(a.P) + crow * a.ldp : nullptr;
     if constexpr (WGK == 1) __syncthreads();  // the bias (the sums' barriers have shown it otherwise)
     if (grouped_reads(KIND) && a.wide)
@@ -396,11 +396,12 @@ static hipError_t launch_any(GroupedArgs a, hipStream_t s) {
     if (work > 0x7FFFFFFF) return hipErrorInvalidValue;  // (the caller has refused such sizes)
     if (work == 0) return hipSuccess;
     hipLaunchKernelGGL((grouped_any_kernel<OP, T, TB, OT, Cfg::BM, Cfg::BN, Cfg::WGM, Cfg::WGN, WGK, KIND>),
-                       dim3((unsigned)work, OP != 2 && a.ksplit > 1 ? a.ksplit : 1), dim3(Cfg::WGM * Cfg::WGN * WGK * 64), 0, s, a);
+                       dim3((unsigned)work, a.ksplit > 1 ? a.ksplit : 1), dim3(Cfg::WGM * Cfg::WGN * WGK * 64), 0, s, a);
     return hipGetLastError();
 }
 
-// 64 x 64 tiles where 128 x 128 ones would leave half the CUs without one.  Three wave
+// 64 x 64 tiles where 128 x 128 ones would leave half the CUs without one (and slices of the
+// contraction do not fill them).  Three wave
 // groups where a CU gets no more than one 128 x 128 tile, and with the small ones, for
 // contractions long enough to share (us, one group / three: 2006 rows in 7 groups of
 // 2000 into 1000, 156 tiles, NN 103 / 79, NT 101 / 74; the same TN, 896 tiles of 286 steps,
@@ -412,7 +413,7 @@ static hipError_t launch_any_tiles(const GroupedArgs& a, hipStream_t s) {
     };
     const int cus = device_cu_count();
     const bool split = (OP == 2 ? a.R / a.groups : a.K) >= 256;
-    if (tiles(128) * 2 > cus || (OP != 2 && a.ksplit > 1 && tiles(64) * 2 > cus)) {
+    if (tiles(128) * 2 > cus || (a.ksplit > 1 && tiles(64) * 2 > cus)) {
         if (split && tiles(128) <= cus) return launch_any<OP, T, TB, OT, CfgAMid, kAnyGroups, KIND>(a, s);
         return launch_any<OP, T, TB, OT, CfgAMid, 1, KIND>(a, s);
     }

@@ -753,10 +753,12 @@ def route_topk_bwd(logits: torch.Tensor, ids: torch.Tensor, weights: torch.Tenso
     pi, pw, pg = _ints(ids, "ids", shape, dev), _floats(weights, "weights", shape, dev), \
         _floats(dweights, "dweights", shape, dev)
     if out is None:
-        out = torch.empty((T, E), dtype=torch.float32, device=logits.device)
-    po, To, Eo, ldo = _rows2d(out, "out", torch.float32, dev)
-    if (To, Eo) != (T, E):
-        raise ValueError(f"out must be {T}x{E}")
+        out = logits.new_empty((T, E))
+        po, ldo = out.data_ptr(), E
+    else:
+        po, To, Eo, ldo = _rows2d(out, "out", torch.float32, dev)
+        if (To, Eo) != (T, E):
+            raise ValueError(f"out must be {T}x{E}")
     _check(_lib.load().vedic_route_topk_bwd(p, ld, pi, pw, pg, T, E, shape[1], renorm, po, ldo, _stream()))
     return out
 
@@ -905,10 +907,12 @@ def combine_rows(Y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | N
         if (rr, rc) != (T, D):
             raise ValueError(f"residual must be {T}x{D}")
     if out is None:
-        out = torch.empty((T, D), dtype=torch.float32, device=Y.device)
-    po, To, Do, ldo = _rows2d(out, "out", torch.float32, dev)
-    if (To, Do) != (T, D):
-        raise ValueError(f"out must be {T}x{D}")
+        out = slots.new_empty((T, D), dtype=torch.float32)
+        po, ldo = out.data_ptr(), D
+    else:
+        po, To, Do, ldo = _rows2d(out, "out", torch.float32, dev)
+        if (To, Do) != (T, D):
+            raise ValueError(f"out must be {T}x{D}")
     _check(_lib.load().vedic_combine_rows(p, _DT[Y.dtype], ldy, R, ps, pw, pres, ldr, po, ldo, T, k, D, _stream()))
     return out
 
@@ -932,13 +936,13 @@ def combine_rows_bwd(dout: torch.Tensor, Y: torch.Tensor, slots: torch.Tensor, w
     if (gr, gc) != (T, D):
         raise ValueError(f"dout must be {T}x{D}")
     if dY is None:
-        dY = torch.empty((R, D), dtype=out_dtype, device=Y.device)
+        dY = Y.new_empty((R, D), dtype=out_dtype)
     if dY.dtype not in _DT:
         raise ValueError("dY must be float16 or float32")
     po, orr, oc, ldo = _rows2d(dY, "dY", dY.dtype, dev)
     if (orr, oc) != (R, D):
         raise ValueError(f"dY must be {R}x{D}")
-    dw = torch.empty((T, k), dtype=torch.float32, device=Y.device)
+    dw = torch.empty_like(weights)
     _check(_lib.load().vedic_combine_rows_bwd(pg, ldg, p, _DT[Y.dtype], ldy, R, ps, pw, po, _DT[dY.dtype], ldo,
                                               dw.data_ptr(), T, k, D, _stream()))
     return dY, dw
