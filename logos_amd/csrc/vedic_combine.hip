@@ -1,5 +1,5 @@
 // vedic_combine.hip -- rows sorted by expert back in token order, the backward of
-// that, a gathered copy of rows, and column sums by group.
+// that, gathered and padded copies of rows, sums of slabs, and column sums by group.
 //
 // All are bound by memory: each value is read and written once, 16 bytes a lane
 // where the rows allow it, sums in fp32 in a fixed order.  (8192 tokens of 2 rows of 1024

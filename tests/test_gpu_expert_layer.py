@@ -207,15 +207,17 @@ def test_rows_past_two_gibibytes():
         del X, C, dYf
 
 
-def test_streams_and_threads():
-    """Four threads on streams of their own, all operators at once: the bits of the calls made alone."""
+@pytest.mark.parametrize("shared", [False, True])
+def test_streams_and_threads(shared):
+    """Four threads on streams of their own, or on one, all operators at once: the bits of the calls made alone."""
     layers = [Layer(60 + 31 * i, 4 + i, 2, 64 + 8 * i, 128, 10 + i) for i in range(4)]
     alone = [layer.step() for layer in layers]
     torch.cuda.synchronize()
     bad = []
+    one = torch.cuda.Stream()
 
     def run(i):
-        s = torch.cuda.Stream()
+        s = one if shared else torch.cuda.Stream()
         with torch.cuda.stream(s):
             for _ in range(5):
                 o = layers[i].step()
