@@ -141,3 +141,46 @@ def test_route_backward_against_differences(renorm):
             d[t, e] = h
             up, dn = weights(x + d, ids, renorm), weights(x - d, ids, renorm)
             assert abs(((up - dn) * dw).sum() / (2 * h) - got[t, e]) < 1e-5  # fp32 logits' 3e-7 dominate h^2
+
+
+@pytest.mark.parametrize("T,E,k,pad", [(70001, 32, 2, 4), (200000, 4, 1, 0), (30011, 260, 3, 1), (40000, 64, 8, 0)])
+def test_many_tokens(T, E, k, pad):
+    """More tokens than one pass of the workgroups; pitched logits.  Distinct integers choose; torch sorts them."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(T)
+    noise = torch.rand(T, E, device="cuda", generator=g)
+    logits = torch.full((T, E + pad), 1e9, device="cuda")
+    logits[:, :E] = noise.argsort(1).float() / 8  # a permutation of 0 .. E - 1 in each row: no ties
+    v = vedic()
+    got = v.route_topk(logits[:, :E], k)
+    top = logits[:, :E].topk(k, 1)
+    assert torch.equal(got.ids.long(), top.indices)
+    torch.testing.assert_close(got.weights.double(), top.values.double().softmax(1), rtol=64 * U, atol=0)
+    flat = top.indices.reshape(-1)
+    order = flat.argsort(stable=True)
+    assert torch.equal(got.rows.long(), order // k)
+    assert torch.equal(got.offsets[1:].long(), torch.bincount(flat, minlength=E).cumsum(0)) and got.offsets[0] == 0
+    assert torch.equal(got.slots.reshape(-1)[order].long(), torch.arange(T * k, device="cuda"))
+
+
+def test_smallest_calls_of_the_set():
+    """No tokens at all, and tokens of which none has an expert or an adapter."""
+    v = vedic()
+    rt = v.route_topk(torch.empty(0, 4, device="cuda"), 2)
+    assert rt.offsets.tolist() == [0] * 5
+    Y = v.gemm_grouped(v.OP_NN, torch.empty(0, 8, device="cuda"), torch.ones(4, 8, 16, device="cuda"), rt.offsets, rows=rt.rows)
+    assert Y.shape == (0, 16) and v.combine_rows(Y, rt.slots, rt.weights).shape == (0, 16)
+    dY, dw = v.combine_rows_bwd(torch.empty(0, 16, device="cuda"), Y, rt.slots, rt.weights)
+    assert dY.shape == (0, 16) and dw.shape == (0, 2)
+    rt = v.route_topk(torch.full((3, 4), -float("inf"), device="cuda"), 2)
+    assert rt.ids.eq(-1).all() and rt.slots.eq(-1).all() and rt.weights.eq(0).all() and rt.offsets.eq(0).all()
+    C = torch.full((6, 16), 7.0, device="cuda")
+    X = torch.ones(3, 8, device="cuda")
+    v.gemm_grouped(v.OP_NN, X, torch.ones(4, 8, 16, device="cuda"), rt.offsets, C, rows=rt.rows)
+    assert C.eq(7.0).all()
+    res = torch.randn(3, 16, device="cuda")
+    assert torch.equal(v.combine_rows(C, rt.slots, rt.weights, residual=res), res)
+    off, rows, _ = v.group_rows(torch.full((3,), -1, dtype=torch.int32, device="cuda"), 2)
+    W = torch.randn(8, 16, device="cuda")
+    got = v.gemm_lora(X, W, torch.ones(2, 8, 4, device="cuda"), torch.ones(2, 4, 16, device="cuda"), off, rows)
+    assert torch.equal(got, v.gemm(v.OP_NN, X, W))
