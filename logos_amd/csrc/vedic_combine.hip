@@ -161,22 +161,25 @@ __global__ void __launch_bounds__(256) gather_rows16_kernel(const u32x4_t* src, 
     }
 }
 
-// dst[i][0 .. 8 octs) = binary16 src row i (row rows[i], zeros outside nsrc, where a
-// list is given), zeros past `cols`; src rows in matrices of `per` rows, `stride` apart.
+// dst[i][0 .. 8 octs) = binary16 src row i, zeros past `cols`: of matrices of `per` rows,
+// `stride` apart, or, where a list is given, row rows[i] of the nsrc rows (zeros outside).
 // 16-byte stores; loads of any alignment.
 __global__ void __launch_bounds__(256) pad_rows_kernel(const _Float16* src, int64_t ld, int per, int64_t stride, int nsrc,
                                                         const int* rows, int64_t n, int cols, int octs, half8_t* dst) {
     for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n * octs; q += (int64_t)gridDim.x * 256) {
         const int64_t i = q / octs;
         const int c = (int)(q - i * octs) * 8;
-        int64_t r = i;
+        int64_t at;  // the row's first value
         bool ok = true;
-        if (rows != nullptr) {
-            r = rows[i];
-            ok = (uint64_t)r < (uint64_t)nsrc;
+        if (rows != nullptr) {  // (an entry is the row itself: `per` counts rows without a list)
+            const int r = rows[i];
+            ok = (unsigned)r < (unsigned)nsrc;
+            at = ok ? (int64_t)r * ld : 0;
+        } else {
+            const int64_t m = i / per;
+            at = m * stride + (i - m * per) * ld;
         }
-        const int64_t m = ok ? r / per : 0;
-        const _Float16* s = src + m * stride + (ok ? r - m * per : 0) * ld + c;
+        const _Float16* s = src + at + c;
         half8_t v;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = ok && c + e < cols ? s[e] : (_Float16)0.0f;
