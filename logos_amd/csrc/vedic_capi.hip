@@ -1413,13 +1413,14 @@ static int run_grouped(const vedic_grouped_desc_t* d) {
     }
     // The rows of a list are copied into a workspace first where the kernels
     // cannot follow it: past 32-bit offsets, and along the contraction (TN) but for
-    // the 16-byte binary16 kernels.
+    // the 16-byte binary16 kernels.  (An A that was padded above is below 2 GiB and keeps
+    // its list: these copies have no padding.)
     void* copy = nullptr;
-    if (a.rows && ((tn && !vec) || (int64_t)d->a_rows * d->lda * es >= (int64_t(1) << 31))) {
+    if (a.rows && ((tn && !vec) || (int64_t)d->a_rows * a.lda * es >= (int64_t(1) << 31))) {
         const int64_t ldn = ((int64_t)a_cols + 7) / 8 * 8;
         hipError_t e = ws.get(&copy, (size_t)R * ldn * es);
         if (e == hipSuccess)
-            e = launch_gather_rows(d->A, d->lda, d->a_rows, a.rows, R, a_cols, es, copy, ldn, ws.s);
+            e = launch_gather_rows(a.A, a.lda, d->a_rows, a.rows, R, a_cols, es, copy, ldn, ws.s);
         if (e != hipSuccess) return hip_status(e);
         a.A = copy;
         a.lda = ldn;

@@ -100,3 +100,35 @@ def test_eager_and_captured_rows():
         g.replay()
         torch.cuda.synchronize()
         torch.testing.assert_close(recorded, eager, rtol=0, atol=41 * 2.0 ** -17)  # 2 K u sum |ab|, the sum below 64
+
+
+@pytest.mark.parametrize("K", [41, 48])
+@pytest.mark.parametrize("R", [5, 700])
+def test_column_slice_past_two_gibibytes(K, R):
+    """A few columns of a matrix whose pitch takes its rows past 2 GiB, and a workspace that held NaN before."""
+    v = vedic()
+    T, N, sizes = 600, 72, [R // 2, R - R // 2]
+    rng = np.random.default_rng(K + R)
+    off = sizes_to_offsets(sizes)
+    wide = torch.empty(T, 1 << 21, dtype=F16, device="cuda")
+    X, x = make(rng, (T, K), F16)
+    wide[:, 7:7 + K] = X
+    W, w = make(rng, (2, K, N), F16, K ** -0.5)
+    dY, dy = make(rng, (R, N), F16)
+    rows = rng.integers(0, T, R).astype(np.int32)
+    rows[0] = T - 1
+    a = x[rows]
+    spoil = pitched(torch.full((20000, 48), float("nan"), dtype=F16, device="cuda"), 0, 1)
+    for _ in range(2):  # (the block grows with the first call and is written by the second)
+        v.gemm_grouped(v.OP_NN, spoil, torch.ones(1, 48, 8, dtype=F16, device="cuda"), ints([0, 20000]))
+    dot = np.concatenate([a[off[i]:off[i + 1]] @ w[i] for i in range(2)])
+    absdot = np.concatenate([np.abs(a[off[i]:off[i + 1]]) @ np.abs(w[i]) for i in range(2)])
+    A = wide[:, 7:7 + K]
+    nn = v.gemm_grouped(v.OP_NN, A, W, ints(off), rows=ints(rows))
+    check_rows(nn.double().cpu().numpy(), dot, absdot, K, F32, "NN")
+    nt = v.gemm_grouped(v.OP_NT, A, W.transpose(1, 2).contiguous(), ints(off), rows=ints(rows))
+    check_rows(nt.double().cpu().numpy(), dot, absdot, K, F32, "NT")
+    dW = v.gemm_grouped(v.OP_TN, A, dY, ints(off), rows=ints(rows))
+    for i in range(2):
+        s = slice(off[i], off[i + 1])
+        check_rows(dW[i].double().cpu().numpy(), a[s].T @ dy[s], np.abs(a[s]).T @ np.abs(dy[s]), sizes[i], F32, f"group {i}")
