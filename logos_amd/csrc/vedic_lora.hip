@@ -1,7 +1,7 @@
 // vedic_lora.hip -- low-rank adapters of many requests in one batch: for the rows
 // i of adapter g (list position p, rows[p] = i),
 //   C[i] += scale[g] (X[i] . A_g) . B_g,   A_g [K x r], B_g [r x N].
-// Two launches, H = X A_g into a workspace (fp32, or the same as two binary16
+// Two launches, H = X A_g into a workspace (fp32, or the same as three binary16
 // values), then C.  fp32 operands, and rows that 16-byte loads cannot take, run as two
 // grouped products (vedic_grouped_any.hpp).
 //
@@ -49,14 +49,19 @@ __device__ __forceinline__ half8_t read_tr16(const char* lds, int pitch, int k0,
 // memory; a wave reads what it loaded itself, so no barrier until the sum).  X's
 // rows go straight into the MFMA's operand registers.
 //
-// H stays at fp32 precision as two binary16 values: row p is scaled by 2^-x so that
-// its largest value lies in [2^14, 2^15), and h = hi + lo, hi = f16(h), lo = f16(h -
-// hi), leaves at most 2^-22 of h or 2^-25, 2^-39 of the largest, behind.
+// H's fp32 values are kept as three binary16 ones each: row p is scaled by 2^-x so that
+// its largest finite value lies in [2^14, 2^15), and h = hi + 2^-12 mid + 2^-24 lo, each
+// part the binary16 nearest to 2^12 times what the last left behind (a remainder of at
+// most 2^4: no overflow).  That is h exactly where its last bit is 2^-48 or more, so for
+// every |h| of 2^-25, 2^-39 of the largest; below, at most 2^-49 is lost, 2^-63 of the
+// largest.  (Two parts without the 2^12 lose bits from 2^-18 of the largest on; the fp32
+// MFMA on H itself takes longer: 4096 rows, 1024 into 4096, projection included, two parts
+// / three / fp32 MFMA, rank 64 89 / 93 / 98 us, rank 128 113 / 119 / 147.)
 // factor[p] = scale 2^x then multiplies the product's fp32 sums.
 template <int RP, int KC>
 __global__ void __launch_bounds__(512) lora_shrink_f16_kernel(LoraArgs a) {
     constexpr int NB = RP / 16, SB = KC * RP * 2, NI = (SB + 1023) / 1024, STAGE = NI * 1024;
-    constexpr int RS = RP < 32 ? 32 : RP;  // columns of hi, of lo
+    constexpr int RS = RP < 32 ? 32 : RP;  // columns of a part
     static_assert(8 * 16 * RP * 4 <= 8 * 2 * STAGE, "the partial sums fit the stages");
     __shared__ __attribute__((aligned(1024))) char s0[8 * STAGE];
     __shared__ __attribute__((aligned(1024))) char s1[8 * STAGE];
@@ -153,35 +158,37 @@ __global__ void __launch_bounds__(512) lora_shrink_f16_kernel(LoraArgs a) {
         h[v] = 0.0f;
         if (c < a.r && c < RP)
             for (int w = 0; w < 8; ++w) h[v] += part(w)[i * RP + c];
-        top = fmaxf(top, fabsf(h[v]));
+        if (fabsf(h[v]) < __builtin_inff()) top = fmaxf(top, fabsf(h[v]));
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 32));
     if (i < np) {
-        // (a row of zeros, or one that is not finite, keeps its scale)
-        int ex = 0;
-        if (top > 0.0f && top < __builtin_inff()) {
+        int ex = 0;  // (a row without finite values other than zero keeps its scale)
+        if (top > 0.0f) {
             (void)frexpf(top, &ex);  // top = m 2^ex, m in [0.5, 1)
             ex -= 15;
         }
         const float down = ldexpf(1.0f, ex < -126 ? 126 : ex > 126 ? -126 : -ex);
-        _Float16* o = a.Hs + (int64_t)(p0 + i) * (2 * RS);
+        _Float16* o = a.Hs + (int64_t)(p0 + i) * (3 * RS);
 #pragma unroll
         for (int v = 0; v < NC; ++v) {
             const int c = c0 + 32 * v;
             const float s = h[v] * down;
             const _Float16 hi = (_Float16)s;
-            const float rest = s - (float)hi;
+            const float r1 = fabsf(s) < __builtin_inff() ? (s - (float)hi) * 4096.0f : 0.0f;
+            const _Float16 mid = (_Float16)r1;
             o[c] = hi;
-            o[RS + c] = fabsf((float)hi) < __builtin_inff() ? (_Float16)rest : (_Float16)0.0f;
+            o[RS + c] = mid;
+            o[2 * RS + c] = (_Float16)((r1 - (float)mid) * 4096.0f);
         }
         if (c0 == 0) a.factor[p0 + i] = (a.scales ? a.scales[g] : 1.0f) / down;
     }
 }
 
-// C[rows[p]] += factor[p] (hi + lo) B_g: 16 places by 256 columns, a wave 64 of
-// them.  B_g's columns are staged in LDS once for both parts; the product is taken
-// transposed, so that a lane holds four neighbouring columns of one row.
+// C[rows[p]] += factor[p] (hi + 2^-12 mid + 2^-24 lo) B_g: 16 places by 256 columns, a wave
+// 64 of them.  B_g's columns are staged in LDS once for the three parts, whose products
+// have accumulators of their own; they are taken transposed, so that a lane holds four
+// neighbouring columns of one row.
 template <int RS>
 __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
     __shared__ __attribute__((aligned(1024))) char sb[RS * 512];
@@ -209,13 +216,12 @@ __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
                                                  in ? (uint32_t)(k * a.N * 2 + slot * 16) : kOob, 0, 0, 0);
     }
     const int p = lane & 15;
-    const _Float16* h = a.Hs + (int64_t)(p0 + (p < np ? p : 0)) * (2 * RS) + 8 * (lane >> 4);
-    half8_t hi[RS / 32], lo[RS / 32];
+    const _Float16* h = a.Hs + (int64_t)(p0 + (p < np ? p : 0)) * (3 * RS) + 8 * (lane >> 4);
+    half8_t part[3][RS / 32];
 #pragma unroll
-    for (int c = 0; c < RS / 32; ++c) {
-        hi[c] = *reinterpret_cast<const half8_t*>(h + 32 * c);
-        lo[c] = *reinterpret_cast<const half8_t*>(h + RS + 32 * c);
-    }
+    for (int q3 = 0; q3 < 3; ++q3)
+#pragma unroll
+        for (int c = 0; c < RS / 32; ++c) part[q3][c] = *reinterpret_cast<const half8_t*>(h + q3 * RS + 32 * c);
     const float f = a.factor[p0 + (p < np ? p : 0)];
     const int row = p < np ? a.rows[p0 + p] : -1;
     const bool ok = (unsigned)row < (unsigned)a.M;
@@ -228,22 +234,28 @@ __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
     }
     wait_vmcnt<0>();
     __syncthreads();
-    float4_t acc[4];
+    float4_t acc[3][4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) acc[b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int q3 = 0; q3 < 3; ++q3)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) acc[q3][b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < RS / 32; ++c)
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const half8_t w = read_tr16<true>(sb, 512, 32 * c, 64 * wave + 16 * b, lane);
-            acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, lo[c], acc[b], 0, 0, 0);
-            acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, hi[c], acc[b], 0, 0, 0);
+#pragma unroll
+            for (int q3 = 0; q3 < 3; ++q3)
+                acc[q3][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, part[q3][c], acc[q3][b], 0, 0, 0);
         }
 #pragma unroll
     for (int b = 0; b < 4; ++b)
         if (ok && n0 + 64 * wave + 16 * b + 4 * (lane >> 4) < a.N) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) old[b][e] = __builtin_fmaf(f, acc[b][e], old[b][e]);
+            for (int e = 0; e < 4; ++e) {
+                const float low = __builtin_fmaf(0x1p-12f, acc[2][b][e], acc[1][b][e]);
+                old[b][e] = __builtin_fmaf(f, __builtin_fmaf(0x1p-12f, low, acc[0][b][e]), old[b][e]);
+            }
             store16_hold(crow + 16 * b, old[b]);
         }
 }
@@ -322,13 +334,13 @@ bool vec16(const LoraArgs& a) {
 
 }  // namespace
 
+// Columns of a part of H.
+static size_t part_columns(int r) { return r <= 32 ? 32 : r <= 64 ? 64 : 128; }
+
 static size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 size_t lora_bytes(const LoraArgs& a, bool f16) {
-    if (f16 && vec16(a)) {  // hi and lo of rs values each, and the factors
-        const size_t rs = (size_t)(a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128);
-        return (size_t)a.n * (rs * 4 + 4);
-    }
+    if (f16 && vec16(a)) return (size_t)a.n * (part_columns(a.r) * 6 + 4);  // three parts, and the factors
     const size_t h = (size_t)a.n * a.r * 4;
     return rounded(h) + (a.ksplit > 1 ? rounded(a.ksplit * h) : 0) + (copies_rows(a, f16) ? (size_t)a.n * a.K * (f16 ? 2 : 4) : 0);
 }
@@ -340,9 +352,8 @@ hipError_t launch_lora(LoraArgs a, bool f16, void* work, hipStream_t s) {
         char* const slabs = static_cast<char*>(work) + rounded(h);
         return launch_any(a, f16, reinterpret_cast<float*>(slabs), slabs + (a.ksplit > 1 ? rounded(a.ksplit * h) : 0), s);
     }
-    const size_t rs = (size_t)(a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128);
     a.Hs = static_cast<_Float16*>(work);
-    a.factor = reinterpret_cast<float*>(a.Hs + (size_t)a.n * 2 * rs);
+    a.factor = reinterpret_cast<float*>(a.Hs + (size_t)a.n * 3 * part_columns(a.r));
     if (a.r <= 16) return launch_f16<16, 64>(a, s);
     if (a.r <= 32) return launch_f16<32, 64>(a, s);
     if (a.r <= 64) return launch_f16<64, 64>(a, s);

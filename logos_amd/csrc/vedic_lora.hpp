@@ -23,7 +23,7 @@ struct LoraArgs {
     int ksplit;  // slices of K in H's product, where that is a grouped product
     // set by the launch
     float* H;       // [n x r]
-    _Float16* Hs;   // [n][hi, lo]
+    _Float16* Hs;   // [n][hi, mid, lo]
     float* factor;  // [n]
 };
 
