@@ -103,48 +103,50 @@ __global__ void __launch_bounds__(256) combine_kernel(CombineArgs a, int strips)
 template <typename T, typename DT, bool VEC>
 __global__ void __launch_bounds__(256) combine_bwd_kernel(CombineBwdArgs a) {
     const int lane = threadIdx.x & 63;
-    const int64_t p = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (p >= (int64_t)a.T * a.k) return;
-    const int64_t t = p / a.k;
-    const int s = __builtin_amdgcn_readfirstlane(a.slots[p]);
-    float dot = 0.0f;
-    if ((unsigned)s < (unsigned)a.R) {
-        const float w = a.weights[p];
-        const float* g = a.dout + t * a.ldg;
-        const T* y = static_cast<const T*>(a.Y) + (int64_t)s * a.ldy;
-        DT* o = static_cast<DT*>(a.dY) + (int64_t)s * a.ldo;
-        float4_t part = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int c0 = 0; c0 < a.D; c0 += 512) {
-            float4_t gv[2], yv[2];
+    for (int64_t p = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); p < (int64_t)a.T * a.k;
+         p += (int64_t)gridDim.x * 4) {
+        const int64_t t = p / a.k;
+        const int s = __builtin_amdgcn_readfirstlane(a.slots[p]);
+        float dot = 0.0f;
+        if ((unsigned)s < (unsigned)a.R) {
+            const float w = a.weights[p];
+            const float* g = a.dout + t * a.ldg;
+            const T* y = static_cast<const T*>(a.Y) + (int64_t)s * a.ldy;
+            DT* o = static_cast<DT*>(a.dY) + (int64_t)s * a.ldo;
+            float4_t part = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int c0 = 0; c0 < a.D; c0 += 512) {
+                float4_t gv[2], yv[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                gv[h] = load_strip<float, VEC>(g, c0 + 256 * h, lane, a.D);
-                yv[h] = load_strip<T, VEC>(y, c0 + 256 * h, lane, a.D);
+                for (int h = 0; h < 2; ++h) {
+                    gv[h] = load_strip<float, VEC>(g, c0 + 256 * h, lane, a.D);
+                    yv[h] = load_strip<T, VEC>(y, c0 + 256 * h, lane, a.D);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) part[e] = __builtin_fmaf(gv[h][e], yv[h][e], part[e]);
+                    store_strip<DT, VEC>(o, c0 + 256 * h, lane, a.D, gv[h] * w);
+                }
             }
+            dot = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) part[e] = __builtin_fmaf(gv[h][e], yv[h][e], part[e]);
-                store_strip<DT, VEC>(o, c0 + 256 * h, lane, a.D, gv[h] * w);
-            }
+            for (int d = 32; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
         }
-        dot = (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
+        if (lane == 0) a.dweights[p] = dot;
     }
-    if (lane == 0) a.dweights[p] = dot;
 }
 
 // dst[i] = src[rows[i]] (zeros for an index outside), `words` 2-byte words each:
 // element-wise, for any alignment.
 __global__ void __launch_bounds__(256) gather_rows_kernel(const uint16_t* src, int64_t ld, int nsrc, const int* rows, int n,
                                                            int words, uint16_t* dst, int64_t ldd) {
-    const int64_t i = blockIdx.x;
-    const int r = rows[i];
-    const bool ok = (unsigned)r < (unsigned)nsrc;
-    const uint16_t* s = src + (int64_t)(ok ? r : 0) * ld;
-    uint16_t* d = dst + i * ldd;
-    for (int c = threadIdx.x; c < words; c += 256) d[c] = ok ? s[c] : (uint16_t)0;
+    for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
+        const int r = rows[i];
+        const bool ok = (unsigned)r < (unsigned)nsrc;
+        const uint16_t* s = src + (int64_t)(ok ? r : 0) * ld;
+        uint16_t* d = dst + i * ldd;
+        for (int c = threadIdx.x; c < words; c += 256) d[c] = ok ? s[c] : (uint16_t)0;
+    }
 }
 
 // The same by 16-byte chunks.
@@ -282,26 +284,36 @@ bool rows_ok(const void* p, int64_t ld, int es, int chunk) {
 
 }  // namespace
 
-hipError_t launch_combine(const CombineArgs& a, bool f16, hipStream_t s) {
+hipError_t launch_combine(CombineArgs a, bool f16, hipStream_t s) {
     const int strips = (a.D + 255) / 256;
-    const int64_t blocks = ((int64_t)a.T * strips + 3) / 4;
     // (rows padded to whole chunks would be read past D: D itself has to be a multiple)
     const bool vec = a.D % 4 == 0 && rows_ok(a.Y, a.ldy, f16 ? 2 : 4, f16 ? 8 : 16) && rows_ok(a.out, a.ldo, 4, 16) &&
                      rows_ok(a.residual, a.ldr, 4, 16);
-    const dim3 g((unsigned)blocks), b(256);
-    if (f16) {
-        if (vec) hipLaunchKernelGGL((combine_kernel<_Float16, true>), g, b, 0, s, a, strips);
-        else hipLaunchKernelGGL((combine_kernel<_Float16, false>), g, b, 0, s, a, strips);
-    } else {
-        if (vec) hipLaunchKernelGGL((combine_kernel<float, true>), g, b, 0, s, a, strips);
-        else hipLaunchKernelGGL((combine_kernel<float, false>), g, b, 0, s, a, strips);
+    // (in launches of fewer than 2^32 threads; a loop in the kernel costs 1 % of 21 us)
+    const int tokens = ((1 << 26) - 4) / strips;
+    for (int64_t left = a.T; left > 0; left -= tokens) {
+        a.T = (int)(left < tokens ? left : tokens);
+        const dim3 g((unsigned)(((int64_t)a.T * strips + 3) / 4)), b(256);
+        if (f16) {
+            if (vec) hipLaunchKernelGGL((combine_kernel<_Float16, true>), g, b, 0, s, a, strips);
+            else hipLaunchKernelGGL((combine_kernel<_Float16, false>), g, b, 0, s, a, strips);
+        } else {
+            if (vec) hipLaunchKernelGGL((combine_kernel<float, true>), g, b, 0, s, a, strips);
+            else hipLaunchKernelGGL((combine_kernel<float, false>), g, b, 0, s, a, strips);
+        }
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        a.slots += (int64_t)a.T * a.k;
+        if (a.weights) a.weights += (int64_t)a.T * a.k;
+        if (a.residual) a.residual += a.T * a.ldr;
+        a.out += a.T * a.ldo;
     }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 template <typename T, typename DT>
 static hipError_t launch_combine_bwd_t(const CombineBwdArgs& a, hipStream_t s) {
-    const dim3 g((unsigned)(((int64_t)a.T * a.k + 3) / 4)), b(256);
+    const dim3 g(row_blocks(((int64_t)a.T * a.k + 3) / 4)), b(256);
     const bool vec = a.D % 4 == 0 && rows_ok(a.dout, a.ldg, 4, 16) && rows_ok(a.Y, a.ldy, sizeof(T), 4 * sizeof(T)) &&
                      rows_ok(a.dY, a.ldo, sizeof(DT), 4 * sizeof(DT));
     if (vec) hipLaunchKernelGGL((combine_bwd_kernel<T, DT, true>), g, b, 0, s, a);
@@ -323,7 +335,7 @@ hipError_t launch_gather_rows(const void* src, int64_t ld, int nsrc, const int* 
         hipLaunchKernelGGL(gather_rows16_kernel, dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const u32x4_t*>(src),
                            ld * es / 16, nsrc, rows, n, chunks, static_cast<u32x4_t*>(dst), ldd * es / 16);
     } else {
-        hipLaunchKernelGGL(gather_rows_kernel, dim3((unsigned)n), dim3(256), 0, s, static_cast<const uint16_t*>(src),
+        hipLaunchKernelGGL(gather_rows_kernel, dim3(row_blocks(n)), dim3(256), 0, s, static_cast<const uint16_t*>(src),
                            ld * (es / 2), nsrc, rows, n, cols * (es / 2), static_cast<uint16_t*>(dst), ldd * (es / 2));
     }
     return hipGetLastError();

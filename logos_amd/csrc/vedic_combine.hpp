@@ -33,7 +33,7 @@ struct CombineBwdArgs {
     int T, k, D;
 };
 
-hipError_t launch_combine(const CombineArgs& a, bool f16, hipStream_t s);
+hipError_t launch_combine(CombineArgs a, bool f16, hipStream_t s);
 hipError_t launch_combine_bwd(const CombineBwdArgs& a, bool f16, bool out16, hipStream_t s);
 // dst[i] = src[rows[i]], `cols` values of es bytes (2 or 4); n > 0.
 hipError_t launch_gather_rows(const void* src, int64_t ld, int nsrc, const int* rows, int n, int cols, int es, void* dst,

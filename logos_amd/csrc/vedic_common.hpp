@@ -94,6 +94,10 @@ enum : int {
 
 constexpr int kMaxHeads = 64;  // scatter targets per GEMM
 
+// Workgroups of 256 threads for `want` of them: a launch takes fewer than 2^32 threads
+// (more are cut without an error), the kernel strides over the rest.
+inline unsigned row_blocks(int64_t want) { return (unsigned)(want < (1 << 24) ? want : (1 << 24) - 1); }
+
 // Leading dimensions below this keep a tile's row offsets in 32 bits.
 constexpr int64_t kMaxLd = int64_t(1) << 22;
 

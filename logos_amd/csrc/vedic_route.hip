@@ -486,9 +486,16 @@ hipError_t launch_group_rows(const int* ids, int n, int per_row, int groups, int
 
 hipError_t launch_route_topk_bwd(const float* logits, int64_t ld, const int* ids, const float* weights, const float* dweights,
                                  int T, int E, int k, int renorm, float* out, int64_t ldo, hipStream_t s) {
-    hipLaunchKernelGGL(route_bwd_kernel, dim3((T + 3) / 4), dim3(256), 0, s, logits, ld, ids, weights, dweights, T, E, k,
-                       renorm, out, ldo);
-    return hipGetLastError();
+    // (in launches of fewer than 2^32 threads)
+    constexpr int kTokens = (1 << 26) - 4;
+    for (int64_t t = 0; t < T; t += kTokens) {
+        const int n = (int)(T - t < kTokens ? T - t : kTokens);
+        hipLaunchKernelGGL(route_bwd_kernel, dim3((n + 3) / 4), dim3(256), 0, s, logits + t * ld, ld, ids + t * k,
+                           weights + t * k, dweights + t * k, n, E, k, renorm, out + t * ldo, ldo);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace vedic

@@ -1,0 +1,64 @@
+"""More rows, tokens or pairs than one launch has threads for."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F16, F32 = torch.float16, torch.float32
+MANY = (1 << 26) + 5  # 64 threads each pass 2^32
+
+
+def vedic():
+    from logos_amd import vedic as v
+
+    return v
+
+
+def test_combine():
+    v = vedic()
+    Y = torch.randn(7, 2, device="cuda").half()
+    slots = torch.randint(-1, 8, (MANY, 1), device="cuda", dtype=torch.int32)
+    slots[-1] = 6
+    got = v.combine_rows(Y, slots)
+    table = torch.cat([torch.zeros(1, 2, device="cuda"), Y.float(), torch.zeros(1, 2, device="cuda")])
+    assert torch.equal(got, table[(slots[:, 0] + 1).long()])
+
+
+def test_combine_backward():
+    v = vedic()
+    Y = torch.randn(MANY, 1, device="cuda")
+    dout = torch.randn(MANY, 1, device="cuda")
+    w = torch.rand(MANY, 1, device="cuda")
+    slots = torch.arange(MANY - 1, -1, -1, device="cuda", dtype=torch.int32)[:, None].contiguous()
+    dY, dw = v.combine_rows_bwd(dout, Y, slots, w)
+    assert torch.equal(dY, (w * dout).flip(0))
+    assert torch.equal(dw, dout * Y.flip(0))
+
+
+def test_route_and_its_backward():
+    v = vedic()
+    logits = torch.randn(MANY, 2, device="cuda")
+    dw = torch.randn(MANY, 1, device="cuda")
+    r = v.route_topk(logits, 1, renorm=False)
+    second = logits[:, 1] > logits[:, 0]
+    assert torch.equal(r.ids[:, 0], second.int())
+    assert r.offsets.tolist() == [0, MANY - int(second.sum()), MANY]
+    assert torch.equal(r.rows[r.slots[:, 0].long()].long(), torch.arange(MANY, device="cuda"))
+    got = v.route_topk_bwd(logits, r.ids, r.weights, dw, renorm=False)
+    for part in (slice(0, 1 << 25), slice(1 << 25, 1 << 26), slice(1 << 26, MANY)):
+        want = v.route_topk_bwd(logits[part], r.ids[part], r.weights[part], dw[part], renorm=False)
+        assert torch.equal(got[part], want)
+
+
+def test_listed_rows():
+    """The copy of a list of 2^24 rows and more, 256 threads each."""
+    v = vedic()
+    R = (1 << 24) + 9
+    X = torch.tensor([[1.0], [2.0], [4.0]], device="cuda")
+    rows = torch.randint(0, 3, (R,), device="cuda", dtype=torch.int32)
+    rows[-1] = 2
+    dY = torch.zeros(R, 1, device="cuda")
+    dY[[0, 5, R // 2, R - 3, R - 1]] = torch.tensor([[1.0], [3.0], [16.0], [32.0], [0.5]], device="cuda")
+    off = torch.tensor([0, R], dtype=torch.int32, device="cuda")
+    got = v.gemm_grouped(v.OP_TN, X, dY, off, rows=rows)
+    assert got.item() == (X[rows.long()] * dY).sum().item()
