@@ -482,9 +482,12 @@ int vedic_flash_attention_bwd_heads(const float* const* Q, const float* const* K
  * it.  Plans stay on the GPU: no call reads one on the host or waits for it.  What
  * a plan holds is clamped where it is read (an offset to 0 .. n, a row or slot
  * outside its matrix counts as none), so a bad plan gives wrong values but no
- * access outside the arrays.  Limits: 1024 groups, leading dimensions below 2^22,
- * counts below 2^30 (places of a grouped product 2^27, of adapters 2^23;
- * VEDIC_STATUS_TOO_LARGE). */
+ * access outside the arrays.  Limits: 1024 groups; counts below 2^30 (places of a grouped
+ * product 2^27, of adapters 2^23); leading dimensions of grouped products and adapters
+ * below 2^22; and fewer than 2^24 tiles, counted as (places / 128 + groups) x (N / 128) for
+ * grouped products on the general kernels (TN: groups x (M / 128) x (N / 128)) and for
+ * adapters that are F32 or not 16-byte aligned, as (places / 16 + groups) x (N / 256) for
+ * the other adapters, each quotient rounded up.  VEDIC_STATUS_TOO_LARGE past them. */
 
 /* The router: for each of T tokens the k largest of its E logits, a tie to the
  * lower index, and their weights exp(x_j - max) / sum, the sum over the chosen

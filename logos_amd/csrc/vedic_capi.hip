@@ -1292,7 +1292,8 @@ static hipError_t launch_grouped(int op, const GroupedArgs& a, int kind, bool f1
     // At most eight rows a group (us, tiles / few-row kernel, 8 groups: NN 1024 into 4096, 8
     // rows 16.2 / 12.2, 32 rows 20.0 / 18.7, 64 rows 19.6 / 19.4, 128 rows 20.0 / 27.0; 4096
     // into 1024, 64 rows 39.0 / 27.6; NT 4096 into 1024, 64 rows 38.6 / 15.5).
-    if (vec && op != VEDIC_OP_TN && a.R <= 8 * a.groups) return launch_grouped_f16_skinny(op, a, kind, f16out, s);
+    if (vec && op != VEDIC_OP_TN && a.R <= 8 * a.groups && grouped_skinny_fits(op, a.groups, a.R, a.N))
+        return launch_grouped_f16_skinny(op, a, kind, f16out, s);
     if (vec)
         return op == VEDIC_OP_NN   ? launch_grouped_f16_nn(a, kind, f16out, s)
                : op == VEDIC_OP_NT ? launch_grouped_f16_nt(a, kind, f16out, s)
@@ -1411,6 +1412,7 @@ static int run_grouped(const vedic_grouped_desc_t* d) {
             vec = true;
         }
     }
+    if (!vec && !grouped_any_fits(tn ? 2 : 0, d->groups, R, d->M, N)) return VEDIC_STATUS_TOO_LARGE;  // (nothing has run)
     // The rows of a list are copied into a workspace first where the kernels
     // cannot follow it: past 32-bit offsets, and along the contraction (TN) but for
     // the 16-byte binary16 kernels.  (An A that was padded above is below 2 GiB and keeps
@@ -1560,8 +1562,7 @@ static int lora_checks(const void* X, int dtype, int64_t ldx, int M, const void*
                        const int* offsets, const int* rows, int n, const float* C, int64_t ldc, int K, int N) {
     if (dtype != VEDIC_DT_F32 && dtype != VEDIC_DT_F16) return VEDIC_STATUS_BAD_DTYPE;
     if (M < 0 || n < 0 || groups <= 0 || r <= 0 || K <= 0 || N <= 0) return VEDIC_STATUS_BAD_DIM;
-    if (r > kLoraMaxRank || groups > kMaxGroups || M >= kMaxCount || n >= kMaxCount / 128 || ldx >= kMaxLd || ldc >= kMaxLd ||
-        ((int64_t)n / 8 + groups) * ((N + 63) / 64) >= kMaxCount)
+    if (r > kLoraMaxRank || groups > kMaxGroups || M >= kMaxCount || n >= kMaxCount / 128 || ldx >= kMaxLd || ldc >= kMaxLd)
         return VEDIC_STATUS_TOO_LARGE;
     if (ldx < K || ldc < N) return VEDIC_STATUS_BAD_LD;
     if (n > 0 && M > 0 && (!X || !A || !B || !offsets || !rows || !C)) return VEDIC_STATUS_NULL_POINTER;
@@ -1600,6 +1601,7 @@ static int run_base(const vedic_gemm_desc_t* b) {
 // C += the adapters' products, after `base` where one is given (the workspace first: a
 // call that cannot have it has done nothing).
 static int run_lora(const vedic_gemm_desc_t* base, const LoraArgs& a, bool f16, void* stream) {
+    if (!lora_fits(a, f16)) return VEDIC_STATUS_TOO_LARGE;
     Workspace ws;
     ws.s = static_cast<hipStream_t>(stream);
     void* work = nullptr;

@@ -24,6 +24,24 @@ namespace vedic {
 
 constexpr int kMaxGroups = 1024;
 
+// Workgroups of 256 threads that a launch can have: 2^32 threads and more are cut
+// without an error.
+constexpr int64_t kMaxBlocks = int64_t(1) << 24;
+
+// Row tiles of `bm` that R rows in `groups` groups can have at most.
+inline int64_t grouped_row_tiles_max(int R, int groups, int bm) { return R / bm + (groups < R ? groups : R); }
+
+// Whether the general kernels (a workgroup per tile; 128 x 128 where there are many) and
+// the binary16 few-row kernel (16 x 64, NT 16 x 32) can launch a product.
+inline bool grouped_any_fits(int op, int groups, int R, int M, int N) {
+    const int64_t rows = op == 2 ? (int64_t)groups * ((M + 127) / 128) : grouped_row_tiles_max(R, groups, 128);
+    return rows * ((N + 127) / 128) < kMaxBlocks;
+}
+inline bool grouped_skinny_fits(int op, int groups, int R, int N) {
+    const int bn = op == 1 ? 32 : 64;
+    return grouped_row_tiles_max(R, groups, 16) * ((N + bn - 1) / bn) < kMaxBlocks;
+}
+
 enum GroupedKind : int {
     GK_LINEAR = 0,    // C = acc (+ b)
     GK_GELU = 1,      // C = gelu(acc (+ b))

@@ -378,10 +378,7 @@ struct CfgASmall {  // 64 x 64, two waves of 32 x 64
 };
 constexpr int kAnyGroups = 3;  // wave groups of a workgroup where few tiles share the CUs
 
-// Row tiles that R rows in `groups` groups can have at most, and about have.
-inline int64_t grouped_row_tiles_max(int R, int groups, int bm) {
-    return R / bm + (groups < R ? groups : R);
-}
+// Row tiles that R rows in `groups` groups about have.
 inline double grouped_row_tiles(int R, int groups, int bm) {
     return (double)R / bm + 0.5 * (groups < R ? groups : R);
 }
@@ -393,7 +390,7 @@ static hipError_t launch_any(GroupedArgs a, hipStream_t s) {
     a.wide = grouped_wide_rows(a, sizeof(OT));
     const int64_t work = OP == 2 ? (int64_t)a.groups * a.tiles_m * a.tiles_n
                                  : grouped_row_tiles_max(a.R, a.groups, Cfg::BM) * a.tiles_n;
-    if (work > 0x7FFFFFFF) return hipErrorInvalidValue;  // (the caller has refused such sizes)
+    if (work * (Cfg::WGM * Cfg::WGN * WGK * 64) >= int64_t(1) << 32) return hipErrorInvalidValue;  // (grouped_any_fits)
     if (work == 0) return hipSuccess;
     hipLaunchKernelGGL((grouped_any_kernel<OP, T, TB, OT, Cfg::BM, Cfg::BN, Cfg::WGM, Cfg::WGN, WGK, KIND>),
                        dim3((unsigned)work, a.ksplit > 1 ? a.ksplit : 1), dim3(Cfg::WGM * Cfg::WGN * WGK * 64), 0, s, a);

@@ -315,7 +315,7 @@ hipError_t launch_any(const LoraArgs& a, bool f16, float* slabs, void* copy, hip
 
 template <int RP, int KC>
 hipError_t launch_f16(const LoraArgs& a, hipStream_t s) {
-    const int64_t tiles = a.n / 16 + (a.groups < a.n ? a.groups : a.n);
+    const int64_t tiles = grouped_row_tiles_max(a.n, a.groups, 16);
     hipLaunchKernelGGL((lora_shrink_f16_kernel<RP, KC>), dim3((unsigned)tiles), dim3(512), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -338,6 +338,11 @@ bool vec16(const LoraArgs& a) {
 static size_t part_columns(int r) { return r <= 32 ? 32 : r <= 64 ? 64 : 128; }
 
 static size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+bool lora_fits(const LoraArgs& a, bool f16) {
+    if (!f16 || !vec16(a)) return grouped_any_fits(0, a.groups, a.n, 0, a.N);
+    return grouped_row_tiles_max(a.n, a.groups, 16) * ((a.N + 255) / 256) < kMaxBlocks;
+}
 
 size_t lora_bytes(const LoraArgs& a, bool f16) {
     if (f16 && vec16(a)) return (size_t)a.n * (part_columns(a.r) * 6 + 4);  // three parts, and the factors

@@ -27,6 +27,8 @@ struct LoraArgs {
     float* factor;  // [n]
 };
 
+// Whether a launch can have the call's tiles.
+bool lora_fits(const LoraArgs& a, bool f16);
 // Workspace of a call, and the call (work: that many bytes, 256-byte aligned).
 size_t lora_bytes(const LoraArgs& a, bool f16);
 hipError_t launch_lora(LoraArgs a, bool f16, void* work, hipStream_t s);

@@ -62,3 +62,24 @@ def test_listed_rows():
     off = torch.tensor([0, R], dtype=torch.int32, device="cuda")
     got = v.gemm_grouped(v.OP_TN, X, dY, off, rows=rows)
     assert got.item() == (X[rows.long()] * dY).sum().item()
+
+
+@pytest.mark.parametrize("op", ["NN", "NT"])
+def test_few_rows_of_many_columns(op):
+    """One row in each of 1024 groups: more tiles of the few-row kernel than a launch has."""
+    v = vedic()
+    G, K, N = 1024, 8, 1 << 20
+    X = torch.randn(G, K, device="cuda").half()
+    W = torch.randn(N, K, device="cuda").half()
+    off = torch.arange(G + 1, dtype=torch.int32, device="cuda")
+    if op == "NN":
+        got = v.gemm_grouped(v.OP_NN, X, W.t().contiguous().expand(G, K, N), off, out_dtype=F16)
+    else:
+        got = v.gemm_grouped(v.OP_NT, X, W.expand(G, N, K), off, out_dtype=F16)
+    for g in (0, 1, 500, G - 1):
+        want = X[g].double() @ W.double().t()
+        mag = X[g].double().abs() @ W.double().abs().t()
+        # K products and sums in fp32, one rounding to binary16
+        err = (got[g].double() - want).abs()
+        assert (err <= (K * 2.0 ** -24) * mag + 2.0 ** -11 * want.abs() * (1 + 2.0 ** -10) + 2.0 ** -25).all()
+    assert torch.isfinite(got[:, -1]).all()
