@@ -1493,7 +1493,8 @@ extern "C" int vedic_bias_grad_grouped(const void* dY, int dtype, int64_t ld, in
     if (R < 0 || N <= 0 || groups <= 0) return VEDIC_STATUS_BAD_DIM;
     if (!offsets || !db || (R > 0 && !dY)) return VEDIC_STATUS_NULL_POINTER;
     if (ld < N) return VEDIC_STATUS_BAD_LD;
-    if (groups > kMaxGroups) return VEDIC_STATUS_TOO_LARGE;
+    // (row counts stay in int with a phase's step added, columns in a launch's 2^32 threads)
+    if (groups > kMaxGroups || R >= kMaxCount || N >= kMaxCount) return VEDIC_STATUS_TOO_LARGE;
     return hip_status(launch_group_colsum(dY, dtype == VEDIC_DT_F16, ld, R, N, offsets, groups, beta, db,
                                           static_cast<hipStream_t>(stream)));
 }

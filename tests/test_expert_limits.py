@@ -21,3 +21,8 @@ def test_grouped_tiles(kw):
 def test_adapter_tiles(dtype, N):
     args = (P, dtype, 8, 1024, P, P, 1024, 4, P, P, 1024, None, P, N if N % 8 else N + 4, 8, N, None)
     assert _lib.load().vedic_lora_add(*args) == _lib.STATUS_TOO_LARGE
+
+
+@pytest.mark.parametrize("R,N", [(1 << 30, 1), ((1 << 31) - 1, 1), (4, 1 << 30)])
+def test_bias_gradient_counts(R, N):
+    assert _lib.load().vedic_bias_grad_grouped(P, 1, N, R, N, P, 2, 0.0, P, None) == _lib.STATUS_TOO_LARGE
