@@ -268,13 +268,13 @@ struct Workspace {
         if (block && take <= block->cap - block->used) {
             *p = reinterpret_cast<T*>(block->base + block->used);
             block->used += take;
+            note();
             return hipSuccess;
         }
         if (capturing()) return hipErrorStreamCaptureUnsupported;
-        // (with what the calls around this one have, so that the block fits them together)
         pooled += take;
         arena->pooled += take;
-        if (block->used + arena->pooled > arena->want) arena->want = block->used + arena->pooled;
+        note();
         for (void*& slot : extra)
             if (!slot) {
                 const hipError_t e = hipMallocAsync(reinterpret_cast<void**>(p), bytes, s);
@@ -296,6 +296,11 @@ struct Workspace {
     }
 
 private:
+    // What the block has to hold: every piece of this call and of the calls around it,
+    // in the block or from the pool (a piece that fits may follow one that did not).
+    void note() {
+        if (arena->pooled > 0 && block->used + arena->pooled > arena->want) arena->want = block->used + arena->pooled;
+    }
     // Takes the stream's arena for this call.
     void open() {
         if (arena) return;

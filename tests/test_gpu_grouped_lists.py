@@ -132,3 +132,34 @@ def test_column_slice_past_two_gibibytes(K, R):
     for i in range(2):
         s = slice(off[i], off[i + 1])
         check_rows(dW[i].double().cpu().numpy(), a[s].T @ dy[s], np.abs(a[s]).T @ np.abs(dy[s]), sizes[i], F32, f"group {i}")
+
+
+def test_one_call_before_a_capture():
+    """A stream whose block holds a call's first and last piece but not the middle one: after that one call the block fits all
+    three, so the captured call shares its contraction as the eager one does."""
+    from logos_amd import _lib
+
+    v = vedic()
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    X, W = (torch.randn(*s, device="cuda", generator=g).half() for s in ((64, 2051), (3, 2051, 67)))
+    off = ints([0, 40, 40, 64])
+    first = pitched(torch.ones(4700, 64, dtype=F16, device="cuda"), 0, 1)  # 601,600 bytes of padded rows
+    w1 = torch.ones(1, 64, 64, dtype=F16, device="cuda")
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        v.gemm_grouped(v.OP_NN, first, w1, ints([0, 4700]))
+        eager = v.gemm_grouped(v.OP_NN, X, W, off)  # copies of 263,168 and 886,032 bytes, slabs of 68,608
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        recorded = v.gemm_grouped(v.OP_NN, X, W, off)
+    for _ in range(2):
+        recorded.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(recorded, eager)
+    del graph
+    assert _lib.load().vedic_workspace_release(s.cuda_stream) == _lib.STATUS_OK
