@@ -74,6 +74,7 @@ static thread_local int g_last_hip_error = 0;
 static int hip_status(hipError_t e) {
     if (e == hipSuccess) return VEDIC_STATUS_OK;
     g_last_hip_error = (int)e;
+    (void)hipGetLastError();  // (reported here: not the error of the program's next launch)
     return VEDIC_STATUS_HIP_ERROR;
 }
 
@@ -118,10 +119,13 @@ struct StreamArena {
         if (main.used != 0 || want <= main.cap) return;
         if (main.base) (void)hipFreeAsync(main.base, s);
         main = ArenaBlock();
-        if (hipMallocAsync(reinterpret_cast<void**>(&main.base), want, s) == hipSuccess)
+        if (hipMallocAsync(reinterpret_cast<void**>(&main.base), want, s) == hipSuccess) {
             main.cap = want;
-        else
+        } else {  // (calls take their pieces from the pool; what they need is counted anew)
+            (void)hipGetLastError();
             main.base = nullptr;
+            want = 0;
+        }
     }
     // The block of the capture `id`; null if none was there to take over.
     ArenaBlock* captured_block(unsigned long long id) {
@@ -272,14 +276,15 @@ struct Workspace {
             return hipSuccess;
         }
         if (capturing()) return hipErrorStreamCaptureUnsupported;
-        pooled += take;
-        arena->pooled += take;
-        note();
         for (void*& slot : extra)
             if (!slot) {
                 const hipError_t e = hipMallocAsync(reinterpret_cast<void**>(p), bytes, s);
-                if (e == hipSuccess) slot = *p;
-                return e;
+                if (e != hipSuccess) return e;  // (a size that cannot be had is not the block's)
+                slot = *p;
+                pooled += take;
+                arena->pooled += take;
+                note();
+                return hipSuccess;
             }
         return hipErrorOutOfMemory;  // more than 8 pool pieces in one call: not reached by this library
     }
