@@ -592,9 +592,10 @@ int vedic_combine_rows_bwd(const float* dout, int64_t ld_dout, const void* Y, in
 /* Low-rank adapters of many requests beside a shared projection: for the places p
  * of adapter g, i = rows[p]:  C[i] += scales[g] (X[i] . A_g) . B_g, A_g [K x r],
  * B_g [r x N] contiguous, one after another; X, A, B all F32 or all F16, C fp32
- * [M x N], scales NULL: ones.  The product with A_g keeps its fp32 values (the
- * kernel for 16-byte-aligned F16 operands holds them as three binary16 parts: exact from
- * the row's largest down to 2^-39 of it, smaller ones to 2^-63 of it).  A row may be listed
+ * [M x N], scales NULL: ones.  The product with A_g is summed in fp32 and
+ * keeps its values (the kernel for 16-byte-aligned F16 operands holds them as three
+ * binary16 parts: to 2^-24 of a value from the row's largest down to 2^-28 of it, to 2^-22
+ * down to 2^-40, to 2^-51 of the largest below).  A row may be listed
  * once (two adapters on one row would add to it at the same time); rows not listed
  * keep their content.  r <= 128.  Takes about 6 n r bytes of the stream's workspace block
  * (r rounded up to 32, 64 or 128), and n K values where X is 2 GiB or more and is F32 or

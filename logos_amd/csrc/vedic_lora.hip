@@ -52,9 +52,12 @@ __device__ __forceinline__ half8_t read_tr16(const char* lds, int pitch, int k0,
 // H's fp32 values are kept as three binary16 ones each: row p is scaled by 2^-x so that
 // its largest finite value lies in [2^14, 2^15), and h = hi + 2^-12 mid + 2^-24 lo, each
 // part the binary16 nearest to 2^12 times what the last left behind (a remainder of at
-// most 2^4: no overflow).  That is h exactly where its last bit is 2^-48 or more, so for
-// every |h| of 2^-25, 2^-39 of the largest; below, at most 2^-49 is lost, 2^-63 of the
-// largest.  (Two parts without the 2^12 lose bits from 2^-18 of the largest on; the fp32
+// most 2^3: no overflow).  hi and mid are zero rather than subnormal: the MFMA aligns a
+// product by its operands' exponents as they stand, so that a subnormal's product beside
+// another keeps only the bits from 2^-38 of the other operand on.  What is lost is at most
+// 2^-24 of h down to 2^-14, 2^-28 of the largest, 2^-22 (mid and lo alone) down to 2^-26,
+// 2^-40 of it, and 2^-37, 2^-51 of the largest, below.
+// (Two parts without the 2^12 lose bits from 2^-18 of the largest on; the fp32
 // MFMA on H itself takes longer: 4096 rows, 1024 into 4096, projection included, two parts
 // / three / fp32 MFMA, rank 64 89 / 93 / 98 us, rank 128 113 / 119 / 147.)
 // factor[p] = scale 2^x then multiplies the product's fp32 sums.
@@ -174,9 +177,10 @@ __global__ void __launch_bounds__(512) lora_shrink_f16_kernel(LoraArgs a) {
         for (int v = 0; v < NC; ++v) {
             const int c = c0 + 32 * v;
             const float s = h[v] * down;
-            const _Float16 hi = (_Float16)s;
+            auto normal = [](float x) { return (_Float16)(fabsf(x) < 0x1p-14f ? 0.0f : x); };
+            const _Float16 hi = normal(s);
             const float r1 = fabsf(s) < __builtin_inff() ? (s - (float)hi) * 4096.0f : 0.0f;
-            const _Float16 mid = (_Float16)r1;
+            const _Float16 mid = normal(r1);
             o[c] = hi;
             o[RS + c] = mid;
             o[2 * RS + c] = (_Float16)((r1 - (float)mid) * 4096.0f);
