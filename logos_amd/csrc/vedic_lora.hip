@@ -59,7 +59,8 @@ __device__ __forceinline__ half8_t read_tr16(const char* lds, int pitch, int k0,
 // 2^-40 of it, and 2^-37, 2^-51 of the largest, below.
 // (Two parts without the 2^12 lose bits from 2^-18 of the largest on; the fp32
 // MFMA on H itself takes longer: 4096 rows, 1024 into 4096, projection included, two parts
-// / three / fp32 MFMA, rank 64 89 / 93 / 98 us, rank 128 113 / 119 / 147.)
+// / three / three staged by the expansion / fp32 MFMA, rank 64 89 / 93 / 88 / 98 us, rank
+// 128 113 / 119 / 109 / 147.)
 // factor[p] = scale 2^x then multiplies the product's fp32 sums.
 template <int RP, int KC>
 __global__ void __launch_bounds__(512) lora_shrink_f16_kernel(LoraArgs a) {
@@ -192,11 +193,17 @@ __global__ void __launch_bounds__(512) lora_shrink_f16_kernel(LoraArgs a) {
 // C[rows[p]] += factor[p] (hi + 2^-12 mid + 2^-24 lo) B_g: 16 places by 256 columns, a wave
 // 64 of them.  B_g's columns are staged in LDS once for the three parts, whose products
 // have accumulators of their own; they are taken transposed, so that a lane holds four
-// neighbouring columns of one row.
+// neighbouring columns of one row.  Past rank 32 the 16 rows of H are staged too, once for
+// the four waves (4096 rows, 1024 into 4096, projection included, each wave its own / staged:
+// rank 32 79.6 / 82.5 us, 64 93 / 88.8, 128 119 / 110).
 template <int RS>
 __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
+    constexpr bool STAGED = RS > 32;
+    constexpr int HB = 16 * 3 * RS * 2, CPP = RS / 8;  // bytes of the 16 rows, 16-byte chunks of a part
     __shared__ __attribute__((aligned(1024))) char sb[RS * 512];
-    __shared__ GroupIndex ix;
+    __shared__ __attribute__((aligned(1024))) char sh[STAGED ? HB : 16];
+    GroupIndex& ix = *reinterpret_cast<GroupIndex*>(sb);
+    static_assert(sizeof(GroupIndex) <= RS * 512, "the index fits B's buffer");
     GroupedArgs q{};
     q.offsets = a.offsets;
     q.groups = a.groups;
@@ -210,6 +217,7 @@ __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
     const int b0 = (t - __builtin_amdgcn_readfirstlane(ix.pre[g])) * 16, p0 = group_start(q, g) + b0;
     const int np = min(16, group_count(q, g) - b0);
     const int n0 = (blockIdx.x - t * strips) * 256;
+    __syncthreads();  // the index's LDS takes B
     const _Float16* B = static_cast<const _Float16*>(a.B) + (int64_t)g * a.r * a.N + n0;
     const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(B);
 #pragma unroll
@@ -220,12 +228,28 @@ __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
                                                  in ? (uint32_t)(k * a.N * 2 + slot * 16) : kOob, 0, 0, 0);
     }
     const int p = lane & 15;
-    const _Float16* h = a.Hs + (int64_t)(p0 + (p < np ? p : 0)) * (3 * RS) + 8 * (lane >> 4);
+    const _Float16* H = a.Hs + (int64_t)p0 * (3 * RS);
     half8_t part[3][RS / 32];
+    // (staged: a part's chunks of row p are XORed by p, so that the rows' reads spread over
+    // the banks)
+    auto chunk = [](int p, int c) { return c ^ (p & 7); };
+    if constexpr (STAGED) {
+        const __amdgpu_buffer_rsrc_t rh = buffer_rsrc(H);
 #pragma unroll
-    for (int q3 = 0; q3 < 3; ++q3)
+        for (int i = 0; i < (HB / 1024 + 3) / 4; ++i) {
+            const int at = 4 * i + wave, u = at * 64 + lane, pr = u / (3 * CPP), c = u % (3 * CPP), q3 = c / CPP;
+            if (at < HB / 1024)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    rh, (lds_void_t*)(sh + at * 1024), 16,
+                    pr < np ? (uint32_t)((pr * 3 * CPP + q3 * CPP + chunk(pr, c % CPP)) * 16) : kOob, 0, 0, 0);
+        }
+    } else {
+        const _Float16* h = H + (p < np ? p : 0) * (3 * RS) + 8 * (lane >> 4);
 #pragma unroll
-        for (int c = 0; c < RS / 32; ++c) part[q3][c] = *reinterpret_cast<const half8_t*>(h + q3 * RS + 32 * c);
+        for (int q3 = 0; q3 < 3; ++q3)
+#pragma unroll
+            for (int c = 0; c < RS / 32; ++c) part[q3][c] = *reinterpret_cast<const half8_t*>(h + q3 * RS + 32 * c);
+    }
     const float f = a.factor[p0 + (p < np ? p : 0)];
     const int row = p < np ? a.rows[p0 + p] : -1;
     const bool ok = (unsigned)row < (unsigned)a.M;
@@ -238,6 +262,13 @@ __global__ void __launch_bounds__(256) lora_expand_f16_kernel(LoraArgs a) {
     }
     wait_vmcnt<0>();
     __syncthreads();
+    if constexpr (STAGED) {
+#pragma unroll
+        for (int q3 = 0; q3 < 3; ++q3)
+#pragma unroll
+            for (int c = 0; c < RS / 32; ++c)
+                part[q3][c] = *reinterpret_cast<const half8_t*>(sh + ((p * 3 + q3) * CPP + chunk(p, 4 * c + (lane >> 4))) * 16);
+    }
     float4_t acc[3][4];
 #pragma unroll
     for (int q3 = 0; q3 < 3; ++q3)
