@@ -228,11 +228,23 @@ bool try_wave_rows(const TIn* X, const float* gamma, const float* beta, float* Y
     return true;
 }
 
+// Rows of a launch: a workgroup each at most, fewer than 2^32 threads (more are cut
+// without an error); a multiple of 4, so that every launch's rows are aligned alike.
+constexpr int kLnMaxRows = (1 << 24) - 4;
+
 }  // namespace
 
 hipError_t launch_layernorm_f32(const float* X, const float* gamma, const float* beta, float* Y, void* Y16, int seq,
                                 int d, float eps, hipStream_t s) {
     _Float16* y16 = static_cast<_Float16*>(Y16);
+    constexpr int64_t kMost = kLnMaxRows;
+    for (; seq > kMost; seq -= (int)kMost) {
+        const hipError_t e = launch_layernorm_f32(X, gamma, beta, Y, y16, kLnMaxRows, d, eps, s);
+        if (e != hipSuccess) return e;
+        X += kMost * d;
+        if (Y) Y += kMost * d;
+        if (y16) y16 += kMost * d;
+    }
     if (try_wave_rows(X, gamma, beta, Y, y16, seq, d, eps, s)) return hipGetLastError();
     const dim3 grid((unsigned)seq), block(kLnThreads);
     if (Y && y16)
@@ -251,6 +263,13 @@ hipError_t launch_layernorm_f16(const void* X16, const float* gamma, const float
                                 float eps, hipStream_t s) {
     const _Float16* x16 = static_cast<const _Float16*>(X16);
     _Float16* y16 = static_cast<_Float16*>(Y16);
+    constexpr int64_t kMost = kLnMaxRows;
+    for (; seq > kMost; seq -= (int)kMost) {
+        const hipError_t e = launch_layernorm_f16(x16, gamma, beta, y16, kLnMaxRows, d, eps, s);
+        if (e != hipSuccess) return e;
+        x16 += kMost * d;
+        y16 += kMost * d;
+    }
     if (try_wave_rows(x16, gamma, beta, nullptr, y16, seq, d, eps, s)) return hipGetLastError();
     hipLaunchKernelGGL((layernorm_rows_kernel<_Float16, false, true>), dim3((unsigned)seq), dim3(kLnThreads), 0, s,
                        x16, gamma, beta, nullptr, y16, d, eps);

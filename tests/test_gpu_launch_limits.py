@@ -83,3 +83,20 @@ def test_few_rows_of_many_columns(op):
         err = (got[g].double() - want).abs()
         assert (err <= (K * 2.0 ** -24) * mag + 2.0 ** -11 * want.abs() * (1 + 2.0 ** -10) + 2.0 ** -25).all()
     assert torch.isfinite(got[:, -1]).all()
+
+
+@pytest.mark.parametrize("rows,d", [((1 << 24) + 7, 3), (MANY, 4)])
+def test_layer_normalisation(rows, d):
+    v = vedic()
+    X = torch.randn(rows, d, device="cuda")
+    gamma, beta = torch.randn(d, device="cuda"), torch.randn(d, device="cuda")
+    Y, Y16 = v.layernorm(X, gamma, beta, fp16=True)
+    step = 1 << 22
+    for at in (0, step, rows // step // 2 * step, rows // step * step):
+        y, y16 = v.layernorm(X[at:at + step], gamma, beta, fp16=True)
+        assert torch.equal(Y[at:at + step], y) and torch.equal(Y16[at:at + step], y16)
+    h = torch.empty(rows, d, dtype=F16, device="cuda")
+    h.copy_(X)
+    Y16 = v.layernorm_fp16(h, gamma, beta)
+    at = rows // step * step
+    assert torch.equal(Y16[at:], v.layernorm_fp16(h[at:], gamma, beta))
