@@ -5,9 +5,9 @@
 // values), then C.  fp32 operands, and rows that 16-byte loads cannot take, run as two
 // grouped products (vedic_grouped_any.hpp).
 //
-// 4096 rows, 1024 into 4096, 12 adapters of rank 64 (all but a twelfth of the rows): 7.9 us
-// for H, bound by the latency of its few workgroups, and 30.2 us for C, bound by reading and
-// writing it (125 MB, 4.1 TB/s); 16 rows of rank 16 4.6 and 4.8 us, two launches' latency.
+// 4096 rows, 1024 into 4096, 12 adapters of rank 64 (all but a twelfth of the rows): 8.2 us
+// for H, bound by the latency of its few workgroups, and 28.2 us for C, bound by reading and
+// writing it (125 MB, 4.4 TB/s); 16 rows of rank 16 4.8 and 5.2 us, two launches' latency.
 #include "vedic_combine.hpp"
 #include "vedic_common.hpp"
 #include "vedic_gemm_f16.hpp"
