@@ -813,6 +813,7 @@ static int gemm_impl(const vedic_gemm_desc_t* d, float* const* heads, int nheads
     int ks = skinny || scatter || wave_split || (f16 && !direct)
                  ? 1
                  : choose_ksplit(d->op, d->M, d->N, d->K, vec, device_cu_count(), f16);
+    if (ks > 1) (void)split_kslice(d->K, ks, f16);  // (the slices that whole steps leave, as launch_split counts them)
     // (in a capture without memory for the slices the product runs unsplit)
     if (ks > 1 && !ws.room(sizeof(float) * (size_t)d->M * d->N * ks +
                            (d->colsum ? Workspace::rounded(sizeof(float) * colsum_matrix_floats(d->M, d->N)) : 0)))
