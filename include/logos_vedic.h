@@ -612,6 +612,111 @@ int vedic_lora_add(const void* X, int dtype, int64_t ldx, int M, const void* A, 
 int vedic_gemm_lora(const vedic_gemm_desc_t* base, const void* A, const void* B, int groups, int r, const int* offsets,
                     const int* rows, int n, const float* scales);
 
+/* ---- decoding: a paged cache of keys and values, weights in four bits ------ */
+
+/* New: the reference keeps no keys and values (every generated token is a whole forward,
+ * cuda/train_gpu.cu:2045) and multiplies binary16 or fp32 weights only.
+ *
+ * Four bits.  A 32-bit word holds eight consecutive values, value 2i in bits 4i .. 4i + 3 and
+ * value 2i + 1 in bits 16 + 4i .. 19 + 4i; code n of a group with the binary16 pair (s, m)
+ * stands for binary16(s n + m), rounded once.  Groups are quantised from their binary16
+ * values as m = the least, s = binary16((largest - least) / 15), n = (x - m) / s to the
+ * nearest (even) of 0 .. 15, 0 where s is 0; a group with an infinity or NaN stands for NaN. */
+typedef enum {
+    VEDIC_KV_F16 = 0, /* a row: dh binary16 values (dh a multiple of 8)                       */
+    VEDIC_KV_I4 = 1   /* a row: dh / 8 words, then dh / 32 pairs (s, m), one per 32 values:
+                         5 dh / 8 bytes (dh a multiple of 32)                                 */
+} vedic_kv_format_t;
+
+/* A cache and the sequences of one call.  Row `offset` of page p, key head h starts at
+ * p stride_page + h stride_head + offset stride_token (binary16 values with F16, bytes with
+ * I4) of k and of v.  Position t of sequence b lies in page table[b ld_table + t / page_size],
+ * row t % page_size.  lens[b] counts sequence b's tokens, the call's new ones included; its
+ * new ones are the last n_b, the call's rows q_start[b] .. q_start[b + 1] - 1 (q_start NULL: row
+ * b alone, tokens = batch).  Rows before q_start[0] or from q_start[batch] on belong to no
+ * sequence.  The lists stay on the GPU and are clamped where they are read (lengths to what
+ * table_cols pages hold, rows to 0 .. tokens, a page outside the cache is page 0 when read
+ * and is not written), so that bad ones give wrong values but no access outside the arrays.
+ * Limits: dh <= 256; 2^30 positions; fewer than 2^30 query rows (tokens x heads), 2^20
+ * sequences and 2^24 workgroups a launch (VEDIC_STATUS_TOO_LARGE past them).
+ * Alignment: rows, q and outputs of 16 bytes, I4 rows of 4 (VEDIC_STATUS_BAD_LD). */
+typedef struct {
+    int format; /* vedic_kv_format_t */
+    int pages, page_size, heads, dh;
+    void* k;
+    void* v;
+    int64_t stride_page, stride_head, stride_token;
+    const int* table;
+    int64_t ld_table;
+    int table_cols;
+    const int* lens;
+    const int* q_start;
+    int batch, tokens;
+} vedic_kv_t;
+
+/* New tokens into the cache: k and v [tokens x heads x dh], F32 or F16 at any strides (in values),
+ * k turned by its position, both rounded to binary16 (nearest even) and stored in the cache's
+ * format; and, with q_heads > 0, q [tokens x q_heads x dh] turned and rounded into q_out (which
+ * is not q).  Rotation (rope_dims > 0, even): pairs (x_i, x_(i + rope_dims / 2)) of a row, or
+ * (x_2i, x_(2i + 1)) with interleaved, by the angle of row `position` (the last one past the
+ * end) of rope [rope_rows x rope_dims]: rope_dims / 2 cosines, then the sines, fp32:
+ *     (a, b) -> (a cos - b sin, b cos + a sin),  each product and sum rounded to fp32.
+ * No two rows may have one place in the cache.  A row of no sequence, or before its
+ * sequence's first position, writes nothing, q_out included. */
+int vedic_kv_append(const vedic_kv_t* kv, int dtype, const void* q, int64_t q_token, int64_t q_head, int q_heads,
+                    void* q_out, int64_t q_out_token, int64_t q_out_head, const void* k, int64_t k_token,
+                    int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const float* rope, int rope_rows,
+                    int rope_dims, int interleaved, void* stream);
+
+/* The same tokens' rows back from the cache: k and v [tokens x heads x dh] binary16, contiguous,
+ * either NULL (q_start the running sums of lens: whole sequences).  Rows of no sequence are
+ * left as they are. */
+int vedic_kv_read(const vedic_kv_t* kv, void* k, void* v, void* stream);
+
+/* Attention of the new rows over the cache: q [tokens x q_heads x dh] binary16, head j of q with key
+ * head j / (q_heads / heads).  The row at position p = lens[b] - n_b + i sees keys
+ * t <= p (causal; else all lens[b]) and, with window > 0 (causal only), of those t >= p - window and,
+ * with stride > 0, also t a multiple of stride -- the masks of vedic_flash_attention_fwd:
+ *     out = sum over t of e^(scale q.k_t - M) v_t / sum of the same without v_t,
+ * 0 for a row that sees no key.  lse (NULL, or [tokens x q_heads]): ln of sum e^(scale q.k_t), +inf for
+ * such a row.  out binary16, rounded once; scores and sums fp32, weights binary16 relative to
+ * their largest.  What a masked key or a page's unused row holds, NaN included, does not
+ * reach the output.  Rows of no sequence are left as they are.
+ * Sequences of up to 64 rows (n_b x q_heads / heads) share out their keys evenly over the GPU,
+ * others take 128 rows a workgroup and share keys where that leaves CUs idle; parts are added in
+ * a fixed order, 2 x (CUs x 4 x 16 + CUs x 2 x 128) x (dh + 2) fp32 of the stream's workspace block at
+ * most.  A captured call without such a block does not split (results may then differ in
+ * rounding). */
+int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_t q_token, int64_t q_head, int q_heads, void* out,
+                          int64_t out_token, int64_t out_head, float* lse, float scale, int causal, int window,
+                          int stride, void* stream);
+
+/* A weight W [K x N] in four bits: column n's ceil(K / 32) * 4 words (values past K are not used, but
+ * their codes are there) at codes + n * that, and its ceil(K / group) pairs (s, m); group 32, 64 or
+ * 128 consecutive values of K.  codes 16-byte, scales 4-byte aligned. */
+typedef struct {
+    const void* codes;
+    const void* scales;
+    int K, N, group;
+} vedic_w4_t;
+
+/* W (F32 or F16, row-major; F32 values rounded to binary16 with the clamp of vedic_cast_f32_to_f16,
+ * infinities and NaN kept) into that form. */
+int vedic_w4_quantize(const void* W, int dtype, int64_t ldw, int K, int N, int group, void* codes, void* scales,
+                      void* stream);
+
+/* The values it stands for, binary16 [K x N]. */
+int vedic_w4_unpack(const vedic_w4_t* w, void* W16, int64_t ldw, void* stream);
+
+/* C[M x N] = epi(X[M x K] . W): X F16, or F32 clamped and rounded to binary16 as it is read; products of
+ * binary16 values summed in fp32; C F32 or F16.  Epilogues NONE, BIAS, BIAS_GELU, and (F32 C)
+ * RESIDUAL, BIAS_RESIDUAL.  Up to 64 rows read the codes themselves; more rows expand W into the
+ * stream's workspace block first, in slabs of columns of up to 64 MiB (and copy an X that is F32
+ * or whose rows are not whole 16 bytes), and run the binary16 tiles; a captured call without such a block takes
+ * 64 rows at a time (results may then differ in rounding). */
+int vedic_gemm_w4(const vedic_w4_t* w, const void* X, int x_dtype, int64_t ldx, int M, void* C, int c_dtype, int64_t ldc,
+                  const float* bias, int epilogue, void* stream);
+
 /* ---- test hooks --------------------------------------------------------- */
 
 /* Off by default.  When on, every GEMM with column sums allocates its

@@ -32,6 +32,7 @@ OP_NN, OP_NT, OP_TN = 0, 1, 2
 EPI_NONE, EPI_BIAS, EPI_BIAS_GELU, EPI_GELU, EPI_GELU_BWD = 0, 1, 2, 3, 4
 EPI_RESIDUAL, EPI_BIAS_RESIDUAL = 5, 6
 DT_F32, DT_F16, DT_F32_F16 = 0, 1, 2
+KV_F16, KV_I4 = 0, 1
 
 
 class GemmDesc(ctypes.Structure):
@@ -93,6 +94,42 @@ class GroupedDesc(ctypes.Structure):
         ("db", c_vp),
         ("db_beta", c_float),
         ("stream", c_vp),
+    ]
+
+
+class Kv(ctypes.Structure):
+    """Mirror of vedic_kv_t."""
+
+    _fields_ = [
+        ("format", c_int),
+        ("pages", c_int),
+        ("page_size", c_int),
+        ("heads", c_int),
+        ("dh", c_int),
+        ("k", c_vp),
+        ("v", c_vp),
+        ("stride_page", c_i64),
+        ("stride_head", c_i64),
+        ("stride_token", c_i64),
+        ("table", c_vp),
+        ("ld_table", c_i64),
+        ("table_cols", c_int),
+        ("lens", c_vp),
+        ("q_start", c_vp),
+        ("batch", c_int),
+        ("tokens", c_int),
+    ]
+
+
+class W4Desc(ctypes.Structure):
+    """Mirror of vedic_w4_t."""
+
+    _fields_ = [
+        ("codes", c_vp),
+        ("scales", c_vp),
+        ("K", c_int),
+        ("N", c_int),
+        ("group", c_int),
     ]
 
 
@@ -174,6 +211,20 @@ SIGNATURES = {
     ),
     "vedic_gemm_lora": (
         c_int, [ctypes.POINTER(GemmDesc), c_vp, c_vp, c_int, c_int, c_vp, c_vp, c_int, c_vp]),
+    "vedic_kv_append": (
+        c_int,
+        [ctypes.POINTER(Kv), c_int, c_vp, c_i64, c_i64, c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,
+         c_vp, c_int, c_int, c_int, c_vp],
+    ),
+    "vedic_kv_read": (c_int, [ctypes.POINTER(Kv), c_vp, c_vp, c_vp]),
+    "vedic_paged_attention": (
+        c_int,
+        [ctypes.POINTER(Kv), c_vp, c_i64, c_i64, c_int, c_vp, c_i64, c_i64, c_vp, c_float, c_int, c_int, c_int, c_vp],
+    ),
+    "vedic_w4_quantize": (c_int, [c_vp, c_int, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_vp]),
+    "vedic_w4_unpack": (c_int, [ctypes.POINTER(W4Desc), c_vp, c_i64, c_vp]),
+    "vedic_gemm_w4": (
+        c_int, [ctypes.POINTER(W4Desc), c_vp, c_int, c_i64, c_int, c_vp, c_int, c_i64, c_vp, c_int, c_vp]),
     "vedic_debug_set_workspace_guard": (None, [c_int]),
     "vedic_debug_workspace_guard_hits": (ctypes.c_long, []),
     "vedic_uses_vendor_blas": (c_int, []),

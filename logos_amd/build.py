@@ -46,6 +46,12 @@ SOURCES = [
     "vedic_route.hip",
     "vedic_combine.hip",
     "vedic_lora.hip",
+    "vedic_cache.hip",
+    "vedic_paged_few_f16.hip",
+    "vedic_paged_few_i4.hip",
+    "vedic_paged_many_f16.hip",
+    "vedic_paged_many_i4.hip",
+    "vedic_w4.hip",
     "vedic_capi.hip",
 ]
 

@@ -1,0 +1,164 @@
+// vedic_cache.hpp -- a paged cache of keys and values, as the kernels that write it
+// (vedic_cache.hip) and read it (vedic_paged.hip) see it, and the four-bit format that
+// the cache and the weights of vedic_w4.hip share.
+#pragma once
+
+#include "vedic_common.hpp"
+
+namespace vedic {
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+// 16 bytes at a 4-byte-aligned address (gfx950 loads and stores them as one access).
+typedef uint32_t u32x4_a4_t __attribute__((ext_vector_type(4), aligned(4)));
+
+// Positions stay below this.
+constexpr int kMaxTokens = 1 << 30;
+
+struct KvView {
+    char* k;
+    char* v;
+    int64_t page, head, token;  // strides in bytes
+    int pages, ps, H, D;
+    const int* table;  // [B x ldt]
+    int64_t ldt;
+    int tcols;
+    const int* lens;     // [B]
+    const int* q_start;  // [B + 1], or null: row b is sequence b's only new one
+    int B, T;
+    // pos / ps = pos * magic >> shift for pos < 2^30 (kv_divider)
+    uint32_t magic;
+    int shift;
+
+    __device__ __forceinline__ int page_of(int pos) const { return (int)((uint64_t)(uint32_t)pos * magic >> shift); }
+    // Tokens of sequence b, as many as its pages can hold at most.
+    __device__ __forceinline__ int len_of(int b) const {
+        const int64_t cap = (int64_t)tcols * ps;
+        const int most = cap < kMaxTokens ? (int)cap : kMaxTokens - 1;
+        return max(0, min(lens[b], most));
+    }
+    // First new row and count of new rows of sequence b (clamped to 0 .. T).
+    __device__ __forceinline__ void rows_of(int b, int& first, int& n) const {
+        if (q_start == nullptr) {
+            first = b;
+            n = b < T ? 1 : 0;
+            return;
+        }
+        first = max(0, min(q_start[b], T));
+        n = max(0, min(q_start[b + 1], T) - first);
+    }
+    // Byte offset of the row of position pos < len (head 0); a page that is none counts as page 0.
+    __device__ __forceinline__ int64_t row_offset(int b, int pos) const {
+        const int t = page_of(pos);
+        int p = table[b * ldt + t];
+        if ((unsigned)p >= (unsigned)pages) p = 0;
+        return p * page + (pos - t * ps) * token;
+    }
+};
+
+inline void kv_divider(KvView& v) {
+    int l = 0;
+    while ((1 << l) < v.ps) ++l;
+    v.shift = 30 + l;
+    v.magic = (uint32_t)((uint64_t(1) << v.shift) / v.ps + 1);
+}
+
+// Four-bit words: 32 bits hold eight consecutive values, value 2 i in bits 4 i .. 4 i + 3 and
+// value 2 i + 1 in bits 16 + 4 i ..; code n of a group with the binary16 pair (s, m) stands
+// for binary16(s n + m), one rounding.  n | 0x6400 is the binary16 1024 + n, and a nibble at
+// bits 4 .. 7 under 0x5400 is 64 + n, so that a pair of values takes one and-or, one exact
+// subtraction and one fused multiply-add.
+__device__ __forceinline__ half8_t four_bit_values(uint32_t w, half2_t s, half2_t m) {
+    const half2_t k1024 = {(_Float16)1024.0f, (_Float16)1024.0f}, k64 = {(_Float16)64.0f, (_Float16)64.0f};
+    const uint32_t w8 = w >> 8;
+    const half2_t n0 = __builtin_bit_cast(half2_t, (w & 0x000F000Fu) | 0x64006400u) - k1024;
+    const half2_t n1 = __builtin_bit_cast(half2_t, (w & 0x00F000F0u) | 0x54005400u) - k64;
+    const half2_t n2 = __builtin_bit_cast(half2_t, (w8 & 0x000F000Fu) | 0x64006400u) - k1024;
+    const half2_t n3 = __builtin_bit_cast(half2_t, (w8 & 0x00F000F0u) | 0x54005400u) - k64;
+    union {
+        half2_t p[4];
+        half8_t h;
+    } u;
+    u.p[0] = __builtin_elementwise_fma(s, n0, m);
+    u.p[1] = __builtin_elementwise_fma(s, n1, m);
+    u.p[2] = __builtin_elementwise_fma(s, n2, m);
+    u.p[3] = __builtin_elementwise_fma(s, n3, m);
+    return u.h;
+}
+__device__ __forceinline__ void four_bit_pair(uint32_t sm, half2_t& s, half2_t& m) {
+    const half2_t p = __builtin_bit_cast(half2_t, sm);
+    s = half2_t{p[0], p[0]};
+    m = half2_t{p[1], p[1]};
+}
+
+// store16_hold of eight binary16 values.
+__device__ __forceinline__ void store_half8(void* p, half8_t h) {
+    store16_hold(static_cast<float*>(p), __builtin_bit_cast(float4_t, h));
+}
+
+// A value that no multiply-add is formed across (the library is compiled with
+// -ffp-contract=fast, which fuses a product into the sum that takes it).
+__device__ __forceinline__ float rounded(float x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// The pair (s, m) of a group whose least and largest binary16 values are lo and hi.
+__device__ __forceinline__ uint32_t four_bit_scale(float lo, float hi, bool bad) {
+    if (bad) return 0x7E007E00u;  // NaN, NaN
+    const half2_t sm = {(_Float16)((hi - lo) / 15.0f), (_Float16)lo};
+    return __builtin_bit_cast(uint32_t, sm);
+}
+__device__ __forceinline__ uint32_t four_bit_code(float x, float s, float lo) {
+    if (!(s > 0.0f)) return 0u;
+    return (uint32_t)__builtin_fminf(__builtin_fmaxf(__builtin_rintf((x - lo) / s), 0.0f), 15.0f);
+}
+__device__ __forceinline__ uint32_t four_bit_word(const float (&x)[8], float s, float lo) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= four_bit_code(x[i], s, lo) << (4 * (i >> 1) + 16 * (i & 1));
+    return w;
+}
+
+struct KvAppendArgs {
+    KvView c;
+    bool i4, f32;  // cache format, type of q, k, v
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;  // strides in values
+    _Float16* q_out;
+    int Hq;
+    const float* rope;  // [rope_rows x rot]: cosines, then sines
+    int rope_rows, rot;
+    bool inter;
+};
+hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t s);
+// k, v: [T x H x D] binary16, either may be null.
+hipError_t launch_kv_read(const KvView& c, bool i4, _Float16* k, _Float16* v, hipStream_t s);
+
+// Attention of the new rows over the cache.
+struct PagedArgs {
+    KvView c;
+    const _Float16* q;
+    _Float16* out;
+    float* lse;  // [T x Hq] or null
+    int64_t q_token, q_head, o_token, o_head;  // strides in values
+    int Hq, G;
+    float scale;  // times log2(e)
+    int causal, window, stride;
+    // set by the rules in vedic_capi.hip: `target` workgroups' worth of keys per item
+    // (0: items are not split), and the partial results of split items
+    int64_t target;
+    int few_most;  // sequences of at most so many rows (new rows x G) are the few-row kernel's
+    int slots;
+    float* part_o;   // [slots x rows x D]
+    float* part_ml;  // [slots x rows x 2]
+};
+constexpr int kFewRows = 16, kManyRows = 128;
+hipError_t launch_paged_few_f16(const PagedArgs& a, hipStream_t s);
+hipError_t launch_paged_few_i4(const PagedArgs& a, hipStream_t s);
+hipError_t launch_paged_many_f16(const PagedArgs& a, hipStream_t s);
+hipError_t launch_paged_many_i4(const PagedArgs& a, hipStream_t s);
+
+}  // namespace vedic

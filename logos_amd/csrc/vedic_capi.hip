@@ -19,10 +19,12 @@
 #include "vedic_flash_attn.hpp"
 #include "vedic_common.hpp"
 #include "vedic_epilogue.hpp"
+#include "vedic_cache.hpp"
 #include "vedic_combine.hpp"
 #include "vedic_grouped.hpp"
 #include "vedic_lora.hpp"
 #include "vedic_route.hpp"
+#include "vedic_w4.hpp"
 
 namespace vedic {
 hipError_t launch_grouped_f16_nn(const GroupedArgs& a, int kind, bool f16out, hipStream_t s);
@@ -1679,6 +1681,298 @@ extern "C" int vedic_gemm_lora(const vedic_gemm_desc_t* base, const void* A, con
                     lora_args(base->A, base->lda, base->M, A, B, groups, r, offsets, rows, n, scales,
                               static_cast<float*>(base->C), base->ldc, base->K, base->N),
                     base->in_dtype == VEDIC_DT_F16, base->stream);
+}
+
+// ------------------------------------------------- paged cache, four-bit weights
+
+// Checks of a cache and its call's sequences; v: what the kernels take.  `some`: whether there is work.
+static int kv_view(const vedic_kv_t* d, KvView& v, bool& some) {
+    some = false;
+    if (!d) return VEDIC_STATUS_NULL_POINTER;
+    if (d->format != VEDIC_KV_F16 && d->format != VEDIC_KV_I4) return VEDIC_STATUS_BAD_DTYPE;
+    const bool i4 = d->format == VEDIC_KV_I4;
+    if (d->pages <= 0 || d->page_size <= 0 || d->heads <= 0 || d->dh <= 0 || d->dh > 256 || d->table_cols <= 0 ||
+        d->batch < 0 || d->tokens < 0 || d->dh % (i4 ? 32 : 8) != 0)
+        return VEDIC_STATUS_BAD_DIM;
+    if (!d->q_start && d->tokens != d->batch) return VEDIC_STATUS_BAD_DIM;
+    if (d->page_size >= kMaxTokens || d->batch >= (1 << 20) || (int64_t)d->tokens * d->heads >= kMaxCount ||
+        d->heads >= (1 << 16))
+        return VEDIC_STATUS_TOO_LARGE;
+    if (d->batch == 0 || d->tokens == 0) return VEDIC_STATUS_OK;
+    if (!d->k || !d->v || !d->table || !d->lens) return VEDIC_STATUS_NULL_POINTER;
+    const int64_t es = i4 ? 1 : 2, row = i4 ? d->dh / 8 * 5 : d->dh, unit = i4 ? 4 : 8;
+    for (int64_t s : {d->stride_page, d->stride_head, d->stride_token})
+        if (s < row || s % unit != 0) return VEDIC_STATUS_BAD_LD;
+    if ((((uintptr_t)d->k | (uintptr_t)d->v) & (i4 ? 3 : 15)) != 0 || d->ld_table < d->table_cols)
+        return VEDIC_STATUS_BAD_LD;
+    some = true;
+    v.k = static_cast<char*>(d->k);
+    v.v = static_cast<char*>(d->v);
+    v.page = d->stride_page * es;
+    v.head = d->stride_head * es;
+    v.token = d->stride_token * es;
+    v.pages = d->pages;
+    v.ps = d->page_size;
+    v.H = d->heads;
+    v.D = d->dh;
+    v.table = d->table;
+    v.ldt = d->ld_table;
+    v.tcols = d->table_cols;
+    v.lens = d->lens;
+    v.q_start = d->q_start;
+    v.B = d->batch;
+    v.T = d->tokens;
+    kv_divider(v);
+    return VEDIC_STATUS_OK;
+}
+
+// Rows of 16-byte pieces at these strides (values of 2 bytes).
+static bool half_rows(const void* p, int64_t token, int64_t head) {
+    return aligned16(p) && token % 8 == 0 && head % 8 == 0;
+}
+
+extern "C" int vedic_kv_append(const vedic_kv_t* kv, int dtype, const void* q, int64_t q_token, int64_t q_head, int q_heads,
+                               void* q_out, int64_t q_out_token, int64_t q_out_head, const void* k, int64_t k_token,
+                               int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const float* rope,
+                               int rope_rows, int rope_dims, int interleaved, void* stream) {
+    KvAppendArgs a{};
+    bool some;
+    const int st = kv_view(kv, a.c, some);
+    if (st != VEDIC_STATUS_OK) return st;
+    if (dtype != VEDIC_DT_F32 && dtype != VEDIC_DT_F16) return VEDIC_STATUS_BAD_DTYPE;
+    if (q_heads < 0 || rope_dims < 0 || rope_dims % 2 != 0 || rope_dims > kv->dh || (rope_dims > 0 && rope_rows <= 0))
+        return VEDIC_STATUS_BAD_DIM;
+    if (q_heads >= (1 << 16) || (int64_t)kv->tokens * q_heads >= kMaxCount) return VEDIC_STATUS_TOO_LARGE;
+    // (launches of fewer than 2^32 threads; a thread takes eight values)
+    const int64_t blocks = ((int64_t)(q_heads + 2 * kv->heads) * (kv->dh / 8) + 255) / 256;
+    if (blocks * kv->tokens >= (1 << 24)) return VEDIC_STATUS_TOO_LARGE;
+    if (!some) return VEDIC_STATUS_OK;
+    if (!k || !v || (q_heads > 0 && (!q || !q_out)) || (rope_dims > 0 && !rope)) return VEDIC_STATUS_NULL_POINTER;
+    if (q_token < 0 || q_head < 0 || k_token < 0 || k_head < 0 || v_token < 0 || v_head < 0) return VEDIC_STATUS_BAD_LD;
+    if (q_heads > 0 && (!half_rows(q_out, q_out_token, q_out_head) || q_out == q || (kv->tokens > 1 && q_out_token < kv->dh) ||
+                        (q_heads > 1 && q_out_head < kv->dh)))
+        return VEDIC_STATUS_BAD_LD;
+    a.i4 = kv->format == VEDIC_KV_I4;
+    a.f32 = dtype == VEDIC_DT_F32;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_token = q_token;
+    a.q_head = q_head;
+    a.k_token = k_token;
+    a.k_head = k_head;
+    a.v_token = v_token;
+    a.v_head = v_head;
+    a.o_token = q_out_token;
+    a.o_head = q_out_head;
+    a.q_out = static_cast<_Float16*>(q_out);
+    a.Hq = q_heads;
+    a.rope = rope;
+    a.rope_rows = rope_rows;
+    a.rot = rope_dims;
+    a.inter = interleaved != 0;
+    return hip_status(launch_kv_append(a, static_cast<hipStream_t>(stream)));
+}
+
+extern "C" int vedic_kv_read(const vedic_kv_t* kv, void* k, void* v, void* stream) {
+    KvView c{};
+    bool some;
+    const int st = kv_view(kv, c, some);
+    if (st != VEDIC_STATUS_OK) return st;
+    const int64_t blocks = ((int64_t)kv->heads * (kv->dh / 8) + 255) / 256;
+    if (blocks * kv->tokens >= (1 << 24)) return VEDIC_STATUS_TOO_LARGE;
+    if (!some || (!k && !v)) return VEDIC_STATUS_OK;
+    if (!aligned16(k) || !aligned16(v)) return VEDIC_STATUS_BAD_LD;
+    return hip_status(launch_kv_read(c, kv->format == VEDIC_KV_I4, static_cast<_Float16*>(k), static_cast<_Float16*>(v),
+                                     static_cast<hipStream_t>(stream)));
+}
+
+// Rows (new tokens x heads that share a key head) up to which a sequence is the few-row kernel's.
+static constexpr int kFewMost = 64;
+
+// Workgroups' worth of keys that a call's items are cut to: as many as a GPU has at work.
+static int64_t paged_target(bool many, int dh, int cus) { return many ? cus * (dh <= 128 ? 2 : 1) : cus * 4; }
+
+extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_t q_token, int64_t q_head, int q_heads,
+                                     void* out, int64_t out_token, int64_t out_head, float* lse, float scale, int causal,
+                                     int window, int stride, void* stream) {
+    PagedArgs a{};
+    bool some;
+    const int st = kv_view(kv, a.c, some);
+    if (st != VEDIC_STATUS_OK) return st;
+    if (q_heads <= 0 || q_heads % kv->heads != 0 || window < 0 || stride < 0 || (window > 0 && !causal) ||
+        (stride > 0 && window == 0))
+        return VEDIC_STATUS_BAD_DIM;
+    if (q_heads >= (1 << 16) || (int64_t)kv->tokens * q_heads >= kMaxCount) return VEDIC_STATUS_TOO_LARGE;
+    a.G = q_heads / kv->heads;
+    const int64_t rows = (int64_t)kv->tokens * a.G;
+    const int64_t tiles = (rows / kFewRows + (kv->batch < kv->tokens ? kv->batch : kv->tokens)) * kv->heads;
+    if (tiles + 4096 >= (1 << 24)) return VEDIC_STATUS_TOO_LARGE;
+    if (!some) return VEDIC_STATUS_OK;
+    if (!q || !out) return VEDIC_STATUS_NULL_POINTER;
+    if (!half_rows(q, q_token, q_head) || !half_rows(out, out_token, out_head) || q_token < 0 || q_head < 0 ||
+        (kv->tokens > 1 && out_token < kv->dh) || (q_heads > 1 && out_head < kv->dh))
+        return VEDIC_STATUS_BAD_LD;
+    a.q = static_cast<const _Float16*>(q);
+    a.out = static_cast<_Float16*>(out);
+    a.lse = lse;
+    a.q_token = q_token;
+    a.q_head = q_head;
+    a.o_token = out_token;
+    a.o_head = out_head;
+    a.Hq = q_heads;
+    a.scale = scale * 1.44269504088896340736f;
+    a.causal = causal != 0;
+    a.window = window < kMaxTokens ? window : kMaxTokens;
+    a.stride = stride;
+    const bool i4 = kv->format == VEDIC_KV_I4;
+    const int cus = device_cu_count();
+    // Which kernels: sequences' rows are known on the GPU only, so a call whose sequences may be of both kinds runs
+    // both, each on its own ones.
+    const bool few = rows < (int64_t)kFewMost * kv->batch || rows <= kFewMost;
+    const bool many = rows > kFewMost && (kv->q_start || a.G > kFewMost);
+    a.few_most = !many ? INT32_MAX : !few ? 0 : kFewMost;
+    Workspace ws;
+    ws.s = static_cast<hipStream_t>(stream);
+    hipError_t e = hipSuccess;
+    for (int kind = 0; kind < 2 && e == hipSuccess; ++kind) {
+        if (kind == 0 ? !few : !many) continue;
+        PagedArgs b = a;
+        const int tile = kind ? kManyRows : kFewRows;
+        b.target = paged_target(kind != 0, kv->dh, cus);
+        // (where no sequence can have two parts)
+        if ((int64_t)kv->table_cols * kv->page_size <= (kind ? 256 : 128)) b.target = 0;
+        const size_t slots = 2 * (size_t)b.target, bytes = slots * tile * (kv->dh + 2) * 4;
+        if (!ws.room(bytes)) b.target = 0;
+        float* part = nullptr;
+        if (b.target > 0) {
+            e = ws.get(&part, bytes);
+            if (e != hipSuccess) break;
+            b.slots = (int)slots;
+            b.part_o = part;
+            b.part_ml = part + slots * tile * kv->dh;
+        }
+        e = kind ? (i4 ? launch_paged_many_i4(b, ws.s) : launch_paged_many_f16(b, ws.s))
+                 : (i4 ? launch_paged_few_i4(b, ws.s) : launch_paged_few_f16(b, ws.s));
+        const hipError_t f = ws.put(part);
+        if (e == hipSuccess) e = f;
+    }
+    return hip_status(e);
+}
+
+static int w4_view(const vedic_w4_t* d, W4View& w) {
+    if (!d) return VEDIC_STATUS_NULL_POINTER;
+    if (d->K <= 0 || d->N <= 0 || (d->group != 32 && d->group != 64 && d->group != 128)) return VEDIC_STATUS_BAD_DIM;
+    if (d->K >= kMaxLd || d->N >= kMaxLd) return VEDIC_STATUS_TOO_LARGE;
+    if (!d->codes || !d->scales) return VEDIC_STATUS_NULL_POINTER;
+    if (!aligned16(d->codes) || ((uintptr_t)d->scales & 3) != 0) return VEDIC_STATUS_BAD_LD;
+    w.codes = static_cast<const uint32_t*>(d->codes);
+    w.sm = static_cast<const uint32_t*>(d->scales);
+    w.K = d->K;
+    w.N = d->N;
+    w.group = d->group;
+    w.words = (d->K + 31) / 32 * 4;
+    w.G = (d->K + d->group - 1) / d->group;
+    return VEDIC_STATUS_OK;
+}
+
+extern "C" int vedic_w4_quantize(const void* W, int dtype, int64_t ldw, int K, int N, int group, void* codes, void* scales,
+                                 void* stream) {
+    W4View w;
+    const vedic_w4_t d{codes, scales, K, N, group};
+    const int st = w4_view(&d, w);
+    if (st != VEDIC_STATUS_OK) return st;
+    if (dtype != VEDIC_DT_F32 && dtype != VEDIC_DT_F16) return VEDIC_STATUS_BAD_DTYPE;
+    if (!W) return VEDIC_STATUS_NULL_POINTER;
+    if (ldw < N) return VEDIC_STATUS_BAD_LD;
+    return hip_status(launch_w4_quantize(W, dtype == VEDIC_DT_F32, ldw, w, static_cast<uint32_t*>(codes),
+                                         static_cast<uint32_t*>(scales), static_cast<hipStream_t>(stream)));
+}
+
+extern "C" int vedic_w4_unpack(const vedic_w4_t* d, void* W16, int64_t ldw, void* stream) {
+    W4View w;
+    const int st = w4_view(d, w);
+    if (st != VEDIC_STATUS_OK) return st;
+    if (!W16) return VEDIC_STATUS_NULL_POINTER;
+    if (ldw < d->N) return VEDIC_STATUS_BAD_LD;
+    return hip_status(launch_w4_unpack(w, static_cast<_Float16*>(W16), ldw, static_cast<hipStream_t>(stream)));
+}
+
+// Expanded columns at a time (bytes).
+static constexpr size_t kW4Slab = size_t(64) << 20;
+
+extern "C" int vedic_gemm_w4(const vedic_w4_t* d, const void* X, int x_dtype, int64_t ldx, int M, void* C, int c_dtype,
+                             int64_t ldc, const float* bias, int epilogue, void* stream) {
+    W4Args a{};
+    const int st = w4_view(d, a.w);
+    if (st != VEDIC_STATUS_OK) return st;
+    if (M < 0) return VEDIC_STATUS_BAD_DIM;
+    if ((x_dtype != VEDIC_DT_F32 && x_dtype != VEDIC_DT_F16) || (c_dtype != VEDIC_DT_F32 && c_dtype != VEDIC_DT_F16))
+        return VEDIC_STATUS_BAD_DTYPE;
+    const bool wants = epilogue == VEDIC_EPI_BIAS || epilogue == VEDIC_EPI_BIAS_GELU || epilogue == VEDIC_EPI_BIAS_RESIDUAL;
+    const bool resid = epilogue == VEDIC_EPI_RESIDUAL || epilogue == VEDIC_EPI_BIAS_RESIDUAL;
+    if (!(wants || resid || epilogue == VEDIC_EPI_NONE) || (wants && !bias) || (resid && c_dtype != VEDIC_DT_F32))
+        return VEDIC_STATUS_BAD_EPILOGUE;
+    if (ldx >= kMaxLd || ldc >= kMaxLd || M >= kMaxCount) return VEDIC_STATUS_TOO_LARGE;
+    // (launches of fewer than 2^32 threads)
+    if ((int64_t)((M + kW4FewRows - 1) / kW4FewRows) * ((d->N + 15) / 16) >= (1 << 23)) return VEDIC_STATUS_TOO_LARGE;
+    if (M == 0) return VEDIC_STATUS_OK;
+    if (!X || !C) return VEDIC_STATUS_NULL_POINTER;
+    if (ldx < d->K || ldc < d->N) return VEDIC_STATUS_BAD_LD;
+    a.X = X;
+    a.ldx = ldx;
+    a.M = M;
+    a.x32 = x_dtype == VEDIC_DT_F32;
+    a.C = C;
+    a.ldc = ldc;
+    a.c16 = c_dtype == VEDIC_DT_F16;
+    a.bias = wants ? bias : nullptr;
+    a.gelu = epilogue == VEDIC_EPI_BIAS_GELU;
+    a.residual = resid;
+    Workspace ws;
+    ws.s = static_cast<hipStream_t>(stream);
+    if (M > kW4FewRows) {
+        const int64_t kp = (int64_t)a.w.words * 8;
+        const bool rows = a.x32 || d->K % 8 != 0 || !aligned16(X) || ldx % 8 != 0;
+        int64_t cols = (int64_t)(kW4Slab / (kp * 2)) / 256 * 256;
+        if (cols < 256) cols = 256;
+        if (cols > d->N) cols = d->N;
+        const size_t wb = (size_t)cols * kp * 2, xb = rows ? (size_t)M * kp * 2 : 0;
+        if (ws.room(Workspace::rounded(wb) + Workspace::rounded(xb))) {
+            _Float16 *w16 = nullptr, *x16 = nullptr;
+            hipError_t e = ws.get(&w16, wb);
+            if (e == hipSuccess && rows) e = ws.get(&x16, xb);
+            if (e == hipSuccess && rows) e = launch_w4_rows(X, a.x32, ldx, M, d->K, x16, kp, ws.s);
+            int status = VEDIC_STATUS_OK;
+            for (int64_t n0 = 0; n0 < d->N && e == hipSuccess && status == VEDIC_STATUS_OK; n0 += cols) {
+                const int n = (int)(d->N - n0 < cols ? d->N - n0 : cols);
+                e = launch_w4_expand(a.w, (int)n0, n, w16, ws.s);
+                if (e != hipSuccess) break;
+                vedic_gemm_desc_t g{};
+                g.op = VEDIC_OP_NT;
+                g.in_dtype = VEDIC_DT_F16;
+                g.out_dtype = c_dtype;
+                g.M = M;
+                g.N = n;
+                g.K = rows ? (int)kp : d->K;
+                g.A = rows ? x16 : X;
+                g.lda = rows ? kp : ldx;
+                g.B = w16;
+                g.ldb = kp;
+                g.C = static_cast<char*>(C) + n0 * (a.c16 ? 2 : 4);
+                g.ldc = ldc;
+                g.alpha = 1.0f;
+                g.bias = wants ? bias + n0 : nullptr;
+                g.epilogue = epilogue;
+                g.stream = stream;
+                status = gemm_impl(&g, nullptr, 0, 0);
+            }
+            const hipError_t f = ws.put(x16), h = ws.put(w16);
+            if (status != VEDIC_STATUS_OK) return status;
+            return hip_status(e != hipSuccess ? e : f != hipSuccess ? f : h);
+        }
+    }
+    return hip_status(launch_w4_few(a, device_cu_count(), ws.s));
 }
 
 // ----------------------------------------------------------- elementwise

@@ -1,0 +1,240 @@
+// vedic_paged.hpp -- what the attention kernels over a paged cache share: how the work is
+// dealt out, which keys a row sees, a row computed without matrix instructions, and the
+// join of split items.
+//
+// A work item is a tile of ROWS rows of one sequence and one key head, and a range of its
+// keys.  Row rho of a sequence is new token rho / G, head rho % G of the G query heads that
+// share the key head, so that a key is read once for all of them.  Lengths are known on the
+// GPU only: every workgroup adds up the keys of all tiles, takes 1 / target of them (rounded
+// up) as the length of a part, and finds its own item by a scan over the sequences; the
+// host's grid is as large as the items can be.  So a batch of one long and many short
+// sequences is dealt out evenly, whatever the table's width.
+//
+// Parts hold their sums relative to their own maximum: O = sum of 2^(x - m + 14) v and l the
+// same without v, x the score times log2(e); the join multiplies by 2^(m - M) in the order of
+// the parts.  The 2^14 keeps weights normal binary16 numbers down to 2^-28 of the largest.
+#pragma once
+
+#include "vedic_cache.hpp"
+
+namespace vedic {
+
+constexpr float kWeightBits = 14.0f;
+constexpr float kNoScore = -__builtin_inff();
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+struct PagedItem {
+    int b, tile, h;      // sequence, tile of its rows, key head
+    int first, n, len;   // its new rows and its tokens
+    int lo, hi;          // keys of this part
+    int part, parts;
+    int slot;            // of the partial result (parts > 1)
+};
+
+// Keys that some row of the sequence may see: [lo, len).
+__device__ __forceinline__ int first_key(const PagedArgs& a, int len, int n) {
+    return a.window > 0 && a.stride == 0 ? max(0, len - n - a.window) : 0;
+}
+
+template <int ROWS, bool MANY>
+__device__ __forceinline__ void sequence_work(const PagedArgs& a, int b, int& tiles, int& span) {
+    tiles = span = 0;
+    if (b >= a.c.B) return;
+    int first, n;
+    a.c.rows_of(b, first, n);
+    const int64_t rows = (int64_t)n * a.G;
+    if (n == 0 || (rows > a.few_most) != MANY) return;
+    const int len = a.c.len_of(b);
+    tiles = (int)((rows + ROWS - 1) / ROWS);
+    span = max(0, len - first_key(a, len, n));
+}
+
+__device__ __forceinline__ int parts_of(int span, int chunk) { return span > chunk ? (span + chunk - 1) / chunk : 1; }
+
+// Keys of a part: at least UNIT, in whole UNITs.
+template <int ROWS, bool MANY, int UNIT>
+__device__ __forceinline__ int part_length(const PagedArgs& a, int lane) {
+    if (a.target <= 0) return INT32_MAX;
+    int64_t total = 0;
+    for (int b0 = 0; b0 < a.c.B; b0 += 64) {
+        int tiles, span;
+        sequence_work<ROWS, MANY>(a, b0 + lane, tiles, span);
+        total += (int64_t)tiles * span;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d);
+    const int64_t each = (total * a.c.H + a.target - 1) / a.target;
+    return each >= (int64_t)INT32_MAX - UNIT ? INT32_MAX : max(1, (int)((each + UNIT - 1) / UNIT)) * UNIT;
+}
+
+// The item (JOIN: the tile) number id; false if there is none.
+template <int ROWS, bool MANY, int UNIT, bool JOIN>
+__device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, PagedItem& it) {
+    const int chunk = part_length<ROWS, MANY, UNIT>(a, lane);
+    int before = 0, slots = 0;  // items (JOIN: tiles) and split items of the sequences before
+    for (int b0 = 0; b0 < a.c.B; b0 += 64) {
+        int tiles, span;
+        sequence_work<ROWS, MANY>(a, b0 + lane, tiles, span);
+        const int parts = parts_of(span, chunk);
+        // (sums of a list that is not ascending stay in range too)
+        const int items = (int)min((int64_t)tiles * a.c.H * parts, int64_t(1) << 24);
+        const int units = JOIN ? (int)min((int64_t)tiles * a.c.H, int64_t(1) << 24) : items;
+        const int split = parts > 1 ? items : 0;
+        int incl = units, sincl = split;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(incl, d), p = __shfl_up(sincl, d);
+            if (lane >= d) incl += o, sincl += p;
+        }
+        const uint64_t past = __ballot(id - before < incl);
+        if (past) {
+            const int who = __builtin_ctzll(past);
+            it.b = b0 + who;
+            const int at = id - before - (__builtin_amdgcn_readlane(incl, who) - __builtin_amdgcn_readlane(units, who));
+            it.parts = __builtin_amdgcn_readlane(parts, who);
+            const int unit = JOIN ? at : at / it.parts;  // tile * H + head
+            it.part = JOIN ? 0 : at - unit * it.parts;
+            const int s0 = slots + __builtin_amdgcn_readlane(sincl, who) - __builtin_amdgcn_readlane(split, who);
+            it.slot = s0 + unit * it.parts + it.part;
+            const int ntiles = __builtin_amdgcn_readlane(tiles, who);
+            // (the last rows of a prompt see the most keys: they begin first)
+            const int tile = unit / a.c.H;
+            it.h = unit - tile * a.c.H;
+            it.tile = ntiles - 1 - tile;
+            a.c.rows_of(it.b, it.first, it.n);
+            it.first = __builtin_amdgcn_readfirstlane(it.first);
+            it.n = __builtin_amdgcn_readfirstlane(it.n);
+            it.len = __builtin_amdgcn_readfirstlane(a.c.len_of(it.b));
+            const int lo = first_key(a, it.len, it.n), sp = max(0, it.len - lo);
+            const int each = ((sp + it.parts - 1) / it.parts + UNIT - 1) / UNIT * UNIT;
+            // keys that some row of the tile sees
+            const int i0 = it.tile * ROWS / a.G, i1 = min(it.n - 1, (it.tile * ROWS + ROWS - 1) / a.G);
+            const int tlo = a.window > 0 && a.stride == 0 ? max(lo, it.len - it.n + i0 - a.window) : lo;
+            const int thi = a.causal ? max(0, it.len - it.n + i1 + 1) : it.len;
+            const int64_t p0 = lo + (int64_t)it.part * each;
+            it.lo = (int)min(max(p0, (int64_t)tlo), (int64_t)thi);
+            it.hi = (int)min(it.parts == 1 ? (int64_t)thi : p0 + each, (int64_t)thi);
+            it.hi = max(it.hi, it.lo);
+            return JOIN || it.parts == 1 || it.slot < a.slots;  // (at most 2 target of them: vedic_capi.hip)
+        }
+        before += __builtin_amdgcn_readlane(incl, 63);
+        slots = min(slots + __builtin_amdgcn_readlane(sincl, 63), 1 << 29);
+    }
+    return false;
+}
+
+// Whether the row at position pos sees key t < len.
+__device__ __forceinline__ bool sees(const PagedArgs& a, int pos, int t) {
+    if (a.causal && t > pos) return false;
+    return a.window == 0 || t >= pos - a.window || (a.stride > 0 && t % a.stride == 0);
+}
+
+// The value d of a cache row.
+template <bool I4>
+__device__ __forceinline__ float cache_value(const char* row, int D, int d) {
+    if constexpr (!I4) return (float)reinterpret_cast<const _Float16*>(row)[d];
+    half2_t s, m;
+    four_bit_pair(reinterpret_cast<const uint32_t*>(row + D / 2)[d >> 5], s, m);
+    const half8_t v = four_bit_values(reinterpret_cast<const uint32_t*>(row)[d >> 3], s, m);
+    float r = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r = (d & 7) == i ? (float)v[i] : r;
+    return r;
+}
+
+// One row's part by one wave, key by key: what a key outside the row's mask holds never enters
+// a sum.  For rows whose sums came out infinite or NaN: in a product of tiles the zero weight
+// of an unseen key times an infinity is NaN.  o: values lane, lane + 64, ..
+template <int DP, bool I4>
+__device__ __forceinline__ void slow_row(const PagedArgs& a, int b, int h, int pos, int lo, int hi, const _Float16* q, int lane,
+                                      float (&o)[DP / 64], float& m, float& l) {
+    float qv[DP / 64];
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j) {
+        const int d = lane + 64 * j;
+        qv[j] = d < a.c.D ? (float)q[d] : 0.0f;
+        o[j] = 0.0f;
+    }
+    m = kNoScore;
+    l = 0.0f;
+    for (int t = lo; t < hi; ++t) {
+        if (!sees(a, pos, t)) continue;
+        const int64_t at = a.c.row_offset(b, t) + (int64_t)h * a.c.head;
+        float x = 0.0f;
+#pragma unroll
+        for (int j = 0; j < DP / 64; ++j) {
+            const int d = lane + 64 * j;
+            if (d < a.c.D) x += qv[j] * cache_value<I4>(a.c.k + at, a.c.D, d);
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+        x *= a.scale;
+        const float mn = __builtin_fmaxf(m, x), mu = mn == kNoScore ? 0.0f : mn;
+        const float f = exp2_fast(m - mu), p = exp2_fast(x - mu + kWeightBits);
+        l = l * f + p;
+        m = mn;
+#pragma unroll
+        for (int j = 0; j < DP / 64; ++j) {
+            const int d = lane + 64 * j;
+            o[j] = o[j] * f + (d < a.c.D ? p * cache_value<I4>(a.c.v + at, a.c.D, d) : 0.0f);
+        }
+    }
+}
+
+__device__ __forceinline__ float lse_of(float m, float l) {
+    return l > 0.0f || l != l ? (m - kWeightBits + __builtin_log2f(l)) * 0.6931471805599453f : __builtin_inff();
+}
+
+namespace {
+
+// The parts of a tile joined: a wave per row, its lanes D / 4 columns of four and the rest
+// shares of the parts.
+template <int ROWS, bool MANY, int UNIT>
+__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    PagedItem it;
+    if (!find_item<ROWS, MANY, UNIT, true>(a, blockIdx.x, lane, it)) return;
+    if (it.parts == 1 || (int64_t)it.slot + it.parts > a.slots) return;
+    const int r = blockIdx.y * 4 + wave, rho = it.tile * ROWS + r, i = rho / a.G;
+    if (r >= ROWS || i >= it.n) return;
+    const int D = a.c.D, cols = D / 4;
+    const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // of a share
+    const int share = lane / lanes, shares = 64 / lanes, c = lane % lanes;
+    const int64_t s0 = (int64_t)it.slot * ROWS + r;
+    float M = kNoScore;
+    for (int p = lane; p < it.parts; p += 64) M = __builtin_fmaxf(M, a.part_ml[2 * (s0 + (int64_t)p * ROWS)]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) M = __builtin_fmaxf(M, __shfl_xor(M, d));
+    const float mu = M == kNoScore ? 0.0f : M;
+    float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+#pragma unroll 4
+    for (int p = share; p < it.parts; p += shares) {
+        const int64_t s = s0 + (int64_t)p * ROWS;
+        const float f = exp2_fast(a.part_ml[2 * s] - mu), lp = a.part_ml[2 * s + 1];
+        const float4_t v = *reinterpret_cast<const float4_t*>(a.part_o + s * D + 4 * min(c, cols - 1));
+        if (f > 0.0f || f != f || lp != lp) {  // (a part without keys has nothing to add)
+            l += lp * f;
+            o += v * f;
+        }
+    }
+    for (int d = lanes; d < 64; d <<= 1) {
+        l += __shfl_xor(l, d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], d);
+    }
+    const int head = it.h * a.G + rho % a.G;
+    const int64_t t = it.first + i;
+    if (share == 0 && c < cols) {
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+        const half4_t v = {(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
+        *reinterpret_cast<half4_t*>(a.out + t * a.o_token + (int64_t)head * a.o_head + 4 * c) = v;
+    }
+    if (a.lse && lane == 0) a.lse[t * a.Hq + head] = lse_of(M, l);
+}
+
+}  // namespace
+
+}  // namespace vedic

@@ -1,0 +1,366 @@
+// vedic_paged_few.hpp -- attention of a few new rows a sequence over its paged cache: one
+// decoded token, or up to some rows of a key head's group of query heads.
+//
+//   S^T = K Q^T (16 tokens x 16 rows per v_mfma_f32_16x16x32_f16), weights 2^(x - m + 14) with a
+//   running maximum and sum in fp32, O^T += V^T P^T.
+//
+// A workgroup has a tile of 16 rows and a range of keys (vedic_paged.hpp); its four waves
+// take 32 keys each in turn, on their own: a wave reads K into the registers that the MFMA
+// takes, V through a piece of LDS of its own (written as rows, read by the transposing
+// ds_read_b64_tr_b16), and no barrier is met until the four partial results are added.  The
+// scores come out with a row of Q per lane and tokens 4 g + i, 16 + 4 g + i in lane group g, which is
+// the order in which the second product then contracts: the weights stay in registers.
+// K and V of the next 32 keys are loaded as soon as their registers are free; a wave has 16 KB
+// under way (binary16, heads of 128), a CU eight to twelve waves.  Reading the cache bounds it.
+//
+// Four bits: lane group g takes values g DP/4 .. + DP/4 - 1 of a token's row, whole words; K is
+// expanded in registers as the MFMA takes it, V as it goes to LDS.
+#pragma once
+
+#include "vedic_paged.hpp"
+
+namespace vedic {
+
+namespace {
+
+typedef short paged_short4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+
+// A lane's share of one token's row: DP / 4 values.
+template <int DP, bool I4>
+struct RowShare;
+template <int DP>
+struct RowShare<DP, false> {
+    static constexpr int KK = DP / 32;
+    u32x4_t v[KK];
+    // Values 32 kk + 8 g .. + 7, zero past D.
+    __device__ __forceinline__ void load(const char* row, int D, int g) {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            v[kk] = u32x4_t{0, 0, 0, 0};
+            if (D == DP || 32 * kk + 8 * g < D) v[kk] = *reinterpret_cast<const u32x4_t*>(row + 64 * kk + 16 * g);
+        }
+    }
+    __device__ __forceinline__ half8_t frag(int kk) const { return __builtin_bit_cast(half8_t, v[kk]); }
+    __device__ __forceinline__ static int first(int kk, int g) { return 32 * kk + 8 * g; }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) v[kk] = u32x4_t{0, 0, 0, 0};
+    }
+};
+template <int DP>
+struct RowShare<DP, true> {
+    static constexpr int KK = DP / 32, NS = (KK + 3) / 4;
+    uint32_t w[KK];
+    uint32_t sm[NS];
+    // Values g DP / 4 + 8 kk .. + 7; words past D have a pair of zeros.
+    __device__ __forceinline__ void load(const char* row, int D, int g) {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + g * KK;
+        const uint32_t* ps = reinterpret_cast<const uint32_t*>(row + D / 2);
+        const int g0 = g * KK / 4;
+        if (D == DP) {
+            if constexpr (KK == 2) {
+                typedef uint32_t a4 __attribute__((ext_vector_type(2), aligned(4)));
+                const a4 x = *reinterpret_cast<const a4*>(p);
+                w[0] = x[0];
+                w[1] = x[1];
+            } else if constexpr (KK % 4 == 0) {
+#pragma unroll
+                for (int i = 0; i < KK / 4; ++i) {
+                    const u32x4_a4_t x = *reinterpret_cast<const u32x4_a4_t*>(p + 4 * i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < KK; ++i) w[i] = p[i];
+            }
+#pragma unroll
+            for (int i = 0; i < NS; ++i) sm[i] = ps[min(g0 + i, D / 32 - 1)];
+        } else {
+#pragma unroll
+            for (int i = 0; i < KK; ++i) w[i] = 8 * (g * KK + i) < D ? p[i] : 0u;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) sm[i] = 32 * (g0 + i) < D ? ps[g0 + i] : 0u;
+        }
+    }
+    __device__ __forceinline__ half8_t frag(int kk, int g) const {
+        // (the group of word g KK + kk, counted from the lane's first group)
+        uint32_t x = sm[0];
+        if constexpr (NS > 1) {
+            const int at = (g * KK + kk) / 4 - g * KK / 4;
+#pragma unroll
+            for (int i = 1; i < NS; ++i) x = at == i ? sm[i] : x;
+        }
+        half2_t s, m;
+        four_bit_pair(x, s, m);
+        return four_bit_values(w[kk], s, m);
+    }
+    __device__ __forceinline__ static int first(int kk, int g) { return g * KK * 8 + 8 * kk; }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) sm[i] = 0u;
+    }
+};
+template <int DP>
+__device__ __forceinline__ half8_t share_frag(const RowShare<DP, false>& r, int kk, int) { return r.frag(kk); }
+template <int DP>
+__device__ __forceinline__ half8_t share_frag(const RowShare<DP, true>& r, int kk, int g) { return r.frag(kk, g); }
+
+constexpr int kFewUnit = 128;  // keys of a round of four waves
+
+template <int DP, bool I4>
+__global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
+    constexpr int KK = DP / 32, DT = DP / 16, PITCH = 2 * DP + 32, OP = DP + 4;
+    static_assert(16 * OP * 4 <= 32 * PITCH, "a wave's partial result fits its piece of LDS");
+    __shared__ __attribute__((aligned(16))) char lds[4 * 32 * PITCH];
+    __shared__ float ml[4][16][2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    PagedItem it;
+    if (!find_item<kFewRows, false, kFewUnit, false>(a, blockIdx.x, lane, it)) return;
+    const KvView& c = a.c;
+    const int r = lane & 15, g = lane >> 4;
+    char* vb = lds + wave * (32 * PITCH);
+
+    // this lane's row of Q
+    const int rho = it.tile * kFewRows + r, i = rho / a.G;
+    const bool mine = i < it.n;
+    const int pos = mine ? it.len - it.n + i : -1;
+    half8_t qf[KK];
+    {
+        const _Float16* q = a.q + (int64_t)(it.first + (mine ? i : 0)) * a.q_token +
+                            (int64_t)(it.h * a.G + (mine ? rho - i * a.G : 0)) * a.q_head;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const int d = RowShare<DP, I4>::first(kk, g);
+            qf[kk] = half8_t{};
+            if (d < c.D) qf[kk] = *reinterpret_cast<const half8_t*>(q + d);
+        }
+    }
+    // keys [klo, khi) of this row; the sparse mask's keys before klo are looked at one by one
+    const int khi = !mine ? 0 : a.causal ? pos + 1 : it.len;
+    const int klo = a.window > 0 ? pos - a.window : INT32_MIN;
+
+    const char* kb = c.k + (int64_t)it.h * c.head;
+    const char* vbase = c.v + (int64_t)it.h * c.head;
+    const int* table = c.table + it.b * c.ldt;
+    // the page of the lane's two tokens of the block at t, and the rest of their rows' offsets
+    auto place = [&](int t, int (&page)[2], int (&inside)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int p = max(0, min(t + 16 * u + r, it.hi - 1)), tp = c.page_of(p);
+            page[u] = table[tp];
+            inside[u] = p - tp * c.ps;
+        }
+    };
+    auto offset = [&](int page, int inside) {
+        return ((unsigned)page < (unsigned)c.pages ? page : 0) * c.page + inside * c.token;
+    };
+
+    float m = kNoScore, l = 0.0f;
+    float4_t acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+    int t = it.lo + 32 * wave;
+    RowShare<DP, I4> k[2], v[2];
+    int64_t off[2];
+    int page[2], inside[2];
+    if (t < it.hi) {
+        place(t, page, inside);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            off[u] = offset(page[u], inside[u]);
+            k[u].load(kb + off[u], c.D, g);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) v[u].load(vbase + off[u], c.D, g);
+        place(min(t + kFewUnit, it.hi - 1), page, inside);
+    }
+    for (; t < it.hi; t += kFewUnit) {
+        const bool more = t + kFewUnit < it.hi;
+        float4_t s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            s[u] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(share_frag(k[u], kk, g), qf[kk], s[u], 0, 0, 0);
+        }
+        if (more) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                off[u] = offset(page[u], inside[u]);
+                k[u].load(kb + off[u], c.D, g);
+            }
+        }
+        // V of this block to LDS; rows past the range as zeros (what lies there is nobody's)
+        if (t + 32 > it.hi) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (t + 16 * u + r >= it.hi) v[u].clear();
+        }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+                *reinterpret_cast<half8_t*>(vb + (16 * u + r) * PITCH + 2 * RowShare<DP, I4>::first(kk, g)) =
+                    share_frag(v[u], kk, g);
+        asm volatile("" ::: "memory");
+        if (more) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) v[u].load(vbase + off[u], c.D, g);
+            place(min(t + 2 * kFewUnit, it.hi - 1), page, inside);
+        }
+        // weights
+        float x[8];
+        float mx = kNoScore;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int tok = t + 16 * (e >> 2) + 4 * g + (e & 3);
+            bool in = tok < khi && tok < it.hi;
+            if (a.window > 0) in = in && (tok >= klo || (a.stride > 0 && tok % a.stride == 0));
+            x[e] = in ? s[e >> 2][e & 3] * a.scale : kNoScore;
+            mx = __builtin_fmaxf(mx, x[e]);
+        }
+        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
+        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
+        const float mn = __builtin_fmaxf(m, mx), mu = mn == kNoScore ? 0.0f : mn;
+        const float f = exp2_fast(m - mu);
+        m = mn;
+        half8_t p;
+        l *= f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float w = exp2_fast(x[e] - mu + kWeightBits);
+            l += w;
+            p[e] = (_Float16)w;
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            union {
+                paged_short4_t q[2];
+                half8_t h;
+            } u;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+                u.q[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) paged_short4_t*)(vb + (16 * b + 4 * g + (r >> 2)) * PITCH +
+                                                                        2 * (16 * d + 4 * (r & 3))));
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u.h, p, acc[d], 0, 0, 0);
+        }
+        asm volatile("" ::: "memory");
+    }
+
+    // the four waves' results
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g == 0) {
+        ml[wave][r][0] = m;
+        ml[wave][r][1] = l;
+    }
+    float* po = reinterpret_cast<float*>(vb);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<float4_t*>(po + r * OP + 16 * d + 4 * g) = acc[d];
+    __syncthreads();
+    const int row = threadIdx.x >> 4, col = 4 * (threadIdx.x & 15);
+    const int rrho = it.tile * kFewRows + row, ri = rrho / a.G;
+    float M = kNoScore, L = 0.0f, fw[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = __builtin_fmaxf(M, ml[w][row][0]);
+    const float mu = M == kNoScore ? 0.0f : M;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        fw[w] = exp2_fast(ml[w][row][0] - mu);
+        L += ml[w][row][1] * fw[w];
+    }
+    float4_t o[DP / 64];
+    bool fine = L < __builtin_inff();
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j) {
+        o[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            o[j] += *reinterpret_cast<const float4_t*>(lds + w * (32 * PITCH) + 4 * (row * OP + col + 64 * j)) * fw[w];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) fine = fine && __builtin_fabsf(o[j][q]) < __builtin_inff();
+    }
+    const bool here = ri < it.n;
+    const int head = it.h * a.G + rrho - ri * a.G;
+    const int64_t tok = it.first + ri;
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    if (here) {
+        if (it.parts == 1) {
+            _Float16* out = a.out + tok * a.o_token + (int64_t)head * a.o_head + col;
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j)
+                if (col + 64 * j < c.D) {
+                    const half4_t h = {(_Float16)(o[j][0] * inv), (_Float16)(o[j][1] * inv), (_Float16)(o[j][2] * inv),
+                                       (_Float16)(o[j][3] * inv)};
+                    *reinterpret_cast<half4_t*>(out + 64 * j) = h;
+                }
+            if (a.lse && col == 0) a.lse[tok * a.Hq + head] = lse_of(M, L);
+        } else {
+            const int64_t s0 = (int64_t)it.slot * kFewRows + row;
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j)
+                if (col + 64 * j < c.D) *reinterpret_cast<float4_t*>(a.part_o + s0 * c.D + col + 64 * j) = o[j];
+            if (col == 0) {
+                a.part_ml[2 * s0] = M;
+                a.part_ml[2 * s0 + 1] = L;
+            }
+        }
+    }
+    // rows with an infinite or undefined value once more, key by key (slow_row)
+    if (!__syncthreads_or(here && !fine)) return;
+    const uint64_t bad = __ballot(here && !fine);
+    for (int w = 0; w < 4; ++w) {
+        if (((bad >> (16 * w)) & 0xFFFF) == 0) continue;  // row 4 wave + w
+        const int brho = it.tile * kFewRows + 4 * wave + w, bi = brho / a.G, bh = it.h * a.G + brho - bi * a.G;
+        const int64_t bt = it.first + bi;
+        float ov[DP / 64], bm, bl;
+        slow_row<DP, I4>(a, it.b, it.h, it.len - it.n + bi, it.lo, it.hi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
+                         bm, bl);
+        const float bin = bl > 0.0f || bl != bl ? 1.0f / bl : 0.0f;
+        const int64_t s0 = (int64_t)it.slot * kFewRows + 4 * wave + w;
+#pragma unroll
+        for (int j = 0; j < DP / 64; ++j) {
+            const int d = lane + 64 * j;
+            if (d >= c.D) continue;
+            if (it.parts == 1) a.out[bt * a.o_token + (int64_t)bh * a.o_head + d] = (_Float16)(ov[j] * bin);
+            else a.part_o[s0 * c.D + d] = ov[j];
+        }
+        if (lane == 0) {
+            if (it.parts == 1) {
+                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(bm, bl);
+            } else {
+                a.part_ml[2 * s0] = bm;
+                a.part_ml[2 * s0 + 1] = bl;
+            }
+        }
+    }
+}
+
+}  // namespace
+
+template <bool I4>
+hipError_t paged_few(const PagedArgs& a, hipStream_t s) {
+    const int64_t tiles = ((int64_t)a.c.T * a.G / kFewRows + (a.c.B < a.c.T ? a.c.B : a.c.T)) * a.c.H;
+    const dim3 grid((unsigned)(tiles + a.target));
+    if (a.c.D <= 64) paged_few_kernel<64, I4><<<grid, 256, 0, s>>>(a);
+    else if (a.c.D <= 128) paged_few_kernel<128, I4><<<grid, 256, 0, s>>>(a);
+    else if (a.c.D <= 192) paged_few_kernel<192, I4><<<grid, 256, 0, s>>>(a);
+    else paged_few_kernel<256, I4><<<grid, 256, 0, s>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && a.target > 0) {
+        const int rows = a.c.q_start == nullptr && a.G < kFewRows ? a.G : kFewRows;
+        paged_join_kernel<kFewRows, false, kFewUnit><<<dim3((unsigned)tiles, (unsigned)(rows + 3) / 4), 256, 0, s>>>(a);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+}  // namespace vedic

@@ -1,0 +1,319 @@
+// vedic_paged_many.hpp -- attention of many new rows a sequence (a prompt, or the next piece
+// of one) over its paged cache.
+//
+//   S^T = K Q^T (32 tokens x 32 rows per v_mfma_f32_32x32x16_f16), weights 2^(x - m + 14) with a
+//   running maximum and sum in fp32, O^T += V^T P^T.
+//
+// A workgroup has a tile of 128 rows (four waves of 32) and a range of keys (vedic_paged.hpp).
+// Blocks of 64 keys go through two buffers of LDS, one barrier a block: while a block is
+// multiplied, the next one's rows are on their way into registers (from the pages, 16 bytes a
+// thread and load; four bits are expanded on their way to LDS) and the places of the one
+// after that are looked up.  K's rows lie 2 DP + 16 bytes apart (ds_read_b128 of eight rows meets
+// every bank once), V's 2 DP + 32 (the same for the transposing ds_read_b64_tr_b16).  The scores'
+// layout, a row of Q per lane, is what the second product takes: the weights stay in
+// registers.  A wave leaves out blocks none of its rows sees, and looks at masks only where
+// some key of a block is hidden from one of them.
+#pragma once
+
+#include "vedic_paged.hpp"
+
+namespace vedic {
+
+namespace {
+
+typedef short many_short4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 many_half4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kManyKeys = 64;    // of a block
+constexpr int kManyUnit = 256;   // parts are whole multiples of it
+
+// The pieces of a block (64 rows of K, then of V) that a thread carries from the pages to LDS.
+template <int DP, bool I4>
+struct BlockShare {
+    static constexpr int KP = 2 * DP + 16, VP = 2 * DP + 32;
+    static constexpr int PER = I4 ? DP / 32 : DP / 8;  // pieces of a row
+    static constexpr int N = 2 * kManyKeys * PER / 256;
+    u32x4_t v[N];
+    uint32_t sm[I4 ? N : 1];
+    __device__ __forceinline__ static void piece(int x, bool& is_v, int& row, int& at) {
+        const int u = threadIdx.x + 256 * x, w = u % (kManyKeys * PER);
+        is_v = u >= kManyKeys * PER;
+        row = w / PER;
+        at = w % PER;
+    }
+    __device__ __forceinline__ void load(const char* kb, const char* vb, const int64_t* off, int D) {
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            bool is_v;
+            int row, at;
+            piece(x, is_v, row, at);
+            const char* p = (is_v ? vb : kb) + off[row];
+            v[x] = u32x4_t{0, 0, 0, 0};
+            if constexpr (I4) {
+                sm[x] = 0;
+                if (D == DP || 32 * at < D) {
+                    v[x] = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_a4_t*>(p + 16 * at));
+                    sm[x] = *reinterpret_cast<const uint32_t*>(p + D / 2 + 4 * at);
+                }
+            } else {
+                if (D == DP || 8 * at < D) v[x] = *reinterpret_cast<const u32x4_t*>(p + 16 * at);
+            }
+        }
+    }
+    // Rows from `left` on as zeros in V (what lies there is nobody's).
+    __device__ __forceinline__ void store(char* k, char* vl, int left) const {
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            bool is_v;
+            int row, at;
+            piece(x, is_v, row, at);
+            const bool none = is_v && row >= left;
+            char* to = (is_v ? vl + row * VP : k + row * KP) + at * (I4 ? 64 : 16);
+            if constexpr (I4) {
+                half2_t s, m;
+                four_bit_pair(none ? 0u : sm[x], s, m);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<half8_t*>(to + 16 * i) = four_bit_values(v[x][i], s, m);
+            } else {
+                *reinterpret_cast<u32x4_t*>(to) = none ? u32x4_t{0, 0, 0, 0} : v[x];
+            }
+        }
+    }
+};
+
+template <int DP, bool I4>
+__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_many_kernel(PagedArgs a) {
+    typedef BlockShare<DP, I4> Share;
+    constexpr int KK = DP / 16, DT = DP / 32, KP = Share::KP, VP = Share::VP, BUF = kManyKeys * (KP + VP);
+    __shared__ __attribute__((aligned(16))) char lds[2 * BUF];
+    __shared__ int64_t off[2][kManyKeys];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    PagedItem it;
+    if (!find_item<kManyRows, true, kManyUnit, false>(a, blockIdx.x, lane, it)) return;
+    const KvView& c = a.c;
+    const int r = lane & 31, h = lane >> 5;
+
+    const int base = it.tile * kManyRows + 32 * wave;  // the wave's first row
+    const int rho = base + r, i = rho / a.G;
+    const bool mine = i < it.n;
+    const int pos = mine ? it.len - it.n + i : -1;
+    const int64_t tok = it.first + (mine ? i : 0);
+    const int head = it.h * a.G + (mine ? rho - i * a.G : 0);
+    half8_t qf[KK];
+    {
+        const _Float16* q = a.q + tok * a.q_token + (int64_t)head * a.q_head;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const int d = 16 * kk + 8 * h;
+            qf[kk] = half8_t{};
+            if (d < c.D) qf[kk] = *reinterpret_cast<const half8_t*>(q + d);
+        }
+    }
+    const int khi = !mine ? 0 : a.causal ? pos + 1 : it.len;
+    const int klo = a.window > 0 ? pos - a.window : INT32_MIN;
+    // of the wave's rows (whole wave: no row where w_n <= 0)
+    const int64_t rows = (int64_t)it.n * a.G;
+    const bool any = base < rows;
+    const int p0 = it.len - it.n + base / a.G, p1 = it.len - it.n + min(it.n - 1, (base + 31) / a.G);
+    const int khi_all = a.causal ? p0 + 1 : it.len;    // every row sees the keys before it
+    const int khi_some = !any ? 0 : a.causal ? p1 + 1 : it.len;  // none sees those from it on
+    const int klo_all = a.window > 0 ? p1 - a.window : INT32_MIN;
+    const int klo_some = a.window > 0 && a.stride == 0 ? p0 - a.window : INT32_MIN;
+
+    const char* kb = c.k + (int64_t)it.h * c.head;
+    const char* vb = c.v + (int64_t)it.h * c.head;
+    auto place = [&](int t) {  // the offset of key t + tid (tid < 64)
+        return c.row_offset(it.b, min(t + tid, it.hi - 1));
+    };
+
+    float m = kNoScore, l = 0.0f;
+    float16_t acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] = 0.0f;
+
+    Share share;
+    if (it.lo < it.hi) {
+        if (tid < kManyKeys) {
+            off[0][tid] = place(it.lo);
+            off[1][tid] = place(it.lo + kManyKeys);
+        }
+        __syncthreads();
+        share.load(kb, vb, off[0], c.D);
+        share.store(lds, lds + kManyKeys * KP, it.hi - it.lo);
+        __syncthreads();
+    }
+    int buf = 0;
+    for (int t = it.lo; t < it.hi; t += kManyKeys, buf ^= 1) {
+        const bool more = t + kManyKeys < it.hi;
+        int64_t next = 0;
+        if (more) {
+            share.load(kb, vb, off[buf ^ 1], c.D);
+            if (tid < kManyKeys) next = place(t + 2 * kManyKeys);
+        }
+        const char* kl = lds + buf * BUF;
+        const char* vl = kl + kManyKeys * KP;
+        if (t < khi_some && t + kManyKeys > klo_some) {
+            float16_t s[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                        *reinterpret_cast<const half8_t*>(kl + (32 * u + r) * KP + 32 * kk + 16 * h), qf[kk], s[u], 0, 0, 0);
+            }
+            float mx = kNoScore;
+            if (t + kManyKeys > min(khi_all, it.hi) || t < klo_all) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = t + 32 * u + 8 * (e >> 2) + 4 * h + (e & 3);
+                        bool in = key < khi && key < it.hi;
+                        if (a.window > 0) in = in && (key >= klo || (a.stride > 0 && key % a.stride == 0));
+                        s[u][e] = in ? s[u][e] * a.scale : kNoScore;
+                        mx = __builtin_fmaxf(mx, s[u][e]);
+                    }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        s[u][e] *= a.scale;
+                        mx = __builtin_fmaxf(mx, s[u][e]);
+                    }
+            }
+            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
+            const float mn = __builtin_fmaxf(m, mx), mu = mn == kNoScore ? 0.0f : mn;
+            if (__any(mn > m)) {
+                const float f = exp2_fast(m - mu);
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d] *= f;
+                m = mn;
+            }
+            const float bias = kWeightBits - mu;
+            half8_t p[4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float w = exp2_fast(s[u][e] + bias);
+                    l += w;
+                    p[2 * u + (e >> 3)][e & 7] = (_Float16)w;
+                }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    union {
+                        many_short4_t q[2];
+                        half8_t h;
+                    } x;
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        x.q[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) many_short4_t*)(vl + (16 * q + 8 * b + 4 * h + ((lane & 15) >> 2)) * VP +
+                                                                               2 * (32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3))));
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, p[q], acc[d], 0, 0, 0);
+                }
+        }
+        if (more) {
+            char* to = lds + (buf ^ 1) * BUF;
+            share.store(to, to + kManyKeys * KP, it.hi - t - kManyKeys);
+            if (tid < kManyKeys) off[buf][tid] = next;
+        }
+        __syncthreads();
+    }
+
+    l += __shfl_xor(l, 32);
+    bool fine = l < __builtin_inff();
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) fine = fine && __builtin_fabsf(acc[d][e]) < __builtin_inff();
+    const int64_t s0 = (int64_t)it.slot * kManyRows + 32 * wave;
+    if (mine) {
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        if (it.parts == 1) {
+            _Float16* out = a.out + tok * a.o_token + (int64_t)head * a.o_head;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int at = 32 * d + 8 * e + 4 * h;
+                    const many_half4_t v = {(_Float16)(acc[d][4 * e] * inv), (_Float16)(acc[d][4 * e + 1] * inv),
+                                            (_Float16)(acc[d][4 * e + 2] * inv), (_Float16)(acc[d][4 * e + 3] * inv)};
+                    if (at < c.D) *reinterpret_cast<many_half4_t*>(out + at) = v;
+                }
+            if (a.lse && h == 0) a.lse[tok * a.Hq + head] = lse_of(m, l);
+        } else {
+            float* po = a.part_o + (s0 + r) * c.D;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int at = 32 * d + 8 * e + 4 * h;
+                    const float4_t v = {acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
+                    if (at < c.D) *reinterpret_cast<float4_t*>(po + at) = v;
+                }
+            if (h == 0) {
+                a.part_ml[2 * (s0 + r)] = m;
+                a.part_ml[2 * (s0 + r) + 1] = l;
+            }
+        }
+    }
+    // rows with an infinite or undefined value once more, key by key (slow_row)
+    uint64_t bad = __ballot(mine && !fine);
+    bad = (bad | bad >> 32) & 0xFFFFFFFFu;
+    while (bad) {
+        const int w = __builtin_ctzll(bad);
+        bad &= bad - 1;
+        const int brho = base + w, bi = brho / a.G, bh = it.h * a.G + brho - bi * a.G;
+        const int64_t bt = it.first + bi;
+        float ov[DP / 64], bm, bl;
+        slow_row<DP, I4>(a, it.b, it.h, it.len - it.n + bi, it.lo, it.hi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
+                         bm, bl);
+        const float bin = bl > 0.0f || bl != bl ? 1.0f / bl : 0.0f;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the stores above come first)
+#pragma unroll
+        for (int j = 0; j < DP / 64; ++j) {
+            const int d = lane + 64 * j;
+            if (d >= c.D) continue;
+            if (it.parts == 1) a.out[bt * a.o_token + (int64_t)bh * a.o_head + d] = (_Float16)(ov[j] * bin);
+            else a.part_o[(s0 + w) * c.D + d] = ov[j];
+        }
+        if (lane == 0) {
+            if (it.parts == 1) {
+                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(bm, bl);
+            } else {
+                a.part_ml[2 * (s0 + w)] = bm;
+                a.part_ml[2 * (s0 + w) + 1] = bl;
+            }
+        }
+    }
+}
+
+}  // namespace
+
+template <bool I4>
+hipError_t paged_many(const PagedArgs& a, hipStream_t s) {
+    const int64_t tiles = ((int64_t)a.c.T * a.G / kManyRows + (a.c.B < a.c.T ? a.c.B : a.c.T)) * a.c.H;
+    // (a sequence has two parts only where it is longer than the average of `target`)
+    const dim3 grid((unsigned)(tiles + a.target));
+    if (a.c.D <= 64) paged_many_kernel<64, I4><<<grid, 256, 0, s>>>(a);
+    else if (a.c.D <= 128) paged_many_kernel<128, I4><<<grid, 256, 0, s>>>(a);
+    else if (a.c.D <= 192) paged_many_kernel<192, I4><<<grid, 256, 0, s>>>(a);
+    else paged_many_kernel<256, I4><<<grid, 256, 0, s>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && a.target > 0) {
+        paged_join_kernel<kManyRows, true, kManyUnit><<<dim3((unsigned)tiles, kManyRows / 4), 256, 0, s>>>(a);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+}  // namespace vedic

@@ -19,6 +19,10 @@ New here, with no counterpart in the reference: products whose rows choose their
   gemm_grouped(op, A, B, offsets)  the experts' products, forward and backward (bias_grad_grouped, group_rows)
   combine_rows / combine_rows_bwd  the experts' rows in token order, and the backward
   gemm_lora / lora_add             low-rank adapters of many requests beside a shared projection
+and decoding with a paged cache of keys and values (binary16 or four bits) and four-bit weights:
+  kv_cache / kv_append / kv_read   a cache, new tokens into it with their positions' rotation, and rows of it back
+  paged_attention(q, k, v, ...)    attention of new tokens over it: one token a sequence, prompts, pieces of prompts
+  gemm_w4(X, W4)                   products with four-bit weights (w4_quantize, w4_unpack)
 
 Operands are torch tensors resident on the GPU (torch is used for device
 memory and streams only); every call runs on torch's current stream.  Shape
@@ -48,6 +52,7 @@ __all__ = [
     "flash_attention_fwd", "flash_attention_fwd_heads", "flash_attention_bwd", "flash_attention_bwd_heads",
     "Routing", "route_topk", "route_topk_bwd", "group_rows", "gemm_grouped", "bias_grad_grouped", "combine_rows",
     "combine_rows_bwd", "lora_add", "gemm_lora",
+    "kv_cache", "kv_append", "kv_read", "paged_attention", "W4", "w4_quantize", "w4_unpack", "gemm_w4",
 ]
 
 _DT = {torch.float32: DT_F32, torch.float16: DT_F16}
@@ -998,4 +1003,232 @@ def gemm_lora(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Tensor
     d = _lib.GemmDesc(OP_NN, dt, DT_F32, M, N, K, px, ldx, pw, ldw, pc, ldc, 1.0, 0.0, pbias,
                       EPI_NONE if bias is None else EPI_BIAS, None, 0, _stream(), None, 0.0)
     _check(_lib.load().vedic_gemm_lora(ctypes.byref(d), pa, pb, G, r, po, pr, n, psc))
+    return out
+
+
+# ---------------------------------------------------------------- a paged cache, weights in four bits
+
+
+def kv_cache(pages: int, page_size: int, heads: int, dh: int, four_bit: bool = False,
+             device=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Zeroed (k, v) of a cache, [pages, heads, page_size, row]: rows of dh float16 values, or of 5 dh / 8 bytes (uint8)
+    with four_bit (vedic_kv_format_t in logos_vedic.h).  Any tensors of that shape and element type will do whose last
+    dimension is contiguous, and whose other strides are whole rows apart."""
+    if dh <= 0 or dh % (32 if four_bit else 8) != 0 or dh > 256:
+        raise ValueError(f"dh must be a multiple of {32 if four_bit else 8} up to 256, got {dh}")
+    shape = (pages, heads, page_size, dh * 5 // 8 if four_bit else dh)
+    dt = torch.uint8 if four_bit else torch.float16
+    device = torch.device("cuda") if device is None else device
+    return torch.zeros(shape, dtype=dt, device=device), torch.zeros(shape, dtype=dt, device=device)
+
+
+def _kv(k, v, table, lens, q_start, tokens, dev) -> _lib.Kv:
+    """The cache and the sequences of a call, checked."""
+    dt = k.dtype
+    if dt not in (torch.float16, torch.uint8):
+        raise ValueError(f"a cache is float16 or uint8 (four bits), got {dt}")
+    pk, pv = _on_current(k, "the cache's k", dt, dev), _on_current(v, "the cache's v", dt, dev)
+    shape, strides = k.shape, k.stride()
+    if len(shape) != 4 or v.shape != shape or v.stride() != strides:
+        raise ValueError(f"a cache's k and v are [pages, heads, page_size, row] with equal strides, got {tuple(shape)} and "
+                         f"{tuple(v.shape)}")
+    pages, heads, ps, row = shape
+    sp, sh, st, one = strides
+    if row > 1 and one != 1:
+        raise ValueError("a cache's rows must be contiguous")
+    i4 = dt == torch.uint8
+    if i4 and row % 5 != 0:
+        raise ValueError(f"a four-bit row has 5 dh / 8 bytes, got {row}")
+    p_table = _on_current(table, "table", torch.int32, dev)
+    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be [sequences, pages], its rows contiguous")
+    B, W = table.shape
+    ps_start = None
+    if q_start is not None:
+        ps_start = _ints(q_start, "q_start", (B + 1,), dev)
+    elif tokens != B:
+        raise ValueError(f"{tokens} rows for {B} sequences: q_start tells which are whose")
+    # (a dimension of one has any stride)
+    return _lib.Kv(i4, pages, ps, heads, row * 8 // 5 if i4 else row, pk, pv, sp if pages > 1 else max(sp, row),
+                   sh if heads > 1 else max(sh, row), st if ps > 1 else max(st, row), p_table,
+                   table.stride(0) if B > 1 else W, W, _ints(lens, "lens", (B,), dev), ps_start, B, tokens)
+
+
+def _heads3d(t: torch.Tensor, name: str, dtype, dev: int) -> tuple[int, int, int, int, int, int]:
+    """(address, tokens, heads, dh, token stride, head stride) of [tokens, heads, dh] with contiguous rows."""
+    p = _on_current(t, name, dtype, dev)
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, dh], got shape {tuple(t.shape)}")
+    n, h, d = t.shape
+    st, sh, one = t.stride()
+    if d > 1 and one != 1:
+        raise ValueError(f"{name}'s rows must be contiguous")
+    return p, n, h, d, st, sh
+
+
+def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              table: torch.Tensor, lens: torch.Tensor, q_start: torch.Tensor | None = None,
+              rope: torch.Tensor | None = None, interleaved: bool = False,
+              out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """New tokens' keys and values into the cache; returns q turned by the tokens' positions, float16 (None without q).
+
+    q [tokens, q_heads, dh], k and v [tokens, heads, dh], all float32 or all float16 (views of one packed projection do).
+    table int32 [sequences, pages]; lens int32 [sequences]: tokens of each, these included; q_start int32
+    [sequences + 1]: rows q_start[b] .. q_start[b + 1] - 1 are sequence b's (None: one row each).  rope float32
+    [positions, dims]: dims / 2 cosines, then the sines, of each position's angles; pairs (i, i + dims / 2), or
+    (2i, 2i + 1) with interleaved; the values behind dims are not turned.  See vedic_kv_append in logos_vedic.h."""
+    dev = _device(k)
+    dt = k.dtype
+    if dt not in _DT:
+        raise ValueError(f"k must be float16 or float32, got {dt}")
+    pk, T, H, D, kt, kh = _heads3d(k, "k", dt, dev)
+    pv, Tv, Hv, Dv, vt, vh = _heads3d(v, "v", dt, dev)
+    kv = _kv(k_cache, v_cache, table, lens, q_start, T, dev)
+    if (Tv, Hv, Dv) != (T, H, D) or (H, D) != (kv.heads, kv.dh):
+        raise ValueError(f"k and v must be [tokens, {kv.heads}, {kv.dh}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    pq = po = None
+    Hq = qt = qh = ot = oh = 0
+    if q is not None:
+        pq, Tq, Hq, Dq, qt, qh = _heads3d(q, "q", dt, dev)
+        if (Tq, Dq) != (T, D):
+            raise ValueError(f"q must be [{T}, q_heads, {D}], got {tuple(q.shape)}")
+        if out is None:
+            out = torch.empty((T, Hq, D), dtype=torch.float16, device=q.device)
+        po, To, Ho, Do, ot, oh = _heads3d(out, "out", torch.float16, dev)
+        if (To, Ho, Do) != (T, Hq, D):
+            raise ValueError(f"out must be {T}x{Hq}x{D}")
+    pr, rows, dims = None, 0, 0
+    if rope is not None:
+        pr = _on_current(rope, "rope", torch.float32, dev)
+        if rope.dim() != 2 or not rope.is_contiguous() or rope.shape[1] > D or rope.shape[1] % 2 != 0:
+            raise ValueError(f"rope must be contiguous float32 [positions, dims], dims even and at most {D}")
+        rows, dims = rope.shape
+    _check(_lib.load().vedic_kv_append(ctypes.byref(kv), _DT[dt], pq, qt, qh, Hq, po, ot, oh, pk, kt, kh, pv, vt, vh, pr, rows,
+                                       dims, interleaved, _stream()))
+    return out if q is not None else None
+
+
+def kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+            q_start: torch.Tensor | None = None, tokens: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rows that kv_append's arguments name, from the cache: (k, v) float16 [tokens, heads, dh].  q_start the running
+    sums of lens gives whole sequences (tokens: q_start's last value, which is on the GPU).  Rows of no sequence are undefined."""
+    dev = _device(k_cache)
+    if tokens is None:
+        if q_start is not None:
+            raise ValueError("tokens (the last value of q_start) is needed with q_start")
+        tokens = table.shape[0]
+    kv = _kv(k_cache, v_cache, table, lens, q_start, tokens, dev)
+    k = torch.empty((tokens, kv.heads, kv.dh), dtype=torch.float16, device=k_cache.device)
+    v = torch.empty_like(k)
+    _check(_lib.load().vedic_kv_read(ctypes.byref(kv), k.data_ptr(), v.data_ptr(), _stream()))
+    return k, v
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
+                    lens: torch.Tensor, q_start: torch.Tensor | None = None, scale: float | None = None,
+                    causal: bool = True, window: int = 0, stride: int = 0, out: torch.Tensor | None = None,
+                    lse: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of new tokens over a paged cache that holds them (kv_append): q float16 [tokens, q_heads, dh], head j with
+    key head j // (q_heads // heads); float16 out.  A row sees the keys up to its own position (causal; else its
+    sequence's all), with window > 0 those from `window` before it on, and further back, with stride > 0, those at multiples of
+    stride.  scale defaults to 1/sqrt(dh).  lse (float32 [tokens, q_heads]) receives each row's log-sum-exp.  table, lens
+    and q_start as for kv_append.  See vedic_paged_attention in logos_vedic.h."""
+    dev = _device(q)
+    pq, T, Hq, D, qt, qh = _heads3d(q, "q", torch.float16, dev)
+    kv = _kv(k_cache, v_cache, table, lens, q_start, T, dev)
+    if D != kv.dh or Hq % kv.heads != 0:
+        raise ValueError(f"q must be [tokens, a multiple of {kv.heads}, {kv.dh}], got {tuple(q.shape)}")
+    if out is None:
+        out = q.new_empty((T, Hq, D))
+        po, ot, oh = out.data_ptr(), Hq * D, D
+    else:
+        po, To, Ho, Do, ot, oh = _heads3d(out, "out", torch.float16, dev)
+        if (To, Ho, Do) != (T, Hq, D):
+            raise ValueError(f"out must be {T}x{Hq}x{D}")
+    pl = None if lse is None else _floats(lse, "lse", (T, Hq), dev)
+    if scale is None:
+        scale = 1.0 / float(D) ** 0.5
+    _check(_lib.load().vedic_paged_attention(ctypes.byref(kv), pq, qt, qh, Hq, po, ot, oh, pl, scale, causal, window, stride,
+                                             _stream()))
+    return out
+
+
+class W4(NamedTuple):
+    """A weight [K, N] in four bits (vedic_w4_t in logos_vedic.h)."""
+
+    codes: torch.Tensor   # int32 [N, ceil(K / 32) * 4]: words of eight codes along K
+    scales: torch.Tensor  # float16 [N, ceil(K / group), 2]: pairs (s, m)
+    K: int
+    group: int
+
+
+def _w4(w: W4, dev: int) -> _lib.W4Desc:
+    pc = _on_current(w.codes, "codes", torch.int32, dev)
+    ps = _on_current(w.scales, "scales", torch.float16, dev)
+    K, group = w.K, w.group
+    if group not in (32, 64, 128) or K <= 0:
+        raise ValueError(f"group must be 32, 64 or 128 and K positive, got {group} and {K}")
+    N = w.codes.shape[0]
+    if tuple(w.codes.shape) != (N, -(-K // 32) * 4) or tuple(w.scales.shape) != (N, -(-K // group), 2) or \
+            not w.codes.is_contiguous() or not w.scales.is_contiguous():
+        raise ValueError(f"codes must be contiguous [N, {-(-K // 32) * 4}] and scales [N, {-(-K // group)}, 2], got "
+                         f"{tuple(w.codes.shape)} and {tuple(w.scales.shape)}")
+    return _lib.W4Desc(pc, ps, K, N, group)
+
+
+def w4_quantize(W: torch.Tensor, group: int = 64) -> W4:
+    """W (float16 or float32 [K, N]) in four bits, a scale and a minimum per `group` (32, 64, 128) values along K."""
+    dev = _device(W)
+    if W.dtype not in _DT:
+        raise ValueError(f"W must be float16 or float32, got {W.dtype}")
+    p, K, N, ld = _rows2d(W, "W", W.dtype, dev)
+    if group not in (32, 64, 128):
+        raise ValueError(f"group must be 32, 64 or 128, got {group}")
+    w = W4(torch.empty((N, -(-K // 32) * 4), dtype=torch.int32, device=W.device),
+           torch.empty((N, -(-K // group), 2), dtype=torch.float16, device=W.device), K, group)
+    _check(_lib.load().vedic_w4_quantize(p, _DT[W.dtype], ld, K, N, group, w.codes.data_ptr(), w.scales.data_ptr(), _stream()))
+    return w
+
+
+def w4_unpack(w: W4, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values a four-bit weight stands for, float16 [K, N]."""
+    dev = _device(w.codes)
+    d = _w4(w, dev)
+    if out is None:
+        out = torch.empty((d.K, d.N), dtype=torch.float16, device=w.codes.device)
+    p, r, c, ld = _rows2d(out, "out", torch.float16, dev)
+    if (r, c) != (d.K, d.N):
+        raise ValueError(f"out must be {d.K}x{d.N}")
+    _check(_lib.load().vedic_w4_unpack(ctypes.byref(d), p, ld, _stream()))
+    return out
+
+
+def gemm_w4(X: torch.Tensor, w: W4, bias: torch.Tensor | None = None, epilogue: int | None = None,
+            out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """C = epi(X . W) with a four-bit weight: X float16 [M, K], or float32 (clamped and rounded to float16 as it is read);
+    fp32 sums; C float32 or float16.  epilogue EPI_NONE, EPI_BIAS, EPI_BIAS_GELU, or EPI_RESIDUAL, EPI_BIAS_RESIDUAL, which
+    add to a float32 `out`; by default EPI_BIAS with a bias, EPI_NONE without.  See vedic_gemm_w4 in logos_vedic.h."""
+    dev = _device(X)
+    if X.dtype not in _DT:
+        raise ValueError(f"X must be float16 or float32, got {X.dtype}")
+    px, M, K, ldx = _rows2d(X, "X", X.dtype, dev)
+    d = _w4(w, dev)
+    if K != d.K:
+        raise ValueError(f"VedicGEMM: inner dimensions differ (X gives K={K}, W gives K={d.K})")
+    if epilogue is None:
+        epilogue = EPI_NONE if bias is None else EPI_BIAS
+    if out is None:
+        if epilogue in (EPI_RESIDUAL, EPI_BIAS_RESIDUAL):
+            raise ValueError("the residual epilogues add to an existing float32 out")
+        out = X.new_empty((M, d.N), dtype=out_dtype)
+    if out.dtype not in _DT:
+        raise ValueError("out must be float32 or float16")
+    pc, Mc, Nc, ldc = _rows2d(out, "out", out.dtype, dev)
+    if (Mc, Nc) != (M, d.N):
+        raise ValueError(f"out must be {M}x{d.N}, got {Mc}x{Nc}")
+    wants = epilogue in (EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESIDUAL)
+    if wants != (bias is not None):
+        raise ValueError("a bias goes with EPI_BIAS, EPI_BIAS_GELU and EPI_BIAS_RESIDUAL")
+    pb = None if bias is None else _floats(bias, "bias", (d.N,), dev)
+    _check(_lib.load().vedic_gemm_w4(ctypes.byref(d), px, _DT[X.dtype], ldx, M, pc, _DT[out.dtype], ldc, pb, epilogue, _stream()))
     return out

@@ -1,0 +1,295 @@
+"""Attention over a paged cache against 64 bits: formats, head layouts, lengths, pages, masks, strides, what masks hide."""
+import numpy as np
+import pytest
+import torch
+
+import _cache_helpers as plain
+from logos_amd import vedic
+
+pytestmark = pytest.mark.gpu
+
+
+class Batch:
+    """Sequences with new[b] new rows and lens[b] tokens in a cache with its pages in a random order."""
+
+    def __init__(self, seed, Hq, H, D, four_bit, ps, new, lens, before=0, after=0, spare=2, token_major=False):
+        rng = np.random.default_rng(seed)
+        self.Hq, self.H, self.D, self.new, self.lens, self.four = Hq, H, D, new, lens, four_bit
+        most = [-(-n // ps) for n in lens]
+        pages = sum(most) + spare
+        order = rng.permutation(pages)
+        self.table = np.full((len(lens), max(1, max(most)) + 1), -7, np.int32)
+        at = 0
+        for b, m in enumerate(most):
+            self.table[b, :m] = order[at:at + m]
+            at += m
+        self.x = [rng.standard_normal((pages, H, ps, D)).astype(np.float16) for _ in range(2)]
+        self.T = before + sum(new) + after
+        self.q = rng.standard_normal((self.T, Hq, D)).astype(np.float16)
+        self.starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32) + before
+        self.rows = [plain.rows_of(x, four_bit) for x in self.x]
+        self.ps, self.token_major = ps, token_major
+
+    def device(self):
+        caches = []
+        for r in self.rows:
+            t = torch.from_numpy(np.ascontiguousarray(r.transpose(0, 2, 1, 3) if self.token_major else r)).cuda()
+            caches.append(t.transpose(1, 2) if self.token_major else t)
+        return (torch.from_numpy(self.q).cuda(), *caches, torch.from_numpy(self.table).cuda(),
+                torch.tensor(self.lens, dtype=torch.int32, device="cuda"), torch.from_numpy(self.starts).cuda())
+
+    def sequence(self, b):
+        """k and v [L, H, D] of sequence b, as the cache's rows stand for them."""
+        L, ps = self.lens[b], self.ps
+        pages = self.table[b, :-(-L // ps)] if L else np.zeros(0, int)
+        return [plain.values_of(r[pages].swapaxes(1, 2).reshape(-1, self.H, r.shape[-1])[:L], self.four) for r in self.rows]
+
+    def check(self, got, lse=None, scale=None, causal=True, window=0, stride=0, skip=()):
+        got = got.float().cpu().numpy()
+        scale = self.D ** -0.5 if scale is None else scale
+        for b in range(len(self.lens)):
+            r0, r1 = self.starts[b], self.starts[b + 1]
+            pos = np.arange(self.lens[b] - self.new[b], self.lens[b])
+            k, v = self.sequence(b)
+            out, want_lse, tol = plain.attention(self.q[r0:r1], k, v, pos, scale, causal, window, stride)
+            for i in range(r1 - r0):
+                if (b, i) in skip:
+                    continue
+                err = np.abs(got[r0 + i] - out[i])
+                assert (err <= tol[i]).all(), (b, i, float(err.max()), float(tol[i].max()))
+                if lse is not None:
+                    g = lse[r0 + i].cpu().numpy()
+                    fin = np.isfinite(want_lse[i])
+                    assert (np.isinf(g) & (g > 0) == ~fin).all()
+                    # the scores' fp32 sums (|q||k| of a few tens, D roundings) and the logarithm's
+                    assert np.abs(g[fin] - want_lse[i][fin]).max(initial=0) <= 2.0 ** -24 * (self.D + 32) * 64
+
+
+def run(b, one_each=False, **kw):
+    q, k, v, table, lens, starts = b.device()
+    return vedic.paged_attention(q, k, v, table, lens, q_start=None if one_each else starts, **kw)
+
+
+@pytest.mark.parametrize("four_bit,D", [(False, d) for d in (8, 40, 64, 72, 96, 128, 160, 192, 200, 256)] +
+                         [(True, d) for d in (32, 64, 96, 128, 160, 192, 224, 256)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 150, 70]])
+def test_head_sizes(four_bit, D, new):
+    b = Batch(D + four_bit, 6, 2, D, four_bit, 24, new, [n + p for n, p in zip(new, (40, 77, 0))])
+    b.check(run(b))
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("Hq,H", [(1, 1), (3, 3), (6, 2), (16, 1), (20, 1), (34, 2), (72, 1), (130, 1)])
+def test_shared_heads_one_token(four_bit, Hq, H):
+    lens = [1, 31, 64, 129, 200]
+    b = Batch(Hq, Hq, H, 64, four_bit, 16, [1] * 5, lens)
+    b.check(run(b, one_each=True))
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("ps", [1, 7, 16, 33, 64, 100, 256, 1000])
+def test_pages(four_bit, ps):
+    b = Batch(ps, 4, 2, 64, four_bit, ps, [1, 2, 90, 1], [1, 63, 130, 257])
+    b.check(run(b))
+    b = Batch(ps, 4, 2, 64, four_bit, ps, [1, 2, 90, 1], [1, 63, 130, 257], token_major=True)
+    b.check(run(b))
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("lens", [[5000], [9, 4097, 2, 1500, 800], [1] * 70 + [3000] + [2] * 70])
+def test_long_and_ragged_decoding(four_bit, lens):
+    """Long sequences are shared out over workgroups, more than one wave of sequences."""
+    b = Batch(len(lens), 4, 1, 64, four_bit, 64, [1] * len(lens), lens)
+    lse = torch.full((b.T, 4), -5.0, device="cuda")
+    b.check(run(b, one_each=True, lse=lse), lse)
+
+
+@pytest.mark.parametrize("new,lens", [
+    ([300], [300]), ([200, 1, 129, 64], [200, 900, 2000, 64]), ([70, 65, 0, 5], [4000, 70, 33, 5]), ([33], [3001])])
+@pytest.mark.parametrize("four_bit", [False, True])
+def test_prompts_and_pieces(new, lens, four_bit):
+    b = Batch(sum(new), 4, 2, 64, four_bit, 48, new, lens)
+    lse = torch.full((b.T, 4), -5.0, device="cuda")
+    b.check(run(b, lse=lse), lse)
+
+
+@pytest.mark.parametrize("window,stride", [(1, 0), (30, 0), (64, 7), (100, 16), (5, 1), (1 << 30, 0), (50, 100000)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [5, 140, 33]])
+def test_masks(window, stride, new):
+    b = Batch(window % 1000 + stride % 1000, 4, 2, 64, False, 32, new, [n + p for n, p in zip(new, (0, 300, 77))])
+    lse = torch.full((b.T, 4), -5.0, device="cuda")
+    b.check(run(b, window=window, stride=stride, lse=lse), lse, window=window, stride=stride)
+
+
+@pytest.mark.parametrize("new", [[2, 9, 1], [80, 140, 0]])
+def test_not_causal(new):
+    b = Batch(11, 4, 2, 64, False, 32, new, [n + p for n, p in zip(new, (0, 300, 77))])
+    b.check(run(b, causal=False, scale=0.2), causal=False, scale=0.2)
+
+
+@pytest.mark.parametrize("n", [3, 100])
+def test_rows_without_keys_and_rows_of_no_sequence(n):
+    """Rows before the first position see nothing (zeros, lse +inf); rows outside the sequences are left as they are."""
+    b = Batch(n, 4, 2, 64, False, 16, [n, 0, n, n], [n - 2, 9, 0, n + 20], before=3, after=5)
+    q, k, v, table, lens, starts = b.device()
+    out = torch.full((b.T, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+    lse = torch.full((b.T, 4), 7.0, device="cuda")
+    vedic.paged_attention(q, k, v, table, lens, q_start=starts, out=out, lse=lse)
+    b.check(out, lse)
+    for t in (out, lse):
+        assert (t[:3] == 7).all() and (t[-5:] == 7).all()
+    assert (out[3:5] == 0).all() and torch.isinf(lse[3:5]).all()
+    assert (out[3 + n:3 + 2 * n] == 0).all()
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("new,past", [([1, 1], 90), ([9, 3], 40), ([100, 150], 30), ([90, 140], 700)])
+def test_what_is_hidden_does_not_count(four_bit, bad, new, past):
+    """NaN and infinities in unused rows of pages, in keys behind a row's own position, and in keys a window leaves out."""
+    lens = [past + n for n in new]
+    b = Batch(past, 4, 2, 64, four_bit, 32, new, lens)
+    filled = [np.full_like(x, bad) for x in b.x]
+    for s in range(2):
+        for p in range(lens[s]):
+            page, at = b.table[s, p // 32], p % 32
+            for f, x in zip(filled, b.x):
+                f[page, :, at] = x[page, :, at]
+    # sequence 0's last key and value, which only its last row sees; sequence 1's first, which no window reaches
+    for f in filled:
+        f[b.table[0, (lens[0] - 1) // 32], :, (lens[0] - 1) % 32, 5] = bad
+        f[b.table[1, 0], :, 0, 5] = bad
+    b.rows = [plain.rows_of(f, four_bit) for f in filled]
+    got = run(b, window=past - 3)
+    with np.errstate(invalid="ignore"):
+        b.check(got, window=past - 3, skip={(0, new[0] - 1)})
+    assert not torch.isfinite(got[new[0] - 1]).all()
+
+
+def test_large_scores():
+    """Weights far apart: the largest score's key has all but 2^-20 of the weight, a long tail the rest."""
+    b = Batch(5, 2, 1, 64, False, 64, [1, 70], [3000, 3000])
+    b.q *= np.float16(6)
+    b.check(run(b, scale=1.0), scale=1.0)
+
+
+def test_a_tail_of_small_weights_counts():
+    """One key 20 above 16383 others that are alike: they have 16383 e^-20 / (1 + ..) = 3.4e-5 of it, each weight below binary16's
+    smallest normal; their value is 2^14 times the first's, so that a third of the sum is theirs."""
+    L, D = 16384, 64
+    k, v = np.zeros((L, 1, D), np.float16), np.full((L, 1, D), 16384.0, np.float16)
+    k[0, 0, 0] = 20.0
+    v[0] = 1.0
+    q = np.zeros((1, 1, D), np.float16)
+    q[0, 0, 0] = 1.0
+    table = torch.arange(L // 64, dtype=torch.int32, device="cuda")[None]
+    lens = torch.tensor([L], dtype=torch.int32, device="cuda")
+    kc, vc = (torch.from_numpy(np.ascontiguousarray(x.reshape(L // 64, 64, 1, D).transpose(0, 2, 1, 3))).cuda() for x in (k, v))
+    got = vedic.paged_attention(torch.from_numpy(q).cuda(), kc, vc, table, lens, scale=1.0).float().cpu().numpy()
+    out, _, tol = plain.attention(q, k, v, [L - 1], 1.0)
+    assert (np.abs(got - out) <= tol + 2.0 ** -11 * np.abs(out)).all(), (got[0, 0, 0], out[0, 0, 0])
+
+
+def test_strided_q_and_out():
+    """q a view of a packed projection, out a view of a wider buffer."""
+    b = Batch(3, 4, 2, 64, False, 16, [1, 80, 3], [50, 80, 40])
+    q, k, v, table, lens, starts = b.device()
+    packed = torch.randn(b.T, 8, 64, device="cuda").half()
+    packed[:, 2:6] = q
+    wide = torch.full((b.T, 6, 72), 3.0, dtype=torch.float16, device="cuda")
+    vedic.paged_attention(packed[:, 2:6], k, v, table, lens, q_start=starts, out=wide[:, 1:5, :64])
+    b.check(wide[:, 1:5, :64])
+    assert (wide[:, 0] == 3).all() and (wide[:, 5] == 3).all() and (wide[:, :, 64:] == 3).all()
+    # heads before tokens
+    qt = q.transpose(0, 1).contiguous().transpose(0, 1)
+    b.check(vedic.paged_attention(qt, k, v, table, lens, q_start=starts))
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_cache_past_four_gib(new):
+    """Pages whose offsets pass 32 bits."""
+    pages, H, ps, D = 5200, 4, 1024, 128  # 5.2 GiB each
+    free = torch.cuda.mem_get_info()[0]
+    if free < 16 << 30:
+        pytest.skip("needs 16 GiB")
+    b = Batch(9, 8, H, D, False, ps, [new], [new + 1500], spare=0)
+    k, v = (torch.empty(pages, H, ps, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    at = torch.tensor([pages - 1, 4200, 5000][:b.rows[0].shape[0]], device="cuda")
+    for c, r in zip((k, v), b.rows):
+        c[at] = torch.from_numpy(r).cuda()
+    q, _, _, table, lens, starts = b.device()
+    n = b.rows[0].shape[0]
+    table[0, :n] = at[table[0, :n].long()].int()
+    b.check(vedic.paged_attention(q, k, v, table, lens, q_start=starts))
+
+
+def test_bad_lists_stay_in_range():
+    """Lengths past the table, pages that are none, starts that do not ascend: values are wrong, accesses are not."""
+    b = Batch(4, 4, 2, 64, False, 16, [4, 90, 2], [40, 120, 33])
+    q, k, v, table, lens, starts = b.device()
+    wild = torch.tensor([[1 << 30, -5, 2], [3, 1 << 20, -1], [0, 0, 0]], dtype=torch.int32, device="cuda")
+    for ln in ([1 << 31 - 1, 500, -4], [0, 48, 7]):
+        for st in ([0, 90, 20, 96], [-5, 10, 1 << 30, 3], [96, 0, 96, 0]):
+            got = vedic.paged_attention(q, k, v, wild, torch.tensor(ln, dtype=torch.int64).clamp(-2 ** 31, 2 ** 31 - 1).int().cuda(),
+                                        q_start=torch.tensor(st, dtype=torch.int32, device="cuda"))
+            torch.cuda.synchronize()
+            assert got.shape == (96, 4, 64)
+
+
+def test_empty_calls():
+    b = Batch(4, 4, 2, 64, False, 16, [4], [40])
+    q, k, v, table, lens, starts = b.device()
+    assert vedic.paged_attention(q[:0], k, v, table[:0], lens[:0]).shape == (0, 4, 64)
+    out = torch.full_like(q, 2.0)
+    vedic.paged_attention(q, k, v, table[:0], lens[:0], q_start=starts[:1], out=out)
+    assert (out == 2).all()
+
+
+@pytest.mark.parametrize("new,lens", [([1] * 6, [3000, 5, 700, 1, 64, 2000]), ([1, 300, 2, 90], [2500, 300, 50, 4000])])
+def test_captured(new, lens):
+    """Recorded into a graph: with a block from an eager call the same bits on every replay, also with other lengths in the
+    same tensors; and without a block (a stream the library has not seen), unsplit."""
+    b = Batch(21, 8, 2, 64, True, 32, new, lens)
+    q, k, v, table, ln, starts = b.device()
+    kw = dict(q_start=None if set(new) == {1} else starts)
+    for warm in (True, False):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        out = torch.zeros_like(q)
+        with torch.cuda.stream(s):
+            if warm:
+                vedic.paged_attention(q, k, v, table, ln, out=out, **kw)
+            s.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                vedic.paged_attention(q, k, v, table, ln, out=out, **kw)
+        torch.cuda.synchronize()
+        want = vedic.paged_attention(q, k, v, table, ln, **kw)
+        for _ in range(4):
+            out.fill_(9)
+            g.replay()
+            torch.cuda.synchronize()
+            if warm:
+                assert torch.equal(out, want)
+            b.check(out)
+            torch.randn(1000, device="cuda").sum().item()
+        if warm:
+            short = torch.tensor([max(n, L - 37) for n, L in zip(new, lens)], dtype=torch.int32, device="cuda")
+            keep = ln.clone()
+            ln.copy_(short)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, vedic.paged_attention(q, k, v, table, short, **kw))
+            ln.copy_(keep)
+        with torch.cuda.stream(s):
+            del g
+            vedic._lib.load().vedic_workspace_release(s.cuda_stream)
+        torch.cuda.synchronize()
+
+
+def test_repeated_calls_give_the_same_bits():
+    b = Batch(2, 8, 2, 128, False, 64, [1, 1, 100], [6000, 2000, 4000])
+    args = b.device()
+    first = vedic.paged_attention(*args[:5], q_start=args[5])
+    for _ in range(5):
+        assert torch.equal(first, vedic.paged_attention(*args[:5], q_start=args[5]))
