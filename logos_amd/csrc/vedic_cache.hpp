@@ -145,7 +145,8 @@ struct PagedArgs {
     float* lse;  // [T x Hq] or null
     int64_t q_token, q_head, o_token, o_head;  // strides in values
     int Hq, G;
-    float scale;  // times log2(e)
+    float scale;  // |scale| log2(e), > 0
+    float sign;   // of the scale: q is multiplied by it
     int causal, window, stride;
     // set by the rules in vedic_capi.hip: `target` workgroups' worth of keys per item
     // (0: items are not split), and the partial results of split items

@@ -1821,10 +1821,12 @@ extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_
     a.o_token = out_token;
     a.o_head = out_head;
     a.Hq = q_heads;
-    a.scale = scale * 1.44269504088896340736f;
+    // (0 as 2^-126, which leaves every score of binary16 values below 2^-80: a hidden key's -infinity stays one)
+    a.sign = scale < 0.0f ? -1.0f : 1.0f;
+    a.scale = scale == 0.0f ? 0x1p-126f : a.sign * scale * 1.44269504088896340736f;
     a.causal = causal != 0;
     a.window = window < kMaxTokens ? window : kMaxTokens;
-    a.stride = stride;
+    a.stride = stride < kMaxTokens ? stride : kMaxTokens;
     const bool i4 = kv->format == VEDIC_KV_I4;
     const int cus = device_cu_count();
     // Which kernels: sequences' rows are known on the GPU only, so a call whose sequences may be of both kinds runs

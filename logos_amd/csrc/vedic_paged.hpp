@@ -25,18 +25,32 @@ constexpr float kNoScore = -__builtin_inff();
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 struct PagedItem {
-    int b, tile, h;      // sequence, tile of its rows, key head
-    int first, n, len;   // its new rows and its tokens
-    int lo, hi;          // keys of this part
+    int b, tile, h;       // sequence, tile of its rows, key head
+    int first, n, len;    // its new rows and its tokens
+    int base, far, near;  // the tile's keys (tile_keys)
+    int lo, hi;           // places of this part
     int part, parts;
-    int slot;            // of the partial result (parts > 1)
+    int slot;             // of the partial result (parts > 1)
 };
 
-// Keys that some row of the sequence may see: [lo, len).
-__device__ __forceinline__ int first_key(const PagedArgs& a, int len, int n) {
-    return a.window > 0 && a.stride == 0 ? max(0, len - n - a.window) : 0;
+constexpr int kPlaces = 64;  // a block of keys lies in one of the two lists
+
+// The keys that rows i0 .. i1 of a sequence see, as a list: places 0 .. far - 1 are the multiples of
+// the stride before `base` (every row's window begins at or after it), places near .. hi - 1
+// the keys base, base + 1, .., of which a row may see some; near is far in whole blocks.
+__device__ __forceinline__ int tile_keys(const PagedArgs& a, int len, int n, int i0, int i1, int& base, int& far, int& near) {
+    const int end = a.causal ? max(0, len - n + i1 + 1) : len;
+    base = a.window > 0 ? max(0, len - n + i0 - a.window) & ~(kPlaces - 1) : 0;
+    far = a.stride > 0 ? (base + a.stride - 1) / a.stride : 0;
+    near = (far + kPlaces - 1) & ~(kPlaces - 1);
+    return near + max(0, end - base);
+}
+// The key at a place (far ones past the end: the last).
+__device__ __forceinline__ int key_at(const PagedArgs& a, const PagedItem& it, int place) {
+    return place < it.near ? min(place, it.far - 1) * a.stride : it.base + place - it.near;
 }
 
+// Tiles of sequence b, and the longest list of keys among them (the last one's, or near it).
 template <int ROWS, bool MANY>
 __device__ __forceinline__ void sequence_work(const PagedArgs& a, int b, int& tiles, int& span) {
     tiles = span = 0;
@@ -45,9 +59,9 @@ __device__ __forceinline__ void sequence_work(const PagedArgs& a, int b, int& ti
     a.c.rows_of(b, first, n);
     const int64_t rows = (int64_t)n * a.G;
     if (n == 0 || (rows > a.few_most) != MANY) return;
-    const int len = a.c.len_of(b);
     tiles = (int)((rows + ROWS - 1) / ROWS);
-    span = max(0, len - first_key(a, len, n));
+    int base, far, near;
+    span = tile_keys(a, a.c.len_of(b), n, (tiles - 1) * ROWS / a.G, n - 1, base, far, near);
 }
 
 __device__ __forceinline__ int parts_of(int span, int chunk) { return span > chunk ? (span + chunk - 1) / chunk : 1; }
@@ -68,7 +82,7 @@ __device__ __forceinline__ int part_length(const PagedArgs& a, int lane) {
     return each >= (int64_t)INT32_MAX - UNIT ? INT32_MAX : max(1, (int)((each + UNIT - 1) / UNIT)) * UNIT;
 }
 
-// The item (JOIN: the tile) number id; false if there is none.
+// The item (JOIN: the split tile) number id; false if there is none.
 template <int ROWS, bool MANY, int UNIT, bool JOIN>
 __device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, PagedItem& it) {
     const int chunk = part_length<ROWS, MANY, UNIT>(a, lane);
@@ -79,7 +93,7 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, 
         const int parts = parts_of(span, chunk);
         // (sums of a list that is not ascending stay in range too)
         const int items = (int)min((int64_t)tiles * a.c.H * parts, int64_t(1) << 24);
-        const int units = JOIN ? (int)min((int64_t)tiles * a.c.H, int64_t(1) << 24) : items;
+        const int units = !JOIN ? items : parts > 1 ? (int)min((int64_t)tiles * a.c.H, int64_t(1) << 24) : 0;
         const int split = parts > 1 ? items : 0;
         int incl = units, sincl = split;
 #pragma unroll
@@ -106,16 +120,13 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, 
             it.first = __builtin_amdgcn_readfirstlane(it.first);
             it.n = __builtin_amdgcn_readfirstlane(it.n);
             it.len = __builtin_amdgcn_readfirstlane(a.c.len_of(it.b));
-            const int lo = first_key(a, it.len, it.n), sp = max(0, it.len - lo);
-            const int each = ((sp + it.parts - 1) / it.parts + UNIT - 1) / UNIT * UNIT;
-            // keys that some row of the tile sees
             const int i0 = it.tile * ROWS / a.G, i1 = min(it.n - 1, (it.tile * ROWS + ROWS - 1) / a.G);
-            const int tlo = a.window > 0 && a.stride == 0 ? max(lo, it.len - it.n + i0 - a.window) : lo;
-            const int thi = a.causal ? max(0, it.len - it.n + i1 + 1) : it.len;
-            const int64_t p0 = lo + (int64_t)it.part * each;
-            it.lo = (int)min(max(p0, (int64_t)tlo), (int64_t)thi);
-            it.hi = (int)min(it.parts == 1 ? (int64_t)thi : p0 + each, (int64_t)thi);
-            it.hi = max(it.hi, it.lo);
+            const int end = tile_keys(a, it.len, it.n, i0, i1, it.base, it.far, it.near);
+            const int sp = __builtin_amdgcn_readlane(span, who);
+            const int each = ((sp + it.parts - 1) / it.parts + UNIT - 1) / UNIT * UNIT;
+            const int64_t p0 = (int64_t)it.part * each;
+            it.lo = (int)min(p0, (int64_t)end);
+            it.hi = it.part == it.parts - 1 ? end : (int)min(p0 + each, (int64_t)end);
             return JOIN || it.parts == 1 || it.slot < a.slots;  // (at most 2 target of them: vedic_capi.hip)
         }
         before += __builtin_amdgcn_readlane(incl, 63);
@@ -147,7 +158,7 @@ __device__ __forceinline__ float cache_value(const char* row, int D, int d) {
 // a sum.  For rows whose sums came out infinite or NaN: in a product of tiles the zero weight
 // of an unseen key times an infinity is NaN.  o: values lane, lane + 64, ..
 template <int DP, bool I4>
-__device__ __forceinline__ void slow_row(const PagedArgs& a, int b, int h, int pos, int lo, int hi, const _Float16* q, int lane,
+__device__ __forceinline__ void slow_row(const PagedArgs& a, const PagedItem& it, int pos, const _Float16* q, int lane,
                                       float (&o)[DP / 64], float& m, float& l) {
     float qv[DP / 64];
 #pragma unroll
@@ -158,9 +169,11 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, int b, int h, int p
     }
     m = kNoScore;
     l = 0.0f;
-    for (int t = lo; t < hi; ++t) {
+    for (int place = it.lo; place < it.hi; ++place) {
+        if (place >= it.far && place < it.near) continue;
+        const int t = key_at(a, it, place);
         if (!sees(a, pos, t)) continue;
-        const int64_t at = a.c.row_offset(b, t) + (int64_t)h * a.c.head;
+        const int64_t at = a.c.row_offset(it.b, t) + (int64_t)it.h * a.c.head;
         float x = 0.0f;
 #pragma unroll
         for (int j = 0; j < DP / 64; ++j) {
@@ -169,7 +182,7 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, int b, int h, int p
         }
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
-        x *= a.scale;
+        x *= a.sign * a.scale;
         const float mn = __builtin_fmaxf(m, x), mu = mn == kNoScore ? 0.0f : mn;
         const float f = exp2_fast(m - mu), p = exp2_fast(x - mu + kWeightBits);
         l = l * f + p;
@@ -202,27 +215,46 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a) {
     const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // of a share
     const int share = lane / lanes, shares = 64 / lanes, c = lane % lanes;
     const int64_t s0 = (int64_t)it.slot * ROWS + r;
-    float M = kNoScore;
-    for (int p = lane; p < it.parts; p += 64) M = __builtin_fmaxf(M, a.part_ml[2 * (s0 + (int64_t)p * ROWS)]);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) M = __builtin_fmaxf(M, __shfl_xor(M, d));
-    const float mu = M == kNoScore ? 0.0f : M;
     float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
-#pragma unroll 4
-    for (int p = share; p < it.parts; p += shares) {
-        const int64_t s = s0 + (int64_t)p * ROWS;
-        const float f = exp2_fast(a.part_ml[2 * s] - mu), lp = a.part_ml[2 * s + 1];
-        const float4_t v = *reinterpret_cast<const float4_t*>(a.part_o + s * D + 4 * min(c, cols - 1));
-        if (f > 0.0f || f != f || lp != lp) {  // (a part without keys has nothing to add)
-            l += lp * f;
-            o += v * f;
+    float M = kNoScore, l = 0.0f;
+    // (a running maximum: all loads of a round are on their way together)
+    for (int p0 = share; p0 < it.parts; p0 += 8 * shares) {
+        float mp[8], lp[8];
+        float4_t v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t s = s0 + (int64_t)min(p0 + j * shares, it.parts - 1) * ROWS;
+            mp[j] = a.part_ml[2 * s];
+            lp[j] = a.part_ml[2 * s + 1];
+            v[j] = *reinterpret_cast<const float4_t*>(a.part_o + s * D + 4 * min(c, cols - 1));
+        }
+        float top = M;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = __builtin_fmaxf(top, mp[j]);
+        const float mu = top == kNoScore ? 0.0f : top, g = exp2_fast(M - mu);
+        M = top;
+        l *= g;
+        o *= g;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float f = exp2_fast(mp[j] - mu);
+            if (p0 + j * shares < it.parts && !(lp[j] == 0.0f)) {  // (a part without keys has nothing to add)
+                l += lp[j] * f;
+                o += v[j] * f;
+            }
         }
     }
     for (int d = lanes; d < 64; d <<= 1) {
-        l += __shfl_xor(l, d);
+        const float other = __shfl_xor(M, d), top = __builtin_fmaxf(M, other), mu = top == kNoScore ? 0.0f : top;
+        const float g = exp2_fast(M - mu), go = exp2_fast(other - mu);
+        M = top;
+        const float lo = __shfl_xor(l, d);
+        l = l * g + lo * go;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], d);
+        for (int j = 0; j < 4; ++j) {
+            const float oo = __shfl_xor(o[j], d);
+            o[j] = o[j] * g + oo * go;
+        }
     }
     const int head = it.h * a.G + rho % a.G;
     const int64_t t = it.first + i;

@@ -134,27 +134,53 @@ __global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
         for (int kk = 0; kk < KK; ++kk) {
             const int d = RowShare<DP, I4>::first(kk, g);
             qf[kk] = half8_t{};
-            if (d < c.D) qf[kk] = *reinterpret_cast<const half8_t*>(q + d);
+            if (d < c.D) qf[kk] = *reinterpret_cast<const half8_t*>(q + d) * (_Float16)a.sign;
         }
     }
-    // keys [klo, khi) of this row; the sparse mask's keys before klo are looked at one by one
+    // keys [klo, khi) of this row, and of all rows of the tile
     const int khi = !mine ? 0 : a.causal ? pos + 1 : it.len;
     const int klo = a.window > 0 ? pos - a.window : INT32_MIN;
+    const int i0 = it.tile * kFewRows / a.G, i1 = min(it.n - 1, (it.tile * kFewRows + kFewRows - 1) / a.G);
+    const int khi_all = a.causal ? it.len - it.n + i0 + 1 : it.len;
+    const int klo_all = a.window > 0 ? it.len - it.n + i1 - a.window : INT32_MIN;
 
     const char* kb = c.k + (int64_t)it.h * c.head;
     const char* vbase = c.v + (int64_t)it.h * c.head;
     const int* table = c.table + it.b * c.ldt;
-    // the page of the lane's two tokens of the block at t, and the rest of their rows' offsets
+    // The page and the row in it of each of the lane's two tokens of the 32 places at t.  Where pages are
+    // whole sixteens, the sixteen near keys of a tile lie in one: one lookup, and the lane's own row
+    // apart from it (rows behind the sequence's end are some row of its page).
+    const bool whole = c.ps % 16 == 0;
+    const int64_t mine_off = r * c.token;
     auto place = [&](int t, int (&page)[2], int (&inside)[2]) {
+        if (whole && t >= it.near) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int p = max(0, min(t + 16 * u + r, it.hi - 1)), tp = c.page_of(p);
-            page[u] = table[tp];
-            inside[u] = p - tp * c.ps;
+            for (int u = 0; u < 2; ++u) {
+                const int key = it.base + min(t + 16 * u, (it.hi - 1) & ~15) - it.near, tp = c.page_of(key);
+                page[u] = table[tp];
+                inside[u] = key - tp * c.ps;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int key = key_at(a, it, min(t + 16 * u + r, it.hi - 1)), tp = c.page_of(key);
+                page[u] = table[tp];
+                inside[u] = key - tp * c.ps;
+            }
         }
     };
-    auto offset = [&](int page, int inside) {
-        return ((unsigned)page < (unsigned)c.pages ? page : 0) * c.page + inside * c.token;
+    auto offset = [&](int t, int (&page)[2], int (&inside)[2], int64_t (&off)[2]) {
+        if (whole && t >= it.near) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int p = __builtin_amdgcn_readfirstlane(page[u]), i = __builtin_amdgcn_readfirstlane(inside[u]);
+                off[u] = ((unsigned)p < (unsigned)c.pages ? p : 0) * c.page + i * c.token + mine_off;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                off[u] = ((unsigned)page[u] < (unsigned)c.pages ? page[u] : 0) * c.page + inside[u] * c.token;
+        }
     };
 
     float m = kNoScore, l = 0.0f;
@@ -168,14 +194,12 @@ __global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
     int page[2], inside[2];
     if (t < it.hi) {
         place(t, page, inside);
+        offset(t, page, inside, off);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            off[u] = offset(page[u], inside[u]);
-            k[u].load(kb + off[u], c.D, g);
-        }
+        for (int u = 0; u < 2; ++u) k[u].load(kb + off[u], c.D, g);
 #pragma unroll
         for (int u = 0; u < 2; ++u) v[u].load(vbase + off[u], c.D, g);
-        place(min(t + kFewUnit, it.hi - 1), page, inside);
+        if (t + kFewUnit < it.hi) place(t + kFewUnit, page, inside);
     }
     for (; t < it.hi; t += kFewUnit) {
         const bool more = t + kFewUnit < it.hi;
@@ -188,17 +212,17 @@ __global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
                 s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(share_frag(k[u], kk, g), qf[kk], s[u], 0, 0, 0);
         }
         if (more) {
+            offset(t + kFewUnit, page, inside, off);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                off[u] = offset(page[u], inside[u]);
-                k[u].load(kb + off[u], c.D, g);
-            }
+            for (int u = 0; u < 2; ++u) k[u].load(kb + off[u], c.D, g);
         }
         // V of this block to LDS; rows past the range as zeros (what lies there is nobody's)
-        if (t + 32 > it.hi) {
+        const bool isnear = t >= it.near;
+        const int left = min(it.hi, isnear ? it.hi : it.far) - t;  // places that are keys
+        if (left < 32) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
-                if (t + 16 * u + r >= it.hi) v[u].clear();
+                if (16 * u + r >= left) v[u].clear();
         }
         asm volatile("" ::: "memory");
 #pragma unroll
@@ -211,34 +235,45 @@ __global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
         if (more) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) v[u].load(vbase + off[u], c.D, g);
-            place(min(t + 2 * kFewUnit, it.hi - 1), page, inside);
+            if (t + 2 * kFewUnit < it.hi) place(t + 2 * kFewUnit, page, inside);
         }
         // weights
-        float x[8];
+        const int key0 = it.base + t - it.near;
+        if (left < 32 || (isnear && (key0 + 32 > khi_all || key0 < klo_all))) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int at = 16 * (e >> 2) + 4 * g + (e & 3), key = key0 + at;
+                bool in = at < left;
+                if (isnear) {
+                    in = in && key < khi;
+                    if (a.window > 0) in = in && (key >= klo || (a.stride > 0 && key % a.stride == 0));
+                } else {
+                    in = in && mine;
+                }
+                s[e >> 2][e & 3] = in ? s[e >> 2][e & 3] : kNoScore;
+            }
+        }
         float mx = kNoScore;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int tok = t + 16 * (e >> 2) + 4 * g + (e & 3);
-            bool in = tok < khi && tok < it.hi;
-            if (a.window > 0) in = in && (tok >= klo || (a.stride > 0 && tok % a.stride == 0));
-            x[e] = in ? s[e >> 2][e & 3] * a.scale : kNoScore;
-            mx = __builtin_fmaxf(mx, x[e]);
-        }
+        for (int e = 0; e < 8; ++e) mx = __builtin_fmaxf(mx, s[e >> 2][e & 3]);
         mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
         mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = __builtin_fmaxf(m, mx), mu = mn == kNoScore ? 0.0f : mn;
-        const float f = exp2_fast(m - mu);
-        m = mn;
+        mx *= a.scale;
+        if (__any(mx > m)) {
+            const float mn = __builtin_fmaxf(m, mx), f = mn == kNoScore ? 1.0f : exp2_fast(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] *= f;
+        }
+        const float bias = kWeightBits - (m == kNoScore ? 0.0f : m);
         half8_t p;
-        l *= f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float w = exp2_fast(x[e] - mu + kWeightBits);
+            const float w = exp2_fast(__builtin_fmaf(s[e >> 2][e & 3], a.scale, bias));
             l += w;
             p[e] = (_Float16)w;
         }
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] *= f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             union {
@@ -322,7 +357,7 @@ __global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
         const int brho = it.tile * kFewRows + 4 * wave + w, bi = brho / a.G, bh = it.h * a.G + brho - bi * a.G;
         const int64_t bt = it.first + bi;
         float ov[DP / 64], bm, bl;
-        slow_row<DP, I4>(a, it.b, it.h, it.len - it.n + bi, it.lo, it.hi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
+        slow_row<DP, I4>(a, it, it.len - it.n + bi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
                          bm, bl);
         const float bin = bl > 0.0f || bl != bl ? 1.0f / bl : 0.0f;
         const int64_t s0 = (int64_t)it.slot * kFewRows + 4 * wave + w;
@@ -357,7 +392,7 @@ hipError_t paged_few(const PagedArgs& a, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.target > 0) {
         const int rows = a.c.q_start == nullptr && a.G < kFewRows ? a.G : kFewRows;
-        paged_join_kernel<kFewRows, false, kFewUnit><<<dim3((unsigned)tiles, (unsigned)(rows + 3) / 4), 256, 0, s>>>(a);
+        paged_join_kernel<kFewRows, false, kFewUnit><<<dim3((unsigned)(tiles < a.target ? tiles : a.target), (unsigned)(rows + 3) / 4), 256, 0, s>>>(a);
         e = hipGetLastError();
     }
     return e;

@@ -5,7 +5,7 @@
 //   running maximum and sum in fp32, O^T += V^T P^T.
 //
 // A workgroup has a tile of 128 rows (four waves of 32) and a range of keys (vedic_paged.hpp).
-// Blocks of 64 keys go through two buffers of LDS, one barrier a block: while a block is
+// Blocks of 64 keys (32 with heads past 128) go through two buffers of LDS, one barrier a block: while a block is
 // multiplied, the next one's rows are on their way into registers (from the pages, 16 bytes a
 // thread and load; four bits are expanded on their way to LDS) and the places of the one
 // after that are looked up.  K's rows lie 2 DP + 16 bytes apart (ds_read_b128 of eight rows meets
@@ -24,20 +24,22 @@ namespace {
 typedef short many_short4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 many_half4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kManyKeys = 64;    // of a block
+// Keys of a block: with heads past 128 the next block's rows would take 64 registers more.
+constexpr int many_keys(int dp) { return dp <= 128 ? 64 : 32; }
 constexpr int kManyUnit = 256;   // parts are whole multiples of it
 
 // The pieces of a block (64 rows of K, then of V) that a thread carries from the pages to LDS.
 template <int DP, bool I4>
 struct BlockShare {
-    static constexpr int KP = 2 * DP + 16, VP = 2 * DP + 32;
+    static constexpr int KEYS = many_keys(DP), KP = 2 * DP + 16, VP = 2 * DP + 32;
     static constexpr int PER = I4 ? DP / 32 : DP / 8;  // pieces of a row
-    static constexpr int N = 2 * kManyKeys * PER / 256;
+    static constexpr int ALL = 2 * KEYS * PER, N = (ALL + 255) / 256;
     u32x4_t v[N];
     uint32_t sm[I4 ? N : 1];
+    // (the last threads have a piece fewer where they do not come out even: they take the last once more)
     __device__ __forceinline__ static void piece(int x, bool& is_v, int& row, int& at) {
-        const int u = threadIdx.x + 256 * x, w = u % (kManyKeys * PER);
-        is_v = u >= kManyKeys * PER;
+        const int u0 = threadIdx.x + 256 * x, u = ALL % 256 == 0 ? u0 : min(u0, ALL - 1), w = u % (KEYS * PER);
+        is_v = u >= KEYS * PER;
         row = w / PER;
         at = w % PER;
     }
@@ -81,12 +83,16 @@ struct BlockShare {
     }
 };
 
+// Keys among the places from t on (the first of a block), to the end of their list.
+__device__ __forceinline__ int keys_left(const PagedItem& it, int t) { return (t < it.near ? min(it.hi, it.far) : it.hi) - t; }
+
 template <int DP, bool I4>
 __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_many_kernel(PagedArgs a) {
     typedef BlockShare<DP, I4> Share;
-    constexpr int KK = DP / 16, DT = DP / 32, KP = Share::KP, VP = Share::VP, BUF = kManyKeys * (KP + VP);
+    constexpr int KEYS = Share::KEYS, U = KEYS / 32, KK = DP / 16, DT = DP / 32;
+    constexpr int KP = Share::KP, VP = Share::VP, BUF = KEYS * (KP + VP);
     __shared__ __attribute__((aligned(16))) char lds[2 * BUF];
-    __shared__ int64_t off[2][kManyKeys];
+    __shared__ int64_t off[2][KEYS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     PagedItem it;
     if (!find_item<kManyRows, true, kManyUnit, false>(a, blockIdx.x, lane, it)) return;
@@ -106,24 +112,22 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_many_kernel(Page
         for (int kk = 0; kk < KK; ++kk) {
             const int d = 16 * kk + 8 * h;
             qf[kk] = half8_t{};
-            if (d < c.D) qf[kk] = *reinterpret_cast<const half8_t*>(q + d);
+            if (d < c.D) qf[kk] = *reinterpret_cast<const half8_t*>(q + d) * (_Float16)a.sign;
         }
     }
     const int khi = !mine ? 0 : a.causal ? pos + 1 : it.len;
     const int klo = a.window > 0 ? pos - a.window : INT32_MIN;
-    // of the wave's rows (whole wave: no row where w_n <= 0)
-    const int64_t rows = (int64_t)it.n * a.G;
-    const bool any = base < rows;
+    // of the wave's rows: all see the keys [klo_all, khi_all), none those outside [klo_some, khi_some)
+    const bool any = base < (int64_t)it.n * a.G;
     const int p0 = it.len - it.n + base / a.G, p1 = it.len - it.n + min(it.n - 1, (base + 31) / a.G);
-    const int khi_all = a.causal ? p0 + 1 : it.len;    // every row sees the keys before it
-    const int khi_some = !any ? 0 : a.causal ? p1 + 1 : it.len;  // none sees those from it on
+    const int khi_all = a.causal ? p0 + 1 : it.len, khi_some = !any ? 0 : a.causal ? p1 + 1 : it.len;
     const int klo_all = a.window > 0 ? p1 - a.window : INT32_MIN;
     const int klo_some = a.window > 0 && a.stride == 0 ? p0 - a.window : INT32_MIN;
 
     const char* kb = c.k + (int64_t)it.h * c.head;
     const char* vb = c.v + (int64_t)it.h * c.head;
-    auto place = [&](int t) {  // the offset of key t + tid (tid < 64)
-        return c.row_offset(it.b, min(t + tid, it.hi - 1));
+    auto place = [&](int t) {  // the offset of the key at place t + tid (tid < KEYS)
+        return c.row_offset(it.b, key_at(a, it, min(t + tid, it.hi - 1)));
     };
 
     float m = kNoScore, l = 0.0f;
@@ -135,29 +139,31 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_many_kernel(Page
 
     Share share;
     if (it.lo < it.hi) {
-        if (tid < kManyKeys) {
+        if (tid < KEYS) {
             off[0][tid] = place(it.lo);
-            off[1][tid] = place(it.lo + kManyKeys);
+            off[1][tid] = place(it.lo + KEYS);
         }
         __syncthreads();
         share.load(kb, vb, off[0], c.D);
-        share.store(lds, lds + kManyKeys * KP, it.hi - it.lo);
+        share.store(lds, lds + KEYS * KP, keys_left(it, it.lo));
         __syncthreads();
     }
     int buf = 0;
-    for (int t = it.lo; t < it.hi; t += kManyKeys, buf ^= 1) {
-        const bool more = t + kManyKeys < it.hi;
+    for (int t = it.lo; t < it.hi; t += KEYS, buf ^= 1) {
+        const bool more = t + KEYS < it.hi;
         int64_t next = 0;
         if (more) {
             share.load(kb, vb, off[buf ^ 1], c.D);
-            if (tid < kManyKeys) next = place(t + 2 * kManyKeys);
+            if (tid < KEYS) next = place(t + 2 * KEYS);
         }
         const char* kl = lds + buf * BUF;
-        const char* vl = kl + kManyKeys * KP;
-        if (t < khi_some && t + kManyKeys > klo_some) {
-            float16_t s[2];
+        const char* vl = kl + KEYS * KP;
+        const bool isnear = t >= it.near;
+        const int key0 = it.base + t - it.near, left = keys_left(it, t);
+        if (any && (!isnear || (key0 < khi_some && key0 + KEYS > klo_some))) {
+            float16_t s[U];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
 #pragma unroll
@@ -165,50 +171,49 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_many_kernel(Page
                     s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
                         *reinterpret_cast<const half8_t*>(kl + (32 * u + r) * KP + 32 * kk + 16 * h), qf[kk], s[u], 0, 0, 0);
             }
-            float mx = kNoScore;
-            if (t + kManyKeys > min(khi_all, it.hi) || t < klo_all) {
+            if (left < KEYS || (isnear && (key0 + KEYS > khi_all || key0 < klo_all))) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int key = t + 32 * u + 8 * (e >> 2) + 4 * h + (e & 3);
-                        bool in = key < khi && key < it.hi;
-                        if (a.window > 0) in = in && (key >= klo || (a.stride > 0 && key % a.stride == 0));
-                        s[u][e] = in ? s[u][e] * a.scale : kNoScore;
-                        mx = __builtin_fmaxf(mx, s[u][e]);
-                    }
-            } else {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < U; ++u)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        s[u][e] *= a.scale;
-                        mx = __builtin_fmaxf(mx, s[u][e]);
+                        const int at = 32 * u + 8 * (e >> 2) + 4 * h + (e & 3), key = key0 + at;
+                        bool in = at < left;
+                        if (isnear) {
+                            in = in && key < khi;
+                            if (a.window > 0) in = in && (key >= klo || (a.stride > 0 && key % a.stride == 0));
+                        } else {
+                            in = in && mine;
+                        }
+                        s[u][e] = in ? s[u][e] : kNoScore;
                     }
             }
-            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
-            const float mn = __builtin_fmaxf(m, mx), mu = mn == kNoScore ? 0.0f : mn;
-            if (__any(mn > m)) {
-                const float f = exp2_fast(m - mu);
+            float mx = s[0][0];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mx = __builtin_fmaxf(mx, s[u][e]);
+            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * a.scale;
+            if (__any(mx > m)) {
+                const float mn = __builtin_fmaxf(m, mx), f = mn == kNoScore ? 1.0f : exp2_fast(m - mn);
                 l *= f;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) acc[d] *= f;
                 m = mn;
             }
-            const float bias = kWeightBits - mu;
-            half8_t p[4];
+            const float bias = kWeightBits - (m == kNoScore ? 0.0f : m);
+            half8_t p[2 * U];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float w = exp2_fast(s[u][e] + bias);
+                    const float w = exp2_fast(__builtin_fmaf(s[u][e], a.scale, bias));
                     l += w;
                     p[2 * u + (e >> 3)][e & 7] = (_Float16)w;
                 }
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
+                for (int q = 0; q < 2 * U; ++q) {
                     union {
                         many_short4_t q[2];
                         half8_t h;
@@ -223,8 +228,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_many_kernel(Page
         }
         if (more) {
             char* to = lds + (buf ^ 1) * BUF;
-            share.store(to, to + kManyKeys * KP, it.hi - t - kManyKeys);
-            if (tid < kManyKeys) off[buf][tid] = next;
+            share.store(to, to + KEYS * KP, keys_left(it, t + KEYS));
+            if (tid < KEYS) off[buf][tid] = next;
         }
         __syncthreads();
     }
@@ -275,7 +280,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_many_kernel(Page
         const int brho = base + w, bi = brho / a.G, bh = it.h * a.G + brho - bi * a.G;
         const int64_t bt = it.first + bi;
         float ov[DP / 64], bm, bl;
-        slow_row<DP, I4>(a, it.b, it.h, it.len - it.n + bi, it.lo, it.hi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
+        slow_row<DP, I4>(a, it, it.len - it.n + bi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
                          bm, bl);
         const float bin = bl > 0.0f || bl != bl ? 1.0f / bl : 0.0f;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the stores above come first)
@@ -310,7 +315,7 @@ hipError_t paged_many(const PagedArgs& a, hipStream_t s) {
     else paged_many_kernel<256, I4><<<grid, 256, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.target > 0) {
-        paged_join_kernel<kManyRows, true, kManyUnit><<<dim3((unsigned)tiles, kManyRows / 4), 256, 0, s>>>(a);
+        paged_join_kernel<kManyRows, true, kManyUnit><<<dim3((unsigned)(tiles < a.target ? tiles : a.target), kManyRows / 4), 256, 0, s>>>(a);
         e = hipGetLastError();
     }
     return e;

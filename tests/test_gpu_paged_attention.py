@@ -56,7 +56,7 @@ class Batch:
                 if (b, i) in skip:
                     continue
                 err = np.abs(got[r0 + i] - out[i])
-                assert (err <= tol[i]).all(), (b, i, float(err.max()), float(tol[i].max()))
+                assert bool((err <= tol[i]).all()), (b, i, float(err.max()), float(tol[i].max()))
                 if lse is not None:
                     g = lse[r0 + i].cpu().numpy()
                     fin = np.isfinite(want_lse[i])

@@ -56,7 +56,7 @@ def check(seed, M, K, N, group, epilogue=None, out_dtype=torch.float32, x32=Fals
     if out_dtype == torch.float16:
         tol = tol + 2.0 ** -11 * np.abs(y) + 2.0 ** -25
     err = np.abs(got - y)
-    assert (err <= tol).all(), (float(err.max()), float(tol.max()))
+    assert bool((err <= tol).all()), (float(err.max()), float(tol.max()))
 
 
 @pytest.mark.parametrize("M", [1, 2, 5, 16, 17, 32, 33, 63, 64, 65, 128, 200])
