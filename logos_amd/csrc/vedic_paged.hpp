@@ -135,6 +135,14 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, 
     return false;
 }
 
+// Bits j < 64: key + j is a multiple of the stride.
+__device__ __forceinline__ uint64_t stride_bits(int key, int stride) {
+    uint64_t bits = 0;
+    const int past = key % stride;
+    for (int j = past ? stride - past : 0; j < 64; j += stride) bits |= uint64_t(1) << j;
+    return bits;
+}
+
 // Whether the row at position pos sees key t < len.
 __device__ __forceinline__ bool sees(const PagedArgs& a, int pos, int t) {
     if (a.causal && t > pos) return false;

@@ -26,23 +26,31 @@ namespace {
 typedef short paged_short4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 
-// A lane's share of one token's row: DP / 4 values.
+// A lane's share of one token's row, DP / 4 values in KK pieces of eight; `first` is where its
+// pieces begin (a place fixed for the lane).  Heads narrower than DP: pieces past the end hold
+// others once more, which the zeros of Q's registers leave out of the scores, and which are
+// columns of the output that nobody reads.
 template <int DP, bool I4>
 struct RowShare;
 template <int DP>
 struct RowShare<DP, false> {
     static constexpr int KK = DP / 32;
     u32x4_t v[KK];
-    // Values 32 kk + 8 g .. + 7, zero past D.
-    __device__ __forceinline__ void load(const char* row, int D, int g) {
+    // Piece kk: the row's values 32 kk + 8 g .. + 7.
+    struct Place {
+        int at[KK];  // bytes
+        __device__ __forceinline__ Place(int D, int g) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            v[kk] = u32x4_t{0, 0, 0, 0};
-            if (D == DP || 32 * kk + 8 * g < D) v[kk] = *reinterpret_cast<const u32x4_t*>(row + 64 * kk + 16 * g);
+            for (int kk = 0; kk < KK; ++kk) at[kk] = 2 * min(32 * kk + 8 * g, D - 8);
         }
+        __device__ __forceinline__ bool own(int kk, int D, int g) const { return 32 * kk + 8 * g < D; }
+        __device__ __forceinline__ int value(int kk, int g) const { return 32 * kk + 8 * g; }
+    };
+    __device__ __forceinline__ void load(const char* row, const Place& p, int) {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) v[kk] = *reinterpret_cast<const u32x4_t*>(row + p.at[kk]);
     }
-    __device__ __forceinline__ half8_t frag(int kk) const { return __builtin_bit_cast(half8_t, v[kk]); }
-    __device__ __forceinline__ static int first(int kk, int g) { return 32 * kk + 8 * g; }
+    __device__ __forceinline__ half8_t frag(int kk, const Place&) const { return __builtin_bit_cast(half8_t, v[kk]); }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) v[kk] = u32x4_t{0, 0, 0, 0};
@@ -53,64 +61,56 @@ struct RowShare<DP, true> {
     static constexpr int KK = DP / 32, NS = (KK + 3) / 4;
     uint32_t w[KK];
     uint32_t sm[NS];
-    // Values g DP / 4 + 8 kk .. + 7; words past D have a pair of zeros.
-    __device__ __forceinline__ void load(const char* row, int D, int g) {
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + g * KK;
-        const uint32_t* ps = reinterpret_cast<const uint32_t*>(row + D / 2);
-        const int g0 = g * KK / 4;
-        if (D == DP) {
-            if constexpr (KK == 2) {
-                typedef uint32_t a4 __attribute__((ext_vector_type(2), aligned(4)));
-                const a4 x = *reinterpret_cast<const a4*>(p);
-                w[0] = x[0];
-                w[1] = x[1];
-            } else if constexpr (KK % 4 == 0) {
+    // Piece kk: word `first` + kk of the row, first = g KK or so far down that KK words are left.
+    struct Place {
+        int first, pairs[NS];  // word; byte offsets of its groups' pairs
+        __device__ __forceinline__ Place(int D, int g) {
+            first = min(g * KK, D / 8 - KK);
 #pragma unroll
-                for (int i = 0; i < KK / 4; ++i) {
-                    const u32x4_a4_t x = *reinterpret_cast<const u32x4_a4_t*>(p + 4 * i);
+            for (int i = 0; i < NS; ++i) pairs[i] = D / 2 + 4 * min(first / 4 + i, D / 32 - 1);
+        }
+        __device__ __forceinline__ bool own(int kk, int, int g) const { return first + kk >= g * KK; }
+        __device__ __forceinline__ int value(int kk, int) const { return 8 * (first + kk); }
+    };
+    __device__ __forceinline__ void load(const char* row, const Place& q, int) {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + q.first;
+        if constexpr (KK % 4 == 0) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
-                }
-            } else {
+            for (int i = 0; i < KK / 4; ++i) {
+                const u32x4_a4_t x = *reinterpret_cast<const u32x4_a4_t*>(p + 4 * i);
 #pragma unroll
-                for (int i = 0; i < KK; ++i) w[i] = p[i];
+                for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
             }
-#pragma unroll
-            for (int i = 0; i < NS; ++i) sm[i] = ps[min(g0 + i, D / 32 - 1)];
         } else {
+            typedef uint32_t u32x2_a4_t __attribute__((ext_vector_type(2), aligned(4)));
 #pragma unroll
-            for (int i = 0; i < KK; ++i) w[i] = 8 * (g * KK + i) < D ? p[i] : 0u;
-#pragma unroll
-            for (int i = 0; i < NS; ++i) sm[i] = 32 * (g0 + i) < D ? ps[g0 + i] : 0u;
+            for (int i = 0; i < KK / 2; ++i) {
+                const u32x2_a4_t x = *reinterpret_cast<const u32x2_a4_t*>(p + 2 * i);
+                w[2 * i] = x[0];
+                w[2 * i + 1] = x[1];
+            }
         }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) sm[i] = *reinterpret_cast<const uint32_t*>(row + q.pairs[i]);
     }
-    __device__ __forceinline__ half8_t frag(int kk, int g) const {
-        // (the group of word g KK + kk, counted from the lane's first group)
+    __device__ __forceinline__ half8_t frag(int kk, const Place& q) const {
         uint32_t x = sm[0];
-        if constexpr (NS > 1) {
-            const int at = (g * KK + kk) / 4 - g * KK / 4;
-#pragma unroll
-            for (int i = 1; i < NS; ++i) x = at == i ? sm[i] : x;
-        }
+        if constexpr (NS > 1) x = (q.first + kk) / 4 > q.first / 4 ? sm[1] : sm[0];  // (DP / 4 values lie in two groups at most)
         half2_t s, m;
         four_bit_pair(x, s, m);
         return four_bit_values(w[kk], s, m);
     }
-    __device__ __forceinline__ static int first(int kk, int g) { return g * KK * 8 + 8 * kk; }
-    __device__ __forceinline__ void clear() {
+    __device__ __forceinline__ void clear() {  // (a pair of zeros: the value 0 whatever the code)
 #pragma unroll
         for (int i = 0; i < NS; ++i) sm[i] = 0u;
     }
 };
-template <int DP>
-__device__ __forceinline__ half8_t share_frag(const RowShare<DP, false>& r, int kk, int) { return r.frag(kk); }
-template <int DP>
-__device__ __forceinline__ half8_t share_frag(const RowShare<DP, true>& r, int kk, int g) { return r.frag(kk, g); }
 
 constexpr int kFewUnit = 128;  // keys of a round of four waves
 
 template <int DP, bool I4>
-__global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
+__global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel(PagedArgs a) {
+    typedef RowShare<DP, I4> Share;
     constexpr int KK = DP / 32, DT = DP / 16, PITCH = 2 * DP + 32, OP = DP + 4;
     static_assert(16 * OP * 4 <= 32 * PITCH, "a wave's partial result fits its piece of LDS");
     __shared__ __attribute__((aligned(16))) char lds[4 * 32 * PITCH];
@@ -126,15 +126,15 @@ __global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
     const int rho = it.tile * kFewRows + r, i = rho / a.G;
     const bool mine = i < it.n;
     const int pos = mine ? it.len - it.n + i : -1;
+    const typename Share::Place where(c.D, g);
     half8_t qf[KK];
     {
         const _Float16* q = a.q + (int64_t)(it.first + (mine ? i : 0)) * a.q_token +
                             (int64_t)(it.h * a.G + (mine ? rho - i * a.G : 0)) * a.q_head;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
-            const int d = RowShare<DP, I4>::first(kk, g);
             qf[kk] = half8_t{};
-            if (d < c.D) qf[kk] = *reinterpret_cast<const half8_t*>(q + d) * (_Float16)a.sign;
+            if (where.own(kk, c.D, g)) qf[kk] = *reinterpret_cast<const half8_t*>(q + where.value(kk, g)) * (_Float16)a.sign;
         }
     }
     // keys [klo, khi) of this row, and of all rows of the tile
@@ -189,16 +189,16 @@ __global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
     for (int d = 0; d < DT; ++d) acc[d] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
     int t = it.lo + 32 * wave;
-    RowShare<DP, I4> k[2], v[2];
+    Share k[2], v[2];
     int64_t off[2];
     int page[2], inside[2];
     if (t < it.hi) {
         place(t, page, inside);
         offset(t, page, inside, off);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) k[u].load(kb + off[u], c.D, g);
+        for (int u = 0; u < 2; ++u) k[u].load(kb + off[u], where, g);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) v[u].load(vbase + off[u], c.D, g);
+        for (int u = 0; u < 2; ++u) v[u].load(vbase + off[u], where, g);
         if (t + kFewUnit < it.hi) place(t + kFewUnit, page, inside);
     }
     for (; t < it.hi; t += kFewUnit) {
@@ -209,12 +209,12 @@ __global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
             s[u] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
-                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(share_frag(k[u], kk, g), qf[kk], s[u], 0, 0, 0);
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[u].frag(kk, where), qf[kk], s[u], 0, 0, 0);
         }
         if (more) {
             offset(t + kFewUnit, page, inside, off);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) k[u].load(kb + off[u], c.D, g);
+            for (int u = 0; u < 2; ++u) k[u].load(kb + off[u], where, g);
         }
         // V of this block to LDS; rows past the range as zeros (what lies there is nobody's)
         const bool isnear = t >= it.near;
@@ -229,28 +229,32 @@ __global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
-                *reinterpret_cast<half8_t*>(vb + (16 * u + r) * PITCH + 2 * RowShare<DP, I4>::first(kk, g)) =
-                    share_frag(v[u], kk, g);
+                *reinterpret_cast<half8_t*>(vb + (16 * u + r) * PITCH + 2 * where.value(kk, g)) = v[u].frag(kk, where);
         asm volatile("" ::: "memory");
         if (more) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) v[u].load(vbase + off[u], c.D, g);
+            for (int u = 0; u < 2; ++u) v[u].load(vbase + off[u], where, g);
             if (t + 2 * kFewUnit < it.hi) place(t + 2 * kFewUnit, page, inside);
         }
         // weights
         const int key0 = it.base + t - it.near;
         if (left < 32 || (isnear && (key0 + 32 > khi_all || key0 < klo_all))) {
+            // places [0, upto) and, of a window's block, from `from` on or on the stride
+            const int upto = min(isnear ? khi - key0 : mine ? 32 : 0, left) - 4 * g;
+            if (isnear && a.window > 0) {
+                const int from = klo - key0 - 4 * g;
+                const uint32_t bits = a.stride > 0 ? (uint32_t)stride_bits(key0, a.stride) >> (4 * g) : 0u;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int at = 16 * (e >> 2) + 4 * g + (e & 3), key = key0 + at;
-                bool in = at < left;
-                if (isnear) {
-                    in = in && key < khi;
-                    if (a.window > 0) in = in && (key >= klo || (a.stride > 0 && key % a.stride == 0));
-                } else {
-                    in = in && mine;
+                for (int e = 0; e < 8; ++e) {
+                    const int at = 16 * (e >> 2) + (e & 3);
+                    s[e >> 2][e & 3] = at < upto && (at >= from || (bits >> at & 1)) ? s[e >> 2][e & 3] : kNoScore;
                 }
-                s[e >> 2][e & 3] = in ? s[e >> 2][e & 3] : kNoScore;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int at = 16 * (e >> 2) + (e & 3);
+                    s[e >> 2][e & 3] = at < upto ? s[e >> 2][e & 3] : kNoScore;
+                }
             }
         }
         float mx = kNoScore;
@@ -321,7 +325,7 @@ __global__ void __launch_bounds__(256) paged_few_kernel(PagedArgs a) {
         for (int w = 0; w < 4; ++w)
             o[j] += *reinterpret_cast<const float4_t*>(lds + w * (32 * PITCH) + 4 * (row * OP + col + 64 * j)) * fw[w];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) fine = fine && __builtin_fabsf(o[j][q]) < __builtin_inff();
+        for (int q = 0; q < 4; ++q) fine = fine && (col + 64 * j >= c.D || __builtin_fabsf(o[j][q]) < __builtin_inff());
     }
     const bool here = ri < it.n;
     const int head = it.h * a.G + rrho - ri * a.G;

@@ -36,50 +36,65 @@ struct BlockShare {
     static constexpr int ALL = 2 * KEYS * PER, N = (ALL + 255) / 256;
     u32x4_t v[N];
     uint32_t sm[I4 ? N : 1];
-    // (the last threads have a piece fewer where they do not come out even: they take the last once more)
-    __device__ __forceinline__ static void piece(int x, bool& is_v, int& row, int& at) {
-        const int u0 = threadIdx.x + 256 * x, u = ALL % 256 == 0 ? u0 : min(u0, ALL - 1), w = u % (KEYS * PER);
-        is_v = u >= KEYS * PER;
-        row = w / PER;
-        at = w % PER;
-    }
-    __device__ __forceinline__ void load(const char* kb, const char* vb, const int64_t* off, int D) {
+    const char* from[N];  // the piece in the row at offset 0 (heads narrower than DP: the last one again past the end)
+    const char* pair[I4 ? N : 1];
+    __device__ __forceinline__ static bool of_v(int x) { return index(x) >= KEYS * PER; }
+    __device__ __forceinline__ static int row(int x) { return index(x) % (KEYS * PER) / PER; }
+    __device__ __forceinline__ static int piece(int x) { return index(x) % PER; }
+    __device__ __forceinline__ BlockShare(const char* kb, const char* vb, int D) {
 #pragma unroll
         for (int x = 0; x < N; ++x) {
-            bool is_v;
-            int row, at;
-            piece(x, is_v, row, at);
-            const char* p = (is_v ? vb : kb) + off[row];
-            v[x] = u32x4_t{0, 0, 0, 0};
+            const char* base = of_v(x) ? vb : kb;
             if constexpr (I4) {
-                sm[x] = 0;
-                if (D == DP || 32 * at < D) {
-                    v[x] = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_a4_t*>(p + 16 * at));
-                    sm[x] = *reinterpret_cast<const uint32_t*>(p + D / 2 + 4 * at);
-                }
+                const int at = min(piece(x), D / 32 - 1);
+                from[x] = base + 16 * at;
+                pair[x] = base + D / 2 + 4 * at;
             } else {
-                if (D == DP || 8 * at < D) v[x] = *reinterpret_cast<const u32x4_t*>(p + 16 * at);
+                from[x] = base + 16 * min(piece(x), D / 8 - 1);
             }
         }
     }
-    // Rows from `left` on as zeros in V (what lies there is nobody's).
-    __device__ __forceinline__ void store(char* k, char* vl, int left) const {
+    __device__ __forceinline__ void load(const int64_t* off) {
 #pragma unroll
         for (int x = 0; x < N; ++x) {
-            bool is_v;
-            int row, at;
-            piece(x, is_v, row, at);
-            const bool none = is_v && row >= left;
-            char* to = (is_v ? vl + row * VP : k + row * KP) + at * (I4 ? 64 : 16);
+            const int64_t o = off[row(x)];
+            if constexpr (I4) {
+                v[x] = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_a4_t*>(from[x] + o));
+                sm[x] = *reinterpret_cast<const uint32_t*>(pair[x] + o);
+            } else {
+                v[x] = *reinterpret_cast<const u32x4_t*>(from[x] + o);
+            }
+        }
+    }
+    // To LDS, V's rows from `left` on as zeros (what lies there is nobody's).
+    __device__ __forceinline__ void store(char* k, char* vl, int left) {
+        if (left < KEYS) {
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+                if (of_v(x) && row(x) >= left) {
+                    if constexpr (I4) sm[x] = 0u;
+                    else v[x] = u32x4_t{0, 0, 0, 0};
+                }
+        }
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            char* to = (of_v(x) ? vl + row(x) * VP : k + row(x) * KP) + piece(x) * (I4 ? 64 : 16);
             if constexpr (I4) {
                 half2_t s, m;
-                four_bit_pair(none ? 0u : sm[x], s, m);
+                four_bit_pair(sm[x], s, m);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) *reinterpret_cast<half8_t*>(to + 16 * i) = four_bit_values(v[x][i], s, m);
             } else {
-                *reinterpret_cast<u32x4_t*>(to) = none ? u32x4_t{0, 0, 0, 0} : v[x];
+                *reinterpret_cast<u32x4_t*>(to) = v[x];
             }
         }
+    }
+
+private:
+    // (the last threads have a piece fewer where they do not come out even: they take the last once more)
+    __device__ __forceinline__ static int index(int x) {
+        const int u = threadIdx.x + 256 * x;
+        return ALL % 256 == 0 ? u : min(u, ALL - 1);
     }
 };
 
@@ -87,7 +102,7 @@ struct BlockShare {
 __device__ __forceinline__ int keys_left(const PagedItem& it, int t) { return (t < it.near ? min(it.hi, it.far) : it.hi) - t; }
 
 template <int DP, bool I4>
-__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_many_kernel(PagedArgs a) {
+__global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_many_kernel(PagedArgs a) {
     typedef BlockShare<DP, I4> Share;
     constexpr int KEYS = Share::KEYS, U = KEYS / 32, KK = DP / 16, DT = DP / 32;
     constexpr int KP = Share::KP, VP = Share::VP, BUF = KEYS * (KP + VP);
@@ -137,14 +152,14 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_many_kernel(Page
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[d][e] = 0.0f;
 
-    Share share;
+    Share share(kb, vb, c.D);
     if (it.lo < it.hi) {
         if (tid < KEYS) {
             off[0][tid] = place(it.lo);
             off[1][tid] = place(it.lo + KEYS);
         }
         __syncthreads();
-        share.load(kb, vb, off[0], c.D);
+        share.load(off[0]);
         share.store(lds, lds + KEYS * KP, keys_left(it, it.lo));
         __syncthreads();
     }
@@ -153,7 +168,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_many_kernel(Page
         const bool more = t + KEYS < it.hi;
         int64_t next = 0;
         if (more) {
-            share.load(kb, vb, off[buf ^ 1], c.D);
+            share.load(off[buf ^ 1]);
             if (tid < KEYS) next = place(t + 2 * KEYS);
         }
         const char* kl = lds + buf * BUF;
@@ -163,29 +178,50 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_many_kernel(Page
         if (any && (!isnear || (key0 < khi_some && key0 + KEYS > klo_some))) {
             float16_t s[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
+            // (FRAGS of K's operands are on their way before the first product that takes one)
+            constexpr int FRAGS = DP <= 64 ? KK : 4;
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
-                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                        *reinterpret_cast<const half8_t*>(kl + (32 * u + r) * KP + 32 * kk + 16 * h), qf[kk], s[u], 0, 0, 0);
+            for (int k0 = 0; k0 < KK; k0 += FRAGS) {
+                half8_t kf[U][FRAGS];
+#pragma unroll
+                for (int kk = 0; kk < FRAGS; ++kk)
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        kf[u][kk] = *reinterpret_cast<const half8_t*>(kl + (32 * u + r) * KP + 32 * (k0 + kk) + 16 * h);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int kk = 0; kk < FRAGS; ++kk)
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[u][kk], qf[k0 + kk], s[u], 0, 0, 0);
             }
             if (left < KEYS || (isnear && (key0 + KEYS > khi_all || key0 < klo_all))) {
+                // places [0, upto) and, of a window's block, from `from` on or on the stride
+                const int upto = min(isnear ? khi - key0 : mine ? KEYS : 0, left) - 4 * h;
+                if (isnear && a.window > 0) {
+                    const int from = klo - key0 - 4 * h;
+                    const uint64_t bits = a.stride > 0 ? stride_bits(key0, a.stride) >> (4 * h) : 0u;
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+                    for (int u = 0; u < U; ++u) {
+                        const uint32_t half = (uint32_t)(bits >> (32 * u));
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int at = 32 * u + 8 * (e >> 2) + 4 * h + (e & 3), key = key0 + at;
-                        bool in = at < left;
-                        if (isnear) {
-                            in = in && key < khi;
-                            if (a.window > 0) in = in && (key >= klo || (a.stride > 0 && key % a.stride == 0));
-                        } else {
-                            in = in && mine;
+                        for (int e = 0; e < 16; ++e) {
+                            const int at = 32 * u + 8 * (e >> 2) + (e & 3);
+                            s[u][e] = at < upto && (at >= from || (half >> (at & 31) & 1)) ? s[u][e] : kNoScore;
                         }
-                        s[u][e] = in ? s[u][e] : kNoScore;
                     }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int at = 32 * u + 8 * (e >> 2) + (e & 3);
+                            s[u][e] = at < upto ? s[u][e] : kNoScore;
+                        }
+                }
             }
             float mx = s[0][0];
 #pragma unroll
