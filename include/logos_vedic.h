@@ -684,7 +684,7 @@ int vedic_kv_read(const vedic_kv_t* kv, void* k, void* v, void* stream);
  * reach the output.  Rows of no sequence are left as they are.
  * Sequences of up to 64 rows (n_b x q_heads / heads) share out their keys evenly over the GPU,
  * others take 128 rows a workgroup and share keys where that leaves CUs idle; parts are added in
- * a fixed order, 2 x (CUs x 4 x 16 + CUs x 2 x 128) x (dh + 2) fp32 of the stream's workspace block at
+ * a fixed order, 512 x CUs x (dh + 2) fp32 of the stream's workspace block at
  * most.  A captured call without such a block does not split (results may then differ in
  * rounding). */
 int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_t q_token, int64_t q_head, int q_heads, void* out,

@@ -156,7 +156,9 @@ struct PagedArgs {
     float* part_o;   // [slots x rows x D]
     float* part_ml;  // [slots x rows x 2]
 };
+// Rows of a tile, and what parts of a tile's keys are whole multiples of.
 constexpr int kFewRows = 16, kManyRows = 128;
+constexpr int kFewUnit = 128, kManyUnit = 256;
 hipError_t launch_paged_few_f16(const PagedArgs& a, hipStream_t s);
 hipError_t launch_paged_few_i4(const PagedArgs& a, hipStream_t s);
 hipError_t launch_paged_many_f16(const PagedArgs& a, hipStream_t s);

@@ -1790,8 +1790,11 @@ extern "C" int vedic_kv_read(const vedic_kv_t* kv, void* k, void* v, void* strea
 // Rows (new tokens x heads that share a key head) up to which a sequence is the few-row kernel's.
 static constexpr int kFewMost = 64;
 
-// Workgroups' worth of keys that a call's items are cut to: as many as a GPU has at work.
-static int64_t paged_target(bool many, int dh, int cus) { return many ? cus * (dh <= 128 ? 2 : 1) : cus * 4; }
+// Items that a call's keys are cut to.  Few rows: eight a CU, which is bound by reading and gains from even
+// shares (32 sequences of 128-wide binary16 heads, up to 16384 tokens: 261 / 225 / 213 / 210 us at one / four / six / eight;
+// 64 over four bits 284 / 203 / 191 / 188).  Many: one, since a part's sums of 128 rows cost as much as 64 keys
+// (pieces of 500 rows of three prompts: 197 us, 242 at two, 226 at four).
+static int64_t paged_target(bool many, int cus) { return many ? cus : cus * 8; }
 
 extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_t q_token, int64_t q_head, int q_heads,
                                      void* out, int64_t out_token, int64_t out_head, float* lse, float scale, int causal,
@@ -1841,9 +1844,9 @@ extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_
         if (kind == 0 ? !few : !many) continue;
         PagedArgs b = a;
         const int tile = kind ? kManyRows : kFewRows;
-        b.target = paged_target(kind != 0, kv->dh, cus);
+        b.target = paged_target(kind != 0, cus);
         // (where no sequence can have two parts)
-        if ((int64_t)kv->table_cols * kv->page_size <= (kind ? 256 : 128)) b.target = 0;
+        if ((int64_t)kv->table_cols * kv->page_size <= (kind ? kManyUnit : kFewUnit)) b.target = 0;
         const size_t slots = 2 * (size_t)b.target, bytes = slots * tile * (kv->dh + 2) * 4;
         if (!ws.room(bytes)) b.target = 0;
         float* part = nullptr;

@@ -24,6 +24,12 @@ constexpr float kNoScore = -__builtin_inff();
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The larger of a lane's value and that of the lane 32 from it.
+__device__ __forceinline__ float both_halves_max(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
 struct PagedItem {
     int b, tile, h;       // sequence, tile of its rows, key head
     int first, n, len;    // its new rows and its tokens
@@ -112,7 +118,7 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, 
             const int s0 = slots + __builtin_amdgcn_readlane(sincl, who) - __builtin_amdgcn_readlane(split, who);
             it.slot = s0 + unit * it.parts + it.part;
             const int ntiles = __builtin_amdgcn_readlane(tiles, who);
-            // (the last rows of a prompt see the most keys: they begin first)
+            // (a prompt's last rows, which see the most keys, begin first, over all heads)
             const int tile = unit / a.c.H;
             it.h = unit - tile * a.c.H;
             it.tile = ntiles - 1 - tile;
@@ -141,6 +147,13 @@ __device__ __forceinline__ uint64_t stride_bits(int key, int stride) {
     const int past = key % stride;
     for (int j = past ? stride - past : 0; j < 64; j += stride) bits |= uint64_t(1) << j;
     return bits;
+}
+
+// Bits [from, upto) and those of `more` below upto.
+__device__ __forceinline__ uint64_t place_bits(int from, int upto, uint64_t more) {
+    const uint64_t below = upto <= 0 ? 0 : upto >= 64 ? ~uint64_t(0) : (uint64_t(1) << upto) - 1;
+    const uint64_t above = from <= 0 ? ~uint64_t(0) : from >= 64 ? 0 : ~uint64_t(0) << from;
+    return below & (above | more);
 }
 
 // Whether the row at position pos sees key t < len.
@@ -203,76 +216,156 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, const PagedItem& it
     }
 }
 
+typedef _Float16 paged_half4_t __attribute__((ext_vector_type(4)));
+
 __device__ __forceinline__ float lse_of(float m, float l) {
     return l > 0.0f || l != l ? (m - kWeightBits + __builtin_log2f(l)) * 0.6931471805599453f : __builtin_inff();
 }
 
 namespace {
 
-// The parts of a tile joined: a wave per row, its lanes D / 4 columns of four and the rest
-// shares of the parts.
-template <int ROWS, bool MANY, int UNIT>
-__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    PagedItem it;
-    if (!find_item<ROWS, MANY, UNIT, true>(a, blockIdx.x, lane, it)) return;
-    if (it.parts == 1 || (int64_t)it.slot + it.parts > a.slots) return;
-    const int r = blockIdx.y * 4 + wave, rho = it.tile * ROWS + r, i = rho / a.G;
-    if (r >= ROWS || i >= it.n) return;
-    const int D = a.c.D, cols = D / 4;
-    const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // of a share
-    const int share = lane / lanes, shares = 64 / lanes, c = lane % lanes;
-    const int64_t s0 = (int64_t)it.slot * ROWS + r;
-    float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-    float M = kNoScore, l = 0.0f;
-    // (a running maximum: all loads of a round are on their way together)
-    for (int p0 = share; p0 < it.parts; p0 += 8 * shares) {
-        float mp[8], lp[8];
-        float4_t v[8];
+// The sums of 32 rows from `base` on, O^T in 32 x 32 blocks (lane l: row base + l mod 32; element 4 e + f of block
+// d: value 32 d + 8 e + 4 (l / 32) + f), to the output or to the partial results from row s0 on.
+template <int DP, bool I4>
+__device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem& it, int base, int64_t s0,
+                                            const float16_t (&acc)[DP / 32], float m, float l, int lane) {
+    constexpr int DT = DP / 32;
+    const int r = lane & 31, h = lane >> 5, rho = base + r, i = rho / a.G;
+    const bool mine = i < it.n;
+    const int64_t tok = it.first + i;
+    const int head = it.h * a.G + rho - i * a.G;
+    l += __shfl_xor(l, 32);
+    bool fine = l < __builtin_inff();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t s = s0 + (int64_t)min(p0 + j * shares, it.parts - 1) * ROWS;
-            mp[j] = a.part_ml[2 * s];
-            lp[j] = a.part_ml[2 * s + 1];
-            v[j] = *reinterpret_cast<const float4_t*>(a.part_o + s * D + 4 * min(c, cols - 1));
-        }
-        float top = M;
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = __builtin_fmaxf(top, mp[j]);
-        const float mu = top == kNoScore ? 0.0f : top, g = exp2_fast(M - mu);
-        M = top;
-        l *= g;
-        o *= g;
+        for (int e = 0; e < 16; ++e) fine = fine && __builtin_fabsf(acc[d][e]) < __builtin_inff();
+    if (mine) {
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        if (it.parts == 1) {
+            _Float16* out = a.out + tok * a.o_token + (int64_t)head * a.o_head;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float f = exp2_fast(mp[j] - mu);
-            if (p0 + j * shares < it.parts && !(lp[j] == 0.0f)) {  // (a part without keys has nothing to add)
-                l += lp[j] * f;
-                o += v[j] * f;
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int at = 32 * d + 8 * e + 4 * h;
+                    const paged_half4_t v = {(_Float16)(acc[d][4 * e] * inv), (_Float16)(acc[d][4 * e + 1] * inv),
+                                            (_Float16)(acc[d][4 * e + 2] * inv), (_Float16)(acc[d][4 * e + 3] * inv)};
+                    if (at < a.c.D) *reinterpret_cast<paged_half4_t*>(out + at) = v;
+                }
+            if (a.lse && h == 0) a.lse[tok * a.Hq + head] = lse_of(m, l);
+        } else {
+            float* po = a.part_o + (s0 + r) * a.c.D;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int at = 32 * d + 8 * e + 4 * h;
+                    const float4_t v = {acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
+                    if (at < a.c.D) *reinterpret_cast<float4_t*>(po + at) = v;
+                }
+            if (h == 0) {
+                a.part_ml[2 * (s0 + r)] = m;
+                a.part_ml[2 * (s0 + r) + 1] = l;
             }
         }
     }
-    for (int d = lanes; d < 64; d <<= 1) {
-        const float other = __shfl_xor(M, d), top = __builtin_fmaxf(M, other), mu = top == kNoScore ? 0.0f : top;
-        const float g = exp2_fast(M - mu), go = exp2_fast(other - mu);
-        M = top;
-        const float lo = __shfl_xor(l, d);
-        l = l * g + lo * go;
+    // rows with an infinite or undefined value once more, key by key (slow_row)
+    uint64_t bad = __ballot(mine && !fine);
+    bad = (bad | bad >> 32) & 0xFFFFFFFFu;
+    while (bad) {
+        const int w = __builtin_ctzll(bad);
+        bad &= bad - 1;
+        const int brho = base + w, bi = brho / a.G, bh = it.h * a.G + brho - bi * a.G;
+        const int64_t bt = it.first + bi;
+        float ov[DP / 64], bm, bl;
+        slow_row<DP, I4>(a, it, it.len - it.n + bi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
+                         bm, bl);
+        const float bin = bl > 0.0f || bl != bl ? 1.0f / bl : 0.0f;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the stores above come first)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float oo = __shfl_xor(o[j], d);
-            o[j] = o[j] * g + oo * go;
+        for (int j = 0; j < DP / 64; ++j) {
+            const int d = lane + 64 * j;
+            if (d >= a.c.D) continue;
+            if (it.parts == 1) a.out[bt * a.o_token + (int64_t)bh * a.o_head + d] = (_Float16)(ov[j] * bin);
+            else a.part_o[(s0 + w) * a.c.D + d] = ov[j];
+        }
+        if (lane == 0) {
+            if (it.parts == 1) {
+                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(bm, bl);
+            } else {
+                a.part_ml[2 * (s0 + w)] = bm;
+                a.part_ml[2 * (s0 + w) + 1] = bl;
+            }
         }
     }
-    const int head = it.h * a.G + rho % a.G;
-    const int64_t t = it.first + i;
-    if (share == 0 && c < cols) {
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
-        const half4_t v = {(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
-        *reinterpret_cast<half4_t*>(a.out + t * a.o_token + (int64_t)head * a.o_head + 4 * c) = v;
+}
+
+// The parts of a tile joined, `per` of its rows a workgroup: a wave per row, its lanes D / 4 columns of
+// four and the rest shares of the parts.
+template <int ROWS, bool MANY, int UNIT>
+__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    PagedItem it;
+    if (!find_item<ROWS, MANY, UNIT, true>(a, blockIdx.x, lane, it)) return;
+    if ((int64_t)it.slot + it.parts > a.slots) return;
+    const int D = a.c.D, cols = D / 4;
+    const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // of a share
+    const int share = lane / lanes, shares = 64 / lanes, c = lane % lanes;
+    for (int r = blockIdx.y * per + wave; r < (int)(blockIdx.y + 1) * per; r += 4) {
+        const int rho = it.tile * ROWS + r, i = rho / a.G;
+        if (i >= it.n) return;
+        const int64_t s0 = (int64_t)it.slot * ROWS + r;
+        float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+        float M = kNoScore, l = 0.0f;
+        // (a running maximum: all loads of a round are on their way together)
+        for (int p0 = share; p0 < it.parts; p0 += 8 * shares) {
+            float mp[8], lp[8];
+            float4_t v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int64_t s = s0 + (int64_t)min(p0 + j * shares, it.parts - 1) * ROWS;
+                mp[j] = a.part_ml[2 * s];
+                lp[j] = a.part_ml[2 * s + 1];
+                v[j] = *reinterpret_cast<const float4_t*>(a.part_o + s * D + 4 * min(c, cols - 1));
+            }
+            float top = M;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = __builtin_fmaxf(top, mp[j]);
+            const float mu = top == kNoScore ? 0.0f : top, g = exp2_fast(M - mu);
+            M = top;
+            l *= g;
+            o *= g;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float f = exp2_fast(mp[j] - mu);
+                if (p0 + j * shares < it.parts && !(lp[j] == 0.0f)) {  // (a part without keys has nothing to add)
+                    l += lp[j] * f;
+                    o += v[j] * f;
+                }
+            }
+        }
+        for (int d = lanes; d < 64; d <<= 1) {
+            const float other = __shfl_xor(M, d), top = __builtin_fmaxf(M, other), mu = top == kNoScore ? 0.0f : top;
+            const float g = exp2_fast(M - mu), go = exp2_fast(other - mu);
+            M = top;
+            const float lo = __shfl_xor(l, d);
+            l = l * g + lo * go;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float oo = __shfl_xor(o[j], d);
+                o[j] = o[j] * g + oo * go;
+            }
+        }
+        const int head = it.h * a.G + rho % a.G;
+        const int64_t t = it.first + i;
+        if (share == 0 && c < cols) {
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            const paged_half4_t v = {(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
+            *reinterpret_cast<paged_half4_t*>(a.out + t * a.o_token + (int64_t)head * a.o_head + 4 * c) = v;
+        }
+        if (a.lse && lane == 0) a.lse[t * a.Hq + head] = lse_of(M, l);
     }
-    if (a.lse && lane == 0) a.lse[t * a.Hq + head] = lse_of(M, l);
 }
 
 }  // namespace

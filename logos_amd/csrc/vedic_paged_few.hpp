@@ -95,7 +95,7 @@ struct RowShare<DP, true> {
     }
     __device__ __forceinline__ half8_t frag(int kk, const Place& q) const {
         uint32_t x = sm[0];
-        if constexpr (NS > 1) x = (q.first + kk) / 4 > q.first / 4 ? sm[1] : sm[0];  // (DP / 4 values lie in two groups at most)
+        if constexpr (NS > 1) x = (q.first + kk) / 4 > q.first / 4 ? sm[1] : sm[0];  // (DP / 4 values: two groups at most)
         half2_t s, m;
         four_bit_pair(x, s, m);
         return four_bit_values(w[kk], s, m);
@@ -105,8 +105,6 @@ struct RowShare<DP, true> {
         for (int i = 0; i < NS; ++i) sm[i] = 0u;
     }
 };
-
-constexpr int kFewUnit = 128;  // keys of a round of four waves
 
 template <int DP, bool I4>
 __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel(PagedArgs a) {
@@ -239,22 +237,14 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
         // weights
         const int key0 = it.base + t - it.near;
         if (left < 32 || (isnear && (key0 + 32 > khi_all || key0 < klo_all))) {
-            // places [0, upto) and, of a window's block, from `from` on or on the stride
             const int upto = min(isnear ? khi - key0 : mine ? 32 : 0, left) - 4 * g;
-            if (isnear && a.window > 0) {
-                const int from = klo - key0 - 4 * g;
-                const uint32_t bits = a.stride > 0 ? (uint32_t)stride_bits(key0, a.stride) >> (4 * g) : 0u;
+            const bool window = isnear && a.window > 0;
+            const uint64_t more = window && a.stride > 0 ? stride_bits(key0, a.stride) >> (4 * g) : 0;
+            const uint32_t bits = (uint32_t)place_bits(window ? klo - key0 - 4 * g : 0, upto, more);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int at = 16 * (e >> 2) + (e & 3);
-                    s[e >> 2][e & 3] = at < upto && (at >= from || (bits >> at & 1)) ? s[e >> 2][e & 3] : kNoScore;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int at = 16 * (e >> 2) + (e & 3);
-                    s[e >> 2][e & 3] = at < upto ? s[e >> 2][e & 3] : kNoScore;
-                }
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t bit = 1u << (16 * (e >> 2) + (e & 3));
+                s[e >> 2][e & 3] = bits & bit ? s[e >> 2][e & 3] : kNoScore;
             }
         }
         float mx = kNoScore;
@@ -396,7 +386,8 @@ hipError_t paged_few(const PagedArgs& a, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.target > 0) {
         const int rows = a.c.q_start == nullptr && a.G < kFewRows ? a.G : kFewRows;
-        paged_join_kernel<kFewRows, false, kFewUnit><<<dim3((unsigned)(tiles < a.target ? tiles : a.target), (unsigned)(rows + 3) / 4), 256, 0, s>>>(a);
+        paged_join_kernel<kFewRows, false, kFewUnit><<<dim3((unsigned)(tiles < a.target ? tiles : a.target), (unsigned)(rows + 3) / 4), 256, 0,
+                                                          s>>>(a, 4);
         e = hipGetLastError();
     }
     return e;

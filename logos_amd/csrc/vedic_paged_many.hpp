@@ -5,14 +5,13 @@
 //   running maximum and sum in fp32, O^T += V^T P^T.
 //
 // A workgroup has a tile of 128 rows (four waves of 32) and a range of keys (vedic_paged.hpp).
-// Blocks of 64 keys (32 with heads past 128) go through two buffers of LDS, one barrier a block: while a block is
-// multiplied, the next one's rows are on their way into registers (from the pages, 16 bytes a
+// Blocks of 64 keys (32 with heads past 128) go through two buffers of LDS, one barrier a block: while
+// a block is multiplied, the next one's rows are on their way into registers (from the pages, 16 bytes a
 // thread and load; four bits are expanded on their way to LDS) and the places of the one
 // after that are looked up.  K's rows lie 2 DP + 16 bytes apart (ds_read_b128 of eight rows meets
 // every bank once), V's 2 DP + 32 (the same for the transposing ds_read_b64_tr_b16).  The scores'
 // layout, a row of Q per lane, is what the second product takes: the weights stay in
-// registers.  A wave leaves out blocks none of its rows sees, and looks at masks only where
-// some key of a block is hidden from one of them.
+// registers.  Masks are looked at only where some key of a block is hidden from a row of the wave.
 #pragma once
 
 #include "vedic_paged.hpp"
@@ -22,11 +21,9 @@ namespace vedic {
 namespace {
 
 typedef short many_short4_t __attribute__((ext_vector_type(4)));
-typedef _Float16 many_half4_t __attribute__((ext_vector_type(4)));
 
 // Keys of a block: with heads past 128 the next block's rows would take 64 registers more.
 constexpr int many_keys(int dp) { return dp <= 128 ? 64 : 32; }
-constexpr int kManyUnit = 256;   // parts are whole multiples of it
 
 // The pieces of a block (64 rows of K, then of V) that a thread carries from the pages to LDS.
 template <int DP, bool I4>
@@ -105,8 +102,9 @@ template <int DP, bool I4>
 __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_many_kernel(PagedArgs a) {
     typedef BlockShare<DP, I4> Share;
     constexpr int KEYS = Share::KEYS, U = KEYS / 32, KK = DP / 16, DT = DP / 32;
-    constexpr int KP = Share::KP, VP = Share::VP, BUF = KEYS * (KP + VP);
-    __shared__ __attribute__((aligned(16))) char lds[2 * BUF];
+    constexpr int KP = Share::KP, VP = Share::VP;
+    __shared__ __attribute__((aligned(16))) char kbuf[2][KEYS * KP];
+    __shared__ __attribute__((aligned(16))) char vbuf[2][KEYS * VP];
     __shared__ int64_t off[2][KEYS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     PagedItem it;
@@ -132,17 +130,22 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
     }
     const int khi = !mine ? 0 : a.causal ? pos + 1 : it.len;
     const int klo = a.window > 0 ? pos - a.window : INT32_MIN;
-    // of the wave's rows: all see the keys [klo_all, khi_all), none those outside [klo_some, khi_some)
-    const bool any = base < (int64_t)it.n * a.G;
+    // of the wave's rows: all see the keys [klo_all, khi_all)
     const int p0 = it.len - it.n + base / a.G, p1 = it.len - it.n + min(it.n - 1, (base + 31) / a.G);
-    const int khi_all = a.causal ? p0 + 1 : it.len, khi_some = !any ? 0 : a.causal ? p1 + 1 : it.len;
+    const int khi_all = base + 32 > (int64_t)it.n * a.G ? 0 : a.causal ? p0 + 1 : it.len;
     const int klo_all = a.window > 0 ? p1 - a.window : INT32_MIN;
-    const int klo_some = a.window > 0 && a.stride == 0 ? p0 - a.window : INT32_MIN;
 
     const char* kb = c.k + (int64_t)it.h * c.head;
     const char* vb = c.v + (int64_t)it.h * c.head;
-    auto place = [&](int t) {  // the offset of the key at place t + tid (tid < KEYS)
-        return c.row_offset(it.b, key_at(a, it, min(t + tid, it.hi - 1)));
+    // Where the key at place t + tid (tid < KEYS) lies: its page, looked up now, and its row's offset once that is there.
+    const int* table = c.table + it.b * c.ldt;
+    auto find = [&](int t, int& page, int& inside) {
+        const int key = key_at(a, it, min(t + tid, it.hi - 1)), tp = c.page_of(key);
+        page = table[tp];
+        inside = key - tp * c.ps;
+    };
+    auto offset = [&](int page, int inside) {
+        return ((unsigned)page < (unsigned)c.pages ? page : 0) * c.page + inside * c.token;
     };
 
     float m = kNoScore, l = 0.0f;
@@ -151,191 +154,112 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[d][e] = 0.0f;
-
     Share share(kb, vb, c.D);
+
+    const int kat = r * KP + 16 * h, vat = (4 * h + ((lane & 15) >> 2)) * VP + 2 * (16 * ((lane >> 4) & 1) + 4 * (lane & 3));
     if (it.lo < it.hi) {
         if (tid < KEYS) {
-            off[0][tid] = place(it.lo);
-            off[1][tid] = place(it.lo + KEYS);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                int page, inside;
+                find(it.lo + x * KEYS, page, inside);
+                off[x][tid] = offset(page, inside);
+            }
         }
         __syncthreads();
         share.load(off[0]);
-        share.store(lds, lds + KEYS * KP, keys_left(it, it.lo));
+        share.store(kbuf[0], vbuf[0], keys_left(it, it.lo));
         __syncthreads();
     }
     int buf = 0;
     for (int t = it.lo; t < it.hi; t += KEYS, buf ^= 1) {
         const bool more = t + KEYS < it.hi;
-        int64_t next = 0;
+        int page = 0, inside = 0;
         if (more) {
+            if (tid < KEYS) find(t + 2 * KEYS, page, inside);  // (first: the rows that follow need not be there for its answer)
             share.load(off[buf ^ 1]);
-            if (tid < KEYS) next = place(t + 2 * KEYS);
         }
-        const char* kl = lds + buf * BUF;
-        const char* vl = kl + KEYS * KP;
+        float16_t s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
+        // (FRAGS of K's operands are on their way before the first product that takes one)
+        constexpr int FRAGS = 4;
+#pragma unroll
+        for (int k0 = 0; k0 < KK; k0 += FRAGS) {
+            half8_t kf[U][FRAGS];
+#pragma unroll
+            for (int kk = 0; kk < FRAGS; ++kk)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    kf[u][kk] = *reinterpret_cast<const half8_t*>(kbuf[buf] + kat + 32 * u * KP + 32 * (k0 + kk));
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kk = 0; kk < FRAGS; ++kk)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[u][kk], qf[k0 + kk], s[u], 0, 0, 0);
+        }
         const bool isnear = t >= it.near;
         const int key0 = it.base + t - it.near, left = keys_left(it, t);
-        if (any && (!isnear || (key0 < khi_some && key0 + KEYS > klo_some))) {
-            float16_t s[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
-            // (FRAGS of K's operands are on their way before the first product that takes one)
-            constexpr int FRAGS = DP <= 64 ? KK : 4;
-#pragma unroll
-            for (int k0 = 0; k0 < KK; k0 += FRAGS) {
-                half8_t kf[U][FRAGS];
-#pragma unroll
-                for (int kk = 0; kk < FRAGS; ++kk)
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        kf[u][kk] = *reinterpret_cast<const half8_t*>(kl + (32 * u + r) * KP + 32 * (k0 + kk) + 16 * h);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int kk = 0; kk < FRAGS; ++kk)
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[u][kk], qf[k0 + kk], s[u], 0, 0, 0);
-            }
-            if (left < KEYS || (isnear && (key0 + KEYS > khi_all || key0 < klo_all))) {
-                // places [0, upto) and, of a window's block, from `from` on or on the stride
-                const int upto = min(isnear ? khi - key0 : mine ? KEYS : 0, left) - 4 * h;
-                if (isnear && a.window > 0) {
-                    const int from = klo - key0 - 4 * h;
-                    const uint64_t bits = a.stride > 0 ? stride_bits(key0, a.stride) >> (4 * h) : 0u;
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const uint32_t half = (uint32_t)(bits >> (32 * u));
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int at = 32 * u + 8 * (e >> 2) + (e & 3);
-                            s[u][e] = at < upto && (at >= from || (half >> (at & 31) & 1)) ? s[u][e] : kNoScore;
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int at = 32 * u + 8 * (e >> 2) + (e & 3);
-                            s[u][e] = at < upto ? s[u][e] : kNoScore;
-                        }
-                }
-            }
-            float mx = s[0][0];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) mx = __builtin_fmaxf(mx, s[u][e]);
-            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * a.scale;
-            if (__any(mx > m)) {
-                const float mn = __builtin_fmaxf(m, mx), f = mn == kNoScore ? 1.0f : exp2_fast(m - mn);
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d] *= f;
-                m = mn;
-            }
-            const float bias = kWeightBits - (m == kNoScore ? 0.0f : m);
-            half8_t p[2 * U];
+        if (left < KEYS || (isnear ? key0 + KEYS > khi_all || key0 < klo_all : khi_all == 0)) {
+            const int upto = min(isnear ? khi - key0 : mine ? KEYS : 0, left) - 4 * h;
+            const bool window = isnear && a.window > 0;
+            const uint64_t strided = window && a.stride > 0 ? stride_bits(key0, a.stride) >> (4 * h) : 0;
+            const uint64_t bits = place_bits(window ? klo - key0 - 4 * h : 0, upto, strided);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float w = exp2_fast(__builtin_fmaf(s[u][e], a.scale, bias));
-                    l += w;
-                    p[2 * u + (e >> 3)][e & 7] = (_Float16)w;
-                }
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int q = 0; q < 2 * U; ++q) {
-                    union {
-                        many_short4_t q[2];
-                        half8_t h;
-                    } x;
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-                        x.q[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) many_short4_t*)(vl + (16 * q + 8 * b + 4 * h + ((lane & 15) >> 2)) * VP +
-                                                                               2 * (32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3))));
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, p[q], acc[d], 0, 0, 0);
+                    const uint32_t bit = 1u << (8 * (e >> 2) + (e & 3));
+                    s[u][e] = (uint32_t)(bits >> (32 * u)) & bit ? s[u][e] : kNoScore;
                 }
         }
+        float mx = s[0][0];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = __builtin_fmaxf(mx, s[u][e]);
+        mx = both_halves_max(mx) * a.scale;
+        if (__any(mx > m)) {
+            const float mn = __builtin_fmaxf(m, mx), f = mn == kNoScore ? 1.0f : exp2_fast(m - mn);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] *= f;
+            m = mn;
+        }
+        const float bias = kWeightBits - (m == kNoScore ? 0.0f : m);
+        half8_t p[2 * U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float w = exp2_fast(__builtin_fmaf(s[u][e], a.scale, bias));
+                l += w;
+                p[2 * u + (e >> 3)][e & 7] = (_Float16)w;
+            }
+#pragma unroll
+        for (int q = 0; q < 2 * U; ++q)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                union {
+                    many_short4_t q[2];
+                    half8_t h;
+                } x;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    x.q[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) many_short4_t*)(vbuf[buf] + vat + (16 * q + 8 * b) * VP + 64 * d));
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, p[q], acc[d], 0, 0, 0);
+            }
         if (more) {
-            char* to = lds + (buf ^ 1) * BUF;
-            share.store(to, to + KEYS * KP, keys_left(it, t + KEYS));
-            if (tid < KEYS) off[buf][tid] = next;
+            share.store(kbuf[buf ^ 1], vbuf[buf ^ 1], keys_left(it, t + KEYS));
+            if (tid < KEYS) off[buf][tid] = offset(page, inside);
         }
         __syncthreads();
     }
-
-    l += __shfl_xor(l, 32);
-    bool fine = l < __builtin_inff();
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) fine = fine && __builtin_fabsf(acc[d][e]) < __builtin_inff();
-    const int64_t s0 = (int64_t)it.slot * kManyRows + 32 * wave;
-    if (mine) {
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        if (it.parts == 1) {
-            _Float16* out = a.out + tok * a.o_token + (int64_t)head * a.o_head;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int at = 32 * d + 8 * e + 4 * h;
-                    const many_half4_t v = {(_Float16)(acc[d][4 * e] * inv), (_Float16)(acc[d][4 * e + 1] * inv),
-                                            (_Float16)(acc[d][4 * e + 2] * inv), (_Float16)(acc[d][4 * e + 3] * inv)};
-                    if (at < c.D) *reinterpret_cast<many_half4_t*>(out + at) = v;
-                }
-            if (a.lse && h == 0) a.lse[tok * a.Hq + head] = lse_of(m, l);
-        } else {
-            float* po = a.part_o + (s0 + r) * c.D;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int at = 32 * d + 8 * e + 4 * h;
-                    const float4_t v = {acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
-                    if (at < c.D) *reinterpret_cast<float4_t*>(po + at) = v;
-                }
-            if (h == 0) {
-                a.part_ml[2 * (s0 + r)] = m;
-                a.part_ml[2 * (s0 + r) + 1] = l;
-            }
-        }
-    }
-    // rows with an infinite or undefined value once more, key by key (slow_row)
-    uint64_t bad = __ballot(mine && !fine);
-    bad = (bad | bad >> 32) & 0xFFFFFFFFu;
-    while (bad) {
-        const int w = __builtin_ctzll(bad);
-        bad &= bad - 1;
-        const int brho = base + w, bi = brho / a.G, bh = it.h * a.G + brho - bi * a.G;
-        const int64_t bt = it.first + bi;
-        float ov[DP / 64], bm, bl;
-        slow_row<DP, I4>(a, it, it.len - it.n + bi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
-                         bm, bl);
-        const float bin = bl > 0.0f || bl != bl ? 1.0f / bl : 0.0f;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the stores above come first)
-#pragma unroll
-        for (int j = 0; j < DP / 64; ++j) {
-            const int d = lane + 64 * j;
-            if (d >= c.D) continue;
-            if (it.parts == 1) a.out[bt * a.o_token + (int64_t)bh * a.o_head + d] = (_Float16)(ov[j] * bin);
-            else a.part_o[(s0 + w) * c.D + d] = ov[j];
-        }
-        if (lane == 0) {
-            if (it.parts == 1) {
-                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(bm, bl);
-            } else {
-                a.part_ml[2 * (s0 + w)] = bm;
-                a.part_ml[2 * (s0 + w) + 1] = bl;
-            }
-        }
-    }
+    finish_rows<DP, I4>(a, it, base, (int64_t)it.slot * kManyRows + 32 * wave, acc, m, l, lane);
 }
 
 }  // namespace
@@ -343,15 +267,14 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
 template <bool I4>
 hipError_t paged_many(const PagedArgs& a, hipStream_t s) {
     const int64_t tiles = ((int64_t)a.c.T * a.G / kManyRows + (a.c.B < a.c.T ? a.c.B : a.c.T)) * a.c.H;
-    // (a sequence has two parts only where it is longer than the average of `target`)
-    const dim3 grid((unsigned)(tiles + a.target));
+    const dim3 grid((unsigned)(tiles + a.target)), join((unsigned)(tiles < a.target ? tiles : a.target), 4);
     if (a.c.D <= 64) paged_many_kernel<64, I4><<<grid, 256, 0, s>>>(a);
     else if (a.c.D <= 128) paged_many_kernel<128, I4><<<grid, 256, 0, s>>>(a);
     else if (a.c.D <= 192) paged_many_kernel<192, I4><<<grid, 256, 0, s>>>(a);
     else paged_many_kernel<256, I4><<<grid, 256, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.target > 0) {
-        paged_join_kernel<kManyRows, true, kManyUnit><<<dim3((unsigned)(tiles < a.target ? tiles : a.target), kManyRows / 4), 256, 0, s>>>(a);
+        paged_join_kernel<kManyRows, true, kManyUnit><<<join, 256, 0, s>>>(a, kManyRows / 4);
         e = hipGetLastError();
     }
     return e;
