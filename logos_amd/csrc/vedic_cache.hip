@@ -90,14 +90,24 @@ __device__ __forceinline__ void rotate8(const KvAppendArgs& a, const void* src, 
     const int half = a.rot >> 1;
     float c[8], s[8], o[8];
     if (a.inter) {
+        float cc[4], ss[4];
+        if constexpr (VEC) {  // (the rotated values are whole sixteens)
+            const float4_t c4 = *reinterpret_cast<const float4_t*>(cs + (e0 >> 1)), s4 = *reinterpret_cast<const float4_t*>(cs + half + (e0 >> 1));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cc[i] = c4[i], ss[i] = s4[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = (e0 >> 1) + i;
+                cc[i] = j < half ? cs[j] : 1.0f;
+                ss[i] = j < half ? cs[half + j] : 0.0f;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int j = (e0 >> 1) + i;
-            const bool in = j < half;
-            const float cc = in ? cs[j] : 1.0f, ss = in ? cs[half + j] : 0.0f;
-            c[2 * i] = c[2 * i + 1] = cc;
-            s[2 * i] = -ss;
-            s[2 * i + 1] = ss;
+            c[2 * i] = c[2 * i + 1] = cc[i];
+            s[2 * i] = -ss[i];
+            s[2 * i + 1] = ss[i];
             o[2 * i] = x[2 * i + 1];
             o[2 * i + 1] = x[2 * i];
         }

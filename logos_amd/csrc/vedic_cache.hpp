@@ -68,23 +68,33 @@ inline void kv_divider(KvView& v) {
 // for binary16(s n + m), one rounding.  n | 0x6400 is the binary16 1024 + n, and a nibble at
 // bits 4 .. 7 under 0x5400 is 64 + n, so that a pair of values takes one and-or, one exact
 // subtraction and one fused multiply-add.
-__device__ __forceinline__ half8_t four_bit_values(uint32_t w, half2_t s, half2_t m) {
-    const half2_t k1024 = {(_Float16)1024.0f, (_Float16)1024.0f}, k64 = {(_Float16)64.0f, (_Float16)64.0f};
-    const uint32_t w8 = w >> 8;
-    const half2_t n0 = __builtin_bit_cast(half2_t, (w & 0x000F000Fu) | 0x64006400u) - k1024;
-    const half2_t n1 = __builtin_bit_cast(half2_t, (w & 0x00F000F0u) | 0x54005400u) - k64;
-    const half2_t n2 = __builtin_bit_cast(half2_t, (w8 & 0x000F000Fu) | 0x64006400u) - k1024;
-    const half2_t n3 = __builtin_bit_cast(half2_t, (w8 & 0x00F000F0u) | 0x54005400u) - k64;
-    union {
-        half2_t p[4];
-        half8_t h;
-    } u;
-    u.p[0] = __builtin_elementwise_fma(s, n0, m);
-    u.p[1] = __builtin_elementwise_fma(s, n1, m);
-    u.p[2] = __builtin_elementwise_fma(s, n2, m);
-    u.p[3] = __builtin_elementwise_fma(s, n3, m);
-    return u.h;
-}
+// (A VOP3 instruction takes no 32-bit literal here and one scalar register: the masks are kept in scalar
+// registers and the bases in vector registers, or each and-or would be two instructions.)
+struct FourBits {
+    uint32_t low, mid;     // 0x000F000F, 0x00F000F0 (scalar)
+    uint32_t k1024, k64;   // 0x6400, 0x5400 twice (vector)
+    __device__ __forceinline__ FourBits() : low(0x000F000Fu), mid(0x00F000F0u), k1024(0x64006400u), k64(0x54005400u) {
+        asm volatile("" : "+s"(low), "+s"(mid), "+v"(k1024), "+v"(k64));
+    }
+    __device__ __forceinline__ half8_t operator()(uint32_t w, half2_t s, half2_t m) const {
+        const half2_t m1024 = {(_Float16)1024.0f, (_Float16)1024.0f}, m64 = {(_Float16)64.0f, (_Float16)64.0f};
+        const uint32_t w8 = w >> 8;
+        const half2_t n0 = __builtin_bit_cast(half2_t, (w & low) | k1024) - m1024;
+        const half2_t n1 = __builtin_bit_cast(half2_t, (w & mid) | k64) - m64;
+        const half2_t n2 = __builtin_bit_cast(half2_t, (w8 & low) | k1024) - m1024;
+        const half2_t n3 = __builtin_bit_cast(half2_t, (w8 & mid) | k64) - m64;
+        union {
+            half2_t p[4];
+            half8_t h;
+        } u;
+        u.p[0] = __builtin_elementwise_fma(s, n0, m);
+        u.p[1] = __builtin_elementwise_fma(s, n1, m);
+        u.p[2] = __builtin_elementwise_fma(s, n2, m);
+        u.p[3] = __builtin_elementwise_fma(s, n3, m);
+        return u.h;
+    }
+};
+__device__ __forceinline__ half8_t four_bit_values(uint32_t w, half2_t s, half2_t m) { return FourBits()(w, s, m); }
 __device__ __forceinline__ void four_bit_pair(uint32_t sm, half2_t& s, half2_t& m) {
     const half2_t p = __builtin_bit_cast(half2_t, sm);
     s = half2_t{p[0], p[0]};
@@ -109,14 +119,26 @@ __device__ __forceinline__ uint32_t four_bit_scale(float lo, float hi, bool bad)
     const half2_t sm = {(_Float16)((hi - lo) / 15.0f), (_Float16)lo};
     return __builtin_bit_cast(uint32_t, sm);
 }
-__device__ __forceinline__ uint32_t four_bit_code(float x, float s, float lo) {
-    if (!(s > 0.0f)) return 0u;
-    return (uint32_t)__builtin_fminf(__builtin_fmaxf(__builtin_rintf((x - lo) / s), 0.0f), 15.0f);
-}
+// The word of eight values: round((x - lo) / s).  A product with 1 / s is off the quotient by less than 2^-18 at quotients
+// up to 16 (two roundings of 2^-24 and the division's own); only where that could decide the rounding is it divided.
 __device__ __forceinline__ uint32_t four_bit_word(const float (&x)[8], float s, float lo) {
+    if (!(s > 0.0f)) return 0u;
+    const float inv = 1.0f / s;
+    float n[8];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float q = (x[i] - lo) * inv;
+        n[i] = __builtin_rintf(q);
+        near |= __builtin_fabsf(q - n[i]) > 0.5f - 0x1p-17f;
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n[i] = __builtin_rintf((x[i] - lo) / s);
+    }
     uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= four_bit_code(x[i], s, lo) << (4 * (i >> 1) + 16 * (i & 1));
+    for (int i = 0; i < 8; ++i) w |= (uint32_t)__builtin_fminf(__builtin_fmaxf(n[i], 0.0f), 15.0f) << (4 * (i >> 1) + 16 * (i & 1));
     return w;
 }
 

@@ -1903,6 +1903,12 @@ extern "C" int vedic_w4_unpack(const vedic_w4_t* d, void* W16, int64_t ldw, void
     return hip_status(launch_w4_unpack(w, static_cast<_Float16*>(W16), ldw, static_cast<hipStream_t>(stream)));
 }
 
+// Whether a product with a four-bit weight reads the codes itself, 64 rows at a time: up to 192 rows, and where that
+// is one workgroup a CU (us, so / expanded: 128 rows of 1024 into 4096 12.4 / 19.6, 192 17.2 / 19.8, 256 22.4 / 19.6; of
+// 4096 into 16384 57 / 98, 82 / 107, 110 / 113; 512 rows of 512 into 512 4.5 / 9.9).
+static bool w4_direct(int M, int N, int cus) {
+    return M <= 192 || (int64_t)((M + kW4FewRows - 1) / kW4FewRows) * ((N + 15) / 16) <= cus;
+}
 // Expanded columns at a time (bytes).
 static constexpr size_t kW4Slab = size_t(64) << 20;
 
@@ -1936,7 +1942,7 @@ extern "C" int vedic_gemm_w4(const vedic_w4_t* d, const void* X, int x_dtype, in
     a.residual = resid;
     Workspace ws;
     ws.s = static_cast<hipStream_t>(stream);
-    if (M > kW4FewRows) {
+    if (!w4_direct(M, d->N, device_cu_count())) {
         const int64_t kp = (int64_t)a.w.words * 8;
         const bool rows = a.x32 || d->K % 8 != 0 || !aligned16(X) || ldx % 8 != 0;
         int64_t cols = (int64_t)(kW4Slab / (kp * 2)) / 256 * 256;

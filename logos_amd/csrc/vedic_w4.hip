@@ -5,8 +5,8 @@
 // v_mfma_f32_16x16x32_f16 takes eight values of one column of W: it loads 16 bytes of its column, 32
 // consecutive codes of one group with one pair (s, m), expands a word at a time (13
 // instructions for eight values) and multiplies; lane group g has the codes 128 i + 32 g .. + 31, and
-// takes the same values of its row of X, straight from the cache.  The waves of a workgroup take
-// 128 values of K in turn and add up their 16 x 16 blocks through LDS in a fixed order, so no
+// takes the same values of its row of X, straight from the cache.  The waves of a workgroup share
+// K and add up their 16 x 16 blocks through LDS in a fixed order, so no
 // second launch and no workspace are needed.  Column blocks a wave: one for a row or two
 // (many workgroups), more with more rows, so that the rows of X are not read more often than
 // the codes.
@@ -19,28 +19,27 @@ namespace vedic {
 
 namespace {
 
+// Eight values of a row of X from k on, zeros from K on (16 bytes at any alignment are one load).
 template <bool X32>
-__device__ __forceinline__ half8_t load_x(const void* X, int64_t row, int k, int K, bool vec) {
+__device__ __forceinline__ half8_t load_x(const void* X, int64_t row, int k, int K) {
     half8_t h = {};
     if constexpr (X32) {
+        typedef float4_t float4_any_t __attribute__((aligned(4)));
         const float* p = static_cast<const float*>(X) + row + k;
-        if (vec) {
-            if (k < K) {
-                const float4_t a = reinterpret_cast<const float4_t*>(p)[0], b = reinterpret_cast<const float4_t*>(p)[1];
+        if (k + 8 <= K) {
+            const float4_t a = reinterpret_cast<const float4_any_t*>(p)[0], b = reinterpret_cast<const float4_any_t*>(p)[1];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) h[i] = to_half_clamped(a[i]), h[4 + i] = to_half_clamped(b[i]);
-            }
-        } else {
-#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = to_half_clamped(a[i]), h[4 + i] = to_half_clamped(b[i]);
+        } else if (K & 7) {
             for (int i = 0; i < 8; ++i)
                 if (k + i < K) h[i] = to_half_clamped(p[i]);
         }
     } else {
+        typedef half8_t half8_any_t __attribute__((aligned(2)));
         const _Float16* p = static_cast<const _Float16*>(X) + row + k;
-        if (vec) {
-            if (k < K) h = *reinterpret_cast<const half8_t*>(p);
-        } else {
-#pragma unroll
+        if (k + 8 <= K) {
+            h = *reinterpret_cast<const half8_any_t*>(p);
+        } else if (K & 7) {
             for (int i = 0; i < 8; ++i)
                 if (k + i < K) h[i] = p[i];
         }
@@ -48,10 +47,34 @@ __device__ __forceinline__ half8_t load_x(const void* X, int64_t row, int k, int
     return h;
 }
 
-// MT x NT blocks of 16 x 16, WAVES waves that share K, SH: log2(group / 32).
+// Eight values of X as they come (16 bytes at any alignment are one load), and as binary16.
+template <bool X32>
+struct XRaw {
+    u32x4_t v[X32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* X, int64_t at) {
+        if constexpr (X32) {
+            typedef u32x4_t any_t __attribute__((aligned(4)));
+            const any_t* p = reinterpret_cast<const any_t*>(static_cast<const float*>(X) + at);
+            v[0] = p[0];
+            v[1] = p[1];
+        } else {
+            typedef u32x4_t any_t __attribute__((aligned(2)));
+            v[0] = *reinterpret_cast<const any_t*>(static_cast<const _Float16*>(X) + at);
+        }
+    }
+    __device__ __forceinline__ half8_t value() const {
+        if constexpr (!X32) return __builtin_bit_cast(half8_t, v[0]);
+        half8_t h;
+        const float4_t a = __builtin_bit_cast(float4_t, v[0]), b = __builtin_bit_cast(float4_t, v[X32 ? 1 : 0]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = to_half_clamped(a[i]), h[4 + i] = to_half_clamped(b[i]);
+        return h;
+    }
+};
+
+// MT x NT blocks of 16 x 16, WAVES waves that share K; shift: log2(group / 32).
 template <int MT, int NT, int WAVES, bool X32>
-__global__ void __launch_bounds__(64 * WAVES) w4_few_kernel(W4Args a, int shift, bool vec) {
-    constexpr int U = NT * MT >= 4 ? 2 : 4;  // steps whose loads are in flight together
+__global__ void __launch_bounds__(64 * WAVES) w4_few_kernel(W4Args a, int shift) {
     __shared__ __attribute__((aligned(16))) float part[WAVES * MT * NT * 256];
     const W4View& w = a.w;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -76,45 +99,91 @@ __global__ void __launch_bounds__(64 * WAVES) w4_few_kernel(W4Args a, int shift,
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-    const int steps = (K + 127) / 128, chunks = w.words / 4;
-    for (int s0 = wave; s0 < steps; s0 += WAVES * U) {
-        u32x4_t c[U][NT];
-        uint32_t p[U][NT];
+    // A wave's steps of 128 values lie together; the first waves have one more where they do not come out even, and the
+    // last one what is left of K.
+    const int steps = K / 128, each = steps / WAVES, rest = steps % WAVES;
+    const int first = wave * each + min(wave, rest), n = each + (wave < rest ? 1 : 0);
+    const FourBits expand;
+    struct Step {
+        u32x4_t c[NT];
+        uint32_t p[NT];
+        XRaw<X32> x[MT][4];
+    };
+    auto load = [&](Step& b, int step) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int step = s0 + u * WAVES, chunk = 4 * step + g;
-            const bool in = chunk < chunks;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                // (a pair of zeros: the value 0 whatever the codes)
-                c[u][j] = u32x4_t{0, 0, 0, 0};
-                p[u][j] = 0;
-                if (in) {
-                    c[u][j] = *reinterpret_cast<const u32x4_t*>(codes[j] + 16 * step);
-                    p[u][j] = sm[j][chunk >> shift];
-                }
-            }
+        for (int j = 0; j < NT; ++j) {
+            b.c[j] = *reinterpret_cast<const u32x4_t*>(codes[j] + 16 * step);
+            b.p[j] = sm[j][(4 * step + g) >> shift];
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int step = s0 + u * WAVES;
-            if (step >= steps) break;
-            half8_t x[MT][4];
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int q = 0; q < 4; ++q) b.x[i][q].load(a.X, row[i] + 128 * step + 32 * g + 8 * q);
+    };
+    auto multiply = [&](const Step& b) {
+        half8_t x[MT][4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) x[i][q] = load_x<X32>(a.X, row[i], 128 * step + 32 * g + 8 * q, K, vec);
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[i][q] = b.x[i][q].value();
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            half2_t s, m;
+            four_bit_pair(b.p[j], s, m);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const half8_t w = expand(b.c[j][q], s, m);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i][q], w, acc[i][j], 0, 0, 0);
+            }
+        }
+    };
+    // The next step is under way while one is multiplied (its loads without conditions, so that how many are under way
+    // is known where the first one's are waited for).
+    Step b0, b1;
+    if (n > 0) {
+        load(b0, first);
+        int t = 0;
+        for (; t + 2 < n; t += 2) {
+            load(b1, first + t + 1);
+            multiply(b0);
+            load(b0, first + t + 2);
+            multiply(b1);
+        }
+        if (t + 1 < n) {
+            load(b1, first + t + 1);
+            multiply(b0);
+            multiply(b1);
+        } else {
+            multiply(b0);
+        }
+    }
+    if (wave == WAVES - 1 && 128 * steps < K) {
+        const int chunk = 4 * steps + g;
+        Step b;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            // (a pair of zeros: the value 0 whatever the codes)
+            b.c[j] = u32x4_t{0, 0, 0, 0};
+            b.p[j] = 0;
+            if (32 * chunk < K) {
+                b.c[j] = *reinterpret_cast<const u32x4_t*>(codes[j] + 16 * steps);
+                b.p[j] = sm[j][chunk >> shift];
+            }
+        }
+        for (int q = 0; q < 4; ++q) {
+            half8_t x[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) x[i] = load_x<X32>(a.X, row[i], 32 * chunk + 8 * q, K);
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 half2_t s, m;
-                four_bit_pair(p[u][j], s, m);
+                four_bit_pair(b.p[j], s, m);
+                const uint32_t w = q == 0 ? b.c[j][0] : q == 1 ? b.c[j][1] : q == 2 ? b.c[j][2] : b.c[j][3];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const half8_t b = four_bit_values(c[u][j][q], s, m);
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i][q], b, acc[i][j], 0, 0, 0);
-                }
+                for (int i = 0; i < MT; ++i)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i], expand(w, s, m), acc[i][j], 0, 0, 0);
             }
         }
     }
@@ -143,34 +212,27 @@ __global__ void __launch_bounds__(64 * WAVES) w4_few_kernel(W4Args a, int shift,
     }
 }
 
-// A thread per 32 codes.
-__global__ void __launch_bounds__(256) w4_expand_kernel(W4View w, int n0, int64_t pieces, half8_t* out, int shift) {
-    const int chunks = w.words / 4;
-    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < pieces; at += (int64_t)gridDim.x * 256) {
-        const int n = (int)(at / chunks), c = (int)(at - (int64_t)n * chunks);
-        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(w.codes + (int64_t)(n0 + n) * w.words + 4 * c);
+// A thread per word.
+__global__ void __launch_bounds__(256) w4_expand_kernel(W4View w, int n0, int64_t words, half8_t* out, int shift) {
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < words; at += (int64_t)gridDim.x * 256) {
+        const int n = (int)(at / w.words), c = (int)(at - (int64_t)n * w.words);
         half2_t s, m;
-        four_bit_pair(w.sm[(int64_t)(n0 + n) * w.G + (c >> shift)], s, m);
+        four_bit_pair(w.sm[(int64_t)(n0 + n) * w.G + (min(c, (w.K - 1) >> 3) >> (shift + 2))], s, m);
+        half8_t v = four_bit_values(w.codes[(int64_t)(n0 + n) * w.words + c], s, m);
+        if (8 * c + 8 > w.K) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            half8_t v = four_bit_values(x[i], s, m);
-            const int k = 32 * c + 8 * i;
-            if (k + 8 > w.K) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (k + j >= w.K) v[j] = (_Float16)0.0f;
-            }
-            store_half8(out + at * 4 + i, v);
+            for (int j = 0; j < 8; ++j)
+                if (8 * c + j >= w.K) v[j] = (_Float16)0.0f;
         }
+        store_half8(out + at, v);
     }
 }
 
 template <bool X32>
-__global__ void __launch_bounds__(256) w4_rows_kernel(const void* X, int64_t ldx, int64_t M, int K, half8_t* out, int eights,
-                                                      bool vec) {
+__global__ void __launch_bounds__(256) w4_rows_kernel(const void* X, int64_t ldx, int64_t M, int K, half8_t* out, int eights) {
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < M * eights; at += (int64_t)gridDim.x * 256) {
         const int64_t m = at / eights;
-        store_half8(out + at, load_x<X32>(X, m * ldx, 8 * (int)(at - m * eights), K, vec));
+        store_half8(out + at, load_x<X32>(X, m * ldx, 8 * (int)(at - m * eights), K));
     }
 }
 
@@ -224,36 +286,50 @@ __global__ void __launch_bounds__(256) w4_unpack_kernel(W4View w, _Float16* out,
 int group_shift(int group) { return group == 32 ? 0 : group == 64 ? 1 : 2; }
 
 template <int MT, int NT, int WAVES>
-void few(const W4Args& a, hipStream_t s, bool vec) {
+void few(const W4Args& a, hipStream_t s) {
     const dim3 grid((unsigned)((a.w.N + 16 * NT - 1) / (16 * NT)), (unsigned)((a.M + kW4FewRows - 1) / kW4FewRows));
-    if (a.x32) w4_few_kernel<MT, NT, WAVES, true><<<grid, 64 * WAVES, 0, s>>>(a, group_shift(a.w.group), vec);
-    else w4_few_kernel<MT, NT, WAVES, false><<<grid, 64 * WAVES, 0, s>>>(a, group_shift(a.w.group), vec);
+    // (fp32 rows take twice the registers: four waves where 16 rows of binary16 do with half of a SIMD's)
+    constexpr int W32 = MT >= 2 ? 4 : WAVES;
+    if (a.x32) w4_few_kernel<MT, NT, W32, true><<<grid, 64 * W32, 0, s>>>(a, group_shift(a.w.group));
+    else w4_few_kernel<MT, NT, WAVES, false><<<grid, 64 * WAVES, 0, s>>>(a, group_shift(a.w.group));
 }
 
 }  // namespace
 
 hipError_t launch_w4_few(const W4Args& a, int cus, hipStream_t s) {
-    const int es = a.x32 ? 4 : 2;
-    const bool vec = a.w.K % 8 == 0 && (((uintptr_t)a.X | (uintptr_t)(a.ldx * es)) & 15) == 0;
-    if (a.M <= 16) few<1, 1, 8>(a, s, vec);
-    else if (a.M <= 32) few<2, 2, 8>(a, s, vec);
-    else few<4, 2, 8>(a, s, vec);
+    // Column blocks a wave: as many as leave a workgroup for every CU, so that X is not read more often than that
+    // needs (us with 1 / 2 / 4: 16 rows of 1024 into 4096 3.9 / 4.2 / 5.4, of 2048 into 8192 8.7 / 6.9 / 8.9, of 4096
+    // into 16384 25.5 / 18.5 / 15.8; 64 rows of 1024 into 4096 7.0 / 7.7 / 11.2, of 4096 into 16384 74 / 46 / 32).
+    const int64_t blocks = (a.w.N + 15) / 16;
+    const int nt = blocks >= 4 * cus ? 4 : blocks >= 2 * cus ? 2 : 1;
+    if (a.M <= 16) {
+        if (nt == 1) few<1, 1, 8>(a, s);
+        else if (nt == 2) few<1, 2, 8>(a, s);
+        else few<1, 4, 8>(a, s);
+    } else if (a.M <= 32) {
+        if (nt == 1) few<2, 1, 8>(a, s);
+        else if (nt == 2) few<2, 2, 8>(a, s);
+        else few<2, 4, 8>(a, s);
+    } else {
+        if (nt == 1) few<4, 1, 8>(a, s);
+        else if (nt == 2) few<4, 2, 4>(a, s);
+        else few<4, 4, 4>(a, s);
+    }
     return hipGetLastError();
 }
 
 hipError_t launch_w4_expand(const W4View& w, int n0, int n, _Float16* out, hipStream_t s) {
-    const int64_t pieces = (int64_t)n * (w.words / 4);
-    w4_expand_kernel<<<row_blocks((pieces + 255) / 256), 256, 0, s>>>(w, n0, pieces, reinterpret_cast<half8_t*>(out),
-                                                                      group_shift(w.group));
+    const int64_t words = (int64_t)n * w.words;
+    w4_expand_kernel<<<row_blocks((words + 255) / 256), 256, 0, s>>>(w, n0, words, reinterpret_cast<half8_t*>(out),
+                                                                     group_shift(w.group));
     return hipGetLastError();
 }
 
 hipError_t launch_w4_rows(const void* X, bool x32, int64_t ldx, int M, int K, _Float16* out, int64_t ld, hipStream_t s) {
     const int eights = (int)(ld / 8);
-    const bool vec = K % 8 == 0 && (((uintptr_t)X | (uintptr_t)(ldx * (x32 ? 4 : 2))) & 15) == 0;
     const unsigned blocks = row_blocks(((int64_t)M * eights + 255) / 256);
-    if (x32) w4_rows_kernel<true><<<blocks, 256, 0, s>>>(X, ldx, M, K, reinterpret_cast<half8_t*>(out), eights, vec);
-    else w4_rows_kernel<false><<<blocks, 256, 0, s>>>(X, ldx, M, K, reinterpret_cast<half8_t*>(out), eights, vec);
+    if (x32) w4_rows_kernel<true><<<blocks, 256, 0, s>>>(X, ldx, M, K, reinterpret_cast<half8_t*>(out), eights);
+    else w4_rows_kernel<false><<<blocks, 256, 0, s>>>(X, ldx, M, K, reinterpret_cast<half8_t*>(out), eights);
     return hipGetLastError();
 }
 

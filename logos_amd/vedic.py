@@ -1034,24 +1034,27 @@ def _kv(k, v, table, lens, q_start, tokens, dev) -> _lib.Kv:
                          f"{tuple(v.shape)}")
     pages, heads, ps, row = shape
     sp, sh, st, one = strides
-    if row > 1 and one != 1:
+    if one != 1 and row > 1:
         raise ValueError("a cache's rows must be contiguous")
-    i4 = dt == torch.uint8
+    i4 = dt is torch.uint8
     if i4 and row % 5 != 0:
         raise ValueError(f"a four-bit row has 5 dh / 8 bytes, got {row}")
-    p_table = _on_current(table, "table", torch.int32, dev)
-    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("table must be [sequences, pages], its rows contiguous")
+    pt, pl, pq = _on_current(table, "table", torch.int32, dev), _on_current(lens, "lens", torch.int32, dev), None
+    if table.dim() != 2:
+        raise ValueError("table must be [sequences, pages]")
     B, W = table.shape
-    ps_start = None
+    tb, tw = table.stride()
+    if tw != 1 and W > 1:
+        raise ValueError("table's rows must be contiguous")
+    if lens.dim() != 1 or lens.shape[0] != B or not lens.is_contiguous():
+        raise ValueError(f"lens must be contiguous int32 of shape ({B},), got {tuple(lens.shape)}")
     if q_start is not None:
-        ps_start = _ints(q_start, "q_start", (B + 1,), dev)
+        pq = _ints(q_start, "q_start", (B + 1,), dev)
     elif tokens != B:
         raise ValueError(f"{tokens} rows for {B} sequences: q_start tells which are whose")
     # (a dimension of one has any stride)
     return _lib.Kv(i4, pages, ps, heads, row * 8 // 5 if i4 else row, pk, pv, sp if pages > 1 else max(sp, row),
-                   sh if heads > 1 else max(sh, row), st if ps > 1 else max(st, row), p_table,
-                   table.stride(0) if B > 1 else W, W, _ints(lens, "lens", (B,), dev), ps_start, B, tokens)
+                   sh if heads > 1 else max(sh, row), st if ps > 1 else max(st, row), pt, tb if B > 1 else W, W, pl, pq, B, tokens)
 
 
 def _heads3d(t: torch.Tensor, name: str, dtype, dev: int) -> tuple[int, int, int, int, int, int]:
@@ -1093,10 +1096,12 @@ def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache:
         if (Tq, Dq) != (T, D):
             raise ValueError(f"q must be [{T}, q_heads, {D}], got {tuple(q.shape)}")
         if out is None:
-            out = torch.empty((T, Hq, D), dtype=torch.float16, device=q.device)
-        po, To, Ho, Do, ot, oh = _heads3d(out, "out", torch.float16, dev)
-        if (To, Ho, Do) != (T, Hq, D):
-            raise ValueError(f"out must be {T}x{Hq}x{D}")
+            out = q.new_empty((T, Hq, D), dtype=torch.float16)
+            po, ot, oh = out.data_ptr(), Hq * D, D
+        else:
+            po, To, Ho, Do, ot, oh = _heads3d(out, "out", torch.float16, dev)
+            if (To, Ho, Do) != (T, Hq, D):
+                raise ValueError(f"out must be {T}x{Hq}x{D}")
     pr, rows, dims = None, 0, 0
     if rope is not None:
         pr = _on_current(rope, "rope", torch.float32, dev)
