@@ -8,11 +8,12 @@
 // once more to binary16.  Rows of four bits: 32 values share (s, m) = (binary16((hi - lo) / 15), lo)
 // of their binary16 values, code = round((x - m) / s).
 //
-// A thread takes eight consecutive values of a row (16 bytes of binary16): it reads them,
-// their partners (cached: a neighbouring thread's own) and the angles, and writes 16 bytes, or
-// a word; the four threads of a group of 32 exchange its least and largest value by DPP.  A
-// workgroup takes 256 such eights of kTok tokens, whose loads are in flight together; the
-// sequence of a token is the count of q_start values up to it (a ballot per 64 sequences).
+// A thread takes eight consecutive values of a row: it reads them, their partners (a neighbouring
+// thread's own: cached) and the angles, and writes 16 bytes, or a word; the four threads of a group of 32
+// exchange its least and largest value by DPP.  Memory bounds it, and what comes before the angles can
+// be asked for: a workgroup has one token, so that many are at it (8192 tokens of 48 heads of 64 from fp32, cold
+// caches: 36 us, 4.3 TB/s; with four tokens a workgroup 46); the sequence of a token is the one whose rows it lies among
+// (a ballot per 64 sequences).
 #include "vedic_cache.hpp"
 
 namespace vedic {
@@ -23,32 +24,26 @@ constexpr int kThreads = 256;
 
 typedef float float8_t __attribute__((ext_vector_type(8)));
 
-// The sequence of new row t and its position (-1: none).
-template <int TOK>
-__device__ __forceinline__ void find_rows(const KvView& c, int t0, int lane, int (&seq)[TOK], int (&pos)[TOK]) {
+// The sequence of new row t and its position (-1: none).  A lane looks at a sequence's rows and length at once: all
+// comes from one round of loads.
+__device__ __forceinline__ void find_row(const KvView& c, int t, int lane, int& seq, int& pos) {
+    seq = 0;
+    pos = -1;
     if (c.q_start == nullptr) {
-#pragma unroll
-        for (int i = 0; i < TOK; ++i) seq[i] = t0 + i;
-    } else {
-#pragma unroll
-        for (int i = 0; i < TOK; ++i) seq[i] = -1;
-        for (int b0 = 0; b0 < c.B + 1; b0 += 64) {
-            const int b = b0 + lane;
-            const int start = b <= c.B ? c.q_start[b] : INT32_MAX;
-#pragma unroll
-            for (int i = 0; i < TOK; ++i) seq[i] += __popcll(__ballot(start <= t0 + i));
-        }
+        seq = t;
+        pos = __builtin_amdgcn_readfirstlane(c.len_of(t)) - 1;
+        return;
     }
-#pragma unroll
-    for (int i = 0; i < TOK; ++i) {
-        const int b = __builtin_amdgcn_readfirstlane(seq[i]), t = t0 + i;
-        seq[i] = b;
-        pos[i] = -1;
-        if (t >= c.T || b < 0 || b >= c.B) continue;
+    for (int b0 = 0; b0 < c.B; b0 += 64) {
+        const int b = min(b0 + lane, c.B - 1);
         int first, n;
         c.rows_of(b, first, n);
-        if (t < first || t >= first + n) continue;  // (a list that is not ascending)
-        pos[i] = c.len_of(b) - n + (t - first);
+        const int at = c.len_of(b) - n - first;  // the row's position less t
+        const uint64_t who = __ballot(b0 + lane < c.B && t >= first && t < first + n);
+        if (who == 0) continue;
+        seq = b0 + __builtin_ctzll(who);
+        pos = t + __builtin_amdgcn_readlane(at, __builtin_ctzll(who));
+        return;
     }
 }
 
@@ -177,61 +172,51 @@ __device__ __forceinline__ void store_row(char* row, bool i4, int D, int e0, con
     if ((e0 & 31) == 0) *reinterpret_cast<uint32_t*>(row + D / 2 + e0 / 8) = sm;
 }
 
-// Items of a token: (Hq + 2 H) rows of D / 8 eights.
-template <bool F32, int TOK>
+// A workgroup per token and 256 of its (Hq + 2 H) D / 8 eights.
+template <bool F32>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(KvAppendArgs a, int items, bool vec_in, bool vec_rot) {
     const KvView& c = a.c;
-    const int lane = threadIdx.x & 63;
-    const int t0 = blockIdx.x * TOK, item = blockIdx.y * kThreads + threadIdx.x;
+    const int t = blockIdx.x, item = blockIdx.y * kThreads + threadIdx.x;
     const int eights = c.D >> 3;
     const bool mine = item < items;
     const int head = mine ? item / eights : 0, e0 = mine ? 8 * (item - head * eights) : 0;
     const int kind = head < a.Hq ? 0 : head < a.Hq + c.H ? 1 : 2;
     const int hk = kind == 0 ? head : kind == 1 ? head - a.Hq : head - a.Hq - c.H;
     const void* src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    const int64_t st = kind == 0 ? a.q_token : kind == 1 ? a.k_token : a.v_token;
-    const int64_t base = hk * (kind == 0 ? a.q_head : kind == 1 ? a.k_head : a.v_head);
-    float x[TOK][8];
+    const int64_t row = hk * (kind == 0 ? a.q_head : kind == 1 ? a.k_head : a.v_head) +
+                        t * (kind == 0 ? a.q_token : kind == 1 ? a.k_token : a.v_token);
+    float x[8];
+    load8<F32>(src, row + e0, vec_in, x);
+    int seq, pos;
+    find_row(c, t, threadIdx.x & 63, seq, pos);
+    if (pos < 0) return;
+    const int tp = c.page_of(pos);
+    const int page = c.table[seq * c.ldt + tp];
+    if (kind < 2 && e0 < a.rot) {
+        const float* cs = a.rope + (int64_t)min(pos, a.rope_rows - 1) * a.rot;
+        if (vec_rot) rotate8<F32, true>(a, src, row, e0, cs, x);
+        else rotate8<F32, false>(a, src, row, e0, cs, x);
+    }
+    if (kind == 0) {
+        if (!mine) return;
+        half8_t h;
 #pragma unroll
-    for (int i = 0; i < TOK; ++i)
-        load8<F32>(src, base + (int64_t)min(t0 + i, c.T - 1) * st + e0, vec_in, x[i]);
-    int seq[TOK], pos[TOK];
-    find_rows<TOK>(c, t0, lane, seq, pos);
-#pragma unroll
-    for (int i = 0; i < TOK; ++i) {
-        if (pos[i] < 0) continue;  // (the same for the whole workgroup)
-        if (kind < 2 && e0 < a.rot) {
-            const float* cs = a.rope + (int64_t)min(pos[i], a.rope_rows - 1) * a.rot;
-            const int64_t row = base + (int64_t)(t0 + i) * st;
-            if (vec_rot) rotate8<F32, true>(a, src, row, e0, cs, x[i]);
-            else rotate8<F32, false>(a, src, row, e0, cs, x[i]);
-        }
-        const int tp = c.page_of(pos[i]);
-        const int page = c.table[seq[i] * c.ldt + tp];
-        const bool there = (unsigned)page < (unsigned)c.pages;
-        if (kind == 0) {
-            if (mine) {
-                half8_t h;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) h[j] = (_Float16)x[i][j];
-                store_half8(a.q_out + (t0 + i) * a.o_token + hk * a.o_head + e0, h);
-            }
-        } else {
-            char* row = (kind == 1 ? c.k : c.v) + (int64_t)page * c.page + (int64_t)hk * c.head +
-                        (int64_t)(pos[i] - tp * c.ps) * c.token;
-            store_row(row, a.i4, c.D, e0, x[i], mine && there);
-        }
+        for (int j = 0; j < 8; ++j) h[j] = (_Float16)x[j];
+        store_half8(a.q_out + t * a.o_token + hk * a.o_head + e0, h);
+    } else {
+        char* to = (kind == 1 ? c.k : c.v) + (int64_t)page * c.page + (int64_t)hk * c.head + (int64_t)(pos - tp * c.ps) * c.token;
+        store_row(to, a.i4, c.D, e0, x, mine && (unsigned)page < (unsigned)c.pages);
     }
 }
 
 // One thread per eight values of K and of V.
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvView c, bool i4, _Float16* k, _Float16* v, int items) {
     const int t = blockIdx.x, item = blockIdx.y * kThreads + threadIdx.x;
-    int seq[1], pos[1];
-    find_rows<1>(c, t, threadIdx.x & 63, seq, pos);
-    if (pos[0] < 0 || item >= items) return;
+    int seq, pos;
+    find_row(c, t, threadIdx.x & 63, seq, pos);
+    if (pos < 0 || item >= items) return;
     const int eights = c.D >> 3, head = item / eights, e0 = 8 * (item - head * eights);
-    const int64_t at = c.row_offset(seq[0], pos[0]) + (int64_t)head * c.head;
+    const int64_t at = c.row_offset(seq, pos) + (int64_t)head * c.head;
     const int64_t to = ((int64_t)t * c.H + head) * c.D + e0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -264,17 +249,9 @@ hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t s) {
     const bool vrot = vec && a.rot % 16 == 0 && aligned(a.rope, 0, 0, 16);
     const int items = (a.Hq + 2 * c.H) * (c.D / 8);
     const unsigned y = (unsigned)((items + kThreads - 1) / kThreads);
-    auto go = [&](auto kernel, int tok) {
-        kernel<<<dim3((unsigned)((c.T + tok - 1) / tok), y), kThreads, 0, s>>>(a, items, vec, vrot);
-    };
-    // (four tokens a workgroup where that leaves workgroups for every CU)
-    if ((int64_t)c.T * y >= 4096) {
-        if (a.f32) go(kv_append_kernel<true, 4>, 4);
-        else go(kv_append_kernel<false, 4>, 4);
-    } else {
-        if (a.f32) go(kv_append_kernel<true, 1>, 1);
-        else go(kv_append_kernel<false, 1>, 1);
-    }
+    const dim3 grid((unsigned)c.T, y);
+    if (a.f32) kv_append_kernel<true><<<grid, kThreads, 0, s>>>(a, items, vec, vrot);
+    else kv_append_kernel<false><<<grid, kThreads, 0, s>>>(a, items, vec, vrot);
     return hipGetLastError();
 }
 
