@@ -15,6 +15,18 @@ typedef uint32_t u32x4_a4_t __attribute__((ext_vector_type(4), aligned(4)));
 // Positions stay below this.
 constexpr int kMaxTokens = 1 << 30;
 
+// Quotients of numbers below 2^30: n / d = n * magic >> shift.
+struct Divider {
+    uint32_t magic;
+    int shift;
+    __device__ __forceinline__ int operator()(int n) const { return (int)((uint64_t)(uint32_t)n * magic >> shift); }
+};
+inline Divider divider(int d) {
+    int l = 0;
+    while ((int64_t(1) << l) < d) ++l;
+    return Divider{(uint32_t)((uint64_t(1) << (30 + l)) / d + 1), 30 + l};
+}
+
 struct KvView {
     char* k;
     char* v;
@@ -26,11 +38,9 @@ struct KvView {
     const int* lens;     // [B]
     const int* q_start;  // [B + 1], or null: row b is sequence b's only new one
     int B, T;
-    // pos / ps = pos * magic >> shift for pos < 2^30 (kv_divider)
-    uint32_t magic;
-    int shift;
+    Divider by_page;  // of positions by ps
 
-    __device__ __forceinline__ int page_of(int pos) const { return (int)((uint64_t)(uint32_t)pos * magic >> shift); }
+    __device__ __forceinline__ int page_of(int pos) const { return by_page(pos); }
     // Tokens of sequence b, as many as its pages can hold at most.
     __device__ __forceinline__ int len_of(int b) const {
         const int64_t cap = (int64_t)tcols * ps;
@@ -55,13 +65,6 @@ struct KvView {
         return p * page + (pos - t * ps) * token;
     }
 };
-
-inline void kv_divider(KvView& v) {
-    int l = 0;
-    while ((1 << l) < v.ps) ++l;
-    v.shift = 30 + l;
-    v.magic = (uint32_t)((uint64_t(1) << v.shift) / v.ps + 1);
-}
 
 // Four-bit words: 32 bits hold eight consecutive values, value 2 i in bits 4 i .. 4 i + 3 and
 // value 2 i + 1 in bits 16 + 4 i ..; code n of a group with the binary16 pair (s, m) stands
@@ -167,6 +170,7 @@ struct PagedArgs {
     float* lse;  // [T x Hq] or null
     int64_t q_token, q_head, o_token, o_head;  // strides in values
     int Hq, G;
+    Divider by_group, by_heads;  // of rows by G, of units by the key heads
     float scale;  // |scale| log2(e), > 0
     float sign;   // of the scale: q is multiplied by it
     int causal, window, stride;

@@ -1722,7 +1722,7 @@ static int kv_view(const vedic_kv_t* d, KvView& v, bool& some) {
     v.q_start = d->q_start;
     v.B = d->batch;
     v.T = d->tokens;
-    kv_divider(v);
+    v.by_page = divider(d->page_size);
     return VEDIC_STATUS_OK;
 }
 
@@ -1808,6 +1808,8 @@ extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_
         return VEDIC_STATUS_BAD_DIM;
     if (q_heads >= (1 << 16) || (int64_t)kv->tokens * q_heads >= kMaxCount) return VEDIC_STATUS_TOO_LARGE;
     a.G = q_heads / kv->heads;
+    a.by_group = divider(a.G);
+    a.by_heads = divider(kv->heads);
     const int64_t rows = (int64_t)kv->tokens * a.G;
     const int64_t tiles = (rows / kFewRows + (kv->batch < kv->tokens ? kv->batch : kv->tokens)) * kv->heads;
     if (tiles + 4096 >= (1 << 24)) return VEDIC_STATUS_TOO_LARGE;
@@ -1847,6 +1849,8 @@ extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_
         b.target = paged_target(kind != 0, cus);
         // (where no sequence can have two parts)
         if ((int64_t)kv->table_cols * kv->page_size <= (kind ? kManyUnit : kFewUnit)) b.target = 0;
+        // (of sequences with two parts and more: a part is longer than 1 / target of all keys, and they have fewer than
+        // twice as many as of their lengths over that)
         const size_t slots = 2 * (size_t)b.target, bytes = slots * tile * (kv->dh + 2) * 4;
         if (!ws.room(bytes)) b.target = 0;
         float* part = nullptr;

@@ -30,6 +30,7 @@ __device__ __forceinline__ float both_halves_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
     return __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
 }
+
 struct PagedItem {
     int b, tile, h;       // sequence, tile of its rows, key head
     int first, n, len;    // its new rows and its tokens
@@ -56,83 +57,109 @@ __device__ __forceinline__ int key_at(const PagedArgs& a, const PagedItem& it, i
     return place < it.near ? min(place, it.far - 1) * a.stride : it.base + place - it.near;
 }
 
-// Tiles of sequence b, and the longest list of keys among them (the last one's, or near it).
+// A sequence's new rows and tokens, its tiles, and the longest list of keys among them (the last one's, or near it).
+struct SequenceWork {
+    int first, n, len, tiles, span;
+};
 template <int ROWS, bool MANY>
-__device__ __forceinline__ void sequence_work(const PagedArgs& a, int b, int& tiles, int& span) {
-    tiles = span = 0;
-    if (b >= a.c.B) return;
-    int first, n;
-    a.c.rows_of(b, first, n);
-    const int64_t rows = (int64_t)n * a.G;
-    if (n == 0 || (rows > a.few_most) != MANY) return;
-    tiles = (int)((rows + ROWS - 1) / ROWS);
+__device__ __forceinline__ SequenceWork sequence_work(const PagedArgs& a, int b) {
+    SequenceWork w{0, 0, 0, 0, 0};
+    if (b >= a.c.B) return w;
+    a.c.rows_of(b, w.first, w.n);
+    w.len = a.c.len_of(b);
+    const int rows = w.n * a.G;  // (below 2^30)
+    if (w.n == 0 || (rows > a.few_most) != MANY) return w;
+    w.tiles = (rows + ROWS - 1) / ROWS;
     int base, far, near;
-    span = tile_keys(a, a.c.len_of(b), n, (tiles - 1) * ROWS / a.G, n - 1, base, far, near);
+    w.span = tile_keys(a, w.len, w.n, a.by_group((w.tiles - 1) * ROWS), w.n - 1, base, far, near);
+    return w;
 }
 
-__device__ __forceinline__ int parts_of(int span, int chunk) { return span > chunk ? (span + chunk - 1) / chunk : 1; }
-
-// Keys of a part: at least UNIT, in whole UNITs.
-template <int ROWS, bool MANY, int UNIT>
-__device__ __forceinline__ int part_length(const PagedArgs& a, int lane) {
-    if (a.target <= 0) return INT32_MAX;
-    int64_t total = 0;
-    for (int b0 = 0; b0 < a.c.B; b0 += 64) {
-        int tiles, span;
-        sequence_work<ROWS, MANY>(a, b0 + lane, tiles, span);
-        total += (int64_t)tiles * span;
-    }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d);
-    const int64_t each = (total * a.c.H + a.target - 1) / a.target;
-    return each >= (int64_t)INT32_MAX - UNIT ? INT32_MAX : max(1, (int)((each + UNIT - 1) / UNIT)) * UNIT;
+// Sums over the lanes up to each (DPP: shifts within rows of 16, then the rows' last lanes).
+template <int CTRL, int ROWS_OF>
+__device__ __forceinline__ int dpp_or_0(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS_OF, 0xF, true); }
+__device__ __forceinline__ int lane_sums(int v) {
+    v += dpp_or_0<0x111, 0xF>(v);
+    v += dpp_or_0<0x112, 0xF>(v);
+    v += dpp_or_0<0x114, 0xF>(v);
+    v += dpp_or_0<0x118, 0xF>(v);
+    v += dpp_or_0<0x142, 0xA>(v);
+    return v + dpp_or_0<0x143, 0xC>(v);
+}
+template <int CTRL, int ROWS_OF>
+__device__ __forceinline__ float dpp_or_0(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS_OF, 0xF, true));
+}
+__device__ __forceinline__ float wave_total(float v) {
+    v += dpp_or_0<0x111, 0xF>(v);
+    v += dpp_or_0<0x112, 0xF>(v);
+    v += dpp_or_0<0x114, 0xF>(v);
+    v += dpp_or_0<0x118, 0xF>(v);
+    v += dpp_or_0<0x142, 0xA>(v);
+    v += dpp_or_0<0x143, 0xC>(v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// The item (JOIN: the split tile) number id; false if there is none.
+// a / b for a below 2^24, b > 0.
+__device__ __forceinline__ int small_quotient(int a, int b) {
+    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+    if ((int64_t)q * b > a) --q;
+    if ((int64_t)(q + 1) * b <= a) ++q;
+    return q;
+}
+
+// The item (JOIN: the split tile) number id; false if there is none.  A part has at least UNIT keys, in whole UNITs.
 template <int ROWS, bool MANY, int UNIT, bool JOIN>
 __device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, PagedItem& it) {
-    const int chunk = part_length<ROWS, MANY, UNIT>(a, lane);
+    SequenceWork w = sequence_work<ROWS, MANY>(a, lane);
+    int chunk = INT32_MAX;
+    if (a.target > 0) {
+        float total = (float)w.tiles * (float)w.span;
+        for (int b0 = 64; b0 < a.c.B; b0 += 64) {
+            const SequenceWork x = sequence_work<ROWS, MANY>(a, b0 + lane);
+            total += (float)x.tiles * (float)x.span;
+        }
+        // (rounded up by more than the sums' and products' roundings: no more items than there are slots for)
+        const float each = wave_total(total) * (float)a.c.H / (float)a.target * 1.0001f + 1.0f;
+        if (each < 1e9f) chunk = ((int)each + UNIT - 1) / UNIT * UNIT;
+    }
     int before = 0, slots = 0;  // items (JOIN: tiles) and split items of the sequences before
     for (int b0 = 0; b0 < a.c.B; b0 += 64) {
-        int tiles, span;
-        sequence_work<ROWS, MANY>(a, b0 + lane, tiles, span);
-        const int parts = parts_of(span, chunk);
+        if (b0 > 0) w = sequence_work<ROWS, MANY>(a, b0 + lane);
+        const int parts = w.span > chunk ? (int)(((int64_t)w.span + chunk - 1) / chunk) : 1;
         // (sums of a list that is not ascending stay in range too)
-        const int items = (int)min((int64_t)tiles * a.c.H * parts, int64_t(1) << 24);
-        const int units = !JOIN ? items : parts > 1 ? (int)min((int64_t)tiles * a.c.H, int64_t(1) << 24) : 0;
+        const int tiles = (int)min((int64_t)w.tiles * a.c.H, int64_t(1) << 24), items = (int)min((int64_t)tiles * parts, int64_t(1) << 24);
+        const int units = !JOIN ? items : parts > 1 ? tiles : 0;
         const int split = parts > 1 ? items : 0;
-        int incl = units, sincl = split;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(incl, d), p = __shfl_up(sincl, d);
-            if (lane >= d) incl += o, sincl += p;
-        }
+        const int incl = lane_sums(units), sincl = lane_sums(split);
         const uint64_t past = __ballot(id - before < incl);
         if (past) {
             const int who = __builtin_ctzll(past);
             it.b = b0 + who;
             const int at = id - before - (__builtin_amdgcn_readlane(incl, who) - __builtin_amdgcn_readlane(units, who));
             it.parts = __builtin_amdgcn_readlane(parts, who);
-            const int unit = JOIN ? at : at / it.parts;  // tile * H + head
+            const int unit = JOIN || it.parts == 1 ? at : __builtin_amdgcn_readfirstlane(small_quotient(at, it.parts));
             it.part = JOIN ? 0 : at - unit * it.parts;
             const int s0 = slots + __builtin_amdgcn_readlane(sincl, who) - __builtin_amdgcn_readlane(split, who);
             it.slot = s0 + unit * it.parts + it.part;
-            const int ntiles = __builtin_amdgcn_readlane(tiles, who);
             // (a prompt's last rows, which see the most keys, begin first, over all heads)
-            const int tile = unit / a.c.H;
+            const int tile = a.by_heads(unit);
             it.h = unit - tile * a.c.H;
-            it.tile = ntiles - 1 - tile;
-            a.c.rows_of(it.b, it.first, it.n);
-            it.first = __builtin_amdgcn_readfirstlane(it.first);
-            it.n = __builtin_amdgcn_readfirstlane(it.n);
-            it.len = __builtin_amdgcn_readfirstlane(a.c.len_of(it.b));
-            const int i0 = it.tile * ROWS / a.G, i1 = min(it.n - 1, (it.tile * ROWS + ROWS - 1) / a.G);
+            it.tile = __builtin_amdgcn_readlane(w.tiles, who) - 1 - tile;
+            it.first = __builtin_amdgcn_readlane(w.first, who);
+            it.n = __builtin_amdgcn_readlane(w.n, who);
+            it.len = __builtin_amdgcn_readlane(w.len, who);
+            const int i0 = a.by_group(it.tile * ROWS), i1 = min(it.n - 1, a.by_group(it.tile * ROWS + ROWS - 1));
             const int end = tile_keys(a, it.len, it.n, i0, i1, it.base, it.far, it.near);
-            const int sp = __builtin_amdgcn_readlane(span, who);
-            const int each = ((sp + it.parts - 1) / it.parts + UNIT - 1) / UNIT * UNIT;
-            const int64_t p0 = (int64_t)it.part * each;
-            it.lo = (int)min(p0, (int64_t)end);
-            it.hi = it.part == it.parts - 1 ? end : (int)min(p0 + each, (int64_t)end);
+            it.lo = 0;
+            it.hi = end;
+            if (it.parts > 1) {
+                const int sp = __builtin_amdgcn_readlane(w.span, who);
+                const int each = ((sp + it.parts - 1) / it.parts + UNIT - 1) / UNIT * UNIT;
+                const int64_t p0 = (int64_t)it.part * each;
+                it.lo = (int)min(p0, (int64_t)end);
+                if (it.part < it.parts - 1) it.hi = (int)min(p0 + each, (int64_t)end);
+            }
             return JOIN || it.parts == 1 || it.slot < a.slots;  // (at most 2 target of them: vedic_capi.hip)
         }
         before += __builtin_amdgcn_readlane(incl, 63);
@@ -230,7 +257,7 @@ template <int DP, bool I4>
 __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem& it, int base, int64_t s0,
                                             const float16_t (&acc)[DP / 32], float m, float l, int lane) {
     constexpr int DT = DP / 32;
-    const int r = lane & 31, h = lane >> 5, rho = base + r, i = rho / a.G;
+    const int r = lane & 31, h = lane >> 5, rho = base + r, i = a.by_group(rho);
     const bool mine = i < it.n;
     const int64_t tok = it.first + i;
     const int head = it.h * a.G + rho - i * a.G;
@@ -276,7 +303,7 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
     while (bad) {
         const int w = __builtin_ctzll(bad);
         bad &= bad - 1;
-        const int brho = base + w, bi = brho / a.G, bh = it.h * a.G + brho - bi * a.G;
+        const int brho = base + w, bi = a.by_group(brho), bh = it.h * a.G + brho - bi * a.G;
         const int64_t bt = it.first + bi;
         float ov[DP / 64], bm, bl;
         slow_row<DP, I4>(a, it, it.len - it.n + bi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
@@ -313,7 +340,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
     const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // of a share
     const int share = lane / lanes, shares = 64 / lanes, c = lane % lanes;
     for (int r = blockIdx.y * per + wave; r < (int)(blockIdx.y + 1) * per; r += 4) {
-        const int rho = it.tile * ROWS + r, i = rho / a.G;
+        const int rho = it.tile * ROWS + r, i = a.by_group(rho);
         if (i >= it.n) return;
         const int64_t s0 = (int64_t)it.slot * ROWS + r;
         float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -357,7 +384,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
                 o[j] = o[j] * g + oo * go;
             }
         }
-        const int head = it.h * a.G + rho % a.G;
+        const int head = it.h * a.G + rho - i * a.G;
         const int64_t t = it.first + i;
         if (share == 0 && c < cols) {
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;

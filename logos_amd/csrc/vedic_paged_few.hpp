@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
     char* vb = lds + wave * (32 * PITCH);
 
     // this lane's row of Q
-    const int rho = it.tile * kFewRows + r, i = rho / a.G;
+    const int rho = it.tile * kFewRows + r, i = a.by_group(rho);
     const bool mine = i < it.n;
     const int pos = mine ? it.len - it.n + i : -1;
     const typename Share::Place where(c.D, g);
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
     // keys [klo, khi) of this row, and of all rows of the tile
     const int khi = !mine ? 0 : a.causal ? pos + 1 : it.len;
     const int klo = a.window > 0 ? pos - a.window : INT32_MIN;
-    const int i0 = it.tile * kFewRows / a.G, i1 = min(it.n - 1, (it.tile * kFewRows + kFewRows - 1) / a.G);
+    const int i0 = a.by_group(it.tile * kFewRows), i1 = min(it.n - 1, a.by_group(it.tile * kFewRows + kFewRows - 1));
     const int khi_all = a.causal ? it.len - it.n + i0 + 1 : it.len;
     const int klo_all = a.window > 0 ? it.len - it.n + i1 - a.window : INT32_MIN;
 
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
     for (int d = 0; d < DT; ++d) *reinterpret_cast<float4_t*>(po + r * OP + 16 * d + 4 * g) = acc[d];
     __syncthreads();
     const int row = threadIdx.x >> 4, col = 4 * (threadIdx.x & 15);
-    const int rrho = it.tile * kFewRows + row, ri = rrho / a.G;
+    const int rrho = it.tile * kFewRows + row, ri = a.by_group(rrho);
     float M = kNoScore, L = 0.0f, fw[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) M = __builtin_fmaxf(M, ml[w][row][0]);
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
     const uint64_t bad = __ballot(here && !fine);
     for (int w = 0; w < 4; ++w) {
         if (((bad >> (16 * w)) & 0xFFFF) == 0) continue;  // row 4 wave + w
-        const int brho = it.tile * kFewRows + 4 * wave + w, bi = brho / a.G, bh = it.h * a.G + brho - bi * a.G;
+        const int brho = it.tile * kFewRows + 4 * wave + w, bi = a.by_group(brho), bh = it.h * a.G + brho - bi * a.G;
         const int64_t bt = it.first + bi;
         float ov[DP / 64], bm, bl;
         slow_row<DP, I4>(a, it, it.len - it.n + bi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,

@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
     const int r = lane & 31, h = lane >> 5;
 
     const int base = it.tile * kManyRows + 32 * wave;  // the wave's first row
-    const int rho = base + r, i = rho / a.G;
+    const int rho = base + r, i = a.by_group(rho);
     const bool mine = i < it.n;
     const int pos = mine ? it.len - it.n + i : -1;
     const int64_t tok = it.first + (mine ? i : 0);
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
     const int khi = !mine ? 0 : a.causal ? pos + 1 : it.len;
     const int klo = a.window > 0 ? pos - a.window : INT32_MIN;
     // of the wave's rows: all see the keys [klo_all, khi_all)
-    const int p0 = it.len - it.n + base / a.G, p1 = it.len - it.n + min(it.n - 1, (base + 31) / a.G);
+    const int p0 = it.len - it.n + a.by_group(base), p1 = it.len - it.n + min(it.n - 1, a.by_group(base + 31));
     const int khi_all = base + 32 > (int64_t)it.n * a.G ? 0 : a.causal ? p0 + 1 : it.len;
     const int klo_all = a.window > 0 ? p1 - a.window : INT32_MIN;
 
