@@ -328,18 +328,29 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
     }
 }
 
-// The parts of a tile joined, `per` of its rows a workgroup: a wave per row, its lanes D / 4 columns of
-// four and the rest shares of the parts.
+// Sums o, l relative to a maximum m, and others' o2, l2, m2, as one.
+__device__ __forceinline__ void join_sums(float4_t& o, float& m, float& l, float4_t o2, float m2, float l2) {
+    const float top = __builtin_fmaxf(m, m2), mu = top == kNoScore ? 0.0f : top;
+    const float f = exp2_fast(m - mu), f2 = exp2_fast(m2 - mu);
+    m = top;
+    l = l * f + l2 * f2;
+    o = o * f + o2 * f2;
+}
+
+// The parts of a tile joined.  A lane has four columns of a row's share of the parts: D / 4 lanes a share, a wave's
+// shares of one row (MANY: `per` rows a workgroup, a wave each in turn), or a workgroup's.
 template <int ROWS, bool MANY, int UNIT>
 __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
+    __shared__ float4_t wave_o[MANY ? 1 : 4][64];
+    __shared__ float wave_ml[MANY ? 1 : 4][2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     PagedItem it;
     if (!find_item<ROWS, MANY, UNIT, true>(a, blockIdx.x, lane, it)) return;
     if ((int64_t)it.slot + it.parts > a.slots) return;
     const int D = a.c.D, cols = D / 4;
     const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // of a share
-    const int share = lane / lanes, shares = 64 / lanes, c = lane % lanes;
-    for (int r = blockIdx.y * per + wave; r < (int)(blockIdx.y + 1) * per; r += 4) {
+    const int shares = (MANY ? 1 : 4) * (64 / lanes), share = (MANY ? 0 : wave * (64 / lanes)) + lane / lanes, c = lane % lanes;
+    for (int r = blockIdx.y * per + (MANY ? wave : 0); r < (int)(blockIdx.y + 1) * per; r += MANY ? 4 : 1) {
         const int rho = it.tile * ROWS + r, i = a.by_group(rho);
         if (i >= it.n) return;
         const int64_t s0 = (int64_t)it.slot * ROWS + r;
@@ -373,20 +384,21 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
             }
         }
         for (int d = lanes; d < 64; d <<= 1) {
-            const float other = __shfl_xor(M, d), top = __builtin_fmaxf(M, other), mu = top == kNoScore ? 0.0f : top;
-            const float g = exp2_fast(M - mu), go = exp2_fast(other - mu);
-            M = top;
-            const float lo = __shfl_xor(l, d);
-            l = l * g + lo * go;
+            const float4_t oo = {__shfl_xor(o[0], d), __shfl_xor(o[1], d), __shfl_xor(o[2], d), __shfl_xor(o[3], d)};
+            join_sums(o, M, l, oo, __shfl_xor(M, d), __shfl_xor(l, d));
+        }
+        if constexpr (!MANY) {
+            wave_o[wave][lane] = o;
+            wave_ml[wave][0] = M;
+            wave_ml[wave][1] = l;
+            __syncthreads();
+            if (wave > 0) return;  // (per is 1)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float oo = __shfl_xor(o[j], d);
-                o[j] = o[j] * g + oo * go;
-            }
+            for (int x = 1; x < 4; ++x) join_sums(o, M, l, wave_o[x][lane], wave_ml[x][0], wave_ml[x][1]);
         }
         const int head = it.h * a.G + rho - i * a.G;
         const int64_t t = it.first + i;
-        if (share == 0 && c < cols) {
+        if (lane < lanes && c < cols) {
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
             const paged_half4_t v = {(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
             *reinterpret_cast<paged_half4_t*>(a.out + t * a.o_token + (int64_t)head * a.o_head + 4 * c) = v;

@@ -386,8 +386,8 @@ hipError_t paged_few(const PagedArgs& a, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.target > 0) {
         const int rows = a.c.q_start == nullptr && a.G < kFewRows ? a.G : kFewRows;
-        paged_join_kernel<kFewRows, false, kFewUnit><<<dim3((unsigned)(tiles < a.target ? tiles : a.target), (unsigned)(rows + 3) / 4), 256, 0,
-                                                          s>>>(a, 4);
+        const dim3 join((unsigned)(tiles < a.target ? tiles : a.target), (unsigned)rows);
+        paged_join_kernel<kFewRows, false, kFewUnit><<<join, 256, 0, s>>>(a, 1);
         e = hipGetLastError();
     }
     return e;
