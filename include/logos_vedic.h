@@ -657,7 +657,7 @@ typedef struct {
 /* New tokens into the cache: k and v [tokens x heads x dh], F32 or F16 at any strides (in values),
  * k turned by its position, both rounded to binary16 (nearest even) and stored in the cache's
  * format; and, with q_heads > 0, q [tokens x q_heads x dh] turned and rounded into q_out (which
- * is not q).  Rotation (rope_dims > 0, even): pairs (x_i, x_(i + rope_dims / 2)) of a row, or
+ * overlaps none of q, k and v).  Rotation (rope_dims > 0, even): pairs (x_i, x_(i + rope_dims / 2)) of a row, or
  * (x_2i, x_(2i + 1)) with interleaved, by the angle of row `position` (the last one past the
  * end) of rope [rope_rows x rope_dims]: rope_dims / 2 cosines, then the sines, fp32:
  *     (a, b) -> (a cos - b sin, b cos + a sin),  each product and sum rounded to fp32.
@@ -679,7 +679,7 @@ int vedic_kv_read(const vedic_kv_t* kv, void* k, void* v, void* stream);
  * with stride > 0, also t a multiple of stride -- the masks of vedic_flash_attention_fwd:
  *     out = sum over t of e^(scale q.k_t - M) v_t / sum of the same without v_t,
  * 0 for a row that sees no key.  lse (NULL, or [tokens x q_heads]): ln of sum e^(scale q.k_t), +inf for
- * such a row.  out binary16, rounded once; scores and sums fp32, weights binary16 relative to
+ * such a row.  out (which does not overlap q) binary16, rounded once; scores and sums fp32, weights binary16 relative to
  * their largest.  What a masked key or a page's unused row holds, NaN included, does not
  * reach the output.  Rows of no sequence are left as they are.
  * Sequences of up to 64 rows (n_b x q_heads / heads) share out their keys evenly over the GPU,
@@ -710,10 +710,11 @@ int vedic_w4_unpack(const vedic_w4_t* w, void* W16, int64_t ldw, void* stream);
 
 /* C[M x N] = epi(X[M x K] . W): X F16, or F32 clamped and rounded to binary16 as it is read; products of
  * binary16 values summed in fp32; C F32 or F16.  Epilogues NONE, BIAS, BIAS_GELU, and (F32 C)
- * RESIDUAL, BIAS_RESIDUAL.  Up to 64 rows read the codes themselves; more rows expand W into the
- * stream's workspace block first, in slabs of columns of up to 64 MiB (and copy an X that is F32
- * or whose rows are not whole 16 bytes), and run the binary16 tiles; a captured call without such a block takes
- * 64 rows at a time (results may then differ in rounding). */
+ * RESIDUAL, BIAS_RESIDUAL.  Up to 192 rows, and more where 64 rows x 16 columns make no more
+ * workgroups than CUs, read the codes themselves; others expand W into the stream's workspace
+ * block first, in slabs of columns of up to 64 MiB (and copy an X that is F32 or whose rows are
+ * not whole 16 bytes), and run the binary16 tiles; a captured call without such a block reads the codes
+ * (results may then differ in rounding). */
 int vedic_gemm_w4(const vedic_w4_t* w, const void* X, int x_dtype, int64_t ldx, int M, void* C, int c_dtype, int64_t ldc,
                   const float* bias, int epilogue, void* stream);
 

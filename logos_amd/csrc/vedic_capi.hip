@@ -1815,7 +1815,7 @@ extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_
     if (tiles + 4096 >= (1 << 24)) return VEDIC_STATUS_TOO_LARGE;
     if (!some) return VEDIC_STATUS_OK;
     if (!q || !out) return VEDIC_STATUS_NULL_POINTER;
-    if (!half_rows(q, q_token, q_head) || !half_rows(out, out_token, out_head) || q_token < 0 || q_head < 0 ||
+    if (!half_rows(q, q_token, q_head) || !half_rows(out, out_token, out_head) || q_token < 0 || q_head < 0 || out == q ||
         (kv->tokens > 1 && out_token < kv->dh) || (q_heads > 1 && out_head < kv->dh))
         return VEDIC_STATUS_BAD_LD;
     a.q = static_cast<const _Float16*>(q);
