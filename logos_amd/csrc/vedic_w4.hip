@@ -180,10 +180,14 @@ __global__ void __launch_bounds__(64 * WAVES) w4_few_kernel(W4Args a, int shift)
             for (int j = 0; j < NT; ++j) {
                 half2_t s, m;
                 four_bit_pair(b.p[j], s, m);
-                const uint32_t w = q == 0 ? b.c[j][0] : q == 1 ? b.c[j][1] : q == 2 ? b.c[j][2] : b.c[j][3];
+                half8_t w = expand(q == 0 ? b.c[j][0] : q == 1 ? b.c[j][1] : q == 2 ? b.c[j][2] : b.c[j][3], s, m);
+                // (codes from K on may be any: an infinity times the row's zero would count)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (32 * chunk + 8 * q + e >= K) w[e] = (_Float16)0.0f;
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i], expand(w, s, m), acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i], w, acc[i][j], 0, 0, 0);
             }
         }
     }

@@ -143,3 +143,18 @@ def test_captured():
                 del g
                 vedic._lib.load().vedic_workspace_release(s.cuda_stream)
             torch.cuda.synchronize()
+
+
+def test_codes_behind_the_last_value():
+    """Codes behind K may be any; with their column's scale they overflow binary16 here, and do not count."""
+    for M, N in ((1, 32), (40, 32), (300, 1000)):
+        K, rng = 40, np.random.default_rng(M)
+        n = rng.integers(0, 10, (N, 64)).astype(np.uint32)
+        n[:, K:] = 15
+        s, m = np.full((N, 2), 6000, np.float16), np.zeros((N, 2), np.float16)
+        v = plain.values(n.reshape(N, 2, 32), s, m).reshape(N, -1)[:, :K].T
+        w = vedic.W4(torch.from_numpy(plain.words(n).view(np.int32)).cuda(), torch.from_numpy(np.stack([s, m], -1)).cuda(), K, 32)
+        x = rng.standard_normal((M, K)).astype(np.float16)
+        got = vedic.gemm_w4(torch.from_numpy(x).cuda(), w).double().cpu().numpy()
+        x64, v64 = x.astype(np.float64), v.astype(np.float64)
+        assert (np.abs(got - x64 @ v64) <= K * 2.0 ** -24 * (np.abs(x64) @ np.abs(v64))).all()
