@@ -1913,6 +1913,14 @@ extern "C" int vedic_w4_unpack(const vedic_w4_t* d, void* W16, int64_t ldw, void
 static bool w4_direct(int M, int N, int cus) {
     return M <= 192 || (int64_t)((M + kW4FewRows - 1) / kW4FewRows) * ((N + 15) / 16) <= cus;
 }
+// Otherwise whether tiles expand the codes as they go, or the codes are expanded once for the binary16 tiles: those
+// are 5 to 10 % faster, share a long K among workgroups where tiles are few, and cost N K 4.5 bytes and two launches first
+// (us, tiles / expanded first: 2048 rows of 1024 into 4096 28.0 / 36.9, 1024 of 4096 into 16384 151 / 188, 2048 298 / 298, 8192
+// 1163 / 1100; 1024 of 1024 into 1024 15.4 / 23.9, of 4096 into 1024 40 / 27, 8192 75 / 86).
+static bool w4_tiled(int M, int K, int N, int cus) {
+    const bool filled = (int64_t)((M + 127) / 128) * ((N + 127) / 128) >= cus;
+    return (filled || K <= 2048) && (M <= 2048 || (int64_t)N * K <= (1 << 23));
+}
 // Expanded columns at a time (bytes).
 static constexpr size_t kW4Slab = size_t(64) << 20;
 
@@ -1946,18 +1954,30 @@ extern "C" int vedic_gemm_w4(const vedic_w4_t* d, const void* X, int x_dtype, in
     a.residual = resid;
     Workspace ws;
     ws.s = static_cast<hipStream_t>(stream);
-    if (!w4_direct(M, d->N, device_cu_count())) {
+    const int cus = device_cu_count();
+    if (!w4_direct(M, d->N, cus)) {
         const int64_t kp = (int64_t)a.w.words * 8;
-        const bool rows = a.x32 || d->K % 8 != 0 || !aligned16(X) || ldx % 8 != 0;
+        const bool rows = a.x32 || d->K % 8 != 0 || !aligned16(X) || ldx % 8 != 0, tiled = w4_tiled(M, d->K, d->N, cus);
         int64_t cols = (int64_t)(kW4Slab / (kp * 2)) / 256 * 256;
         if (cols < 256) cols = 256;
         if (cols > d->N) cols = d->N;
-        const size_t wb = (size_t)cols * kp * 2, xb = rows ? (size_t)M * kp * 2 : 0;
-        if (ws.room(Workspace::rounded(wb) + Workspace::rounded(xb))) {
+        const size_t wb = tiled ? 0 : (size_t)cols * kp * 2, xb = rows ? (size_t)M * kp * 2 : 0;
+        if (wb + xb == 0 || ws.room(Workspace::rounded(wb) + Workspace::rounded(xb))) {
             _Float16 *w16 = nullptr, *x16 = nullptr;
-            hipError_t e = ws.get(&w16, wb);
+            hipError_t e = hipSuccess;
+            if (wb) e = ws.get(&w16, wb);
             if (e == hipSuccess && rows) e = ws.get(&x16, xb);
             if (e == hipSuccess && rows) e = launch_w4_rows(X, a.x32, ldx, M, d->K, x16, kp, ws.s);
+            if (tiled) {
+                if (rows) {
+                    a.X = x16;
+                    a.ldx = kp;
+                    a.x32 = false;
+                }
+                if (e == hipSuccess) e = launch_w4_tile(a, cus, ws.s);
+                const hipError_t f = ws.put(x16);
+                return hip_status(e != hipSuccess ? e : f);
+            }
             int status = VEDIC_STATUS_OK;
             for (int64_t n0 = 0; n0 < d->N && e == hipSuccess && status == VEDIC_STATUS_OK; n0 += cols) {
                 const int n = (int)(d->N - n0 < cols ? d->N - n0 : cols);
@@ -1987,7 +2007,7 @@ extern "C" int vedic_gemm_w4(const vedic_w4_t* d, const void* X, int x_dtype, in
             return hip_status(e != hipSuccess ? e : f != hipSuccess ? f : h);
         }
     }
-    return hip_status(launch_w4_few(a, device_cu_count(), ws.s));
+    return hip_status(launch_w4_few(a, cus, ws.s));
 }
 
 // ----------------------------------------------------------- elementwise

@@ -28,6 +28,8 @@ struct W4Args {
 };
 constexpr int kW4FewRows = 64;  // rows of a workgroup of the few-row kernel
 hipError_t launch_w4_few(const W4Args& a, int cus, hipStream_t s);
+// Many rows: X binary16 in whole 16 bytes (K and ldx multiples of 8, aligned).
+hipError_t launch_w4_tile(const W4Args& a, int cus, hipStream_t s);
 // Binary16 rows n0 .. n0 + n - 1 of the transposed weight, [n x 8 words], zeros from K on.
 hipError_t launch_w4_expand(const W4View& w, int n0, int n, _Float16* out, hipStream_t s);
 // X as binary16 [M x ld], zeros from K on.

@@ -158,3 +158,65 @@ def test_codes_behind_the_last_value():
         got = vedic.gemm_w4(torch.from_numpy(x).cuda(), w).double().cpu().numpy()
         x64, v64 = x.astype(np.float64), v.astype(np.float64)
         assert (np.abs(got - x64 @ v64) <= K * 2.0 ** -24 * (np.abs(x64) @ np.abs(v64))).all()
+
+
+@pytest.mark.parametrize("M,K,N,group", [(300, 200, 900, 32), (257, 1024, 1300, 64), (700, 40, 700, 128), (700, 1999, 515, 64), (1000, 96, 1000, 32),
+                                         (2100, 136, 2100, 128), (2049, 640, 2070, 32), (2100, 2056, 3700, 64), (300, 2100, 900, 64),
+                                         (200, 4096, 1500, 128), (385, 64, 1025, 64), (500, 72, 777, 32)])
+def test_many_rows(M, K, N, group):
+    """Tiles of both heights, whole and ragged in rows, columns, steps and words of K; and weights expanded first."""
+    check(M + K, M, K, N, group)
+
+
+@pytest.mark.parametrize("x32", [False, True])
+@pytest.mark.parametrize("epilogue,out", [(vedic.EPI_NONE, torch.float16), (vedic.EPI_BIAS, torch.float32), (vedic.EPI_BIAS_GELU, torch.float16),
+                                          (vedic.EPI_RESIDUAL, torch.float32), (vedic.EPI_BIAS_RESIDUAL, torch.float32)])
+@pytest.mark.parametrize("N", [1301, 1280])
+def test_many_rows_epilogues(x32, epilogue, out, N):
+    check(1, 333, 320, N, 64, epilogue, out, x32)
+
+
+@pytest.mark.parametrize("x32", [False, True])
+@pytest.mark.parametrize("ldx,align", [(264, 0), (256, 1), (257, 0), (259, 3)])
+def test_many_rows_strides(x32, ldx, align):
+    check(2, 333, 256, 1000, 32, x32=x32, ldx=ldx, align=align)
+
+
+def test_whole_rows_of_out():
+    """Rows of C that are whole 16-byte pieces, which the tiles store as such; what is behind them stays."""
+    w, _ = weight(3, 256, 1024, 64)
+    X = torch.randn(400, 256, device="cuda").half()
+    wide = vedic.gemm_w4(X, w)
+    for dt in (torch.float32, torch.float16):
+        out = torch.full((400, 1032), 7.0, dtype=dt, device="cuda")
+        vedic.gemm_w4(X, w, out=out[:, :1024])
+        assert torch.equal(out[:, :1024], wide.to(dt)) and (out[:, 1024:] == 7).all()
+
+
+def test_many_rows_captured():
+    """fp32 rows, which the tiles take as binary16 from the workspace: with a block the eager bits, without one 64 rows at a time."""
+    w, v = weight(6, 256, 700, 64)
+    X = torch.randn(700, 256, device="cuda")
+    want = vedic.gemm_w4(X, w)
+    tol = 260 * 2.0 ** -23 * (X.half().double().abs().cpu() @ torch.from_numpy(np.abs(v.astype(np.float64))))
+    for warm in (True, False):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        out = torch.zeros_like(want)
+        with torch.cuda.stream(s):
+            if warm:
+                vedic.gemm_w4(X, w, out=out)
+            s.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                vedic.gemm_w4(X, w, out=out)
+        for _ in range(4):
+            out.fill_(9)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) if warm else bool(((out - want).double().cpu().abs() <= tol).all())
+            torch.randn(1000, device="cuda").sum().item()
+        with torch.cuda.stream(s):
+            del g
+            vedic._lib.load().vedic_workspace_release(s.cuda_stream)
+        torch.cuda.synchronize()
