@@ -710,11 +710,11 @@ int vedic_w4_unpack(const vedic_w4_t* w, void* W16, int64_t ldw, void* stream);
 
 /* C[M x N] = epi(X[M x K] . W): X F16, or F32 clamped and rounded to binary16 as it is read; products of
  * binary16 values summed in fp32; C F32 or F16.  Epilogues NONE, BIAS, BIAS_GELU, and (F32 C)
- * RESIDUAL, BIAS_RESIDUAL.  Up to 192 rows, and more where 64 rows x 16 columns make no more
- * workgroups than CUs, read the codes themselves; others expand W into the stream's workspace
- * block first, in slabs of columns of up to 64 MiB (and copy an X that is F32 or whose rows are
- * not whole 16 bytes), and run the binary16 tiles; a captured call without such a block reads the codes
- * (results may then differ in rounding). */
+ * RESIDUAL, BIAS_RESIDUAL.  Rows are taken 64 at a time (up to 96 or 128 of them, or where that is
+ * a workgroup a CU), in tiles, or by the binary16 tiles from W expanded into the stream's workspace
+ * block, in slabs of columns of up to 64 MiB (large products, and a long K of few tiles).  The tiles take an X that is
+ * F32, or whose rows are not whole 16 bytes, from a binary16 copy in that block.  A captured call
+ * without such a block goes 64 rows at a time (results may then differ in rounding). */
 int vedic_gemm_w4(const vedic_w4_t* w, const void* X, int x_dtype, int64_t ldx, int M, void* C, int c_dtype, int64_t ldc,
                   const float* bias, int epilogue, void* stream);
 

@@ -1907,19 +1907,19 @@ extern "C" int vedic_w4_unpack(const vedic_w4_t* d, void* W16, int64_t ldw, void
     return hip_status(launch_w4_unpack(w, static_cast<_Float16*>(W16), ldw, static_cast<hipStream_t>(stream)));
 }
 
-// Whether a product with a four-bit weight reads the codes itself, 64 rows at a time: up to 192 rows, and where that
-// is one workgroup a CU (us, so / expanded: 128 rows of 1024 into 4096 12.4 / 19.6, 192 17.2 / 19.8, 256 22.4 / 19.6; of
-// 4096 into 16384 57 / 98, 82 / 107, 110 / 113; 512 rows of 512 into 512 4.5 / 9.9).
-static bool w4_direct(int M, int N, int cus) {
-    return M <= 192 || (int64_t)((M + kW4FewRows - 1) / kW4FewRows) * ((N + 15) / 16) <= cus;
+// Whether a product with a four-bit weight reads the codes itself, 64 rows at a time: up to 128 rows, 96 of a long K,
+// and where that is one workgroup a CU (us, so / as below: 128 rows of 1024 into 4096 12.4 / 15.0, 160 15.9 / 15.1; of
+// 2048 into 8192 22.2 / 23.4, 27.7 / 23.8; 96 of 4096 into 4096 30.9 / 28.9, 65 25.8 / 28.2; 512 rows of 512 into 512 4.5 / 9.9).
+static bool w4_direct(int M, int K, int N, int cus) {
+    return M <= (K <= 2048 ? 128 : 96) || (int64_t)((M + kW4FewRows - 1) / kW4FewRows) * ((N + 15) / 16) <= cus;
 }
 // Otherwise whether tiles expand the codes as they go, or the codes are expanded once for the binary16 tiles: those
 // are 5 to 10 % faster, share a long K among workgroups where tiles are few, and cost N K 4.5 bytes and two launches first
 // (us, tiles / expanded first: 2048 rows of 1024 into 4096 28.0 / 36.9, 1024 of 4096 into 16384 151 / 188, 2048 298 / 298, 8192
-// 1163 / 1100; 1024 of 1024 into 1024 15.4 / 23.9, of 4096 into 1024 40 / 27, 8192 75 / 86).
+// 1163 / 1100; 1024 of 1024 into 1024 15.4 / 23.9, of 4096 into 1024 40 / 27, 8192 75 / 86; 128 of 4096 into 16384 46 / 77).
 static bool w4_tiled(int M, int K, int N, int cus) {
     const bool filled = (int64_t)((M + 127) / 128) * ((N + 127) / 128) >= cus;
-    return (filled || K <= 2048) && (M <= 2048 || (int64_t)N * K <= (1 << 23));
+    return (filled || K <= 2048 || N >= 8192) && (M <= 2048 || (int64_t)N * K <= (1 << 23));
 }
 // Expanded columns at a time (bytes).
 static constexpr size_t kW4Slab = size_t(64) << 20;
@@ -1955,7 +1955,7 @@ extern "C" int vedic_gemm_w4(const vedic_w4_t* d, const void* X, int x_dtype, in
     Workspace ws;
     ws.s = static_cast<hipStream_t>(stream);
     const int cus = device_cu_count();
-    if (!w4_direct(M, d->N, cus)) {
+    if (!w4_direct(M, d->K, d->N, cus)) {
         const int64_t kp = (int64_t)a.w.words * 8;
         const bool rows = a.x32 || d->K % 8 != 0 || !aligned16(X) || ldx % 8 != 0, tiled = w4_tiled(M, d->K, d->N, cus);
         int64_t cols = (int64_t)(kW4Slab / (kp * 2)) / 256 * 256;

@@ -169,6 +169,12 @@ def test_many_rows(M, K, N, group):
 
 
 @pytest.mark.parametrize("x32", [False, True])
+def test_slabs_of_many_rows(x32):
+    """Expanded columns in two slabs, with a bias and the rows' copy beside them."""
+    check(3, 130, 16384, 2500, 128, vedic.EPI_BIAS, x32=x32)
+
+
+@pytest.mark.parametrize("x32", [False, True])
 @pytest.mark.parametrize("epilogue,out", [(vedic.EPI_NONE, torch.float16), (vedic.EPI_BIAS, torch.float32), (vedic.EPI_BIAS_GELU, torch.float16),
                                           (vedic.EPI_RESIDUAL, torch.float32), (vedic.EPI_BIAS_RESIDUAL, torch.float32)])
 @pytest.mark.parametrize("N", [1301, 1280])
