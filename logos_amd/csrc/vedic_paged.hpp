@@ -202,43 +202,57 @@ __device__ __forceinline__ float cache_value(const char* row, int D, int d) {
     return r;
 }
 
-// One row's part by one wave, key by key: what a key outside the row's mask holds never enters
-// a sum.  For rows whose sums came out infinite or NaN: in a product of tiles the zero weight
-// of an unseen key times an infinity is NaN.  o: values lane, lane + 64, ..
+// One row's part by one wave, key by key (KEYS on their way at a time): what a key outside the row's mask
+// holds never enters a sum.  For rows whose weights are fine and whose outputs came out infinite or NaN: in a product of
+// tiles the zero weight of an unseen key times an infinity is NaN.  (A row with a score that is NaN or +infinity has a
+// sum of weights that is NaN, and is NaN.)  o: values lane, lane + 64, ..
 template <int DP, bool I4>
 __device__ __forceinline__ void slow_row(const PagedArgs& a, const PagedItem& it, int pos, const _Float16* q, int lane,
                                       float (&o)[DP / 64], float& m, float& l) {
-    float qv[DP / 64];
+    constexpr int N = DP / 64, KEYS = I4 ? 2 : 8;  // (more of four bits cost the kernels that hold this a wave a SIMD)
+    float qv[N];
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j) {
+    for (int j = 0; j < N; ++j) {
         const int d = lane + 64 * j;
         qv[j] = d < a.c.D ? (float)q[d] : 0.0f;
         o[j] = 0.0f;
     }
     m = kNoScore;
     l = 0.0f;
-    for (int place = it.lo; place < it.hi; ++place) {
-        if (place >= it.far && place < it.near) continue;
-        const int t = key_at(a, it, place);
-        if (!sees(a, pos, t)) continue;
-        const int64_t at = a.c.row_offset(it.b, t) + (int64_t)it.h * a.c.head;
-        float x = 0.0f;
+    for (int p0 = it.lo; p0 < it.hi; p0 += KEYS) {
+        bool seen[KEYS];
+        float x[KEYS], v[KEYS][N], mn = m;
 #pragma unroll
-        for (int j = 0; j < DP / 64; ++j) {
-            const int d = lane + 64 * j;
-            if (d < a.c.D) x += qv[j] * cache_value<I4>(a.c.k + at, a.c.D, d);
+        for (int e = 0; e < KEYS; ++e) {
+            const int place = min(p0 + e, it.hi - 1), t = key_at(a, it, place);
+            seen[e] = p0 + e < it.hi && !(place >= it.far && place < it.near) && sees(a, pos, t);
+            const int64_t at = a.c.row_offset(it.b, t) + (int64_t)it.h * a.c.head;
+            x[e] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int d = min(lane + 64 * j, a.c.D - 1);
+                x[e] += lane + 64 * j < a.c.D ? qv[j] * cache_value<I4>(a.c.k + at, a.c.D, d) : 0.0f;
+                v[e][j] = cache_value<I4>(a.c.v + at, a.c.D, d);
+            }
         }
 #pragma unroll
-        for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
-        x *= a.sign * a.scale;
-        const float mn = __builtin_fmaxf(m, x), mu = mn == kNoScore ? 0.0f : mn;
-        const float f = exp2_fast(m - mu), p = exp2_fast(x - mu + kWeightBits);
-        l = l * f + p;
-        m = mn;
+        for (int e = 0; e < KEYS; ++e) {
 #pragma unroll
-        for (int j = 0; j < DP / 64; ++j) {
-            const int d = lane + 64 * j;
-            o[j] = o[j] * f + (d < a.c.D ? p * cache_value<I4>(a.c.v + at, a.c.D, d) : 0.0f);
+            for (int d = 32; d > 0; d >>= 1) x[e] += __shfl_xor(x[e], d);
+            x[e] = seen[e] ? x[e] * a.sign * a.scale : kNoScore;
+            mn = __builtin_fmaxf(mn, x[e]);
+        }
+        const float mu = mn == kNoScore ? 0.0f : mn, f = exp2_fast(m - mu);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] *= f;
+#pragma unroll
+        for (int e = 0; e < KEYS; ++e) {
+            const float p = exp2_fast(x[e] - mu + kWeightBits);
+            l += p;
+#pragma unroll
+            for (int j = 0; j < N; ++j) o[j] += seen[e] ? p * v[e][j] : 0.0f;
         }
     }
 }
@@ -262,13 +276,14 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
     const int64_t tok = it.first + i;
     const int head = it.h * a.G + rho - i * a.G;
     l += __shfl_xor(l, 32);
-    bool fine = l < __builtin_inff();
+    bool fine = true;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) fine = fine && __builtin_fabsf(acc[d][e]) < __builtin_inff();
+    fine |= l != l;
     if (mine) {
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         if (it.parts == 1) {
             _Float16* out = a.out + tok * a.o_token + (int64_t)head * a.o_head;
 #pragma unroll
@@ -338,19 +353,19 @@ __device__ __forceinline__ void join_sums(float4_t& o, float& m, float& l, float
 }
 
 // The parts of a tile joined.  A lane has four columns of a row's share of the parts: D / 4 lanes a share, a wave's
-// shares of one row (MANY: `per` rows a workgroup, a wave each in turn), or a workgroup's.
-template <int ROWS, bool MANY, int UNIT>
+// shares of one row (`per` rows a workgroup, a wave each in turn), or with WHOLE a workgroup's.
+template <int ROWS, bool MANY, int UNIT, bool WHOLE>
 __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
-    __shared__ float4_t wave_o[MANY ? 1 : 4][64];
-    __shared__ float wave_ml[MANY ? 1 : 4][2];
+    __shared__ float4_t wave_o[WHOLE ? 4 : 1][64];
+    __shared__ float wave_ml[WHOLE ? 4 : 1][2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     PagedItem it;
     if (!find_item<ROWS, MANY, UNIT, true>(a, blockIdx.x, lane, it)) return;
     if ((int64_t)it.slot + it.parts > a.slots) return;
     const int D = a.c.D, cols = D / 4;
     const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // of a share
-    const int shares = (MANY ? 1 : 4) * (64 / lanes), share = (MANY ? 0 : wave * (64 / lanes)) + lane / lanes, c = lane % lanes;
-    for (int r = blockIdx.y * per + (MANY ? wave : 0); r < (int)(blockIdx.y + 1) * per; r += MANY ? 4 : 1) {
+    const int shares = (WHOLE ? 4 : 1) * (64 / lanes), share = (WHOLE ? wave * (64 / lanes) : 0) + lane / lanes, c = lane % lanes;
+    for (int r = blockIdx.y * per + (WHOLE ? 0 : wave); r < (int)(blockIdx.y + 1) * per; r += WHOLE ? 1 : 4) {
         const int rho = it.tile * ROWS + r, i = a.by_group(rho);
         if (i >= it.n) return;
         const int64_t s0 = (int64_t)it.slot * ROWS + r;
@@ -387,7 +402,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
             const float4_t oo = {__shfl_xor(o[0], d), __shfl_xor(o[1], d), __shfl_xor(o[2], d), __shfl_xor(o[3], d)};
             join_sums(o, M, l, oo, __shfl_xor(M, d), __shfl_xor(l, d));
         }
-        if constexpr (!MANY) {
+        if constexpr (WHOLE) {
             wave_o[wave][lane] = o;
             wave_ml[wave][0] = M;
             wave_ml[wave][1] = l;

@@ -274,7 +274,7 @@ hipError_t paged_many(const PagedArgs& a, hipStream_t s) {
     else paged_many_kernel<256, I4><<<grid, 256, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.target > 0) {
-        paged_join_kernel<kManyRows, true, kManyUnit><<<join, 256, 0, s>>>(a, kManyRows / 4);
+        paged_join_kernel<kManyRows, true, kManyUnit, false><<<join, 256, 0, s>>>(a, kManyRows / 4);
         e = hipGetLastError();
     }
     return e;

@@ -293,3 +293,30 @@ def test_repeated_calls_give_the_same_bits():
     first = vedic.paged_attention(*args[:5], q_start=args[5])
     for _ in range(5):
         assert torch.equal(first, vedic.paged_attention(*args[:5], q_start=args[5]))
+
+
+def test_many_sequences_of_which_two_are_split():
+    """More rows that might have parts than workgroups to give each one: a wave joins a row."""
+    b = Batch(33, 4, 2, 64, False, 16, [1] * 300, [5000, 1200] + [3] * 298)
+    b.check(run(b))
+
+
+@pytest.mark.parametrize("new", [1, 20, 500])
+@pytest.mark.parametrize("where,bad", [(0, np.nan), (0, np.inf), (1, np.nan), (1, -np.inf)])
+def test_infinities_and_nan_that_are_seen(new, where, bad):
+    """A key or value of position 350: what the formula gives for the rows that see it (few and many rows, split and not), and
+    for the others what it gives without."""
+    b = Batch(31, 4, 2, 64, False, 16, [new, 1], [700, 3000])
+    page, row = b.table[0, 350 // 16], 350 % 16
+    b.rows[where][page, 1, row, 5] = bad
+    lse = torch.empty(b.T, 4, device="cuda")
+    got = run(b, lse=lse).double().cpu().numpy()
+    for s in range(2):
+        r = slice(b.starts[s], b.starts[s + 1])
+        k, v = b.sequence(s)
+        with np.errstate(invalid="ignore"):
+            want, want_lse, tol = plain.attention(b.q[r], k, v, np.arange(b.lens[s] - b.new[s], b.lens[s]), 64 ** -0.5)
+        fin = np.isfinite(want)
+        assert (np.isnan(got[r]) == np.isnan(want)).all() and (got[r][np.isinf(want)] == want[np.isinf(want)]).all()
+        assert (np.abs(got[r][fin] - want[fin]) <= tol[fin]).all()
+        assert (np.isnan(lse[r].cpu().numpy()) == np.isnan(want_lse)).all()
