@@ -1,6 +1,6 @@
 // vedic_cache.hpp -- a paged cache of keys and values, as the kernels that write it
-// (vedic_cache.hip) and read it (vedic_paged.hip) see it, and the four-bit format that
-// the cache and the weights of vedic_w4.hip share.
+// (vedic_cache.hip) and read it (vedic_paged.hpp) see it, and the four-bit format that
+// the cache and the weights of vedic_w4.hip and vedic_w4_tile.hip share.
 #pragma once
 
 #include "vedic_common.hpp"

@@ -1791,9 +1791,9 @@ extern "C" int vedic_kv_read(const vedic_kv_t* kv, void* k, void* v, void* strea
 static constexpr int kFewMost = 64;
 
 // Items that a call's keys are cut to.  Few rows: eight a CU, which is bound by reading and gains from even
-// shares (32 sequences of 128-wide binary16 heads, up to 16384 tokens: 261 / 225 / 213 / 210 us at one / four / six / eight;
-// 64 over four bits 284 / 203 / 191 / 188).  Many: one, since a part's sums of 128 rows cost as much as 64 keys
-// (pieces of 500 rows of three prompts: 197 us, 242 at two, 226 at four).
+// shares (us at one / four / six / eight, before the last steps took 5 to 10 off each: 32 sequences of 128-wide binary16 heads,
+// up to 16384 tokens, 261 / 225 / 213 / 210; 64 over four bits 284 / 203 / 191 / 188).  Many: one, since a part's sums
+// of 128 rows cost as much as 64 keys (pieces of 500 rows of three prompts: 197 us, 242 at two, 226 at four).
 static int64_t paged_target(bool many, int cus) { return many ? cus : cus * 8; }
 
 extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_t q_token, int64_t q_head, int q_heads,

@@ -167,3 +167,52 @@ def test_pages_past_four_gib():
     assert torch.equal(k[4100], x[:1024].transpose(0, 1)) and torch.equal(v[pages - 1, :, :476], x[1024:].transpose(0, 1))
     a, b = vedic.kv_read(k, v, table, lens, starts, 1500)
     assert torch.equal(a, x) and torch.equal(b, x)
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+def test_a_padded_batch(four_bit):
+    """Rows before the first sequence and behind the last one write nothing: not the cache, not q's output, not what is read back."""
+    k_cache, v_cache = vedic.kv_cache(6, 8, 2, 64, four_bit)
+    for c in (k_cache, v_cache):
+        bits(c).fill_(77)
+    x = torch.randn(12, 6, 64, device="cuda").half()
+    table = torch.tensor([[4, 1], [2, 0]], dtype=torch.int32, device="cuda")
+    lens, starts = (torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([9, 3], [2, 6, 9]))
+    out = torch.full((12, 2, 64), 5.0, dtype=torch.float16, device="cuda")
+    vedic.kv_append(x[:, :2], x[:, 2:4], x[:, 4:], k_cache, v_cache, table, lens, starts, out=out)
+    assert torch.equal(out[2:9], x[2:9, :2]) and (out[:2] == 5).all() and (out[9:] == 5).all()
+    there = torch.zeros(6, 8, dtype=torch.bool)
+    there[4, 5:], there[1, 0], there[2, :3] = True, True, True  # positions 5 .. 8 and 0 .. 2
+    for c in (k_cache, v_cache):
+        touched = (bits(c) != 77).any(-1).any(1).cpu()
+        assert (touched == there).all()
+    kr, vr = vedic.kv_read(k_cache, v_cache, table, lens, starts, 12)
+    want = [torch.from_numpy(plain.values_of(plain.rows_of(x[2:9, i:i + 2].cpu().numpy(), four_bit), four_bit)).cuda() for i in (2, 4)]
+    assert torch.equal(kr[2:9], want[0]) and torch.equal(vr[2:9], want[1])
+
+
+def test_recorded_beside_another_stream():
+    """An append recorded on one stream, replayed while lengths grow in place, with eager appends to another cache on a second one."""
+    caches = [vedic.kv_cache(4, 16, 2, 64) for _ in range(2)]
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4)
+    lens = [torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(2)]
+    x = torch.randn(40, 1, 2, 64, device="cuda").half()
+    step = torch.empty(1, 2, 64, dtype=torch.float16, device="cuda")
+    s, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            lens[0] += 1
+            vedic.kv_append(None, step, step, *caches[0], table, lens[0])
+    for i in range(40):
+        with torch.cuda.stream(s):
+            step.copy_(x[i])
+            graph.replay()
+        with torch.cuda.stream(other):
+            lens[1] += 1
+            vedic.kv_append(None, x[i], x[i], *caches[1], table, lens[1])
+    torch.cuda.synchronize()
+    for c in caches:
+        assert torch.equal(c[0].transpose(1, 2).reshape(64, 2, 64)[:40], x[:, 0])
+    assert torch.equal(caches[0][1], caches[1][1])

@@ -320,3 +320,19 @@ def test_infinities_and_nan_that_are_seen(new, where, bad):
         assert (np.isnan(got[r]) == np.isnan(want)).all() and (got[r][np.isinf(want)] == want[np.isinf(want)]).all()
         assert (np.abs(got[r][fin] - want[fin]) <= tol[fin]).all()
         assert (np.isnan(lse[r].cpu().numpy()) == np.isnan(want_lse)).all()
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 0.004, 1.5])
+@pytest.mark.parametrize("new", [2, 200])
+def test_scales(scale, new):
+    b = Batch(41, 4, 2, 64, False, 16, [new], [600])
+    lse = torch.empty(b.T, 4, device="cuda")
+    b.check(run(b, scale=scale, lse=lse), lse, scale=scale)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [300, 3]])
+def test_sequences_that_share_pages(new):
+    """Two sequences with one beginning: the same pages in both rows of the table."""
+    b = Batch(43, 4, 2, 64, True, 32, new, [800, 640])
+    b.table[1, :15] = b.table[0, :15]
+    b.check(run(b))

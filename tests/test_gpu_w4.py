@@ -226,3 +226,8 @@ def test_many_rows_captured():
             del g
             vedic._lib.load().vedic_workspace_release(s.cuda_stream)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("M,K,N", [(20000, 64, 17), (17000, 33, 5), (4000, 264, 129)])
+def test_narrow_weights_of_many_rows(M, K, N):
+    check(M + N, M, K, N, 32, vedic.EPI_BIAS)
