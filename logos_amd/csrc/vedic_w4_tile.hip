@@ -160,18 +160,18 @@ __global__ void __launch_bounds__(256) w4_tile_kernel(W4Args a, int shift, int t
     auto step = [&](auto tail, auto odd, int s, Codes& now, Codes& next) {
         rows(s, 1, xv[1]);
         values(tail, now, s, 1, wv[1]);
+        if constexpr (!odd) load_codes((s >> 1) + AHEAD);
         multiply(no, 0);
         rows(s, 2, xv[0]);
         values(tail, now, s, 2, wv[0]);
         multiply(no, 1);
         asm volatile("" ::: "memory");
-        wait_vmcnt<(ST - 3) * SideX::NLD + (ST - 3 + odd) / 2 * CODES>();
+        wait_vmcnt<(ST - 3) * SideX::NLD + (ST - 2 + !odd) / 2 * CODES>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         rows(s, 3, xv[1]);
         read_codes(s + 1, next);
         values(tail, now, s, 3, wv[1]);
-        if constexpr (!odd) load_codes((s >> 1) + AHEAD);
         load_x(tail, s + ST - 1);
         multiply(yes, 2);
         rows(s + 1, 0, xv[0]);
