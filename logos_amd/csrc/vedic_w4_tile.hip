@@ -53,8 +53,8 @@ __global__ void __launch_bounds__(256) w4_tile_kernel(W4Args a, int shift, int t
     const _Float16* tile = static_cast<const _Float16*>(a.X) + (int64_t)m0 * a.ldx;
     // X's rows of step s; TAIL: any K (X has zeros from K to the next multiple of eight), else steps that lie in K or
     // behind it as a whole (a resource without records then: zeros), which takes no vector instruction.
-    auto load_x = [&](auto tail, int s) {
-        char* to = lds + (s % ST) * STAGE;
+    auto load_x = [&](auto tail, int s, int place) {
+        char* to = lds + place;
         const _Float16* from = tile + (int64_t)s * kBK;
         if constexpr (tail) {
             sx.load(from, to, wave, lane, (K + 7) / 8 * 8 - s * kBK);
@@ -77,12 +77,12 @@ __global__ void __launch_bounds__(256) w4_tile_kernel(W4Args a, int shift, int t
         const int col = (wave * 2 + i) * 16 + (lane >> 2);
         pair_at[i] = n0 + col < w.N ? (uint32_t)col * w.G * 4u : kOob;
     }
-    auto load_codes = [&](int d) {
-        sc.load(codes + (int64_t)d * 32, lds_codes + (d % RING) * SideC::BYTES, wave, lane, 2 * w.words - 32 * d);
+    auto load_codes = [&](int d, int place) {
+        sc.load(codes + (int64_t)d * 32, lds_codes + place * SideC::BYTES, wave, lane, 2 * w.words - 32 * d);
         const int chunk = 4 * d + (lane & 3);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rp, (lds_void_t*)(lds_pairs + (d % RING) * PAIRS + (wave * 2 + i) * 256), 4,
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rp, (lds_void_t*)(lds_pairs + place * PAIRS + (wave * 2 + i) * 256), 4,
                                                      32 * chunk < K ? pair_at[i] + 4u * (chunk >> shift) : kOob, 0, 0, 0);
     };
     constexpr int CODES = SideC::NLD + 2;  // loads
@@ -90,14 +90,16 @@ __global__ void __launch_bounds__(256) w4_tile_kernel(W4Args a, int shift, int t
         u32x4_t c[2];
         uint32_t p[2];
     };
-    auto read_codes = [&](int s, Codes& b) {
-        const char* pc = lds_codes + ((s >> 1) % RING) * SideC::BYTES;
-        const char* pp = lds_pairs + ((s >> 1) % RING) * PAIRS;
+    // (column 64 (wave mod 2) + 32 j + r, piece 2 odd + h of its four: of two steps)
+    const int code_col = 64 * (wave & 1) + r;
+    const int code_at[2] = {code_col * 64 + ((h ^ swz_kc<4>(code_col)) << 4), code_col * 64 + (((2 + h) ^ swz_kc<4>(code_col)) << 4)};
+    auto read_codes = [&](auto odd, int place, Codes& b) {
+        const char* pc = lds_codes + place * SideC::BYTES + code_at[odd];
+        const char* pp = lds_pairs + place * PAIRS + code_col * 16 + 4 * h;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int col = 64 * (wave & 1) + 32 * j + r, chunk = 2 * (s & 1) + h;
-            b.c[j] = *reinterpret_cast<const u32x4_t*>(pc + col * 64 + ((chunk ^ swz_kc<4>(col)) << 4));
-            b.p[j] = *reinterpret_cast<const uint32_t*>(pp + col * 16 + chunk * 4);
+            b.c[j] = *reinterpret_cast<const u32x4_t*>(pc + 32 * 64 * j);
+            b.p[j] = *reinterpret_cast<const uint32_t*>(pp + 32 * 16 * j + 8 * odd);
         }
     };
     const FourBits expand;
@@ -117,13 +119,13 @@ __global__ void __launch_bounds__(256) w4_tile_kernel(W4Args a, int shift, int t
         }
     };
     const int xr = BM / 2 * (wave >> 1);
-    auto rows = [&](int s, int q, half8_t (&v)[MI]) {
-        const char* p = lds + (s % ST) * STAGE;
+    int row_at[4];
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const int row = xr + 32 * i + r;
-            v[i] = *reinterpret_cast<const half8_t*>(p + row * 128 + (((4 * h + q) ^ swz_kc<8>(row)) << 4));
-        }
+    for (int q = 0; q < 4; ++q) row_at[q] = (xr + r) * 128 + (((4 * h + q) ^ swz_kc<8>(r)) << 4);
+    auto rows = [&](int place, int q, half8_t (&v)[MI]) {
+        const char* p = lds + place + row_at[q];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) v[i] = *reinterpret_cast<const half8_t*>(p + 32 * 128 * i);
     };
 
     float16_t acc[MI][2];
@@ -157,40 +159,53 @@ __global__ void __launch_bounds__(256) w4_tile_kernel(W4Args a, int shift, int t
     // A step: the fragments of its next products are read and expanded beside the present ones; half way, the next
     // step's rows and codes have arrived (wait, barrier) and the places of the step before this one are free.  Issued
     // after those rows, and perhaps under way: the loads of ST - 3 steps, NLD of rows each, and of codes in the even ones.
+    // (x0, x1, x2: bytes to X's places of the step before, of this and of the next one; d0, d1, d2: the codes' places, by two steps;
+    // counted along, since the remainder by 3 or 5 would take vector instructions for every address)
+    int x0 = (ST - 1) * STAGE, x1 = 0, x2 = STAGE, d0 = RING - 1, d1 = 0, d2 = 1;
     auto step = [&](auto tail, auto odd, int s, Codes& now, Codes& next) {
-        rows(s, 1, xv[1]);
+        rows(x1, 1, xv[1]);
         values(tail, now, s, 1, wv[1]);
-        if constexpr (!odd) load_codes((s >> 1) + AHEAD);
+        if constexpr (!odd) load_codes((s >> 1) + AHEAD, d0);
         multiply(no, 0);
-        rows(s, 2, xv[0]);
+        rows(x1, 2, xv[0]);
         values(tail, now, s, 2, wv[0]);
         multiply(no, 1);
         asm volatile("" ::: "memory");
         wait_vmcnt<(ST - 3) * SideX::NLD + (ST - 2 + !odd) / 2 * CODES>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        rows(s, 3, xv[1]);
-        read_codes(s + 1, next);
+        rows(x1, 3, xv[1]);
+        if constexpr (odd) read_codes(no, d2, next);
+        else read_codes(yes, d1, next);
         values(tail, now, s, 3, wv[1]);
-        load_x(tail, s + ST - 1);
+        load_x(tail, s + ST - 1, x0);
         multiply(yes, 2);
-        rows(s + 1, 0, xv[0]);
+        rows(x2, 0, xv[0]);
         values(tail, next, s + 1, 0, wv[0]);
         multiply(no, 3);
+        x0 = x1;
+        x1 = x2;
+        x2 = x2 == (ST - 1) * STAGE ? 0 : x2 + STAGE;
+        if constexpr (odd) {
+            d0 = d1;
+            d1 = d2;
+            d2 = d2 == RING - 1 ? 0 : d2 + 1;
+        }
     };
     // The loads in the steps' order, as if ST - 1 steps had been before.
-    if constexpr (ST % 2 == 0) load_codes(0);
+    if constexpr (ST % 2 == 0) load_codes(0, 0);
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i) {
-        if ((ST - 1 - i) % 2 == 0) load_codes((i - ST + 1) / 2 + AHEAD);
-        load_x(yes, i);
+        constexpr int FIRST = ST - 1;
+        if ((FIRST - i) % 2 == 0) load_codes((i - FIRST) / 2 + AHEAD, (i - FIRST) / 2 + AHEAD);
+        load_x(yes, i, i * STAGE);
         asm volatile("" ::: "memory");
     }
     wait_vmcnt<(ST - 2) * SideX::NLD + (ST - 2) / 2 * CODES>();
     stage_barrier();
     Codes c0, c1;
     rows(0, 0, xv[0]);
-    read_codes(0, c0);
+    read_codes(no, 0, c0);
     values(yes, c0, 0, 0, wv[0]);
     // Steps without masks: all of a K of whole steps (but an odd last one), else those whose loads lie within K.
     const int plain = (K % kBK == 0 ? steps : max(K / kBK - ST + 1, 0)) & ~1;
