@@ -1915,8 +1915,8 @@ static bool w4_direct(int M, int K, int N, int cus) {
 }
 // Otherwise whether tiles expand the codes as they go, or the codes are expanded once for the binary16 tiles: those
 // are 5 to 10 % faster, share a long K among workgroups where tiles are few, and cost N K 4.5 bytes and two launches first
-// (us, tiles / expanded first: 2048 rows of 1024 into 4096 28.0 / 36.9, 1024 of 4096 into 16384 151 / 188, 2048 298 / 298, 8192
-// 1163 / 1100; 1024 of 1024 into 1024 15.4 / 23.9, of 4096 into 1024 40 / 27, 8192 75 / 86; 128 of 4096 into 16384 46 / 77).
+// (us, tiles / expanded first: 2048 rows of 1024 into 4096 27.3 / 36.9, 1024 of 4096 into 16384 151 / 188, 2048 290 / 298, 8192
+// 1163 / 1100; 1024 of 1024 into 1024 14.1 / 23.9, of 4096 into 1024 40 / 27, 8192 75 / 86; 128 of 4096 into 16384 46 / 77).
 static bool w4_tiled(int M, int K, int N, int cus) {
     const bool filled = (int64_t)((M + 127) / 128) * ((N + 127) / 128) >= cus;
     return (filled || K <= 2048 || N >= 8192) && (M <= 2048 || (int64_t)N * K <= (1 << 23));

@@ -9,8 +9,9 @@
 // lanes 32 .. 63 its words 4 .. 7, read as one 16-byte piece and expanded a word a product (13 instructions,
 // beside BM / 64 matrix instructions).
 //
-// Bound by a wave's own issue: matrix instructions and expanding take turns more than they overlap (a step of 256 rows 0.77
-// us, its matrix instructions alone 0.52; of 128 rows 0.50 and 0.26).
+// Bound by a wave's own issue where tiles are few (a step of 128 rows 0.48 us, its matrix instructions alone 0.26: they
+// and the expanding take turns more than they overlap); with every CU at it 600 to 950 TFLOP/s by K (2048 rows of 4096 into
+// 16384 290 us, 8192 of 2048 into 1024 47), and what surrounds the steps: 7 us a launch with its first loads, GELU and stores.
 //
 // The sums pass through LDS by 32 rows, so that a lane has eight consecutive columns for the bias, GELU and stores of
 // 16 bytes.
@@ -283,8 +284,8 @@ hipError_t launch_w4_tile(const W4Args& a, int cus, hipStream_t s) {
     const int shift = a.w.group == 32 ? 0 : a.w.group == 64 ? 1 : 2;
     // 256 rows (twice the products an expanded value) where a tile for every CU and a K of some length are there, else
     // 128: two workgroups a CU, or one with its loads further ahead (us of 256 / two of 128 / one: 8192 rows of 4096 into
-    // 1024 75 / 83 / 92, 1024 of 4096 into 16384 151 / 160 / 183, 2048 of 1024 into 4096 27.8 / 28.0 / 33.5, 8192 102 / 99 /
-    // 125, 1024 of 4096 into 1024 59 / 42 / 40).
+    // 1024 84 / 88, 1024 of 4096 into 16384 151 / 159, 2048 of 1024 into 4096 29.0 / 29.6 / 35.4, 8192 103 / 95 / 119, 4096 of
+    // 512 into 4096 37.3 / 33.4 / 42.9).
     if ((int64_t)tall * tn >= cus && a.w.K >= 2048) w4_tile_kernel<256, 4><<<(unsigned)(tall * tn), 256, 0, s>>>(a, shift, tall, tn);
     else if ((int64_t)low * tn > cus) w4_tile_kernel<128, 3><<<(unsigned)(low * tn), 256, 0, s>>>(a, shift, low, tn);
     else w4_tile_kernel<128, 5><<<(unsigned)(low * tn), 256, 0, s>>>(a, shift, low, tn);
