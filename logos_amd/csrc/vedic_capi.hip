@@ -1835,9 +1835,9 @@ extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_
     const bool i4 = kv->format == VEDIC_KV_I4;
     const int cus = device_cu_count();
     // Which kernels: sequences' rows are known on the GPU only, so a call whose sequences may be of both kinds runs
-    // both, each on its own ones.
-    const bool few = rows < (int64_t)kFewMost * kv->batch || rows <= kFewMost;
+    // both, each on its own ones.  (Without q_start every sequence has G rows.)
     const bool many = rows > kFewMost && (kv->q_start || a.G > kFewMost);
+    const bool few = !many || (kv->q_start && rows < (int64_t)kFewMost * kv->batch);
     a.few_most = !many ? INT32_MAX : !few ? 0 : kFewMost;
     Workspace ws;
     ws.s = static_cast<hipStream_t>(stream);

@@ -336,3 +336,16 @@ def test_sequences_that_share_pages(new):
     b = Batch(43, 4, 2, 64, True, 32, new, [800, 640])
     b.table[1, :15] = b.table[0, :15]
     b.check(run(b))
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("one_each", [True, False])
+@pytest.mark.parametrize("sequences", [1, 2, 5])
+@pytest.mark.parametrize("group", [63, 64, 65, 128])
+def test_query_heads_around_the_few_rows(group, sequences, one_each, four_bit):
+    """As many query heads a key head as the kernel of few rows takes of one token, one fewer and more."""
+    b = Batch(group, group, 1, 64, four_bit, 16, [1] * sequences, [200, 1, 129, 64, 31][:sequences])
+    out = torch.full((b.T, group, 64), float("nan"), dtype=torch.float16, device="cuda")
+    lse = torch.full((b.T, group), float("nan"), device="cuda")
+    run(b, one_each=one_each, out=out, lse=lse)
+    b.check(out, lse)
