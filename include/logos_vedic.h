@@ -683,7 +683,8 @@ int vedic_kv_read(const vedic_kv_t* kv, void* k, void* v, void* stream);
  * their largest.  What a masked key or a page's unused row holds, NaN included, does not
  * reach the output.  Rows of no sequence are left as they are.
  * Sequences of up to 64 rows (n_b x q_heads / heads) share out their keys evenly over the GPU,
- * others take 128 rows a workgroup and share keys where that leaves CUs idle; parts are added in
+ * others -- and, with q_start and heads up to 192, all those of a call with 64 rows and more a
+ * sequence on average -- take 128 rows a workgroup and share keys where that leaves CUs idle; parts are added in
  * a fixed order, 512 x CUs x (dh + 2) fp32 of the stream's workspace block at
  * most.  A captured call without such a block does not split (results may then differ in
  * rounding). */

@@ -349,3 +349,21 @@ def test_query_heads_around_the_few_rows(group, sequences, one_each, four_bit):
     lse = torch.full((b.T, group), float("nan"), device="cuda")
     run(b, one_each=one_each, out=out, lse=lse)
     b.check(out, lse)
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("D", [224, 256])
+def test_single_tokens_of_wide_heads_beside_a_long_piece(four_bit, D):
+    """They are the few-row kernel's: the bits of a call without the piece (no key is shared out in either, so that the order of
+    the sums is the same)."""
+    b = Batch(47, 8, 2, D, four_bit, 32, [1] * 9 + [700], [128, 1, 90, 31, 64, 127, 5, 100, 77, 900])
+    q, k, v, table, lens, starts = b.device()
+    got = vedic.paged_attention(q, k, v, table, lens, q_start=starts)
+    b.check(got)
+    assert torch.equal(got[:9], vedic.paged_attention(q[:9], k, v, table[:9, :4], lens[:9]))
+
+
+@pytest.mark.parametrize("four_bit,D", [(False, 64), (True, 128), (False, 160)])
+def test_single_tokens_beside_a_long_piece(four_bit, D):
+    b = Batch(48, 8, 2, D, four_bit, 32, [1] * 9 + [700], [128, 1, 90, 31, 64, 1270, 5, 100, 77, 900])
+    b.check(run(b))
