@@ -30,8 +30,8 @@ typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 
 // A lane's share of one token's row, DP / 4 values in KK pieces of eight; `first` is where its
 // pieces begin (a place fixed for the lane).  Heads narrower than DP: pieces past the end hold
-// others once more, which the zeros of Q's registers leave out of the scores, and which are
-// columns of the output that nobody reads.
+// others once more, which of V are columns of the output that nobody reads; K's are taken as
+// zeros (Q's alone would not do: what they hold may be infinite).
 template <int DP, bool I4>
 struct RowShare;
 template <int DP>
@@ -53,6 +53,10 @@ struct RowShare<DP, false> {
         for (int kk = 0; kk < KK; ++kk) v[kk] = *reinterpret_cast<const u32x4_t*>(row + p.at[kk]);
     }
     __device__ __forceinline__ half8_t frag(int kk, const Place&) const { return __builtin_bit_cast(half8_t, v[kk]); }
+    // (the last two pieces are the only ones that may lie past the end: D > DP - 64)
+    __device__ __forceinline__ half8_t key(int kk, const Place& p, int D, int g) const {
+        return kk >= KK - 2 && !p.own(kk, D, g) ? half8_t{} : frag(kk, p);
+    }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) v[kk] = u32x4_t{0, 0, 0, 0};
@@ -95,12 +99,19 @@ struct RowShare<DP, true> {
 #pragma unroll
         for (int i = 0; i < NS; ++i) sm[i] = *reinterpret_cast<const uint32_t*>(row + q.pairs[i]);
     }
-    __device__ __forceinline__ half8_t frag(int kk, const Place& q) const {
-        uint32_t x = sm[0];
-        if constexpr (NS > 1) x = (q.first + kk) / 4 > q.first / 4 ? sm[1] : sm[0];  // (DP / 4 values: two groups at most)
+    __device__ __forceinline__ uint32_t pair(int kk, const Place& q) const {
+        if constexpr (NS > 1) return (q.first + kk) / 4 > q.first / 4 ? sm[1] : sm[0];  // (DP / 4 values: two groups at most)
+        return sm[0];
+    }
+    __device__ __forceinline__ half8_t values(int kk, uint32_t x) const {
         half2_t s, m;
         four_bit_pair(x, s, m);
         return four_bit_values(w[kk], s, m);
+    }
+    __device__ __forceinline__ half8_t frag(int kk, const Place& q) const { return values(kk, pair(kk, q)); }
+    // (at most the first four pieces are another lane group's: D >= DP - 32)
+    __device__ __forceinline__ half8_t key(int kk, const Place& q, int D, int g) const {
+        return values(kk, kk < 4 && !q.own(kk, D, g) ? 0u : pair(kk, q));
     }
     __device__ __forceinline__ void clear() {  // (a pair of zeros: the value 0 whatever the code)
 #pragma unroll
@@ -108,7 +119,8 @@ struct RowShare<DP, true> {
     }
 };
 
-template <int DP, bool I4>
+// NARROW: heads of fewer than DP values.  (Looked at here instead, K's zeros cost full heads over four bits 2 to 5 %.)
+template <int DP, bool I4, bool NARROW>
 __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel(PagedArgs a) {
     typedef RowShare<DP, I4> Share;
     constexpr int KK = DP / 32, DT = DP / 16, PITCH = 2 * DP + 32, OP = DP + 4;
@@ -209,7 +221,8 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
             s[u] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
-                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[u].frag(kk, where), qf[kk], s[u], 0, 0, 0);
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(NARROW ? k[u].key(kk, where, c.D, g) : k[u].frag(kk, where), qf[kk], s[u], 0,
+                                                              0, 0);
         }
         if (more) {
             offset(t + kFewUnit, page, inside, off);
@@ -378,14 +391,20 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
 
 }  // namespace
 
+template <int DP, bool I4>
+void paged_few_of(const PagedArgs& a, const dim3& grid, hipStream_t s) {
+    if (a.c.D < DP) paged_few_kernel<DP, I4, true><<<grid, 256, 0, s>>>(a);
+    else paged_few_kernel<DP, I4, false><<<grid, 256, 0, s>>>(a);
+}
+
 template <bool I4>
 hipError_t paged_few(const PagedArgs& a, hipStream_t s) {
     const int64_t tiles = ((int64_t)a.c.T * a.G / kFewRows + (a.c.B < a.c.T ? a.c.B : a.c.T)) * a.c.H;
     const dim3 grid((unsigned)(tiles + a.target));
-    if (a.c.D <= 64) paged_few_kernel<64, I4><<<grid, 256, 0, s>>>(a);
-    else if (a.c.D <= 128) paged_few_kernel<128, I4><<<grid, 256, 0, s>>>(a);
-    else if (a.c.D <= 192) paged_few_kernel<192, I4><<<grid, 256, 0, s>>>(a);
-    else paged_few_kernel<256, I4><<<grid, 256, 0, s>>>(a);
+    if (a.c.D <= 64) paged_few_of<64, I4>(a, grid, s);
+    else if (a.c.D <= 128) paged_few_of<128, I4>(a, grid, s);
+    else if (a.c.D <= 192) paged_few_of<192, I4>(a, grid, s);
+    else paged_few_of<256, I4>(a, grid, s);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.target > 0) {
         const int rows = a.c.q_start == nullptr && a.G < kFewRows ? a.G : kFewRows;

@@ -67,12 +67,13 @@ struct BlockShare {
             }
         }
     }
-    // To LDS, V's rows from `left` on as zeros (what lies there is nobody's).
-    __device__ __forceinline__ void store(char* k, char* vl, int left) {
-        if (left < KEYS) {
+    // To LDS, V's rows from `left` on as zeros (what lies there is nobody's), and pieces past the end of a head narrower than DP
+    // (Q has zeros there, but what the last piece holds may be infinite).
+    __device__ __forceinline__ void store(char* k, char* vl, int left, int D) {
+        if (left < KEYS || D < DP) {
 #pragma unroll
             for (int x = 0; x < N; ++x)
-                if (of_v(x) && row(x) >= left) {
+                if ((of_v(x) && row(x) >= left) || piece(x) * (I4 ? 32 : 8) >= D) {
                     if constexpr (I4) sm[x] = 0u;
                     else v[x] = u32x4_t{0, 0, 0, 0};
                 }
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
         }
         __syncthreads();
         share.load(off[0]);
-        share.store(kbuf[0], vbuf[0], keys_left(it, it.lo));
+        share.store(kbuf[0], vbuf[0], keys_left(it, it.lo), c.D);
         __syncthreads();
     }
     int buf = 0;
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
                 acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, p[q], acc[d], 0, 0, 0);
             }
         if (more) {
-            share.store(kbuf[buf ^ 1], vbuf[buf ^ 1], keys_left(it, t + KEYS));
+            share.store(kbuf[buf ^ 1], vbuf[buf ^ 1], keys_left(it, t + KEYS), c.D);
             if (tid < KEYS) off[buf][tid] = offset(page, inside);
         }
         __syncthreads();

@@ -367,3 +367,34 @@ def test_single_tokens_of_wide_heads_beside_a_long_piece(four_bit, D):
 def test_single_tokens_beside_a_long_piece(four_bit, D):
     b = Batch(48, 8, 2, D, four_bit, 32, [1] * 9 + [700], [128, 1, 90, 31, 64, 1270, 5, 100, 77, 900])
     b.check(run(b))
+
+
+@pytest.mark.parametrize("new", [1, 20, 500])
+@pytest.mark.parametrize("four_bit,D,bad", [(False, d, s * np.inf) for d in (8, 40, 64, 96, 104, 160, 200, 224, 256) for s in (1, -1)] +
+                         [(True, d, np.inf) for d in (32, 64, 96, 160, 224)])
+def test_infinities_at_the_end_of_a_row(four_bit, D, bad, new):
+    """A seen key with an infinity among its last eight values (in four bits: a group whose last code stands for more than binary16's
+    largest): weight 0 where the score is -infinity, for heads that fill the kernels' widths and for narrower ones."""
+    b = Batch(53 + D, 4, 2, D, four_bit, 16, [new, 1], [700, 3000])
+    page, row = b.table[0, 350 // 16], 350 % 16
+    x = b.x[0][page, 1, row].copy()
+    x[D - 3] = bad
+    if four_bit:
+        x[D - 32:] = -65504
+        x[D - 3] = 65504
+    b.rows[0][page, 1, row] = plain.rows_of(x, four_bit)
+    assert np.isinf(plain.values_of(b.rows[0][page, 1, row], four_bit)).nonzero()[0].tolist() == [D - 3]
+    lse = torch.empty(b.T, 4, device="cuda")
+    got = run(b, lse=lse).double().cpu().numpy()
+    for s in range(2):
+        r = slice(b.starts[s], b.starts[s + 1])
+        k, v = b.sequence(s)
+        at = (b.q[r], k, v, np.arange(b.lens[s] - b.new[s], b.lens[s]), D ** -0.5)
+        with np.errstate(invalid="ignore"):
+            want, want_lse, _ = plain.attention(*at)
+        k0 = k.copy()
+        k0[~np.isfinite(k).all(-1)] = 0  # (that key's score has no error: the tolerance is the other keys')
+        tol = plain.attention(at[0], k0, *at[2:])[2]
+        fin = np.isfinite(want)
+        assert (np.isnan(got[r]) == np.isnan(want)).all() and (np.isnan(lse[r].cpu().numpy()) == np.isnan(want_lse)).all()
+        assert (np.abs(got[r][fin] - want[fin]) <= tol[fin]).all()
