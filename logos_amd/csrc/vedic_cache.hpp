@@ -180,7 +180,7 @@ struct PagedArgs {
     int few_most;  // sequences of at most so many rows (new rows x G) are the few-row kernel's
     int slots;
     float* part_o;   // [slots x rows x D]
-    float* part_ml;  // [slots x rows x 2]
+    float* part_ml;  // [slots x rows x 2]: largest score, sum
 };
 // Rows of a tile, and what parts of a tile's keys are whole multiples of.
 constexpr int kFewRows = 16, kManyRows = 128;

@@ -10,9 +10,10 @@
 // host's grid is as large as the items can be.  So a batch of one long and many short
 // sequences is dealt out evenly, whatever the table's width.
 //
-// Parts hold their sums relative to their own maximum: O = sum of 2^(x - m + 14) v and l the
-// same without v, x the score times log2(e); the join multiplies by 2^(m - M) in the order of
-// the parts.  The 2^14 keeps weights normal binary16 numbers down to 2^-28 of the largest.
+// Parts hold their sums relative to their own largest score m: O = sum of 2^(c (q.k - m) + 14) v and l
+// the same without v, c the scale times log2(e); the join multiplies by 2^(c (m - M)) in the order of
+// the parts.  The 2^14 keeps weights normal binary16 numbers down to 2^-28 of the largest.  (Differences of scores, not of
+// c times them: c m is rounded, by more than a weight's range from 2^29 on.)
 #pragma once
 
 #include "vedic_cache.hpp"
@@ -239,17 +240,17 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, const PagedItem& it
         for (int e = 0; e < KEYS; ++e) {
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) x[e] += __shfl_xor(x[e], d);
-            x[e] = seen[e] ? x[e] * a.sign * a.scale : kNoScore;
+            x[e] = seen[e] ? x[e] * a.sign : kNoScore;
             mn = __builtin_fmaxf(mn, x[e]);
         }
-        const float mu = mn == kNoScore ? 0.0f : mn, f = exp2_fast(m - mu);
+        const float mu = mn == kNoScore ? 0.0f : mn, f = exp2_fast((m - mu) * a.scale);
         m = mn;
         l *= f;
 #pragma unroll
         for (int j = 0; j < N; ++j) o[j] *= f;
 #pragma unroll
         for (int e = 0; e < KEYS; ++e) {
-            const float p = exp2_fast(x[e] - mu + kWeightBits);
+            const float p = exp2_fast(__builtin_fmaf(x[e] - mu, a.scale, kWeightBits));
             l += p;
 #pragma unroll
             for (int j = 0; j < N; ++j) o[j] += seen[e] ? p * v[e][j] : 0.0f;
@@ -259,8 +260,10 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, const PagedItem& it
 
 typedef _Float16 paged_half4_t __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ float lse_of(float m, float l) {
-    return l > 0.0f || l != l ? (m - kWeightBits + __builtin_log2f(l)) * 0.6931471805599453f : __builtin_inff();
+// A row's 1 / l and log-sum-exp from its largest score m and its sum l.
+__device__ __forceinline__ float inverse_of(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
+__device__ __forceinline__ float lse_of(const PagedArgs& a, float m, float l) {
+    return l > 0.0f || l != l ? (__builtin_fmaf(m, a.scale, -kWeightBits) + __builtin_log2f(l)) * 0.6931471805599453f : __builtin_inff();
 }
 
 namespace {
@@ -283,7 +286,7 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
         for (int e = 0; e < 16; ++e) fine = fine && __builtin_fabsf(acc[d][e]) < __builtin_inff();
     fine |= l != l;
     if (mine) {
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const float inv = inverse_of(l);
         if (it.parts == 1) {
             _Float16* out = a.out + tok * a.o_token + (int64_t)head * a.o_head;
 #pragma unroll
@@ -295,7 +298,7 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
                                             (_Float16)(acc[d][4 * e + 2] * inv), (_Float16)(acc[d][4 * e + 3] * inv)};
                     if (at < a.c.D) *reinterpret_cast<paged_half4_t*>(out + at) = v;
                 }
-            if (a.lse && h == 0) a.lse[tok * a.Hq + head] = lse_of(m, l);
+            if (a.lse && h == 0) a.lse[tok * a.Hq + head] = lse_of(a, m, l);
         } else {
             float* po = a.part_o + (s0 + r) * a.c.D;
 #pragma unroll
@@ -319,11 +322,12 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
         const int w = __builtin_ctzll(bad);
         bad &= bad - 1;
         const int brho = base + w, bi = a.by_group(brho), bh = it.h * a.G + brho - bi * a.G;
+        const int bpos = it.len - it.n + bi;
         const int64_t bt = it.first + bi;
         float ov[DP / 64], bm, bl;
-        slow_row<DP, I4>(a, it, it.len - it.n + bi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
+        slow_row<DP, I4>(a, it, bpos, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
                          bm, bl);
-        const float bin = bl > 0.0f || bl != bl ? 1.0f / bl : 0.0f;
+        const float bin = inverse_of(bl);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the stores above come first)
 #pragma unroll
         for (int j = 0; j < DP / 64; ++j) {
@@ -334,7 +338,7 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
         }
         if (lane == 0) {
             if (it.parts == 1) {
-                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(bm, bl);
+                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(a, bm, bl);
             } else {
                 a.part_ml[2 * (s0 + w)] = bm;
                 a.part_ml[2 * (s0 + w) + 1] = bl;
@@ -344,9 +348,9 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
 }
 
 // Sums o, l relative to a maximum m, and others' o2, l2, m2, as one.
-__device__ __forceinline__ void join_sums(float4_t& o, float& m, float& l, float4_t o2, float m2, float l2) {
+__device__ __forceinline__ void join_sums(float scale, float4_t& o, float& m, float& l, float4_t o2, float m2, float l2) {
     const float top = __builtin_fmaxf(m, m2), mu = top == kNoScore ? 0.0f : top;
-    const float f = exp2_fast(m - mu), f2 = exp2_fast(m2 - mu);
+    const float f = exp2_fast((m - mu) * scale), f2 = exp2_fast((m2 - mu) * scale);
     m = top;
     l = l * f + l2 * f2;
     o = o * f + o2 * f2;
@@ -385,13 +389,13 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
             float top = M;
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = __builtin_fmaxf(top, mp[j]);
-            const float mu = top == kNoScore ? 0.0f : top, g = exp2_fast(M - mu);
+            const float mu = top == kNoScore ? 0.0f : top, g = exp2_fast((M - mu) * a.scale);
             M = top;
             l *= g;
             o *= g;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float f = exp2_fast(mp[j] - mu);
+                const float f = exp2_fast((mp[j] - mu) * a.scale);
                 if (p0 + j * shares < it.parts && !(lp[j] == 0.0f)) {  // (a part without keys has nothing to add)
                     l += lp[j] * f;
                     o += v[j] * f;
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
         }
         for (int d = lanes; d < 64; d <<= 1) {
             const float4_t oo = {__shfl_xor(o[0], d), __shfl_xor(o[1], d), __shfl_xor(o[2], d), __shfl_xor(o[3], d)};
-            join_sums(o, M, l, oo, __shfl_xor(M, d), __shfl_xor(l, d));
+            join_sums(a.scale, o, M, l, oo, __shfl_xor(M, d), __shfl_xor(l, d));
         }
         if constexpr (WHOLE) {
             wave_o[wave][lane] = o;
@@ -409,16 +413,16 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
             __syncthreads();
             if (wave > 0) return;  // (per is 1)
 #pragma unroll
-            for (int x = 1; x < 4; ++x) join_sums(o, M, l, wave_o[x][lane], wave_ml[x][0], wave_ml[x][1]);
+            for (int x = 1; x < 4; ++x) join_sums(a.scale, o, M, l, wave_o[x][lane], wave_ml[x][0], wave_ml[x][1]);
         }
         const int head = it.h * a.G + rho - i * a.G;
         const int64_t t = it.first + i;
         if (lane < lanes && c < cols) {
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            const float inv = inverse_of(l);
             const paged_half4_t v = {(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
             *reinterpret_cast<paged_half4_t*>(a.out + t * a.o_token + (int64_t)head * a.o_head + 4 * c) = v;
         }
-        if (a.lse && lane == 0) a.lse[t * a.Hq + head] = lse_of(M, l);
+        if (a.lse && lane == 0) a.lse[t * a.Hq + head] = lse_of(a, M, l);
     }
 }
 

@@ -267,19 +267,18 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
         for (int e = 0; e < 8; ++e) mx = __builtin_fmaxf(mx, s[e >> 2][e & 3]);
         mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
         mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
-        mx *= a.scale;
         if (__any(mx > m)) {
-            const float mn = __builtin_fmaxf(m, mx), f = mn == kNoScore ? 1.0f : exp2_fast(m - mn);
+            const float mn = __builtin_fmaxf(m, mx), f = mn == kNoScore ? 1.0f : exp2_fast((m - mn) * a.scale);
             m = mn;
             l *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) acc[d] *= f;
         }
-        const float bias = kWeightBits - (m == kNoScore ? 0.0f : m);
+        const float mu = m == kNoScore ? 0.0f : m;
         half8_t p;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float w = exp2_fast(__builtin_fmaf(s[e >> 2][e & 3], a.scale, bias));
+            const float w = exp2_fast(__builtin_fmaf(s[e >> 2][e & 3] - mu, a.scale, kWeightBits));
             l += w;
             p[e] = (_Float16)w;
         }
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
     const float mu = M == kNoScore ? 0.0f : M;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        fw[w] = exp2_fast(ml[w][row][0] - mu);
+        fw[w] = exp2_fast((ml[w][row][0] - mu) * a.scale);
         L += ml[w][row][1] * fw[w];
     }
     float4_t o[DP / 64];
@@ -336,7 +335,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
     const bool here = ri < it.n;
     const int head = it.h * a.G + rrho - ri * a.G;
     const int64_t tok = it.first + ri;
-    const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+    const float inv = inverse_of(L);
     if (here) {
         if (it.parts == 1) {
             _Float16* out = a.out + tok * a.o_token + (int64_t)head * a.o_head + col;
@@ -347,7 +346,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
                                        (_Float16)(o[j][3] * inv)};
                     *reinterpret_cast<half4_t*>(out + 64 * j) = h;
                 }
-            if (a.lse && col == 0) a.lse[tok * a.Hq + head] = lse_of(M, L);
+            if (a.lse && col == 0) a.lse[tok * a.Hq + head] = lse_of(a, M, L);
         } else {
             const int64_t s0 = (int64_t)it.slot * kFewRows + row;
 #pragma unroll
@@ -365,11 +364,12 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
     for (int w = 0; w < 4; ++w) {
         if (((bad >> (16 * w)) & 0xFFFF) == 0) continue;  // row 4 wave + w
         const int brho = it.tile * kFewRows + 4 * wave + w, bi = a.by_group(brho), bh = it.h * a.G + brho - bi * a.G;
+        const int bpos = it.len - it.n + bi;
         const int64_t bt = it.first + bi;
         float ov[DP / 64], bm, bl;
-        slow_row<DP, I4>(a, it, it.len - it.n + bi, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
+        slow_row<DP, I4>(a, it, bpos, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
                          bm, bl);
-        const float bin = bl > 0.0f || bl != bl ? 1.0f / bl : 0.0f;
+        const float bin = inverse_of(bl);
         const int64_t s0 = (int64_t)it.slot * kFewRows + 4 * wave + w;
 #pragma unroll
         for (int j = 0; j < DP / 64; ++j) {
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
         }
         if (lane == 0) {
             if (it.parts == 1) {
-                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(bm, bl);
+                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(a, bm, bl);
             } else {
                 a.part_ml[2 * s0] = bm;
                 a.part_ml[2 * s0 + 1] = bl;

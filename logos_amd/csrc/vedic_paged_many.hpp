@@ -226,15 +226,23 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = __builtin_fmaxf(mx, s[u][e]);
-        mx = both_halves_max(mx) * a.scale;
+        mx = both_halves_max(mx);
         if (__any(mx > m)) {
-            const float mn = __builtin_fmaxf(m, mx), f = mn == kNoScore ? 1.0f : exp2_fast(m - mn);
+            const float mn = __builtin_fmaxf(m, mx), f = mn == kNoScore ? 1.0f : exp2_fast((m - mn) * a.scale);
             l *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) acc[d] *= f;
             m = mn;
         }
-        const float bias = kWeightBits - (m == kNoScore ? 0.0f : m);
+        const float mu = m == kNoScore ? 0.0f : m;
+        float bias = __builtin_fmaf(-mu, a.scale, kWeightBits);
+        if (__any(__builtin_fabsf(bias) > 0x1p20f)) {  // (c m far from its rounding: differences of scores, as everywhere else)
+            bias = kWeightBits;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[u][e] -= mu;
+        }
         half8_t p[2 * U];
 #pragma unroll
         for (int u = 0; u < U; ++u)

@@ -398,3 +398,33 @@ def test_infinities_at_the_end_of_a_row(four_bit, D, bad, new):
         fin = np.isfinite(want)
         assert (np.isnan(got[r]) == np.isnan(want)).all() and (np.isnan(lse[r].cpu().numpy()) == np.isnan(want_lse)).all()
         assert (np.abs(got[r][fin] - want[fin]) <= tol[fin]).all()
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("size", [100.0, 4000.0, 60000.0])
+@pytest.mark.parametrize("new,lens", [([1, 1], [1, 300]), ([1, 3], [5000, 3]), ([200, 90], [200, 2000])])
+def test_scores_far_from_zero(new, lens, size, four_bit):
+    """Finite scores of up to 2^38, whose fp32 step is far above 1: a row is the value of its largest score (all of some rows' are
+    below zero), wherever the next one is further away than the rounding of the sums."""
+    b = Batch(59, 4, 2, 64, four_bit, 32, new, lens)
+    rng = np.random.default_rng(7)
+    b.x[0][:] = (0.5 + 0.5 * rng.random(b.x[0].shape)) * size
+    b.rows = [plain.rows_of(x, four_bit) for x in b.x]
+    b.q[:] = (0.5 + 0.5 * rng.random(b.q.shape)) * size * np.where(rng.random((b.T, 4, 1)) < 0.5, -1, 1)
+    lse = torch.empty(b.T, 4, device="cuda")
+    got = run(b, lse=lse).double().cpu().numpy()
+    lse, clear = lse.double().cpu().numpy(), 0
+    for s in range(2):
+        k, v = (x.astype(np.float64) for x in b.sequence(s))
+        for i in range(new[s]):
+            r, p = b.starts[s] + i, lens[s] - new[s] + i
+            for h in range(4):
+                x = k[:p + 1, h // 2] @ b.q[r, h].astype(np.float64) / 8
+                top = x.argmax()
+                step = 67 * 2.0 ** -24 * np.abs(x[top])  # (64 products' sum, the scale and log2(e), each half a step)
+                assert abs(lse[r, h] - x[top]) <= step + 10
+                if (np.delete(x, top) < x[top] - 2 * step - 30).all():
+                    clear += 1
+                    want = v[top, h // 2]
+                    assert (np.abs(got[r, h] - want) <= 2.0 ** -10 * np.abs(want) + 2.0 ** -11).all(), (s, i, h)
+    assert clear > b.T
