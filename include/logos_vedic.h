@@ -678,8 +678,8 @@ int vedic_kv_read(const vedic_kv_t* kv, void* k, void* v, void* stream);
  * t <= p (causal; else all lens[b]) and, with window > 0 (causal only), of those t >= p - window and,
  * with stride > 0, also t a multiple of stride -- the masks of vedic_flash_attention_fwd:
  *     out = sum over t of e^(scale q.k_t - M) v_t / sum of the same without v_t,
- * 0 for a row that sees no key.  lse (NULL, or [tokens x q_heads]): ln of sum e^(scale q.k_t), +inf for
- * such a row.  out (which does not overlap q) binary16, rounded once; scores and sums fp32, weights binary16 relative to
+ * 0 for a row that sees no key, NaN for one that sees only keys of score -infinity.  lse (NULL, or [tokens x q_heads]): ln of
+ * sum e^(scale q.k_t), +inf and NaN for such rows.  out (which does not overlap q) binary16, rounded once; scores and sums fp32, weights binary16 relative to
  * their largest.  What a masked key or a page's unused row holds, NaN included, does not
  * reach the output.  Rows of no sequence are left as they are.
  * Sequences of up to 64 rows (n_b x q_heads / heads) share out their keys evenly over the GPU,

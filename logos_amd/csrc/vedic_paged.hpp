@@ -260,10 +260,17 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, const PagedItem& it
 
 typedef _Float16 paged_half4_t __attribute__((ext_vector_type(4)));
 
-// A row's 1 / l and log-sum-exp from its largest score m and its sum l.
-__device__ __forceinline__ float inverse_of(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
-__device__ __forceinline__ float lse_of(const PagedArgs& a, float m, float l) {
-    return l > 0.0f || l != l ? (__builtin_fmaf(m, a.scale, -kWeightBits) + __builtin_log2f(l)) * 0.6931471805599453f : __builtin_inff();
+// A row's 1 / l and log-sum-exp from its largest score m and its sum l.  A sum of 0: the row at position pos sees no key (0 and
+// +infinity), or only keys whose scores are -infinity (nothing over nothing: NaN).
+__device__ __forceinline__ float empty_row(const PagedArgs& a, int pos, int len, float unseen) {
+    return (a.causal ? pos >= 0 : len > 0) ? __builtin_nanf("") : unseen;
+}
+__device__ __forceinline__ float inverse_of(const PagedArgs& a, int pos, int len, float l) {
+    return l > 0.0f || l != l ? 1.0f / l : empty_row(a, pos, len, 0.0f);
+}
+__device__ __forceinline__ float lse_of(const PagedArgs& a, int pos, int len, float m, float l) {
+    return l > 0.0f || l != l ? (__builtin_fmaf(m, a.scale, -kWeightBits) + __builtin_log2f(l)) * 0.6931471805599453f
+                              : empty_row(a, pos, len, __builtin_inff());
 }
 
 namespace {
@@ -277,7 +284,7 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
     const int r = lane & 31, h = lane >> 5, rho = base + r, i = a.by_group(rho);
     const bool mine = i < it.n;
     const int64_t tok = it.first + i;
-    const int head = it.h * a.G + rho - i * a.G;
+    const int head = it.h * a.G + rho - i * a.G, pos = it.len - it.n + i;
     l += __shfl_xor(l, 32);
     bool fine = true;
 #pragma unroll
@@ -286,7 +293,7 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
         for (int e = 0; e < 16; ++e) fine = fine && __builtin_fabsf(acc[d][e]) < __builtin_inff();
     fine |= l != l;
     if (mine) {
-        const float inv = inverse_of(l);
+        const float inv = inverse_of(a, pos, it.len, l);
         if (it.parts == 1) {
             _Float16* out = a.out + tok * a.o_token + (int64_t)head * a.o_head;
 #pragma unroll
@@ -298,7 +305,7 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
                                             (_Float16)(acc[d][4 * e + 2] * inv), (_Float16)(acc[d][4 * e + 3] * inv)};
                     if (at < a.c.D) *reinterpret_cast<paged_half4_t*>(out + at) = v;
                 }
-            if (a.lse && h == 0) a.lse[tok * a.Hq + head] = lse_of(a, m, l);
+            if (a.lse && h == 0) a.lse[tok * a.Hq + head] = lse_of(a, pos, it.len, m, l);
         } else {
             float* po = a.part_o + (s0 + r) * a.c.D;
 #pragma unroll
@@ -327,7 +334,7 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
         float ov[DP / 64], bm, bl;
         slow_row<DP, I4>(a, it, bpos, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
                          bm, bl);
-        const float bin = inverse_of(bl);
+        const float bin = inverse_of(a, bpos, it.len, bl);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the stores above come first)
 #pragma unroll
         for (int j = 0; j < DP / 64; ++j) {
@@ -338,7 +345,7 @@ __device__ __forceinline__ void finish_rows(const PagedArgs& a, const PagedItem&
         }
         if (lane == 0) {
             if (it.parts == 1) {
-                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(a, bm, bl);
+                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(a, bpos, it.len, bm, bl);
             } else {
                 a.part_ml[2 * (s0 + w)] = bm;
                 a.part_ml[2 * (s0 + w) + 1] = bl;
@@ -415,14 +422,14 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
 #pragma unroll
             for (int x = 1; x < 4; ++x) join_sums(a.scale, o, M, l, wave_o[x][lane], wave_ml[x][0], wave_ml[x][1]);
         }
-        const int head = it.h * a.G + rho - i * a.G;
+        const int head = it.h * a.G + rho - i * a.G, pos = it.len - it.n + i;
         const int64_t t = it.first + i;
         if (lane < lanes && c < cols) {
-            const float inv = inverse_of(l);
+            const float inv = inverse_of(a, pos, it.len, l);
             const paged_half4_t v = {(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
             *reinterpret_cast<paged_half4_t*>(a.out + t * a.o_token + (int64_t)head * a.o_head + 4 * c) = v;
         }
-        if (a.lse && lane == 0) a.lse[t * a.Hq + head] = lse_of(a, M, l);
+        if (a.lse && lane == 0) a.lse[t * a.Hq + head] = lse_of(a, pos, it.len, M, l);
     }
 }
 

@@ -333,9 +333,9 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
     }
     fine |= L != L;
     const bool here = ri < it.n;
-    const int head = it.h * a.G + rrho - ri * a.G;
+    const int head = it.h * a.G + rrho - ri * a.G, rpos = it.len - it.n + ri;
     const int64_t tok = it.first + ri;
-    const float inv = inverse_of(L);
+    const float inv = inverse_of(a, rpos, it.len, L);
     if (here) {
         if (it.parts == 1) {
             _Float16* out = a.out + tok * a.o_token + (int64_t)head * a.o_head + col;
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
                                        (_Float16)(o[j][3] * inv)};
                     *reinterpret_cast<half4_t*>(out + 64 * j) = h;
                 }
-            if (a.lse && col == 0) a.lse[tok * a.Hq + head] = lse_of(a, M, L);
+            if (a.lse && col == 0) a.lse[tok * a.Hq + head] = lse_of(a, rpos, it.len, M, L);
         } else {
             const int64_t s0 = (int64_t)it.slot * kFewRows + row;
 #pragma unroll
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
         float ov[DP / 64], bm, bl;
         slow_row<DP, I4>(a, it, bpos, a.q + bt * a.q_token + (int64_t)bh * a.q_head, lane, ov,
                          bm, bl);
-        const float bin = inverse_of(bl);
+        const float bin = inverse_of(a, bpos, it.len, bl);
         const int64_t s0 = (int64_t)it.slot * kFewRows + 4 * wave + w;
 #pragma unroll
         for (int j = 0; j < DP / 64; ++j) {
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
         }
         if (lane == 0) {
             if (it.parts == 1) {
-                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(a, bm, bl);
+                if (a.lse) a.lse[bt * a.Hq + bh] = lse_of(a, bpos, it.len, bm, bl);
             } else {
                 a.part_ml[2 * s0] = bm;
                 a.part_ml[2 * s0 + 1] = bl;

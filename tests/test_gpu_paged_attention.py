@@ -428,3 +428,24 @@ def test_scores_far_from_zero(new, lens, size, four_bit):
                     want = v[top, h // 2]
                     assert (np.abs(got[r, h] - want) <= 2.0 ** -10 * np.abs(want) + 2.0 ** -11).all(), (s, i, h)
     assert clear > b.T
+
+
+@pytest.mark.parametrize("new", [1, 30, 300])
+def test_rows_whose_scores_are_all_minus_infinity(new):
+    """Undefined by the formula (nothing over nothing), unlike a row that sees no key; the rows beside them are not touched."""
+    b = Batch(61, 4, 2, 64, False, 16, [new, 2], [new + 3, 1])
+    for p in range(4):
+        b.rows[0][b.table[0, p // 16], :, p % 16, 7] = -np.inf
+    b.q[:, :, 7] = np.abs(b.q[:, :, 7]) + np.float16(0.5)
+    b.q[0, 1, 7] = -1.0
+    lse = torch.empty(b.T, 4, device="cuda")
+    got = run(b, lse=lse, window=2).float().cpu().numpy()
+    lse = lse.cpu().numpy()
+    for i in range(new + 2):
+        for h in range(4):
+            if i == 0:  # position 3 sees 1 .. 3 only, of -infinity, or +infinity for the head whose value is below zero
+                assert np.isnan(got[0, h]).all() and np.isnan(lse[0, h])
+            elif i == new:  # before the first position of a sequence with one token
+                assert (got[i, h] == 0).all() and lse[i, h] == np.inf
+            else:
+                assert np.isfinite(got[i, h]).all() and np.isfinite(lse[i, h])
