@@ -678,10 +678,12 @@ int vedic_kv_read(const vedic_kv_t* kv, void* k, void* v, void* stream);
  * t <= p (causal; else all lens[b]) and, with window > 0 (causal only), of those t >= p - window and,
  * with stride > 0, also t a multiple of stride -- the masks of vedic_flash_attention_fwd:
  *     out = sum over t of e^(scale q.k_t - M) v_t / sum of the same without v_t,
- * 0 for a row that sees no key, NaN for one that sees only keys of score -infinity.  lse (NULL, or [tokens x q_heads]): ln of
- * sum e^(scale q.k_t), +inf and NaN for such rows.  out (which does not overlap q) binary16, rounded once; scores and sums fp32, weights binary16 relative to
- * their largest.  What a masked key or a page's unused row holds, NaN included, does not
- * reach the output.  Rows of no sequence are left as they are.
+ * 0 for a row that sees no key, NaN for one that sees only keys of score -infinity.  lse (NULL, or
+ * [tokens x q_heads]): ln of sum e^(scale q.k_t), +inf and NaN for such rows.  out (which does not overlap q)
+ * binary16, rounded once; scores and sums fp32.  The weights that multiply v_t are binary16 relative to the row's
+ * largest: of two parts (22 bits) for the sequences that share out their keys over a binary16 cache (below), else of
+ * one.  What a masked key or a page's unused row holds, NaN included, does not reach the output.  Rows of no sequence
+ * are left as they are.
  * Sequences of up to 64 rows (n_b x q_heads / heads) share out their keys evenly over the GPU,
  * others -- and, with q_start and heads up to 192, all those of a call with 64 rows and more a
  * sequence on average -- take 128 rows a workgroup and share keys where that leaves CUs idle; parts are added in

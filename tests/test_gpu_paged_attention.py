@@ -449,3 +449,18 @@ def test_rows_whose_scores_are_all_minus_infinity(new):
                 assert (got[i, h] == 0).all() and lse[i, h] == np.inf
             else:
                 assert np.isfinite(got[i, h]).all() and np.isfinite(lse[i, h])
+
+
+@pytest.mark.parametrize("D", [8, 40, 64, 128, 160, 256])
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [700, 3, 6000]), ([3, 9, 16], [40, 9, 3000])])
+def test_weights_of_few_rows_over_binary16(D, new, lens):
+    """In two binary16 parts, 2^-22 of a weight instead of 2^-11: the output's own rounding and the scores' are what is left."""
+    b = Batch(67 + D, 4, 2, D, False, 32, new, lens)
+    got = run(b).double().cpu().numpy()
+    for s in range(3):
+        r = slice(b.starts[s], b.starts[s + 1])
+        k, v = b.sequence(s)
+        at = (np.arange(lens[s] - new[s], lens[s]), D ** -0.5)
+        out, _, tol = plain.attention(b.q[r], k, v, *at)
+        size = plain.attention(b.q[r], k, np.abs(v), *at)[0]  # the weights' sum of |v|
+        assert (np.abs(got[r] - out) <= tol - (2.0 ** -11 - 2.0 ** -22) * size).all()
