@@ -689,7 +689,8 @@ int vedic_kv_read(const vedic_kv_t* kv, void* k, void* v, void* stream);
  * sequence on average -- take 128 rows a workgroup and share keys where that leaves CUs idle; parts are added in
  * a fixed order, 512 x CUs x (dh + 2) fp32 of the stream's workspace block at
  * most.  A captured call without such a block does not split (results may then differ in
- * rounding). */
+ * rounding), and of more than 2^14 sequences it is refused (VEDIC_STATUS_HIP_ERROR).  Calls of more than 128 sequences
+ * sum up their work in one more launch. */
 int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_t q_token, int64_t q_head, int q_heads, void* out,
                           int64_t out_token, int64_t out_head, float* lse, float scale, int causal, int window,
                           int stride, void* stream);

@@ -51,6 +51,7 @@ SOURCES = [
     "vedic_paged_few_i4.hip",
     "vedic_paged_many_f16.hip",
     "vedic_paged_many_i4.hip",
+    "vedic_paged_plan.hip",
     "vedic_w4.hip",
     "vedic_w4_tile.hip",
     "vedic_capi.hip",

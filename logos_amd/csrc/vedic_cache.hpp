@@ -177,6 +177,9 @@ struct PagedArgs {
     // set by the rules in vedic_capi.hip: `target` workgroups' worth of keys per item
     // (0: items are not split), and the partial results of split items
     int64_t target;
+    // null, or of many sequences the keys of a part, and for each 64 of them the items, split tiles and split
+    // items of those before (launch_paged_plan)
+    const int* plan;
     int few_most;  // sequences of at most so many rows (new rows x G) are the few-row kernel's
     int slots;
     float* part_o;   // [slots x rows x D]
@@ -185,6 +188,9 @@ struct PagedArgs {
 // Rows of a tile, and what parts of a tile's keys are whole multiples of.
 constexpr int kFewRows = 16, kManyRows = 128;
 constexpr int kFewUnit = 128, kManyUnit = 256;
+// Ints of a plan, and the plan of one kind of rows.
+inline int64_t paged_plan_ints(int sequences) { return 1 + 3 * (((int64_t)sequences + 63) / 64); }
+hipError_t launch_paged_plan(const PagedArgs& a, bool many, int* plan, hipStream_t s);
 hipError_t launch_paged_few_f16(const PagedArgs& a, hipStream_t s);
 hipError_t launch_paged_few_i4(const PagedArgs& a, hipStream_t s);
 hipError_t launch_paged_many_f16(const PagedArgs& a, hipStream_t s);

@@ -1796,6 +1796,12 @@ static constexpr int kFewMost = 64;
 // of 128 rows cost as much as 64 keys (pieces of 500 rows of three prompts: 197 us, 242 at two, 226 at four).
 static int64_t paged_target(bool many, int cus) { return many ? cus : cus * 8; }
 
+// Sequences past which the items' places are summed up beforehand, and up to which a captured call without a workspace block
+// goes without (every workgroup then walks all of them: us a call of single tokens over up to 300 keys, walked / summed up,
+// 65 sequences 36.8 / 38.1, 129 57.7 / 50.7, 512 184 / 122, 4096 3634 / 880; over up to 30, 129 16.9 / 18.2, 256 27.8 / 26.4, 16384
+// 22700 / 1650).
+static constexpr int kPlanFrom = 128, kNoPlanMost = 1 << 14;
+
 extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_t q_token, int64_t q_head, int q_heads,
                                      void* out, int64_t out_token, int64_t out_head, float* lse, float scale, int causal,
                                      int window, int stride, void* stream) {
@@ -1865,10 +1871,21 @@ extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_
             b.part_o = part;
             b.part_ml = part + slots * tile * kv->dh;
         }
+        int* plan = nullptr;
+        const size_t plan_bytes = (size_t)paged_plan_ints(kv->batch) * 4;
+        if (kv->batch > kPlanFrom && ws.room(plan_bytes)) {
+            e = ws.get(&plan, plan_bytes);
+            if (e == hipSuccess) e = launch_paged_plan(b, kind != 0, plan, ws.s);
+            if (e != hipSuccess) break;
+            b.plan = plan;
+        } else if (kv->batch > kNoPlanMost) {
+            e = hipErrorStreamCaptureUnsupported;
+            break;
+        }
         e = kind ? (i4 ? launch_paged_many_i4(b, ws.s) : launch_paged_many_f16(b, ws.s))
                  : (i4 ? launch_paged_few_i4(b, ws.s) : launch_paged_few_f16(b, ws.s));
-        const hipError_t f = ws.put(part);
-        if (e == hipSuccess) e = f;
+        const hipError_t f = ws.put(part), g = ws.put(plan);
+        if (e == hipSuccess) e = f != hipSuccess ? f : g;
     }
     return hip_status(e);
 }

@@ -8,7 +8,8 @@
 // GPU only: every workgroup adds up the keys of all tiles, takes 1 / target of them (rounded
 // up) as the length of a part, and finds its own item by a scan over the sequences; the
 // host's grid is as large as the items can be.  So a batch of one long and many short
-// sequences is dealt out evenly, whatever the table's width.
+// sequences is dealt out evenly, whatever the table's width.  Of many sequences the sums are made
+// beforehand, by 64 sequences (vedic_paged_plan.hip).
 //
 // Parts hold their sums relative to their own largest score m: O = sum of 2^(c (q.k - m) + 14) v and l
 // the same without v, c the scale times log2(e); the join multiplies by 2^(c (m - M)) in the order of
@@ -109,29 +110,71 @@ __device__ __forceinline__ int small_quotient(int a, int b) {
     return q;
 }
 
-// The item (JOIN: the split tile) number id; false if there is none.  A part has at least UNIT keys, in whole UNITs.
-template <int ROWS, bool MANY, int UNIT, bool JOIN>
-__device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, PagedItem& it) {
-    SequenceWork w = sequence_work<ROWS, MANY>(a, lane);
-    int chunk = INT32_MAX;
-    if (a.target > 0) {
-        float total = (float)w.tiles * (float)w.span;
-        for (int b0 = 64; b0 < a.c.B; b0 += 64) {
-            const SequenceWork x = sequence_work<ROWS, MANY>(a, b0 + lane);
-            total += (float)x.tiles * (float)x.span;
-        }
-        // (rounded up by more than the sums' and products' roundings: no more items than there are slots for)
-        const float each = wave_total(total) * (float)a.c.H / (float)a.target * 1.0001f + 1.0f;
-        if (each < 1e9f) chunk = ((int)each + UNIT - 1) / UNIT * UNIT;
+// Keys of a part, from `total`, the sum of all tiles' keys: whole UNITs, and no more parts than there are slots for (rounded up
+// by more than the sums' and products' roundings).
+template <int UNIT>
+__device__ __forceinline__ int part_keys(const PagedArgs& a, float total) {
+    const float each = total * (float)a.c.H / (float)a.target * 1.0001f + 1.0f;
+    return each < 1e9f ? ((int)each + UNIT - 1) / UNIT * UNIT : INT32_MAX;
+}
+// A sequence's parts a tile, tiles, items, and those of its tiles and items that are split (sums of a list that is not ascending
+// stay in range too).
+struct SequenceUnits {
+    int parts, tiles, items, split_tiles, split_items;
+    __device__ __forceinline__ SequenceUnits(const PagedArgs& a, const SequenceWork& w, int chunk) {
+        parts = w.span > chunk ? (int)(((int64_t)w.span + chunk - 1) / chunk) : 1;
+        tiles = (int)min((int64_t)w.tiles * a.c.H, int64_t(1) << 24);
+        items = (int)min((int64_t)tiles * parts, int64_t(1) << 24);
+        split_tiles = parts > 1 ? tiles : 0;
+        split_items = parts > 1 ? items : 0;
     }
+};
+
+// The last of n ascending values that is at most id (the first one is).
+__device__ __forceinline__ int last_at_most(const int* v, int n, int id, int lane) {
+    int lo = 0;
+    for (int span = n; span > 1;) {
+        const int step = (span + 63) >> 6, at = lane * step;
+        const uint64_t ok = __ballot(at < span && v[lo + min(at, span - 1)] <= id);
+        const int past = (63 - __builtin_clzll(ok | 1)) * step;
+        lo += past;
+        span = min(step, span - past);
+    }
+    return lo;
+}
+
+// The item (JOIN: the split tile) number id; false if there is none.  A part has at least UNIT keys, in whole UNITs.  PLAN: the
+// sums are there.  (Looked at here instead, other registers cost the kernels of few sequences 2 %.)
+template <int ROWS, bool MANY, int UNIT, bool JOIN, bool PLAN>
+__device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, PagedItem& it) {
+    int chunk = INT32_MAX, b0 = 0, end = a.c.B;
     int before = 0, slots = 0;  // items (JOIN: tiles) and split items of the sequences before
-    for (int b0 = 0; b0 < a.c.B; b0 += 64) {
-        if (b0 > 0) w = sequence_work<ROWS, MANY>(a, b0 + lane);
-        const int parts = w.span > chunk ? (int)(((int64_t)w.span + chunk - 1) / chunk) : 1;
-        // (sums of a list that is not ascending stay in range too)
-        const int tiles = (int)min((int64_t)w.tiles * a.c.H, int64_t(1) << 24), items = (int)min((int64_t)tiles * parts, int64_t(1) << 24);
-        const int units = !JOIN ? items : parts > 1 ? tiles : 0;
-        const int split = parts > 1 ? items : 0;
+    SequenceWork w;
+    if constexpr (PLAN) {
+        const int blocks = (a.c.B + 63) >> 6;
+        const int* items = a.plan + 1 + (JOIN ? blocks : 0);
+        const int block = __builtin_amdgcn_readfirstlane(last_at_most(items, blocks, id, lane));
+        chunk = __builtin_amdgcn_readfirstlane(a.plan[0]);
+        before = __builtin_amdgcn_readfirstlane(items[block]);
+        slots = __builtin_amdgcn_readfirstlane(a.plan[1 + 2 * blocks + block]);
+        b0 = 64 * block;
+        end = b0 + 64;
+        w = sequence_work<ROWS, MANY>(a, b0 + lane);
+    } else {
+        w = sequence_work<ROWS, MANY>(a, lane);
+        if (a.target > 0) {
+            float total = (float)w.tiles * (float)w.span;
+            for (int b = 64; b < a.c.B; b += 64) {
+                const SequenceWork x = sequence_work<ROWS, MANY>(a, b + lane);
+                total += (float)x.tiles * (float)x.span;
+            }
+            chunk = __builtin_amdgcn_readfirstlane(part_keys<UNIT>(a, wave_total(total)));
+        }
+    }
+    for (const int first = b0; b0 < end; b0 += 64) {
+        if (b0 > first) w = sequence_work<ROWS, MANY>(a, b0 + lane);
+        const SequenceUnits u(a, w, chunk);
+        const int parts = u.parts, units = JOIN ? u.split_tiles : u.items, split = u.split_items;
         const int incl = lane_sums(units), sincl = lane_sums(split);
         const uint64_t past = __ballot(id - before < incl);
         if (past) {
@@ -365,13 +408,13 @@ __device__ __forceinline__ void join_sums(float scale, float4_t& o, float& m, fl
 
 // The parts of a tile joined.  A lane has four columns of a row's share of the parts: D / 4 lanes a share, a wave's
 // shares of one row (`per` rows a workgroup, a wave each in turn), or with WHOLE a workgroup's.
-template <int ROWS, bool MANY, int UNIT, bool WHOLE>
+template <int ROWS, bool MANY, int UNIT, bool WHOLE, bool PLAN>
 __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, int per) {
     __shared__ float4_t wave_o[WHOLE ? 4 : 1][64];
     __shared__ float wave_ml[WHOLE ? 4 : 1][2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     PagedItem it;
-    if (!find_item<ROWS, MANY, UNIT, true>(a, blockIdx.x, lane, it)) return;
+    if (!find_item<ROWS, MANY, UNIT, true, PLAN>(a, blockIdx.x, lane, it)) return;
     if ((int64_t)it.slot + it.parts > a.slots) return;
     const int D = a.c.D, cols = D / 4;
     const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // of a share

@@ -120,7 +120,7 @@ struct RowShare<DP, true> {
 };
 
 // NARROW: heads of fewer than DP values.  (Looked at here instead, K's zeros cost full heads over four bits 2 to 5 %.)
-template <int DP, bool I4, bool NARROW>
+template <int DP, bool I4, bool NARROW, bool PLAN>
 __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel(PagedArgs a) {
     typedef RowShare<DP, I4> Share;
     constexpr int KK = DP / 32, DT = DP / 16, PITCH = 2 * DP + 32, OP = DP + 4;
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
     __shared__ float ml[4][16][2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     PagedItem it;
-    if (!find_item<kFewRows, false, kFewUnit, false>(a, blockIdx.x, lane, it)) return;
+    if (!find_item<kFewRows, false, kFewUnit, false, PLAN>(a, blockIdx.x, lane, it)) return;
     const KvView& c = a.c;
     const int r = lane & 15, g = lane >> 4;
     char* vb = lds + wave * (32 * PITCH);
@@ -397,31 +397,36 @@ __global__ void __launch_bounds__(256, I4 || DP <= 192 ? 2 : 1) paged_few_kernel
 
 }  // namespace
 
-template <int DP, bool I4>
+template <int DP, bool I4, bool PLAN>
 void paged_few_of(const PagedArgs& a, const dim3& grid, hipStream_t s) {
-    if (a.c.D < DP) paged_few_kernel<DP, I4, true><<<grid, 256, 0, s>>>(a);
-    else paged_few_kernel<DP, I4, false><<<grid, 256, 0, s>>>(a);
+    if (a.c.D < DP) paged_few_kernel<DP, I4, true, PLAN><<<grid, 256, 0, s>>>(a);
+    else paged_few_kernel<DP, I4, false, PLAN><<<grid, 256, 0, s>>>(a);
 }
 
-template <bool I4>
-hipError_t paged_few(const PagedArgs& a, hipStream_t s) {
+template <bool I4, bool PLAN>
+hipError_t paged_few_by(const PagedArgs& a, hipStream_t s) {
     const int64_t tiles = ((int64_t)a.c.T * a.G / kFewRows + (a.c.B < a.c.T ? a.c.B : a.c.T)) * a.c.H;
     const dim3 grid((unsigned)(tiles + a.target));
-    if (a.c.D <= 64) paged_few_of<64, I4>(a, grid, s);
-    else if (a.c.D <= 128) paged_few_of<128, I4>(a, grid, s);
-    else if (a.c.D <= 192) paged_few_of<192, I4>(a, grid, s);
-    else paged_few_of<256, I4>(a, grid, s);
+    if (a.c.D <= 64) paged_few_of<64, I4, PLAN>(a, grid, s);
+    else if (a.c.D <= 128) paged_few_of<128, I4, PLAN>(a, grid, s);
+    else if (a.c.D <= 192) paged_few_of<192, I4, PLAN>(a, grid, s);
+    else paged_few_of<256, I4, PLAN>(a, grid, s);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.target > 0) {
         const int rows = a.c.q_start == nullptr && a.G < kFewRows ? a.G : kFewRows;
         const unsigned units = (unsigned)(tiles < a.target ? tiles : a.target);
         // A workgroup a row of few tiles (one sequence of 16000 tokens, 8 heads of 128: 12.3 us by a wave a row, 5.4), a wave
         // a row of many.
-        if ((int64_t)units * rows <= 2 * a.target) paged_join_kernel<kFewRows, false, kFewUnit, true><<<dim3(units, rows), 256, 0, s>>>(a, 1);
-        else paged_join_kernel<kFewRows, false, kFewUnit, false><<<dim3(units, (rows + 3) / 4), 256, 0, s>>>(a, 4);
+        if ((int64_t)units * rows <= 2 * a.target) paged_join_kernel<kFewRows, false, kFewUnit, true, PLAN><<<dim3(units, rows), 256, 0, s>>>(a, 1);
+        else paged_join_kernel<kFewRows, false, kFewUnit, false, PLAN><<<dim3(units, (rows + 3) / 4), 256, 0, s>>>(a, 4);
         e = hipGetLastError();
     }
     return e;
+}
+
+template <bool I4>
+hipError_t paged_few(const PagedArgs& a, hipStream_t s) {
+    return a.plan ? paged_few_by<I4, true>(a, s) : paged_few_by<I4, false>(a, s);
 }
 
 }  // namespace vedic

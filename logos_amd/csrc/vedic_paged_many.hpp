@@ -103,7 +103,7 @@ private:
 // Keys among the places from t on (the first of a block), to the end of their list.
 __device__ __forceinline__ int keys_left(const PagedItem& it, int t) { return (t < it.near ? min(it.hi, it.far) : it.hi) - t; }
 
-template <int DP, bool I4>
+template <int DP, bool I4, bool PLAN>
 __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_many_kernel(PagedArgs a) {
     typedef BlockShare<DP, I4> Share;
     constexpr int KEYS = Share::KEYS, U = KEYS / 32, KK = DP / 16, DT = DP / 32;
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
     __shared__ int64_t off[2][KEYS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     PagedItem it;
-    if (!find_item<kManyRows, true, kManyUnit, false>(a, blockIdx.x, lane, it)) return;
+    if (!find_item<kManyRows, true, kManyUnit, false, PLAN>(a, blockIdx.x, lane, it)) return;
     const KvView& c = a.c;
     const int r = lane & 31, h = lane >> 5;
 
@@ -279,20 +279,25 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
 
 }  // namespace
 
-template <bool I4>
-hipError_t paged_many(const PagedArgs& a, hipStream_t s) {
+template <bool I4, bool PLAN>
+hipError_t paged_many_by(const PagedArgs& a, hipStream_t s) {
     const int64_t tiles = ((int64_t)a.c.T * a.G / kManyRows + (a.c.B < a.c.T ? a.c.B : a.c.T)) * a.c.H;
     const dim3 grid((unsigned)(tiles + a.target)), join((unsigned)(tiles < a.target ? tiles : a.target), 4);
-    if (a.c.D <= 64) paged_many_kernel<64, I4><<<grid, 256, 0, s>>>(a);
-    else if (a.c.D <= 128) paged_many_kernel<128, I4><<<grid, 256, 0, s>>>(a);
-    else if (a.c.D <= 192) paged_many_kernel<192, I4><<<grid, 256, 0, s>>>(a);
-    else paged_many_kernel<256, I4><<<grid, 256, 0, s>>>(a);
+    if (a.c.D <= 64) paged_many_kernel<64, I4, PLAN><<<grid, 256, 0, s>>>(a);
+    else if (a.c.D <= 128) paged_many_kernel<128, I4, PLAN><<<grid, 256, 0, s>>>(a);
+    else if (a.c.D <= 192) paged_many_kernel<192, I4, PLAN><<<grid, 256, 0, s>>>(a);
+    else paged_many_kernel<256, I4, PLAN><<<grid, 256, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.target > 0) {
-        paged_join_kernel<kManyRows, true, kManyUnit, false><<<join, 256, 0, s>>>(a, kManyRows / 4);
+        paged_join_kernel<kManyRows, true, kManyUnit, false, PLAN><<<join, 256, 0, s>>>(a, kManyRows / 4);
         e = hipGetLastError();
     }
     return e;
+}
+
+template <bool I4>
+hipError_t paged_many(const PagedArgs& a, hipStream_t s) {
+    return a.plan ? paged_many_by<I4, true>(a, s) : paged_many_by<I4, false>(a, s);
 }
 
 }  // namespace vedic

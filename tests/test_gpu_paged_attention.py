@@ -464,3 +464,92 @@ def test_weights_of_few_rows_over_binary16(D, new, lens):
         out, _, tol = plain.attention(b.q[r], k, v, *at)
         size = plain.attention(b.q[r], k, np.abs(v), *at)[0]  # the weights' sum of |v|
         assert (np.abs(got[r] - out) <= tol - (2.0 ** -11 - 2.0 ** -22) * size).all()
+
+
+def many_sequences(seed, count, long, four_bit=False, one_each=True):
+    """Short sequences and, at the places of `long`, (new rows, tokens) of others."""
+    rng = np.random.default_rng(seed)
+    lens = rng.integers(int(four_bit), 12, count).tolist()
+    new = [1] * count if one_each else [min(n, int(rng.integers(0, 3))) for n in lens]
+    for at, (n, L) in long.items():
+        lens[at], new[at] = L, 1 if one_each else n
+    return Batch(seed, 4, 2, 64, four_bit, 16, new, lens)
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("one_each", [True, False])
+@pytest.mark.parametrize("count,long", [(65, {64: (300, 900)}), (200, {0: (1, 1200), 128: (70, 3000)}), (4161, {4160: (90, 700), 63: (5, 2000)}),
+                                        (9000, {4100: (200, 1500)})])
+def test_many_sequences(count, long, one_each, four_bit):
+    """More than a wave's lanes, and more blocks of 64 than that; first and last ones long, parts among them."""
+    b = many_sequences(count, count, long, four_bit, one_each)
+    lse = torch.full((b.T, 4), -5.0, device="cuda")
+    out = run(b, one_each=one_each, lse=lse)
+    b.check(out, lse)
+    assert torch.equal(out, run(b, one_each=one_each))
+
+
+def test_many_sequences_captured():
+    """Recorded with a block and without, replayed after the lengths have changed in place."""
+    b = many_sequences(3, 300, {7: (1, 2000), 299: (1, 900)})
+    q, k, v, table, ln, _ = b.device()
+    keep, other = ln.clone(), ln.clone()
+    other[7], other[0], other[299] = 20, 3, 0
+    want = [vedic.paged_attention(q, k, v, table, x) for x in (keep, other)]
+    for warm in (True, False):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        out = torch.zeros_like(q)
+        with torch.cuda.stream(s):
+            if warm:
+                vedic.paged_attention(q, k, v, table, ln, out=out)
+            s.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                vedic.paged_attention(q, k, v, table, ln, out=out)
+        torch.cuda.synchronize()
+        for i in (0, 1, 0, 1):
+            ln.copy_((keep, other)[i])
+            out.fill_(9)
+            g.replay()
+            torch.cuda.synchronize()
+            if warm:
+                assert torch.equal(out, want[i])
+            assert (out - want[i]).abs().max() <= 2.0 ** -9 * 4
+            torch.randn(1000, device="cuda").sum().item()
+        ln.copy_(keep)
+        with torch.cuda.stream(s):
+            del g
+            vedic._lib.load().vedic_workspace_release(s.cuda_stream)
+        torch.cuda.synchronize()
+
+
+def test_bad_lists_of_many_sequences_stay_in_range():
+    b = many_sequences(5, 300, {5: (60, 500)}, one_each=False)
+    q, k, v, table, ln, starts = b.device()
+    table[::3, 0] = 1 << 30
+    for st in (starts.flip(0).contiguous(), starts * 0 + b.T, torch.randint(-5, b.T + 9, (301,), dtype=torch.int32, device="cuda")):
+        for lens in (ln, ln * 0 + 2 ** 31 - 1, -ln):
+            vedic.paged_attention(q, k, v, table, lens, q_start=st)
+            torch.cuda.synchronize()
+
+
+def test_more_sequences_than_a_captured_call_walks():
+    """Refused without a workspace block, where every workgroup would walk all of them; the capture goes on."""
+    n = 16385
+    k_cache, v_cache = vedic.kv_cache(1, 1, 1, 8)
+    q, table = torch.zeros(n, 1, 8, dtype=torch.float16, device="cuda"), torch.zeros(n, 1, dtype=torch.int32, device="cuda")
+    lens, out = torch.ones(n, dtype=torch.int32, device="cuda"), torch.ones_like(q)
+    v_cache.fill_(3)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            with pytest.raises(RuntimeError):
+                vedic.paged_attention(q, k_cache, v_cache, table, lens, out=out)
+            vedic.paged_attention(q[:100], k_cache, v_cache, table[:100], lens[:100], out=out[:100])
+        g.replay()
+    torch.cuda.synchronize()
+    assert (out[:100] == 3).all() and (out[100:] == 1).all()
+    assert (vedic.paged_attention(q, k_cache, v_cache, table, lens) == 3).all()
