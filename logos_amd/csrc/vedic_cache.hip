@@ -13,7 +13,7 @@
 // exchange its least and largest value by DPP.  Memory bounds it, and what comes before the angles can
 // be asked for: a workgroup has one token, so that many are at it (8192 tokens of 48 heads of 64 from fp32, cold
 // caches: 36 us, 4.3 TB/s; with four tokens a workgroup 46); the sequence of a token is the one whose rows it lies among
-// (a ballot per 64 sequences).
+// (a ballot, after a search by 64ths among more than 64: 4096 tokens of as many sequences, 16 heads of 64, 50 us by a walk, 19 so).
 #include "vedic_cache.hpp"
 
 namespace vedic {
@@ -34,17 +34,15 @@ __device__ __forceinline__ void find_row(const KvView& c, int t, int lane, int& 
         pos = __builtin_amdgcn_readfirstlane(c.len_of(t)) - 1;
         return;
     }
-    for (int b0 = 0; b0 < c.B; b0 += 64) {
-        const int b = min(b0 + lane, c.B - 1);
-        int first, n;
-        c.rows_of(b, first, n);
-        const int at = c.len_of(b) - n - first;  // the row's position less t
-        const uint64_t who = __ballot(b0 + lane < c.B && t >= first && t < first + n);
-        if (who == 0) continue;
-        seq = b0 + __builtin_ctzll(who);
-        pos = t + __builtin_amdgcn_readlane(at, __builtin_ctzll(who));
-        return;
-    }
+    // (of many sequences the last that begins at the row or before it: empty ones begin where the next one does)
+    const int b0 = c.B > 64 ? last_at_most(c.q_start, c.B, t, lane) : 0, b = min(b0 + lane, c.B - 1);
+    int first, n;
+    c.rows_of(b, first, n);
+    const int at = c.len_of(b) - n - first;  // the row's position less t
+    const uint64_t who = __ballot(b0 + lane < c.B && t >= first && t < first + n);
+    if (who == 0) return;
+    seq = b0 + __builtin_ctzll(who);
+    pos = t + __builtin_amdgcn_readlane(at, __builtin_ctzll(who));
 }
 
 template <bool F32>

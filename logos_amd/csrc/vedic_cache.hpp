@@ -66,6 +66,19 @@ struct KvView {
     }
 };
 
+// The last of n ascending values that is at most id (the first one is).
+__device__ __forceinline__ int last_at_most(const int* v, int n, int id, int lane) {
+    int lo = 0;
+    for (int span = n; span > 1;) {
+        const int step = (span + 63) >> 6, at = lane * step;
+        const uint64_t ok = __ballot(at < span && v[lo + min(at, span - 1)] <= id);
+        const int past = (63 - __builtin_clzll(ok | 1)) * step;
+        lo += past;
+        span = min(step, span - past);
+    }
+    return lo;
+}
+
 // Four-bit words: 32 bits hold eight consecutive values, value 2 i in bits 4 i .. 4 i + 3 and
 // value 2 i + 1 in bits 16 + 4 i ..; code n of a group with the binary16 pair (s, m) stands
 // for binary16(s n + m), one rounding.  n | 0x6400 is the binary16 1024 + n, and a nibble at

@@ -130,19 +130,6 @@ struct SequenceUnits {
     }
 };
 
-// The last of n ascending values that is at most id (the first one is).
-__device__ __forceinline__ int last_at_most(const int* v, int n, int id, int lane) {
-    int lo = 0;
-    for (int span = n; span > 1;) {
-        const int step = (span + 63) >> 6, at = lane * step;
-        const uint64_t ok = __ballot(at < span && v[lo + min(at, span - 1)] <= id);
-        const int past = (63 - __builtin_clzll(ok | 1)) * step;
-        lo += past;
-        span = min(step, span - past);
-    }
-    return lo;
-}
-
 // The item (JOIN: the split tile) number id; false if there is none.  A part has at least UNIT keys, in whole UNITs.  PLAN: the
 // sums are there.  (Looked at here instead, other registers cost the kernels of few sequences 2 %.)
 template <int ROWS, bool MANY, int UNIT, bool JOIN, bool PLAN>

@@ -216,3 +216,31 @@ def test_recorded_beside_another_stream():
     for c in caches:
         assert torch.equal(c[0].transpose(1, 2).reshape(64, 2, 64)[:40], x[:, 0])
     assert torch.equal(caches[0][1], caches[1][1])
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("count", [64, 65, 300, 4160])
+def test_many_sequences(count, four_bit):
+    """Empty ones among them, at both ends too, more than a wave's lanes and more blocks of 64 than that."""
+    rng = np.random.default_rng(count)
+    lens = rng.integers(0, 9, count)
+    new = np.minimum(lens, rng.integers(0, 4, count))
+    new[0] = new[-1] = new[count // 2:count // 2 + 20] = 0
+    append_and_check(count, 1, 1, 32, four_bit, 4, new.tolist(), lens.tolist(), 32, False, torch.float16)
+
+
+def test_a_padded_batch_of_many_sequences():
+    """Rows before the first of 200 sequences and behind the last one belong to none."""
+    n = 200
+    k_cache, v_cache = vedic.kv_cache(n, 4, 1, 8)
+    x = torch.randn(n + 9, 1, 8, device="cuda").half()
+    table = torch.arange(n, dtype=torch.int32, device="cuda")[:, None]
+    lens, starts = torch.full((n,), 2, dtype=torch.int32, device="cuda"), torch.arange(n + 1, dtype=torch.int32, device="cuda") + 5
+    out = torch.full((n + 9, 1, 8), 5.0, dtype=torch.float16, device="cuda")
+    vedic.kv_append(x, x, x, k_cache, v_cache, table, lens, starts, out=out)
+    assert torch.equal(out[5:-4], x[5:-4]) and (out[:5] == 5).all() and (out[-4:] == 5).all()
+    assert torch.equal(k_cache[:, 0, 1], x[5:-4, 0]) and (k_cache[:, 0, [0, 2, 3]] == 0).all()
+    for st in (starts.flip(0).contiguous(), torch.randint(-9, n + 30, (n + 1,), dtype=torch.int32, device="cuda")):
+        vedic.kv_append(x, x, x, k_cache, v_cache, table, lens, st)
+        vedic.kv_read(k_cache, v_cache, table, lens, st, tokens=n + 9)
+        torch.cuda.synchronize()
