@@ -302,7 +302,21 @@ void few(const W4Args& a, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_w4_few(const W4Args& a, int cus, hipStream_t s) {
+hipError_t launch_w4_few(const W4Args& all, int cus, hipStream_t s) {
+    // (a launch's second dimension ends at 2^16: only a captured call without a workspace block comes here with so many rows)
+    constexpr int kMostRows = kW4FewRows * ((1 << 16) - 1);
+    if (all.M > kMostRows) {
+        W4Args part = all;
+        for (int m = 0; m < all.M; m += part.M) {
+            part.X = static_cast<const char*>(all.X) + m * all.ldx * (all.x32 ? 4 : 2);
+            part.C = static_cast<char*>(all.C) + m * all.ldc * (all.c16 ? 2 : 4);
+            part.M = all.M - m < kMostRows ? all.M - m : kMostRows;
+            const hipError_t e = launch_w4_few(part, cus, s);
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
+    }
+    const W4Args& a = all;
     // Column blocks a wave: as many as leave a workgroup for every CU, so that X is not read more often than that
     // needs (us with 1 / 2 / 4: 16 rows of 1024 into 4096 3.9 / 4.2 / 5.4, of 2048 into 8192 8.7 / 6.9 / 8.9, of 4096
     // into 16384 25.5 / 18.5 / 15.8; 64 rows of 1024 into 4096 7.0 / 7.7 / 11.2, of 4096 into 16384 74 / 46 / 32).

@@ -231,3 +231,23 @@ def test_many_rows_captured():
 @pytest.mark.parametrize("M,K,N", [(20000, 64, 17), (17000, 33, 5), (4000, 264, 129)])
 def test_narrow_weights_of_many_rows(M, K, N):
     check(M + N, M, K, N, 32, vedic.EPI_BIAS)
+
+
+def test_more_rows_than_one_launch_takes_captured():
+    """fp32 rows past 64 * 65535, without a workspace block: whole numbers, exact in any order."""
+    M, K, N = 64 * 65535 + 200, 8, 3
+    n = torch.randint(0, 16, (N, 32), generator=torch.Generator().manual_seed(1))
+    codes = plain.words(n.numpy().astype(np.uint32)).view(np.int32)
+    w = vedic.W4(torch.from_numpy(codes).cuda(), torch.tensor([[[1.0, -8.0]]] * N, dtype=torch.float16, device="cuda"), K, 32)
+    X = torch.randint(-9, 10, (M, K), device="cuda").float()
+    out = torch.full((M, N), 7.0, dtype=torch.float16, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            vedic.gemm_w4(X, w, out=out)
+        g.replay()
+    torch.cuda.synchronize()
+    want = (X.double().cpu() @ (n[:, :K].double().t() - 8)).half()
+    assert torch.equal(out.cpu(), want)
