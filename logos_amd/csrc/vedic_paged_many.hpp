@@ -236,7 +236,9 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
         }
         const float mu = m == kNoScore ? 0.0f : m;
         float bias = __builtin_fmaf(-mu, a.scale, kWeightBits);
-        if (__any(__builtin_fabsf(bias) > 0x1p20f)) {  // (c m far from its rounding: differences of scores, as everywhere else)
+        // (c m's rounding is in all of a block's weights, but not the same in the next block's, and below 2^-14 of them up to
+        // here; past it differences of scores, as everywhere else)
+        if (__any(__builtin_fabsf(bias) > 0x1p10f)) {
             bias = kWeightBits;
 #pragma unroll
             for (int u = 0; u < U; ++u)

@@ -553,3 +553,30 @@ def test_more_sequences_than_a_captured_call_walks():
     torch.cuda.synchronize()
     assert (out[:100] == 3).all() and (out[100:] == 1).all()
     assert (vedic.paged_attention(q, k_cache, v_cache, table, lens) == 3).all()
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+def test_scores_of_some_thousands(four_bit):
+    """Rows whose scores rise from key to key, all near -2^12 or 2^12 times the scale's unit, so that every block brings a new largest
+    one: weights of different blocks against each other, at the scores' own rounding."""
+    b = Batch(71, 4, 2, 64, four_bit, 32, [200, 90], [900, 3000])
+    for x in b.x:
+        x[:] = 0
+    for s in range(2):
+        for t in range(b.lens[s]):
+            page, at = b.table[s, t // 32], t % 32
+            b.x[0][page, :, at, :2] = 64 * t / b.lens[s], 64.0
+            b.x[1][page, :, at] = np.float16(np.random.default_rng(t).standard_normal(64))
+    b.rows = [plain.rows_of(x, four_bit) for x in b.x]
+    b.q[:] = 0
+    b.q[:, :, 0], b.q[:, ::2, 1], b.q[:, 1::2, 1] = 0.125, 48.0, -48.0
+    got = run(b, scale=1.0).double().cpu().numpy()
+    for s in range(2):
+        r = slice(b.starts[s], b.starts[s + 1])
+        k, v = b.sequence(s)
+        at = (np.arange(b.lens[s] - b.new[s], b.lens[s]), 1.0)
+        out = plain.attention(b.q[r], k, v, *at)[0]
+        size = plain.attention(b.q[r], k, np.abs(v), *at)[0]
+        # (two products of a score that are not 0, both exact, and a sum below 2^12: 2^-13 off, above and below the division; the
+        # weights' half step, 2^-11; c times the differences, exponentials and sums, 2^-13)
+        assert (np.abs(got[r] - out) <= 2.0 ** -11 * np.abs(out) + (2.0 ** -11 + 2.0 ** -12 + 2.0 ** -13) * size + 2.0 ** -25).all()
