@@ -580,3 +580,30 @@ def test_scores_of_some_thousands(four_bit):
         # (two products of a score that are not 0, both exact, and a sum below 2^12: 2^-13 off, above and below the division; the
         # weights' half step, 2^-11; c times the differences, exponentials and sums, 2^-13)
         assert (np.abs(got[r] - out) <= 2.0 ** -11 * np.abs(out) + (2.0 ** -11 + 2.0 ** -12 + 2.0 ** -13) * size + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("four_bit,D,ps", [(True, 64, 16), (True, 128, 48), (True, 160, 7), (True, 256, 33), (False, 40, 5), (False, 128, 100),
+                                           (False, 160, 7), (False, 256, 32)])
+@pytest.mark.parametrize("window,stride", [(40, 0), (33, 100), (64, 16), (200, 3), (7, 1)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [5, 140, 33]])
+def test_masks_of_other_shapes(four_bit, D, ps, window, stride, new):
+    """Lists of 0 to some hundred far keys, that end within a block of 32 or 64, over pages of any size and both formats."""
+    b = Batch(window + stride + D, 4, 2, D, four_bit, ps, new, [n + p for n, p in zip(new, (1, 1700, 380))])
+    lse = torch.full((b.T, 4), -5.0, device="cuda")
+    b.check(run(b, window=window, stride=stride, lse=lse), lse, window=window, stride=stride)
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+def test_the_largest_lengths_and_rows_stay_in_range(four_bit):
+    """INT_MAX and INT_MIN in the lists, far keys of a window among them."""
+    b = Batch(4, 4, 2, 64, four_bit, 16, [4, 90, 2], [40, 120, 33])
+    q, k, v, table, _, _ = b.device()
+    top, low = 2 ** 31 - 1, -2 ** 31
+    wild = torch.tensor([[top, low, 2], [3, low, -1], [0, top, 0]], dtype=torch.int32, device="cuda")
+    for ln in ([top, 500, low], [top, top, top]):
+        for st in ([0, 90, 20, 96], [low, 10, top, 3], [0, 4, 94, top]):
+            for mask in (dict(), dict(window=20, stride=3), dict(causal=False)):
+                got = vedic.paged_attention(q, k, v, wild, torch.tensor(ln, dtype=torch.int32, device="cuda"),
+                                            q_start=torch.tensor(st, dtype=torch.int32, device="cuda"), **mask)
+                torch.cuda.synchronize()
+                assert got.shape == (96, 4, 64)
