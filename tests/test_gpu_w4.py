@@ -251,3 +251,35 @@ def test_more_rows_than_one_launch_takes_captured():
     torch.cuda.synchronize()
     want = (X.double().cpu() @ (n[:, :K].double().t() - 8)).half()
     assert torch.equal(out.cpu(), want)
+
+
+@pytest.mark.parametrize("x32", [False, True])
+@pytest.mark.parametrize("epilogue,out", [(vedic.EPI_NONE, torch.float32), (vedic.EPI_BIAS_GELU, torch.float16), (vedic.EPI_BIAS_RESIDUAL, torch.float32)])
+@pytest.mark.parametrize("M,K,N,group", [(2048, 2048, 4096, 128), (2040, 2112, 4100, 64), (2048, 2176, 4224, 32)])
+def test_tall_tiles(M, K, N, group, epilogue, out, x32):
+    """Tiles of 256 rows: K in whole steps, an even and an odd number of them, whole and ragged rows and columns."""
+    check(M + K, M, K, N, group, epilogue, out, x32)
+
+
+def test_captured_without_a_block_to_fp32():
+    """Rows that go 64 at a time in a graph whose stream has no workspace block, against 64 bits."""
+    w, v = weight(5, 512, 384, 64)
+    v = v.astype(np.float64)
+    for M in (1, 40, 300):
+        X = torch.randn(M, 512, device="cuda").half()
+        x64 = X.double().cpu().numpy()
+        want, tol = x64 @ v, 516 * 2.0 ** -24 * (np.abs(x64) @ np.abs(v))
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        out = torch.zeros(M, 384, device="cuda")
+        with torch.cuda.stream(s):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                vedic.gemm_w4(X, w, out=out)
+        for _ in range(3):
+            out.fill_(9)
+            g.replay()
+            torch.cuda.synchronize()
+            assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()
+            torch.randn(1000, device="cuda").sum().item()
+        del g
