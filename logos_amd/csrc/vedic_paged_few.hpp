@@ -12,8 +12,9 @@
 // the order in which the second product then contracts: the weights stay in registers.
 // K and V of the next 32 keys are loaded as soon as their registers are free; a wave has 16 KB
 // under way (binary16, heads of 128), a CU eight to twelve waves.  Reading the cache bounds it (32 sequences of up to
-// 16384 tokens, 8 key heads of 128: 203 us, 5.5 TB/s), in four bits expanding it as well (64 sequences: 170 us, 4.4 TB/s), and
-// for one sequence what an item looks up one after another: lists, table, rows (4099 tokens in 16 heads of 64: 8.2 us).
+// 16384 tokens, 8 key heads of 128: 203 us, 5.5 TB/s), in four bits expanding it as well (64 sequences: 184 us, 4.0 TB/s, the
+// vector pipes busy 63 % of it), and for one sequence what an item looks up one after another: lists, table, rows (4099 tokens
+// in 16 heads of 64: 8.7 us).
 //
 // Four bits: lane group g takes values g DP/4 .. + DP/4 - 1 of a token's row, whole words; K is
 // expanded in registers as the MFMA takes it, V as it goes to LDS.

@@ -13,9 +13,11 @@
 // layout, a row of Q per lane, is what the second product takes: the weights stay in
 // registers.  Masks are looked at only where some key of a block is hidden from a row of the wave.
 //
-// Bound by the vector instructions of the weights (score to exponential, sum, binary16) beside the matrix instructions: a
-// prompt of 8192 in 16 heads of 64 191 us, 718 TFLOP/s of what its mask leaves; three waves a SIMD hide most of one
-// kind behind the other (two: 237 us).
+// Bound by the vector and the matrix instructions of a wave, which take turns more than they overlap: of a prompt of 8192 in 16
+// heads of 64 (198 us in a row of calls, 690 TFLOP/s of what its mask leaves; 195 to 209 by box) the vector pipes are busy 63 %
+// and the matrix pipes 32 %, the LDS 33 %.  A block of 64 keys takes a wave 16 matrix instructions and about 220 vector ones,
+// 144 of them the weights' (maximum, fma, exponential, sum, half a conversion each), the others rescaling, masks and the next
+// block's way to LDS.  Three waves a SIMD hide some of one kind behind the other (two: 237 us).
 #pragma once
 
 #include "vedic_paged.hpp"
