@@ -1844,7 +1844,7 @@ extern "C" int vedic_paged_attention(const vedic_kv_t* kv, const void* q, int64_
     // sequences may be of both kinds runs both, each on its own ones.  With more than kFewMost rows a sequence on average
     // the many-row kernel takes all of them, but for heads past 192: single tokens cost it little beside a long piece, and
     // the other launches cost 6 us and what the kernels do not overlap (us, both kernels / the many-row one, 2000 rows and 15
-    // single tokens over 4000 keys and more: 16 heads of 64 168 / 148, 16 of 128 258 / 215, 12 over 4 of 96 163 / 150, 32 over 8
+    // single tokens over 4000 keys and more: 16 heads of 64 in four bits 168 / 148, 16 of 128 258 / 215, 12 over 4 of 96 163 / 150, 32 over 8
     // of 128 274 / 280, over 8000 keys 467 / 505, four bits 432 / 526; 8 over 2 of 256 269 / 346).
     const bool many = rows > kFewMost && (kv->q_start || a.G > kFewMost);
     const bool few = !many || (kv->q_start && (rows < (int64_t)kFewMost * kv->batch || (kv->batch > 1 && kv->dh > 192)));
