@@ -247,8 +247,8 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) paged_m
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[u][e] -= mu;
         }
-        // (in 11 bits; a second part would cost 27 to 37 %: a prompt of 8192 in 16 heads of 64 195 / 266 us, three pieces of 500
-        // rows over four bits 187 / 237)
+        // (In 11 bits, which is off about as much as the output's own rounding.  A second part would cost 27 to 37 %: a prompt of
+        // 8192 in 16 heads of 64 195 / 266 us, three pieces of 500 rows over four bits 187 / 237.)
         half8_t p[2 * U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
